@@ -291,7 +291,8 @@ class Kernels:
                      "memory was not 1024-byte aligned)",
                      "attention met a visible position whose page is absent or outside the cache (it read page 0 "
                      "instead; the result is wrong)",
-                     "a token stands at a position past the model's table of positions"]
+                     "a token stands at a position past the model's table of positions",
+                     "the lengths of a step's requests do not fit its rows, its page lists or its page tables"]
             raise KernelError("device error: " + "; ".join(n for n, f in zip(names, flags) if f))
 
     # ------------------------------------------------------------------ row-wise kernels
@@ -719,6 +720,148 @@ class Kernels:
             if rc != 0:
                 raise KernelError(f"attn_mma: {lib.braid_last_error().decode(errors='replace')} (code {rc})")
 
+    # ------------------------------------------------------------------ a cache held in 4 bits
+    def _on_device(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
+        """Refuse tensors that are not on the device these kernels launch on, and launches while another one is current."""
+        for t in tensors:
+            if t is not None and (t.device.type != "cuda" or t.device.index != self._device_index):
+                raise KernelError(f"{what}: a tensor on {t.device}; these kernels run on cuda:{self._device_index}")
+        if torch.cuda.current_device() != self._device_index:
+            raise KernelError(f"{what}: the current device is not cuda:{self._device_index}")
+
+    @staticmethod
+    def _i32(what: str, name: str, t: Optional[torch.Tensor], least: int) -> None:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least):
+            raise KernelError(f"{what}: {name} must be contiguous int32 with at least {least} numbers")
+
+    @staticmethod
+    def kv4_supports(head_dim: int) -> bool:
+        """Head sizes that a 4-bit cache holds: whole groups of 32 numbers, up to 256."""
+        return head_dim % 32 == 0 and 32 <= head_dim <= 256
+
+    @staticmethod
+    def kv4_page_bytes(head_dim: int) -> int:
+        """Bytes that a page's tokens take of one kv head, keys and values: 1.25 a number pair (csrc/kv4.cuh has the layout)."""
+        if not Kernels.kv4_supports(head_dim):
+            raise KernelError(f"a 4-bit cache holds heads of 32, 64, ... 256 numbers, not {head_dim}")
+        return build.page_size() * (head_dim + head_dim // 4)
+
+    def _check_kv4(self, what: str, cache: torch.Tensor, hd: int) -> None:
+        if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[2] != self.kv4_page_bytes(hd):
+            raise KernelError(f"{what}: the cache must be contiguous uint8 [pages, kv_heads, {self.kv4_page_bytes(hd)}], got {cache.dtype} "
+                              f"{tuple(cache.shape)}")
+
+    def step_tables(self, q_len: torch.Tensor, kv_before: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, place: torch.Tensor, *,
+                    num_pages: int, positions: Optional[torch.Tensor] = None, token_seq: Optional[torch.Tensor] = None,
+                    q_start: Optional[torch.Tensor] = None) -> None:
+        """A step's tables from its requests' lengths, all int32 on the device.  Request i brings q_len[i] tokens behind kv_before[i]
+        cached ones and holds the next ceil((kv_before[i] + q_len[i]) / page size) entries of `pages` (-1: given back).  Written:
+        page_table [n, cols] (-1 beyond a request's blocks), place [rows] (the cache place, page * page size + position in the page,
+        of every new token; -1 for rows past the tokens) and, where given, positions and token_seq [rows] (0 and -1 past the tokens)
+        and q_start [n].  Lengths that fit neither the rows, the list nor the table, and pages outside [0, num_pages), raise a device error
+        (`check_device_errors`); what does not fit is not written anywhere else."""
+        lib = self.part_library("kv4")
+        n = q_len.numel()
+        if page_table.dim() != 2 or page_table.shape[0] != n or kv_before.numel() != n:
+            raise KernelError(f"step_tables: {n} requests want as many kv_before and rows of the page table, got {kv_before.numel()} and "
+                              f"{tuple(page_table.shape)}")
+        rows, cols = place.numel(), page_table.shape[1]
+        for name, t, size in (("q_len", q_len, n), ("kv_before", kv_before, n), ("pages", pages, 0), ("page_table", page_table, n * cols),
+                              ("place", place, rows), ("positions", positions, rows), ("token_seq", token_seq, rows), ("q_start", q_start, n)):
+            self._i32("step_tables", name, t, size)
+        self._on_device("step_tables", q_len, kv_before, pages, page_table, place, positions, token_seq, q_start)
+        self.launches += 1
+        self._check_lib(lib, lib.braid_step_tables(
+            q_len.data_ptr(), kv_before.data_ptr(), pages.data_ptr(), page_table.data_ptr(), place.data_ptr(), _ptr(positions),
+            _ptr(token_seq), _ptr(q_start), n, pages.numel(), rows, cols, int(num_pages), self._error_flag.data_ptr() + 24, self._stream()),
+            "step_tables")
+
+    def kv4_store(self, k: torch.Tensor, v: torch.Tensor, place: torch.Tensor, cache: torch.Tensor, hd: int) -> None:
+        """Write keys and values [rows, kv_heads * hd] (rows of any stride, float32 or bfloat16) into a 4-bit cache at the rows'
+        places (`step_tables`; -1: a row of padding, not written; no place twice).  They are rounded to bfloat16 first, as an
+        ordinary cache of a bfloat16 run holds them."""
+        lib = self.part_library("kv4")
+        self._check_kv4("kv4_store", cache, hd)
+        nkh, rows = cache.shape[1], k.shape[0]
+        for x in (k, v):
+            if x.dim() != 2 or x.shape != (rows, nkh * hd) or x.stride(1) != 1 or x.dtype != k.dtype:
+                raise KernelError(f"kv4_store: keys and values are rows of {nkh * hd} numbers of one element type, got {tuple(k.shape)} and "
+                                  f"{tuple(v.shape)}")
+        self._i32("kv4_store", "place", place, rows)
+        self._on_device("kv4_store", k, v, place, cache)
+        self.launches += 1
+        self._check_lib(lib, lib.braid_kv4_store(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), dtype_code(k.dtype), place.data_ptr(),
+                                                 cache.data_ptr(), rows, nkh, hd, cache.shape[0], self._error_flag.data_ptr(),
+                                                 self._stream()), "kv4_store")
+
+    def kv4_expand(self, cache: torch.Tensor, out: torch.Tensor, page_table: torch.Tensor, q_len: torch.Tensor, kv_before: torch.Tensor,
+                   window: Optional[int] = None, keep_first: int = 0) -> None:
+        """Read the pages that a step's queries see back into ordinary ones, out [pages, 2, kv_heads, page size, hd] (float32 or
+        bfloat16), page for page: with a window, from the first block that a sequence's first new token sees, and its kept first
+        blocks.  Places of those pages behind the sequence's end come out zero; other pages stay as they were.  A page belongs to one
+        sequence."""
+        lib = self.part_library("kv4")
+        if out.dim() != 5 or out.shape[0] != cache.shape[0] or out.shape[1] != 2 or out.shape[3] != build.page_size() or not out.is_contiguous():
+            raise KernelError(f"kv4_expand: the pages must be contiguous [{cache.shape[0]}, 2, kv_heads, {build.page_size()}, head_dim], got "
+                              f"{tuple(out.shape)}")
+        hd, n = out.shape[4], page_table.shape[0]
+        self._check_kv4("kv4_expand", cache, hd)
+        if out.shape[2] != cache.shape[1]:
+            raise KernelError(f"kv4_expand: the cache holds {cache.shape[1]} kv heads, the pages {out.shape[2]}")
+        for name, t, size in (("page_table", page_table, 0), ("q_len", q_len, n), ("kv_before", kv_before, n)):
+            self._i32("kv4_expand", name, t, size)
+        self._on_device("kv4_expand", cache, out, page_table, q_len, kv_before)
+        self.launches += 1
+        self._check_lib(lib, lib.braid_kv4_expand(cache.data_ptr(), out.data_ptr(), dtype_code(out.dtype), page_table.data_ptr(), q_len.data_ptr(),
+                                                  kv_before.data_ptr(), n, page_table.shape[1], cache.shape[1], hd, cache.shape[0],
+                                                  int(window or 0), int(keep_first or 0), self._error_flag.data_ptr() + 16, self._stream()),
+                        "kv4_expand")
+
+    def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
+                 q_len: torch.Tensor, kv_before: torch.Tensor, token_seq: torch.Tensor, n_seqs: int, max_q_len: int, max_kv_len: int,
+                 nqh: int, nkh: int, hd: int, window: Optional[int], scale: float, sink: Optional[float] = None, out_scale: float = 1.0,
+                 head_sinks: Optional[torch.Tensor] = None, head_gate: Optional[torch.Tensor] = None, keep_first: int = 0,
+                 head_scale: Optional[torch.Tensor] = None, distance_bias: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                 softcap: Optional[float] = None, backend: str = "auto") -> None:
+        """Attention over a 4-bit cache, of single tokens and of prompts, float32 or bfloat16 (q [rows, >= nqh * hd], a view of
+        wider rows is fine; out [rows, nqh * hd]).  Options as in `attn_simple`.  `max_q_len` and `max_kv_len` bound what a sequence
+        brings and what it holds after the step.  Rows of padding (token_seq -1) are left as they were."""
+        what = "attn_kv4"
+        if backend not in ("auto", "plain"):
+            raise KernelError(f"attn_kv4: unknown backend {backend!r} (auto, plain)")
+        self._check_kv4(what, cache, hd)
+        self._check_head_extras(head_sinks, head_gate, nqh, out.dtype, head_scale, distance_bias)
+        rows = out.shape[0]
+        dtype_code(out.dtype)
+        if q.dim() != 2 or out.dim() != 2 or q.stride(1) != 1 or out.stride(1) != 1 or q.shape[0] < rows or q.shape[1] < nqh * hd \
+                or out.shape[1] < nqh * hd or q.dtype != out.dtype:
+            raise KernelError(f"attn_kv4: queries and result are rows of {nqh} heads of {hd} numbers, of one element type")
+        if cache.shape[1] != nkh or nkh <= 0 or nqh <= 0 or nqh % nkh:
+            raise KernelError(f"attn_kv4: {nqh} query heads over {nkh} kv heads, and a cache of {cache.shape[1]}")
+        if head_gate is not None and head_gate.shape[0] < rows:
+            raise KernelError(f"attn_kv4: gates for {head_gate.shape[0]} of {rows} rows")
+        if softcap is not None and (not softcap > 0 or distance_bias is not None):
+            raise KernelError("attn_kv4: a cap on the scores is positive and does not go with a distance bias")
+        if page_table.dim() != 2 or page_table.shape[0] < n_seqs:
+            raise KernelError(f"attn_kv4: a page table of {n_seqs} sequences is wanted, got {tuple(page_table.shape)}")
+        if int(keep_first or 0) < 0 or int(window or 0) < 0 or max_q_len < 0 or max_kv_len < 0:
+            raise KernelError("attn_kv4: window, keep_first and lengths must not be negative")
+        for name, t, size in (("page_table", page_table, 0), ("q_start", q_start, n_seqs), ("q_len", q_len, n_seqs),
+                              ("kv_before", kv_before, n_seqs), ("token_seq", token_seq, rows)):
+            self._i32(what, name, t, size)
+        self._on_device(what, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, head_sinks, head_gate, head_scale,
+                        *(distance_bias or ()))
+        if rows == 0 or n_seqs == 0:
+            return
+        lib = self.part_library("kv4")
+        self.launches += 1
+        self._check_lib(lib, lib.braid_attn_kv4_simple(
+            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype_code(out.dtype), cache.data_ptr(), page_table.data_ptr(),
+            token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(), rows, nqh, nkh, hd, page_table.shape[1], cache.shape[0],
+            int(window or 0), int(keep_first or 0), float(scale), int(sink is not None), float(sink or 0.0), float(out_scale),
+            _ptr(head_sinks), _ptr(head_gate), head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale),
+            *self._bias_args(distance_bias), float(softcap or 0.0), self._error_flag.data_ptr() + 16, self._stream()), what)
+
     # ------------------------------------------------------------------ element-wise kernels of other models
     def dyt(self, x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, alpha: torch.Tensor, out: torch.Tensor,
             row_index: Optional[torch.Tensor] = None, in_scale: float = 1.0) -> None:
@@ -838,6 +981,14 @@ class Kernels:
                 lib.braid_delta_work_floats.argtypes = [c_int] * 5
                 lib.braid_delta_work_floats.restype = c_longlong
                 names = ("braid_delta_rule", "braid_delta_gated_norm")
+            elif name == "kv4":
+                lib.braid_step_tables.argtypes = [c_void_p] * 8 + [c_int] * 5 + [c_void_p, c_void_p]
+                lib.braid_kv4_store.argtypes = [c_void_p, c_longlong] * 2 + [c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_void_p]
+                lib.braid_kv4_expand.argtypes = [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 7 + [c_void_p, c_void_p]
+                lib.braid_attn_kv4_simple.argtypes = [c_void_p, c_longlong] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 8 + \
+                                                     [c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_longlong] + [c_void_p] * 3 + \
+                                                     [c_float, c_void_p, c_void_p]
+                names = ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand", "braid_attn_kv4_simple")
             elif name == "streams":
                 lib.braid_streams.argtypes = [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
                                               c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,

@@ -33,9 +33,9 @@ CORE_SOURCES = ["errors.cu", "elementwise.cu", "pointwise.cu", "attn_simple.cu",
 # Kernels that only some models use: each a library of its own, compiled when a model that needs it is built.
 PART_SOURCES = {"latent": ["errors.cu", "latent.cu", "latent_attn_tc.cu"], "moe": ["errors.cu", "moe.cu", "moe_tc.cu", "moe_few.cu"], "scan": ["errors.cu", "scan.cu", "scan_mma.cu", "scan_chunk.cu", "scan_step.cu"],
                 "streams": ["errors.cu", "streams.cu"], "conv": ["errors.cu", "conv_heads.cu"],
-                "delta": ["errors.cu", "delta.cu", "delta_chunk.cu"]}
+                "delta": ["errors.cu", "delta.cu", "delta_chunk.cu"], "kv4": ["errors.cu", "kv4.cu"]}
 HEADERS = ["common.cuh", "rowscale.cuh", "streamk.cuh", "tcgen05.cuh", "tcgen05_pair.cuh", "attn_tc.cuh", "attn_noalloc.h", "page.h", "trace.cuh",
-           "mma_tile.cuh", "softcap.cuh", "gated_norm.cuh", "chunk_mma.cuh", "delta.cuh", "few.cuh"]
+           "mma_tile.cuh", "softcap.cuh", "gated_norm.cuh", "chunk_mma.cuh", "delta.cuh", "few.cuh", "kv4.cuh"]
 
 
 class BuildError(RuntimeError):

@@ -1,0 +1,386 @@
+"""The 4-bit cache on the GPU (csrc/kv4.cu, csrc/attn_kv4.cu) against the plain form in 64 bits (plain_kv4.py).
+
+Tolerances.  The codes are exact, so pages have to be equal byte for byte, and read-back values to a float32 or bfloat16 rounding.
+Attention: a score is a sum of 32-bit products.  The tensor cores take the codes 128 higher; with smag[0] a score's products so, and
+U = 2^-24 a unit of float32, a group's sum is cut off twice (4 U each), the queries' own sum is rounded 5 times, and two
+multiply-adds a group join them: 16 U smag[0], which moves every probability by twice that and the exponentials' 2^-21.  In bfloat16 runs each probability times a group's
+step is rounded by 2^-8 of itself, and so is the result; prompts read keys and values as bfloat16 numbers: 2^-8 of a score's
+products and of a value.  Sums over the keys lose 2 U a tile of 16."""
+import math
+
+import pytest
+import torch
+
+import plain_kv4 as P
+from braidinfer_b200.csrc.api import KernelError, get_kernels
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def K():
+    return get_kernels(verbose=False)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def dev(x, dt=torch.int32):
+    return torch.as_tensor(x).to(dt).to(DEV)
+
+
+# ------------------------------------------------------------------ tables
+@pytest.mark.parametrize("q_len, before, pad, extra_cols", [
+    ([1], [0], 0, 0), ([1], [63], 0, 0), ([1], [64], 3, 2), ([3, 0, 5], [0, 0, 128], 0, 0), ([0, 0], [0, 130], 4, 1), ([64, 65, 1], [64, 0, 127], 31, 5),
+    ([1] * 300, [i * 7 for i in range(300)], 0, 0), ([2] * 5000, [i % 70 for i in range(5000)], 9, 0), ([40000], [100000], 1, 0)])
+def test_tables(K, q_len, before, pad, extra_cols):
+    blocks = [-(-(q + b) // 64) for q, b in zip(q_len, before)]
+    num, rows, cols = sum(blocks) + 3, sum(q_len) + pad, max(blocks) + extra_cols
+    pages = torch.randperm(num, generator=gen(len(q_len)))[:sum(blocks)].tolist()
+    at = 0
+    for q, b, n in zip(q_len, before, blocks):               # blocks that a window has given back
+        if b > 200:
+            pages[at] = -1
+        at += n
+    want = P.tables(q_len, before, pages, rows, cols)
+    n = len(q_len)
+    table, place, pos, seq, start = (torch.full(s, 77, dtype=torch.int32, device=DEV) for s in ((n, cols), (rows + 1,), (rows + 1,), (rows + 1,), (n + 1,)))
+    K.step_tables(dev(q_len), dev(before), dev(pages), table, place[:rows], num_pages=num, positions=pos[:rows], token_seq=seq[:rows], q_start=start[:n])
+    K.check_device_errors()
+    for got, w in zip((table, place[:rows], pos[:rows], seq[:rows], start[:n]), want):
+        assert got.tolist() == w
+    assert place[rows] == pos[rows] == seq[rows] == start[n] == 77
+    again, place2 = torch.empty_like(table), torch.empty_like(place[:rows])
+    K.step_tables(dev(q_len), dev(before), dev(pages), again, place2, num_pages=num)     # the others are not asked for
+    assert torch.equal(again, table) and torch.equal(place2, place[:rows])
+
+
+@pytest.mark.parametrize("q_len, before, listed, rows, cols, num", [
+    ([3, 4], [0, 0], [0, 1], 6, 1, 9),             # more tokens than rows
+    ([3, 4], [0, 61], [0, 1], 7, 2, 9),            # fewer pages than blocks
+    ([3, 4], [0, 61], [0, 1, 2], 7, 1, 9),         # a request of more blocks than the table has columns
+    ([3, 4], [0, 0], [0, 9], 7, 1, 9),             # a page outside the cache
+    ([3, 4], [0, 0], [-5, 0], 7, 1, 9),
+    ([3, 4], [0, 0], [0, -1], 7, 1, 9),            # a new token's block was given back
+    ([-3, 4], [0, 0], [0, 1], 7, 1, 9), ([3, 4], [0, -64], [0, 1], 7, 1, 9),
+    ([2 ** 31 - 1, 4], [2 ** 31 - 1, 0], [0, 1], 7, 1, 9), ([2, 4], [2 ** 31 - 2, 0], [0, 1], 7, 1, 9)])
+def test_tables_flag_what_does_not_fit(K, q_len, before, listed, rows, cols, num):
+    table, place, pos, seq = (torch.full((s + 8,), 77, dtype=torch.int32, device=DEV) for s in (2 * cols, rows, rows, rows))
+    K.step_tables(dev(q_len), dev(before), dev(listed), table[:2 * cols].view(2, cols), place[:rows], num_pages=num, positions=pos[:rows], token_seq=seq[:rows])
+    with pytest.raises(KernelError, match="lengths of a step's requests"):
+        K.check_device_errors()
+    assert all((t[-8:] == 77).all() for t in (table, place, pos, seq))
+    assert ((table[:-8] >= -1) & (table[:-8] < num)).all() and ((place[:-8] >= -1) & (place[:-8] < 64 * num)).all()
+
+
+# ------------------------------------------------------------------ write, read back
+def odd_rows(rows, kv, hd, g):
+    x = torch.randn(rows, kv, hd, generator=g, dtype=torch.float64) * torch.rand(rows, 1, 1, generator=g) * 4
+    x[0] = 3.0                                                # a group without a range
+    x[1, 0, :32] = torch.arange(32) * 0.5                     # ties
+    if rows > 8:
+        x[2, -1, 5] = math.nan
+        x[3, -1, 31] = -math.inf
+        x[4, 0, :2] = torch.tensor([3e38, -3e38])             # a range past float32
+        x[5, 0] = torch.randn(hd, generator=g) * 1e-39        # numbers below float32's normal ones
+        x[6, 0] = 1000 + torch.arange(hd)
+        x[7, 0, 1:32] = 0
+    return x
+
+
+@pytest.mark.parametrize("hd", range(32, 257, 32))
+@pytest.mark.parametrize("dt, kv, shift", [(BF, 1, 0), (BF, 2, 8), (F32, 3, 0), (BF, 3, 1), (F32, 2, 3)])
+def test_store_and_read_back(K, hd, dt, kv, shift):
+    g = gen(hd + kv)
+    rows, pages = 37, 4
+    wide = torch.zeros(rows, 2 * kv * hd + shift + 8)
+    k, v = odd_rows(rows, kv, hd, g), odd_rows(rows, kv, hd, g).flip(0)
+    wide[:, shift:shift + kv * hd], wide[:, shift + kv * hd:shift + 2 * kv * hd] = k.flatten(1), v.flatten(1)
+    wide = wide.to(dt)
+    x = [wide[:, shift + i * kv * hd:shift + (i + 1) * kv * hd] for i in (0, 1)]
+    place = torch.randperm(64 * pages, generator=g)[:rows]
+    place[[9, 20]] = -1
+    cache = torch.randint(0, 256, (pages, kv, K.kv4_page_bytes(hd)), generator=g, dtype=torch.uint8)
+    want = cache.clone()
+    for plane in (0, 1):
+        P.write(want, place, plane, x[plane].double().view(rows, kv, hd))
+    got, w = cache.to(DEV), wide.to(DEV)
+    K.kv4_store(w[:, shift:shift + kv * hd], w[:, shift + kv * hd:shift + 2 * kv * hd], dev(place), got, hd)
+    K.check_device_errors()
+    assert_pages_equal(got.cpu(), want, hd)
+    # all of it read back, but the last page: 20 of its places
+    vals = P.numbers(*P.read(got, hd))
+    for ot in (F32, BF):
+        out = torch.full((pages + 1, 2, kv, 64, hd), 5.0, dtype=ot, device=DEV)[:pages]
+        K.kv4_expand(got, out, dev([[2, 0, 3]]), dev([9]), dev([64 * 2 + 11]))
+        K.check_device_errors()
+        o = out.cpu().double()
+        assert (o[1] == 5).all() and (o[3, :, :, 20:] == 0).all()
+        for p, n in ((2, 64), (0, 64), (3, 20)):
+            a, b = o[p, :, :, :n], vals[p, :, :, :n]
+            assert torch.equal(a.isnan(), b.isnan())
+            # (the random bytes hold infinities, numbers past the type's largest, and ones below its normal ones: half a step of those)
+            inside = b.abs() < 3.3e38
+            step, least = (U, 2.0 ** -150) if ot == F32 else (2.0 ** -8 + U, 2.0 ** -134 + 2.0 ** -150)
+            assert ((a - b).abs() <= step * b.abs() + least)[inside].all() and (a[b.abs() > 3.42e38].isinf()).all()
+
+
+def assert_pages_equal(got, want, hd):
+    """Equal bytes; the bits of a NaN are whatever they are."""
+    a, b = P.read(got, hd), P.read(want, hd)
+    assert torch.equal(a[0], b[0])
+    for x, y in zip(a[1:], b[1:]):
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(0), y.nan_to_num(0))
+
+
+def test_store_outside_and_expand_of_absent_pages(K):
+    hd, kv = 64, 2
+    cache = torch.zeros(4, kv, K.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+    x = torch.randn(3, kv * hd, device=DEV)
+    K.kv4_store(x, x, dev([5, 3 * 64, 64]), cache[:2], hd)
+    with pytest.raises(KernelError, match="cache write outside"):
+        K.check_device_errors()
+    assert (cache[2:] == 0).all() and (cache[0] != 0).any() and (cache[1] != 0).any()
+    out = torch.zeros(2, 2, kv, 64, hd, device=DEV)
+    for page in (-1, 2, 1 << 30):
+        K.kv4_expand(cache[:2], out, dev([[0, page]]), dev([1]), dev([70]))
+        with pytest.raises(KernelError, match="visible position"):
+            K.check_device_errors()
+    # blocks behind the window may be absent; kept first ones may not
+    K.kv4_expand(cache[:2], out, dev([[-1, -1, 1]]), dev([2]), dev([140]), window=13)
+    K.check_device_errors()
+    K.kv4_expand(cache[:2], out, dev([[-1, -1, 1]]), dev([2]), dev([140]), window=14)
+    with pytest.raises(KernelError, match="visible position"):
+        K.check_device_errors()
+    K.kv4_expand(cache[:2], out, dev([[0, -1, 1]]), dev([2]), dev([140]), window=13, keep_first=3)
+    K.check_device_errors()
+    K.kv4_expand(cache[:2], out, dev([[-1, -1, 1]]), dev([2]), dev([140]), window=13, keep_first=3)
+    with pytest.raises(KernelError, match="visible position"):
+        K.check_device_errors()
+
+
+# ------------------------------------------------------------------ attention
+class Case:
+    """Sequences over pages in any order, with rows of padding at the end."""
+
+    def __init__(self, K, seqs, nqh, nkh, hd, dt, seed=0, pad=2, spread=1.0, lowest=None):
+        g = gen(seed + hd + nqh)
+        self.q_len, self.before = [n for n, _ in seqs], [b for _, b in seqs]
+        blocks = [-(-(n + b) // 64) for n, b in seqs]
+        self.num, self.rows, self.cols = sum(blocks) + 2, sum(self.q_len) + pad, max(blocks) + 1
+        order = torch.randperm(self.num, generator=g)[:sum(blocks)].tolist()
+        table, place, _, seq, start = P.tables(self.q_len, self.before, order, self.rows, self.cols)
+        self.table, self.seq, self.start = (torch.tensor(x, dtype=torch.int32) for x in (table, seq, start))
+        x = torch.randn(2, self.num * 64, nkh, hd, generator=g) * spread
+        x[0] += torch.randn(1, nkh, hd, generator=g) * (torch.rand(1, nkh, hd, generator=g) < 0.1) * 3
+        self.cache = torch.zeros(self.num, nkh, K.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+        every = dev(torch.arange(self.num * 64))
+        K.kv4_store(x[0].flatten(1).to(DEV), x[1].flatten(1).to(DEV), every, self.cache, hd)
+        self.q = (torch.randn(self.rows, (nqh + 1) * hd, generator=g)).to(dt).to(DEV)[:, :nqh * hd]     # rows wider than the heads
+        self.nqh, self.nkh, self.hd, self.dt = nqh, nkh, hd, dt
+
+    def run(self, K, window=None, scale=None, backend="auto", max_kv=None, max_q=None, out=None, **kw):
+        out = torch.full((self.rows, self.nqh * self.hd), 9.0, dtype=self.dt, device=DEV) if out is None else out
+        K.attn_kv4(self.q, out, self.cache, self.table.to(DEV), self.start.to(DEV), dev(self.q_len), dev(self.before), self.seq.to(DEV), len(self.q_len),
+                   max_q or max(self.q_len), max_kv or max(n + b for n, b in zip(self.q_len, self.before)), self.nqh, self.nkh, self.hd, window,
+                   scale or self.hd ** -0.5, backend=backend, **kw)
+        K.check_device_errors()
+        return out
+
+    def want(self, window=None, scale=None, sink=None, out_scale=1.0, head_sinks=None, head_gate=None, keep_first=0, head_scale=None, distance_bias=None,
+             softcap=None):
+        s = head_sinks if head_sinks is not None else torch.full((self.nqh,), sink) if sink is not None else None
+        return P.attend(self.q.double().view(self.rows, self.nqh, self.hd), self.cache, self.table, self.q_len, self.before, scale or self.hd ** -0.5, window,
+                        keep_first, s, head_gate.double() if head_gate is not None else None, out_scale, head_scale, distance_bias, softcap)
+
+    def check(self, K, **kw):
+        run_only = {k: kw.pop(k) for k in ("backend", "max_kv", "max_q") if k in kw}
+        out = self.run(K, **kw, **run_only)
+        want, mag, smag = self.want(**kw)
+        total = sum(self.q_len)
+        assert (out[total:] == 9.0).all()                    # rows of padding stay as they were
+        off = (out.double().view(want.shape) - want).abs()[:total]
+        score = 16 * U * smag[0]
+        prompt = max(self.q_len) > 8 and self.dt == BF
+        if prompt:
+            score = score + 2.0 ** -8 * smag[1]
+        if kw.get("distance_bias") is not None or kw.get("softcap"):
+            score = score + 2.0 ** -18 * 60                  # their own float32 forms: a part in 2^18 of up to 60
+        keys = max(n + b for n, b in zip(self.q_len, self.before))
+        part = 2 * score[..., None] + 2.0 ** -19 + 4 * U * (keys / 16 + 8)
+        if self.dt == BF:
+            part = part + (2 if prompt else 1) * 2.0 ** -8
+        most = mag * part + (2.0 ** -8 if self.dt == BF else 4 * U) * want.abs() + 1e-30
+        bad = off > most[:total]
+        assert not bad.any(), (bad.sum().item(), off.max().item(), most[:total][bad].min().item())
+        return out
+
+
+SHAPES = [  # sequences (new, before), heads, kv heads, head size
+    ([(1, 0)], 1, 1, 32), ([(1, 62), (1, 63), (1, 64), (1, 700)], 4, 1, 64), ([(1, 15), (1, 16), (1, 2000)], 8, 2, 128), ([(1, 333)], 16, 1, 96),
+    ([(3, 70), (8, 0), (1, 129)], 6, 2, 64), ([(8, 500)], 32, 4, 128), ([(5, 100), (0, 50), (2, 64)], 5, 5, 160), ([(1, 90), (4, 3)], 24, 1, 32),
+    ([(1, 1000)], 40, 2, 192), ([(2, 40), (7, 300)], 9, 3, 224), ([(1, 127), (6, 128)], 8, 1, 256), ([(1, 17)], 66, 1, 64)]
+
+
+@pytest.mark.parametrize("backend", ["plain", "auto"])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("seqs, nqh, nkh, hd", SHAPES)
+def test_few_tokens(K, seqs, nqh, nkh, hd, dt, backend):
+    Case(K, seqs, nqh, nkh, hd, dt).check(K, backend=backend)
+
+
+def test_nothing_to_do(K):
+    c = Case(K, [(1, 5)], 2, 1, 64, BF)
+    K.attn_kv4(c.q[:0], c.q[:0], c.cache, c.table.to(DEV), dev([0]), dev([0]), dev([5]), dev([]), 1, 1, 6, 2, 1, 64, None, 0.1)
+    K.kv4_store(torch.zeros(0, 64, device=DEV), torch.zeros(0, 64, device=DEV), dev([]), c.cache, 64)
+    K.step_tables(dev([]), dev([]), dev([]), torch.empty(0, 4, dtype=torch.int32, device=DEV), dev([]), num_pages=3)
+    K.check_device_errors()
+
+
+OPTIONS = {
+    "window": dict(window=50), "window 1": dict(window=1), "kept": dict(window=40, keep_first=70), "sink": dict(sink=1.5), "low sink": dict(sink=-1e4),
+    "high sink": dict(sink=90.0), "sinks": dict(head_sinks=True, out_scale=0.25), "gate": dict(head_gate=True, window=100), "scaled": dict(head_scale=True, scale=0.3),
+    "bias": dict(distance_bias=True, window=130), "cap": dict(softcap=3.0, scale=0.5), "negative": dict(scale=-0.2, window=33, keep_first=5)}
+
+
+def options(name, rows, nqh, dt, seed=3):
+    g = gen(seed)
+    kw = dict(OPTIONS[name])
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    for key, make in (("head_sinks", lambda: rnd(nqh).to(DEV)), ("head_gate", lambda: rnd(rows, nqh + 3).to(dt).to(DEV)[:, 1:nqh + 1]),
+                      ("head_scale", lambda: rnd(nqh).to(DEV)), ("distance_bias", lambda: (rnd(nqh).abs().to(DEV), rnd(nqh).abs().to(DEV)))):
+        if kw.get(key) is True:
+            kw[key] = make()
+    return kw
+
+
+@pytest.mark.parametrize("backend", ["plain", "auto"])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("name", OPTIONS)
+def test_options(K, name, dt, backend):
+    c = Case(K, [(1, 200), (4, 130), (2, 0), (1, 63)], 10, 2, 64, dt)
+    c.check(K, backend=backend, **options(name, c.rows, c.nqh, dt))
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("seqs, nqh, nkh, hd", [
+    ([(9, 0)], 4, 2, 64), ([(130, 0), (17, 200)], 8, 2, 128), ([(64, 64), (1, 500), (0, 9), (33, 31)], 3, 1, 32), ([(70, 5)], 20, 1, 96), ([(40, 100)], 2, 2, 256),
+    ([(12, 1000)], 6, 1, 160)])
+def test_prompts(K, seqs, nqh, nkh, hd, dt):
+    Case(K, seqs, nqh, nkh, hd, dt).check(K)
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("name", OPTIONS)
+def test_options_of_prompts(K, name, dt):
+    c = Case(K, [(50, 100), (90, 0), (1, 300)], 4, 2, 64, dt)
+    c.check(K, **options(name, c.rows, c.nqh, dt))
+
+
+@pytest.mark.parametrize("new", [1, 6, 40])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+def test_what_is_not_seen_does_not_count(K, dt, new):
+    """NaN in places behind the sequence's end and before its window, and in pages that no sequence holds; the values of a sequence
+    whose own keys hold a NaN are NaN, and its neighbour's are not."""
+    c = Case(K, [(new, 150), (new, 90)], 4, 2, 64, dt)
+    clean = c.run(K, window=20)
+    L = [n + b for n, b in zip(c.q_len, c.before)]
+    held = {}
+    for i in (0, 1):
+        for blk in range(-(-L[i] // 64)):
+            held[int(c.table[i, blk])] = (i, blk)
+    bad = []
+    for p in range(c.num):
+        for t in range(64):
+            i, blk = held.get(p, (None, 0))
+            at = blk * 64 + t
+            if i is None or at >= L[i] or at <= c.before[i] - 20:
+                bad.append(p * 64 + t)
+    nan = torch.full((len(bad), 2 * 64), math.nan, device=DEV)
+    K.kv4_store(nan, nan, dev(bad), c.cache, 64)
+    assert torch.equal(c.run(K, window=20), clean)
+    # the second sequence's own last key
+    last = int(c.table[1, (L[1] - 1) // 64]) * 64 + (L[1] - 1) % 64
+    K.kv4_store(nan[:1], nan[:1], dev([last]), c.cache, 64)
+    out = c.run(K, window=20)
+    assert torch.equal(out[:2 * new - 1], clean[:2 * new - 1]) and out[2 * new - 1].isnan().all() and (out[2 * new:] == 9).all()
+
+
+@pytest.mark.parametrize("backend", ["plain", "auto"])
+@pytest.mark.parametrize("new", [1, 30])
+def test_absent_pages_are_flagged(K, new, backend):
+    c = Case(K, [(new, 100)], 4, 2, 64, BF)
+    for page in (-1, c.num, 1 << 30):
+        c.table[0, 0] = page
+        with pytest.raises(KernelError, match="visible position"):
+            c.run(K, backend=backend)
+    c.table[0, 0] = -1
+    c.run(K, backend=backend, window=30)                      # behind the window: nobody asks for it
+
+
+def test_large_scores_and_small_ones(K):
+    for spread, scale in ((100.0, 1.0), (1e-3, 1.0), (1e4, 1e-9), (1.0, 0.0)):
+        c = Case(K, [(1, 300), (3, 64)], 8, 2, 128, F32, spread=spread)
+        for dt in (F32, BF):
+            c.dt, c.q = dt, c.q.to(dt)
+            out = c.run(K, scale=scale or 1e-30)
+            plain = c.run(K, scale=scale or 1e-30, backend="plain")
+            want, mag, smag = c.want(scale=scale or 1e-30)
+            n = 4
+            smag = smag[0]
+            rows = (smag[:n] < 2.0 ** 10)[..., None]          # rows whose scores are not all rounding
+            for o in (out, plain):
+                off = (o.double().view(want.shape) - want).abs()[:n]
+                most = mag[:n] * (32 * U * smag[:n][..., None] + 2.0 ** -18 + (2.0 ** -8 if dt == BF else 0)) + (2.0 ** -8 if dt == BF else 4 * U) * want[:n].abs()
+                assert o[:n].isfinite().all() and (off <= most)[rows.expand_as(off)].all()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 9000), (1, 10), (1, 4000)], [(4, 5000)], [(33, 3000)]])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+def test_long_contexts_slices_and_repeats(K, seqs, dt):
+    c = Case(K, seqs, 8, 2, 64, dt)
+    out = c.check(K)
+    assert torch.equal(c.run(K), out)
+    # bounds above the true lengths only change the slices
+    wide = c.run(K, max_kv=20000)
+    assert (wide.double() - out.double()).abs().max() <= 2.0 ** -6 * out[:-2].double().abs().max()
+
+
+def test_run_of_all_of_them(K):
+    """A batch as it is served: tables, write and attention step by step, prompts first and then a token each, against one pass
+    over whole sequences."""
+    hd, nqh, nkh, num = 64, 8, 2, 40
+    g = gen(8)
+    lens = [70, 1, 129]
+    cache = torch.zeros(num, nkh, K.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+    free = torch.randperm(num, generator=g).tolist()
+    held = [[], [], []]
+    before = [0, 0, 0]
+    mirror = torch.zeros(num, nkh, K.kv4_page_bytes(hd), dtype=torch.uint8)
+    for step in range(4):
+        new = lens if step == 0 else [1, 1, 1] if step < 3 else [2, 65, 1]
+        rows, pad = sum(new), 5
+        for h, n, b in zip(held, new, before):
+            while len(h) * 64 < n + b:
+                h.append(free.pop())
+        qkv = torch.randn(rows + pad, (nqh + 2 * nkh) * hd, generator=g).to(BF).to(DEV)
+        table, place = torch.empty(3, 8, dtype=torch.int32, device=DEV), torch.empty(rows + pad, dtype=torch.int32, device=DEV)
+        pos, seq, start = torch.empty_like(place), torch.empty_like(place), torch.empty(3, dtype=torch.int32, device=DEV)
+        q_len, kvb = dev(new), dev(before)
+        K.step_tables(q_len, kvb, dev(sum(held, [])), table, place, num_pages=num, positions=pos, token_seq=seq, q_start=start)
+        k, v = qkv[:, nqh * hd:(nqh + nkh) * hd], qkv[:, (nqh + nkh) * hd:]
+        K.kv4_store(k, v, place, cache, hd)
+        out = torch.zeros(rows + pad, nqh * hd, dtype=BF, device=DEV)
+        longest = max(n + b for n, b in zip(new, before))
+        K.attn_kv4(qkv, out, cache, table, start, q_len, kvb, seq, 3, max(new), longest, nqh, nkh, hd, None, hd ** -0.5)
+        K.check_device_errors()
+        for plane, x in ((0, k), (1, v)):
+            P.write(mirror, place.cpu(), plane, x.cpu().double().view(-1, nkh, hd))
+        want, mag, smag = P.attend(qkv[:, :nqh * hd].double().view(-1, nqh, hd).cpu(), mirror, table.cpu(), new, before, hd ** -0.5)
+        off = (out.cpu().double().view(want.shape) - want).abs()
+        assert (off <= mag * (2.0 ** -7 + 2 * (2.0 ** -8 * smag[1] + 16 * U * smag[0])[..., None]) + 2.0 ** -8 * want.abs()).all()
+        before = [n + b for n, b in zip(new, before)]
