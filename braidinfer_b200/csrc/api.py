@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_int, c_longlong, c_float, c_void_p, c_char_p
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
@@ -137,6 +138,8 @@ class RowScale:
         """The scales themselves (for tests and for parts written in torch)."""
         return torch.rsqrt(self.shares.sum(0) / self.width + self.eps)
 
+
+_KV4_ARGS = struct.Struct("<15Q3q12i4f2i")      # Kv4Args of attn_kv4.cu
 
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # torch's own quick way to the stream handle
@@ -822,10 +825,12 @@ class Kernels:
                  nqh: int, nkh: int, hd: int, window: Optional[int], scale: float, sink: Optional[float] = None, out_scale: float = 1.0,
                  head_sinks: Optional[torch.Tensor] = None, head_gate: Optional[torch.Tensor] = None, keep_first: int = 0,
                  head_scale: Optional[torch.Tensor] = None, distance_bias: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
-                 softcap: Optional[float] = None, backend: str = "auto") -> None:
+                 softcap: Optional[float] = None, settled: bool = False, backend: str = "auto") -> None:
         """Attention over a 4-bit cache, of single tokens and of prompts, float32 or bfloat16 (q [rows, >= nqh * hd], a view of
         wider rows is fine; out [rows, nqh * hd]).  Options as in `attn_simple`.  `max_q_len` and `max_kv_len` bound what a sequence
-        brings and what it holds after the step.  Rows of padding (token_seq -1) are left as they were."""
+        brings and what it holds after the step.  Rows of padding (token_seq -1) are left as they were.  `settled`: the tables, and all
+        that earlier steps cached, are in memory before the kernels right ahead in the stream have ended (StepContext.settled).
+        `backend` "plain": the plain kernel, for comparisons."""
         what = "attn_kv4"
         if backend not in ("auto", "plain"):
             raise KernelError(f"attn_kv4: unknown backend {backend!r} (auto, plain)")
@@ -853,6 +858,11 @@ class Kernels:
                         *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
+        if backend == "auto":
+            self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
+                               int(window or 0), scale, sink, out_scale, head_sinks, head_gate, int(keep_first or 0), head_scale, distance_bias,
+                               softcap, settled)
+            return
         lib = self.part_library("kv4")
         self.launches += 1
         self._check_lib(lib, lib.braid_attn_kv4_simple(
@@ -861,6 +871,53 @@ class Kernels:
             int(window or 0), int(keep_first or 0), float(scale), int(sink is not None), float(sink or 0.0), float(out_scale),
             _ptr(head_sinks), _ptr(head_gate), head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale),
             *self._bias_args(distance_bias), float(softcap or 0.0), self._error_flag.data_ptr() + 16, self._stream()), what)
+
+    def kv4_attention_library(self, head_dim: int):
+        """The attention over a 4-bit cache for one head size, compiled at first use."""
+        lib = self._attn_libs.get(("kv4", head_dim))
+        if lib is None:
+            self.kv4_page_bytes(head_dim)                     # (refuses other sizes)
+            lib = ctypes.CDLL(str(build.kv4_attention_library(head_dim, verbose=self._verbose)))
+            lib.braid_last_error.restype = c_char_p
+            lib.braid_attn_kv4.argtypes = [c_char_p, c_void_p]
+            lib.braid_attn_kv4.restype = c_int
+            if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
+                raise KernelError("the attention library over a 4-bit cache is another than was asked for")
+            lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once)
+            self._attn_libs[("kv4", head_dim)] = lib
+        return lib
+
+    def _attn_kv4_mma(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
+                      scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled) -> None:
+        lib = self.kv4_attention_library(hd)
+        f32, g, rows = int(out.dtype == torch.float32), nqh // nkh, out.shape[0]
+        key = (min(g * max_q_len, 9), f32)
+        plan = lib.plans.get(key)
+        if plan is None:
+            columns = lib.braid_attn_kv4_columns(key[0], f32)
+            plan = lib.plans[key] = (columns, lib.braid_attn_kv4_slots(f32, columns))
+        columns, slots = plan
+        hpc = min(g, columns)
+        ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (columns // hpc))
+        span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
+        # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
+        n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
+        partial = None
+        if n_splits > 1:
+            need = rows * nqh * n_splits * (hd + 2)
+            if self._attn_partial is None or self._attn_partial.numel() < need:
+                self._attn_partial = torch.empty(max(need, 1 << 22), dtype=torch.float32, device="cuda")
+                self.workspace_generation += 1
+            partial = self._attn_partial
+        bias = distance_bias or (None, None)
+        args = _KV4_ARGS.pack(
+            q.data_ptr(), out.data_ptr(), _ptr(partial) or 0, cache.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
+            kv_before.data_ptr(), token_seq.data_ptr(), _ptr(head_sinks) or 0, _ptr(head_gate) or 0, _ptr(head_scale) or 0, _ptr(bias[0]) or 0,
+            _ptr(bias[1]) or 0, self._error_flag.data_ptr() + 16, q.stride(0), out.stride(0), head_gate.stride(0) if head_gate is not None else 0,
+            rows, n_seqs, max_q_len, nqh, nkh, page_table.shape[1], cache.shape[0], window, keep_first, n_splits, int(sink is not None),
+            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns)
+        self.launches += 1 + (n_splits > 1)
+        self._check_lib(lib, lib.braid_attn_kv4(args, self._stream()), "attn_kv4")
 
     # ------------------------------------------------------------------ element-wise kernels of other models
     def dyt(self, x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, alpha: torch.Tensor, out: torch.Tensor,

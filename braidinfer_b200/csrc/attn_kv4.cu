@@ -1,0 +1,636 @@
+// Attention over a cache held in 4 bits (kv4.cuh), compiled for one head size: -DBRAID_HD=<32, 64, ... 256>.
+//
+// softmax over the visible keys of scale * q . k_j, with k_j = lowest + step * code a group of 32 numbers, so that
+//   q . k_j = sum over groups g of  step_jg (q_g . code_jg) + lowest_jg sum(q_g)
+//   out     = sum over keys of  (p_j step_jg) code_jg + sum over keys of p_j lowest_jg        (for the numbers of group g)
+// The codes themselves are the tensor cores' operand (mma.sync m16n8k16, bfloat16, float32 sums): a mask and an "or" turn
+// two of them into the bfloat16 pair 128 + code, exact, straight from the bytes as they are stored; the 128 comes off through
+// sum(q_g) for the keys and by a subtraction for the values.  So neither keys nor values are ever rounded, and what scales them is applied
+// to a group's sums (keys) or to the probabilities (values).  Keys and value columns are the 16 rows of a product and the
+// queries its 8 columns (query heads of one kv head, of up to 8 tokens), so that few queries waste little.
+//
+// What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
+// shifts are half.  Every warp walks units of 32 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
+// (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
+// and results; a context longer than that is sliced over CTAs, whose results a second kernel merges.
+// The running maximum of a column is raised only when a unit's scores exceed it by more than 8 (in powers of two): a vote instead
+// of a reduction over the warp; sums are taken against the same maximum, so nothing is lost.
+//
+// float32 runs (PARTS 3): queries and scaled probabilities are three bfloat16 numbers each, whose products with the codes are exact, so
+// that the result has float32's precision.
+#include "kv4.cuh"
+#include "tcgen05.cuh"
+#include "softcap.cuh"
+#include <type_traits>
+
+#ifndef BRAID_HD
+#error "compile with -DBRAID_HD=<head_dim>"
+#endif
+static_assert(BRAID_HD % 32 == 0 && BRAID_HD >= 32 && BRAID_HD <= 256, "head_dim must be a multiple of 32 in [32, 256]");
+
+struct Kv4Args {
+    const void* q;
+    void* out;
+    float* partial;              // n_splits > 1: [rows * nqh][n_splits][HD] results, then [rows * nqh][n_splits][2] maxima and sums
+    const uint8_t* cache;
+    const int* page_table;
+    const int* q_start;
+    const int* q_len;
+    const int* kv_before;
+    const int* token_seq;
+    const float* head_sinks;
+    const void* head_gate;
+    const float* head_scale;
+    const float* bias_slope;
+    const float* bias_rate;
+    int* error_flag;
+    long long q_stride, out_stride, gate_stride;
+    int rows, n_seqs, max_q_len, nqh, nkh, cols, num_pages, window, keep_first, n_splits, has_sink, settled;
+    float scale, sink, out_scale, softcap;
+    int f32, columns;            // float32 rows; columns a CTA
+};
+
+#define LOG2E 1.4426950408889634f
+#define KV4_RAISE 8.f
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// codes n and 4 + n of a word as the bfloat16 pair 128 + code, and as the codes themselves
+template <int N> __device__ __forceinline__ uint32_t codes128(uint32_t x) { return ((x >> (4 * N)) & 0x000f000fu) | 0x43004300u; }
+template <int N> __device__ __forceinline__ uint32_t codes0(uint32_t x) {
+    const uint32_t y = codes128<N>(x);
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(128.f), __float2bfloat16(128.f)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// N neighbouring 32-bit words of shared memory, in the widest loads that their count allows
+template <int N>
+__device__ __forceinline__ void lds_words(const void* p, uint32_t* x) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(x + i) = reinterpret_cast<const uint4*>(p)[i / 4];
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint2*>(x + i) = reinterpret_cast<const uint2*>(p)[i / 2];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+// a bfloat16 pair from two float32 numbers, and what the rounding leaves
+__device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
+    const uint32_t w = pack2(a, b);
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+
+template <int PARTS, int NT, int NW, int SR, int ST>
+struct Kv4Cfg {
+    static constexpr int HD = BRAID_HD, W = HD / 32;
+    static constexpr int US = 16 * SR;                       // tokens a unit
+    static constexpr int SB = SR * kv4_record_bytes(HD);     // bytes a unit
+    static constexpr int BM = 8 * NT;                        // columns a CTA
+    static constexpr int RING = NW * ST * SB;
+    static constexpr int MERGE = NW * BM * (HD + 4) * 4;
+    static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+    static_assert(BRAID_PAGE_SIZE % US == 0, "a unit must not straddle a page");
+};
+
+template <int PARTS, int NT, int NW, int SR, int ST>
+__global__ void __launch_bounds__(NW * 32)
+attn_kv4_kernel(const Kv4Args a) {
+    using C = Kv4Cfg<PARTS, NT, NW, SR, ST>;
+    using T = typename std::conditional<PARTS == 3, float, __nv_bfloat16>::type;
+    constexpr int HD = C::HD, W = C::W;
+    pdl_trigger();
+    // a caller that has made the tables, or this step's older keys, with kernels of this library right before does not say `settled`
+    if (!a.settled) pdl_wait();
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint64_t full[NW][ST];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int r = lane >> 2, j = lane & 3;
+    const int g = a.nqh / a.nkh;
+    const int hpc = min(g, C::BM), tpc = C::BM / hpc, hchunks = (g + hpc - 1) / hpc;
+    const int seq = blockIdx.y;
+    const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
+    const int unit = gridDim.z - 1 - blockIdx.z;              // late tokens, which see the most, first
+    const int tile = unit / a.n_splits, split = unit - tile * a.n_splits;
+    const int q_len = a.q_len[seq], tok0 = tile * tpc;
+    if (tok0 >= q_len) return;
+    const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
+    const int n_tok = min(tpc, q_len - tok0);
+    const int head0 = kvh * g + hchunk * hpc, n_heads = min(hpc, g - hchunk * hpc);
+    const int pos_min = kv_before + tok0, pos_max = pos_min + n_tok - 1;
+    const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
+    const int t_win = k_lo / C::US;                            // the units walked: kept first ones that the window has left, then the window's
+    const int n_first = min((a.keep_first + C::US - 1) / C::US, t_win);
+    int i_lo = 0, i_hi = n_first + pos_max / C::US + 1 - t_win;
+    if (a.n_splits > 1) {
+        const int per = (i_hi + a.n_splits - 1) / a.n_splits;
+        i_lo = min(i_hi, split * per);
+        i_hi = min(i_hi, i_lo + per);
+    }
+    const int n_mine = max(0, (i_hi - i_lo - warp + NW - 1) / NW);
+    auto tile_of = [&](int k) { const int i = i_lo + warp + k * NW; return i < n_first ? i : t_win + (i - n_first); };
+
+    uint8_t* ring = smem + warp * (ST * C::SB);
+    if (tid == 0) abort_flag = 0;
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) mbar_init(&full[warp][s], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    const int* table = a.page_table + (size_t)seq * a.cols;
+    int issued = 0, pages = 0;                                 // a lane's page: of this warp's unit (issued & ~31) + lane
+    auto issue = [&]() {
+        if ((issued & 31) == 0) {
+            pages = 0;
+            if (issued + lane < n_mine) {
+                const int block = tile_of(issued + lane) / (BRAID_PAGE_SIZE / C::US);
+                const int p = block < a.cols ? table[block] : -1;
+                if (p < 0 || p >= a.num_pages) atomicExch(a.error_flag, 1);      // never followed: page 0 is read instead
+                else pages = p;
+            }
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, issued & 31);
+        if (lane == 0) {
+            const int t = tile_of(issued), s = issued % ST;
+            mbar_expect_tx(&full[warp][s], C::SB);
+            bulk_load(ring + s * C::SB, a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t % (BRAID_PAGE_SIZE / C::US)) * C::SB,
+                      C::SB, &full[warp][s]);
+        }
+        ++issued;
+    };
+    // units that hold only tokens cached before this step may be asked for at once
+    if (a.settled) {
+        while (issued < min(ST, n_mine) && (tile_of(issued) + 1) * C::US <= kv_before) issue();
+        pdl_wait();
+    }
+    while (issued < min(ST, n_mine)) issue();
+
+    // ---- queries: column nt * 8 + r, numbers 32 w + 8 j .. + 7 of the head
+    uint32_t q[NT][W][PARTS][4];
+    float qs[NT][2][W];                                        // the sum of a group's numbers, columns nt * 8 + 2 j, + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + r, tl = col / hpc, hl = col - tl * hpc;
+        const bool in = tl < n_tok && hl < n_heads;
+        const T* src = (const T*)a.q + (size_t)(q_start + (in ? tok0 + tl : 0)) * a.q_stride + (size_t)(head0 + (in ? hl : 0)) * HD + 8 * j;
+        const bool wide = !(((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) & 15);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            float x[8];
+            if (wide) {
+                constexpr int VW = 16 / sizeof(T);
+#pragma unroll
+                for (int i = 0; i < 8; i += VW) load_run<T, VW>(src + 32 * w + i, x + i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = to_f32(src[32 * w + i]);
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!in) x[i] = 0.f;
+                sum += x[i];
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            qs[nt][0][w] = __shfl_sync(0xffffffffu, sum, 8 * j);
+            qs[nt][1][w] = __shfl_sync(0xffffffffu, sum, 8 * j + 4);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) q[nt][w][p][n] = split_pair(x[2 * n], x[2 * n + 1]);
+        }
+    }
+    // ---- this lane's columns of scores: nt * 8 + 2 j + c
+    int pos[NT][2], lo[NT][2];
+    float sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int col = nt * 8 + 2 * j + c, tl = col / hpc, hl = col - tl * hpc;
+            const bool in = tl < n_tok && hl < n_heads;
+            pos[nt][c] = in ? pos_min + tl : -1;               // -1: the column sees nothing
+            lo[nt][c] = a.window > 0 ? pos[nt][c] - a.window + 1 : 0;
+            sc[nt][c] = (in && a.head_scale ? a.scale * a.head_scale[head0 + hl] : a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E);
+        }
+
+    float o[NT][2 * W][4], zs[NT][2][W], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            m[nt][c] = -INFINITY;
+            l[nt][c] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) zs[nt][c][w] = 0.f;
+        }
+    }
+
+    bool ok = true;
+    for (int k = 0; k < n_mine && ok; ++k) {
+        const int st = k % ST;
+        ok = mbar_wait(&full[warp][st], (uint32_t)((k / ST) & 1), &abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* base = ring + st * C::SB;
+        const int key0 = tile_of(k) * C::US;
+
+        // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
+        float s[SR][NT][4];
+#pragma unroll
+        for (int rec = 0; rec < SR; ++rec) {
+            const uint8_t* rb = base + rec * kv4_record_bytes(HD);
+            uint32_t ka[W], kb[W], ga[W], gb[W];
+            lds_words<W>(rb + r * (HD / 2) + j * (4 * W), ka);
+            lds_words<W>(rb + (r + 8) * (HD / 2) + j * (4 * W), kb);
+            lds_words<W>(rb + kv4_key_groups(HD) + r * (4 * W), ga);
+            lds_words<W>(rb + kv4_key_groups(HD) + (r + 8) * (4 * W), gb);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[rec][nt][0] = s[rec][nt][1] = s[rec][nt][2] = s[rec][nt][3] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const uint32_t a0 = codes128<0>(ka[w]), a1 = codes128<0>(kb[w]), a2 = codes128<1>(ka[w]), a3 = codes128<1>(kb[w]);
+                const uint32_t b0 = codes128<2>(ka[w]), b1 = codes128<2>(kb[w]), b2 = codes128<3>(ka[w]), b3 = codes128<3>(kb[w]);
+                const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]);
+                const float za = fmaf(-128.f, sa, kv4_lowest(ga[w])), zb = fmaf(-128.f, sb, kv4_lowest(gb[w]));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float raw[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        mma16816(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
+                        mma16816(raw, b0, b1, b2, b3, q[nt][w][p][2], q[nt][w][p][3]);
+                    }
+                    s[rec][nt][0] = fmaf(sa, raw[0], fmaf(za, qs[nt][0][w], s[rec][nt][0]));
+                    s[rec][nt][1] = fmaf(sa, raw[1], fmaf(za, qs[nt][1][w], s[rec][nt][1]));
+                    s[rec][nt][2] = fmaf(sb, raw[2], fmaf(zb, qs[nt][0][w], s[rec][nt][2]));
+                    s[rec][nt][3] = fmaf(sb, raw[3], fmaf(zb, qs[nt][1][w], s[rec][nt][3]));
+                }
+            }
+        }
+        // ---- factors, cap, bias; mask
+#pragma unroll
+        for (int rec = 0; rec < SR; ++rec)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[rec][nt][e] *= sc[nt][e & 1];
+        if (a.softcap > 0.f) softcap_scores<SR * NT * 4>(&s[0][0][0], 1.f, a.softcap * LOG2E);
+        if (a.bias_slope) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = nt * 8 + 2 * j + c, hl = col % hpc;
+                    const float r1 = hl < n_heads ? a.bias_slope[head0 + hl] : 0.f, r2 = hl < n_heads ? a.bias_rate[head0 + hl] : 0.f;
+#pragma unroll
+                    for (int rec = 0; rec < SR; ++rec)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {          // (keys after the query are masked below)
+                            const float d = (float)(pos[nt][c] - (key0 + 16 * rec + 8 * h + r));
+                            s[rec][nt][2 * h + c] -= r1 * LOG2E * log1pf(r2 * fmaxf(d, 0.f));
+                        }
+                }
+        }
+        const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1)) || n_tok < tpc || n_heads < hpc || hpc * tpc < C::BM;
+        if (edge) {
+#pragma unroll
+            for (int rec = 0; rec < SR; ++rec)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + 16 * rec + 8 * (e >> 1) + r, c = e & 1;
+                        if (!(key <= pos[nt][c] && (key >= lo[nt][c] || key < a.keep_first))) s[rec][nt][e] = -INFINITY;
+                    }
+        }
+        // ---- running maximum
+        float top[NT][2];
+        bool raise = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+#pragma unroll
+                for (int rec = 1; rec < SR; ++rec) x = fmaxf(x, fmaxf(s[rec][nt][c], s[rec][nt][2 + c]));
+                top[nt][c] = x;
+                raise |= x > m[nt][c] + KV4_RAISE;
+            }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = top[nt][c];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(x, m[nt][c]);
+                    const float f = x == -INFINITY ? 1.f : exp2f(m[nt][c] - x);      // exp2(-inf) = 0
+                    m[nt][c] = x;
+                    l[nt][c] *= f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) zs[nt][c][w] *= f;
+#pragma unroll
+                    for (int i = 0; i < 2 * W; ++i) { o[nt][i][c] *= f; o[nt][i][2 + c] *= f; }
+                }
+        }
+        // ---- probabilities and values
+#pragma unroll
+        for (int rec = 0; rec < SR; ++rec) {
+            const uint8_t* rb = base + rec * kv4_record_bytes(HD);
+            uint32_t ga[W], gb[W];
+            lds_words<W>(rb + kv4_value_groups(HD) + r * (4 * W), ga);
+            lds_words<W>(rb + kv4_value_groups(HD) + (r + 8) * (4 * W), gb);
+            // value codes of tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9, numbers 32 w + 4 r .. + 3: 16 bits a group
+            const uint8_t* vc = rb + kv4_value_codes(HD) + 2 * j * (HD / 2) + r * (2 * W);
+            uint32_t v01[W], v89[W];
+            if constexpr (W % 2 == 0) {
+                uint32_t x0[W / 2], x1[W / 2], x8[W / 2], x9[W / 2];
+                lds_words<W / 2>(vc, x0);
+                lds_words<W / 2>(vc + HD / 2, x1);
+                lds_words<W / 2>(vc + 8 * (HD / 2), x8);
+                lds_words<W / 2>(vc + 9 * (HD / 2), x9);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    v01[w] = __byte_perm(x0[w / 2], x1[w / 2], w & 1 ? 0x7632 : 0x5410);
+                    v89[w] = __byte_perm(x8[w / 2], x9[w / 2], w & 1 ? 0x7632 : 0x5410);
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint16_t* u = reinterpret_cast<const uint16_t*>(vc) + w;
+                    v01[w] = u[0] | ((uint32_t)u[HD / 4] << 16);
+                    v89[w] = u[8 * (HD / 4)] | ((uint32_t)u[9 * (HD / 4)] << 16);
+                }
+            }
+            float p[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = e & 1;
+                    p[nt][e] = exp2f(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
+                    l[nt][c] += p[nt][e];
+                }
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]), za = kv4_lowest(ga[w]), zb = kv4_lowest(gb[w]);
+                const uint32_t a0 = codes0<0>(v01[w]), a1 = codes0<1>(v01[w]), a2 = codes0<0>(v89[w]), a3 = codes0<1>(v89[w]);
+                const uint32_t b0 = codes0<2>(v01[w]), b1 = codes0<3>(v01[w]), b2 = codes0<2>(v89[w]), b3 = codes0<3>(v89[w]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4] = {p[nt][0] * sa, p[nt][1] * sa, p[nt][2] * sb, p[nt][3] * sb};
+                    float z[4] = {p[nt][0] * za, p[nt][1] * za, p[nt][2] * zb, p[nt][3] * zb};
+                    if (edge) {                                // what a column does not see does not count, whatever it holds
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (s[rec][nt][e] == -INFINITY) x[e] = z[e] = 0.f;
+                    }
+                    zs[nt][0][w] += z[0] + z[2];
+                    zs[nt][1][w] += z[1] + z[3];
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
+                        mma16816(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
+                        mma16816(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
+                    }
+                }
+            }
+        }
+        __syncwarp();                                          // every lane has read the unit
+        if (issued < n_mine) issue();
+    }
+    if (!ok) {
+        // a copy did not arrive in time: wait for the others (bounded too), so that none lands after the CTA has ended
+        if (lane == 0) atomicExch(a.error_flag, 1);
+        for (int s = 0; s < ST; ++s) {
+            const int last = (issued - 1 - s) / ST;            // the last use of stage s
+            if (issued > s) for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&full[warp][s], (uint32_t)(last & 1)); ++i) {}
+        }
+    }
+
+    // ---- the CTA's warps merge
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+#pragma unroll
+                for (int w = 0; w < W; ++w) zs[nt][c][w] += __shfl_xor_sync(0xffffffffu, zs[nt][c][w], x);
+            }
+    __syncthreads();                                           // every warp is done with its ring
+    float* mo = reinterpret_cast<float*>(smem);                // [warp][column][HD]
+    float* ml = mo + NW * C::BM * HD;                          // [warp][column][2]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int col = nt * 8 + 2 * j + c;
+            float* dst = mo + (warp * C::BM + col) * HD + 4 * r;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(o[nt][2 * w][c] + zs[nt][c][w], o[nt][2 * w][2 + c] + zs[nt][c][w],
+                                                                       o[nt][2 * w + 1][c] + zs[nt][c][w], o[nt][2 * w + 1][2 + c] + zs[nt][c][w]);
+            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c]; }
+        }
+    __syncthreads();
+    const bool out_wide = !(((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) & (4 * sizeof(T) - 1));
+    for (int i = tid; i < C::BM * (HD / 4); i += NW * 32) {
+        const int col = i / (HD / 4), d = (i - col * (HD / 4)) * 4;
+        const int tl = col / hpc, hl = col - tl * hpc;
+        if (!(tl < n_tok && hl < n_heads)) continue;
+        const int head = head0 + hl;
+        const size_t row = (size_t)(q_start + tok0 + tl);
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * C::BM + col) * 2]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = M == -INFINITY ? 1.f : exp2f(ml[(w * C::BM + col) * 2] - M);     // nothing finite: zeros, or a NaN that stays
+            const float4 y = *reinterpret_cast<const float4*>(mo + (w * C::BM + col) * HD + d);
+            L = fmaf(ml[(w * C::BM + col) * 2 + 1], f, L);
+            x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+        }
+        if (a.n_splits > 1) {
+            const size_t at = (row * a.nqh + head) * a.n_splits + split;
+            *reinterpret_cast<float4*>(a.partial + at * HD + d) = x;
+            if (d == 0) *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(M, L);
+            continue;
+        }
+        float f = 1.f;
+        if (a.has_sink) {                                      // one more score, with no value
+            const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
+            f = exp2f(M - mn);
+            L = L * f + exp2f(sk - mn);
+        }
+        float inv = f * a.out_scale / L;
+        if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[row * a.gate_stride + head])));
+        T* dst = (T*)a.out + row * a.out_stride + (size_t)head * HD + d;
+        __align__(16) T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
+        if (!out_wide) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = y[e];
+        } else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+    }
+}
+
+// The slices of a (row, head) made one: sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), four numbers a thread.
+template <typename T>
+__global__ void __launch_bounds__(128)
+attn_kv4_merge_kernel(const Kv4Args a) {
+    constexpr int HD = BRAID_HD;
+    pdl_trigger();
+    pdl_wait();
+    const long long it = (long long)blockIdx.x * 128 + threadIdx.x;
+    const long long rh = it / (HD / 4);
+    const int d = (int)(it - rh * (HD / 4)) * 4;
+    if (rh >= (long long)a.rows * a.nqh) return;
+    const long long row = rh / a.nqh;
+    const int head = (int)(rh - row * a.nqh);
+    if (a.token_seq[row] < 0) return;
+    const float* po = a.partial + (size_t)rh * a.n_splits * HD + d;
+    const float2* pm = reinterpret_cast<const float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD) + (size_t)rh * a.n_splits;
+    float M = -INFINITY, L = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int B = 8;                                       // slices in flight
+    for (int s0 = 0; s0 < a.n_splits; s0 += B) {
+        float2 ml[B];
+        float4 y[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const bool in = s0 + i < a.n_splits;
+            ml[i] = in ? pm[s0 + i] : make_float2(-INFINITY, 0.f);
+            y[i] = in ? *reinterpret_cast<const float4*>(po + (size_t)(s0 + i) * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float Mn = M;
+#pragma unroll
+        for (int i = 0; i < B; ++i) Mn = fmaxf(Mn, ml[i].x);
+        const float ref = Mn == -INFINITY ? 0.f : Mn, c = M == -INFINITY && Mn == -INFINITY ? 1.f : exp2f(M - ref);
+        L *= c; x.x *= c; x.y *= c; x.z *= c; x.w *= c;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            // a slice without a finite score has weight 0, which leaves nothing of its zeros and all of a NaN
+            const float f = exp2f(ml[i].x - ref);
+            L = fmaf(ml[i].y, f, L);
+            x.x = fmaf(y[i].x, f, x.x); x.y = fmaf(y[i].y, f, x.y); x.z = fmaf(y[i].z, f, x.z); x.w = fmaf(y[i].w, f, x.w);
+        }
+        M = Mn;
+    }
+    float f = 1.f;
+    if (a.has_sink) {
+        const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
+        f = exp2f(M - mn);
+        L = L * f + exp2f(sk - mn);
+    }
+    float inv = f * a.out_scale / L;
+    if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[row * a.gate_stride + head])));
+    T* dst = (T*)a.out + row * a.out_stride + (size_t)head * HD + d;
+    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(y[e]);
+}
+
+// ------------------------------------------------------------------ host side
+// Warps, records a unit and stages a ring: what fits 227 KB with several CTAs an SM.
+#define KV4_NW 4
+#define KV4_SR 2
+#define KV4_ST (BRAID_HD > 128 ? 2 : 3)
+// Columns a CTA: 8, or 16 where a step has that many and the registers hold their results.
+#define KV4_NT_MAX (BRAID_HD > 128 ? 1 : 2)
+
+template <int PARTS, int NT>
+static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>; }
+
+template <int PARTS, int NT>
+static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
+    using C = Kv4Cfg<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>;
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(kv4_kernel<PARTS, NT>(), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) { braid_set_error("attn_kv4: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e)); return (int)e; }
+        configured = true;
+    }
+    const int g = a.nqh / a.nkh, hpc = g < C::BM ? g : C::BM, tpc = C::BM / hpc, hchunks = (g + hpc - 1) / hpc;
+    const long long gz = (long long)((a.max_q_len + tpc - 1) / tpc) * a.n_splits;
+    if (gz > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
+        BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld tiles, %d heads, %d sequences)", gz, a.nkh * hchunks, a.n_seqs);
+    if (gz == 0) return BRAID_OK;
+    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
+    BRAID_LAUNCH_CHECK();
+}
+
+extern "C" int braid_attn_kv4_head_dim(void) { return BRAID_HD; }
+extern "C" int braid_attn_kv4_args_bytes(void) { return (int)sizeof(Kv4Args); }
+extern "C" int braid_attn_kv4_columns(int wanted, int f32) { return wanted <= 8 || KV4_NT_MAX == 1 || (f32 && BRAID_HD > 64) ? 8 : 16; }
+
+// CTAs that the device holds at once.
+extern "C" int braid_attn_kv4_slots(int f32, int columns) {
+    int dev = 0, sms = 0, per_sm = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int smem = Kv4Cfg<1, 1, KV4_NW, KV4_SR, KV4_ST>::SMEM, smem2 = Kv4Cfg<1, KV4_NT_MAX, KV4_NW, KV4_SR, KV4_ST>::SMEM;
+    const void* f = columns <= 8 ? (f32 ? kv4_kernel<3, 1>() : kv4_kernel<1, 1>()) : (f32 ? kv4_kernel<3, KV4_NT_MAX>() : kv4_kernel<1, KV4_NT_MAX>());
+    const int bytes = columns <= 8 ? smem : smem2;
+    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, f, KV4_NW * 32, bytes);
+    if (e != cudaSuccess || per_sm <= 0 || sms <= 0) return 148 * 2;
+    return per_sm * sms;
+}
+
+// `args`: a Kv4Args, filled in by the caller (csrc/api.py has its layout).
+extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
+    Kv4Args a = *args;
+    if (a.rows <= 0 || a.n_seqs <= 0) return BRAID_OK;
+    if (a.head_sinks) a.has_sink = 1;
+    if (a.window <= 0) a.window = a.keep_first = 0;
+    if (!a.error_flag) BRAID_REFUSE("attn_kv4: error_flag is required");
+    if (a.num_pages <= 0 || a.cols <= 0) BRAID_REFUSE("attn_kv4: the cache has no pages (pages=%d, table columns=%d)", a.num_pages, a.cols);
+    if (a.nqh <= 0 || a.nkh <= 0 || a.nqh % a.nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", a.nqh, a.nkh);
+    if ((uintptr_t)a.cache & 15) BRAID_REFUSE("attn_kv4: the cache must start on 16 bytes");
+    if (a.keep_first < 0 || a.max_q_len < 0) BRAID_REFUSE("attn_kv4: keep_first=%d, max_q_len=%d must not be negative", a.keep_first, a.max_q_len);
+    if (!a.bias_slope != !a.bias_rate) BRAID_REFUSE("attn_kv4: a distance bias has a slope and a rate a head");
+    if (a.softcap > 0.f && a.bias_slope) BRAID_REFUSE("attn_kv4: a cap on the scores and a distance bias are not combined");
+    if (a.n_splits < 1) a.n_splits = 1;
+    if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: n_splits > 1 needs the partial buffer");
+    cudaStream_t s = (cudaStream_t)stream;
+    int rc;
+    if (a.columns <= 8) rc = a.f32 ? launch_kv4<3, 1>(a, s) : launch_kv4<1, 1>(a, s);
+    else rc = a.f32 ? launch_kv4<3, KV4_NT_MAX>(a, s) : launch_kv4<1, KV4_NT_MAX>(a, s);
+    if (rc || a.n_splits == 1) return rc;
+    const long long ctas = ((long long)a.rows * a.nqh * (BRAID_HD / 4) + 127) / 128;
+    if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
+    if (a.f32) braid_launch(attn_kv4_merge_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, s, a);
+    else braid_launch(attn_kv4_merge_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, s, a);
+    BRAID_LAUNCH_CHECK();
+}

@@ -183,6 +183,11 @@ def latent_attention_library(rank: int, rot: int, verbose: bool = True) -> Path:
                          defines=[f"-DBRAID_LAT_RANK={rank}", f"-DBRAID_LAT_ROT={rot}"], verbose=verbose)
 
 
+def kv4_attention_library(head_dim: int, verbose: bool = True) -> Path:
+    """The tensor-core attention over a cache held in 4 bits, compiled for one head size."""
+    return build_library(f"braidinfer_attn_kv4_hd{head_dim}", ["errors.cu", "attn_kv4.cu"], defines=[f"-DBRAID_HD={head_dim}"], verbose=verbose)
+
+
 def attention_library(head_dim: int, verbose: bool = True, value_heads: int = 1) -> Path:
     """The tensor-core attention kernels compiled for one head size (what a model needs
     is compiled when the model is first built).  `value_heads` > 1: the mma.sync kernel alone, compiled so that a
