@@ -62,6 +62,11 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816_zero(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -71,12 +76,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-// codes n and 4 + n of a word as the bfloat16 pair 128 + code, and as the codes themselves
-template <int N> __device__ __forceinline__ uint32_t codes128(uint32_t x) { return ((x >> (4 * N)) & 0x000f000fu) | 0x43004300u; }
-template <int N> __device__ __forceinline__ uint32_t codes0(uint32_t x) {
-    const uint32_t y = codes128<N>(x);
+// codes n and 4 + n of a word as the bfloat16 pair 128 + code, and as the codes themselves.  `magic` is 0x43004300 in a register: mask
+// and "or" are then one instruction (with two constants they are two: the one pass over a code is what bounds the kernel)
+template <int N> __device__ __forceinline__ uint32_t codes128(uint32_t x, uint32_t magic) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(y) : "r"(x >> (4 * N)), "r"(magic));
+    return y;
+}
+template <int N> __device__ __forceinline__ uint32_t codes0(uint32_t x, uint32_t magic) {
+    const uint32_t y = codes128<N>(x, magic);
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(128.f), __float2bfloat16(128.f)));
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float exp2_ftz(float x) {        // to 2 units of the last place; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 // N neighbouring 32-bit words of shared memory, in the widest loads that their count allows
 template <int N>
@@ -160,7 +175,7 @@ attn_kv4_kernel(const Kv4Args a) {
     }
     __syncthreads();
     const int* table = a.page_table + (size_t)seq * a.cols;
-    int issued = 0, pages = 0;                                 // a lane's page: of this warp's unit (issued & ~31) + lane
+    int issued = 0, istage = 0, pages = 0;                     // a lane's page: of this warp's unit (issued & ~31) + lane
     auto issue = [&]() {
         if ((issued & 31) == 0) {
             pages = 0;
@@ -173,12 +188,13 @@ attn_kv4_kernel(const Kv4Args a) {
         }
         const int page = __shfl_sync(0xffffffffu, pages, issued & 31);
         if (lane == 0) {
-            const int t = tile_of(issued), s = issued % ST;
-            mbar_expect_tx(&full[warp][s], C::SB);
-            bulk_load(ring + s * C::SB, a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t % (BRAID_PAGE_SIZE / C::US)) * C::SB,
-                      C::SB, &full[warp][s]);
+            const int t = tile_of(issued);
+            mbar_expect_tx(&full[warp][istage], C::SB);
+            bulk_load(ring + istage * C::SB, a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t % (BRAID_PAGE_SIZE / C::US)) * C::SB,
+                      C::SB, &full[warp][istage]);
         }
         ++issued;
+        if (++istage == ST) istage = 0;
     };
     // units that hold only tokens cached before this step may be asked for at once
     if (a.settled) {
@@ -189,13 +205,17 @@ attn_kv4_kernel(const Kv4Args a) {
 
     // ---- queries: column nt * 8 + r, numbers 32 w + 8 j .. + 7 of the head
     uint32_t q[NT][W][PARTS][4];
-    float qs[NT][2][W];                                        // the sum of a group's numbers, columns nt * 8 + 2 j, + 1
+    constexpr int GH = W > 4 ? 2 : 1;
+    uint32_t qb[NT][3][GH];                                    // -128 and 1 times the sum of group j's (and 4 + j's) numbers, in three parts
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int col = nt * 8 + r, tl = col / hpc, hl = col - tl * hpc;
         const bool in = tl < n_tok && hl < n_heads;
         const T* src = (const T*)a.q + (size_t)(q_start + (in ? tok0 + tl : 0)) * a.q_stride + (size_t)(head0 + (in ? hl : 0)) * HD + 8 * j;
         const bool wide = !(((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) & 15);
+        float sums[GH];
+#pragma unroll
+        for (int h = 0; h < GH; ++h) sums[h] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             float x[8];
@@ -215,12 +235,17 @@ attn_kv4_kernel(const Kv4Args a) {
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            qs[nt][0][w] = __shfl_sync(0xffffffffu, sum, 8 * j);
-            qs[nt][1][w] = __shfl_sync(0xffffffffu, sum, 8 * j + 4);
+            if ((w & 3) == j) sums[w >> 2] = sum;
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
                 for (int n = 0; n < 4; ++n) q[nt][w][p][n] = split_pair(x[2 * n], x[2 * n + 1]);
+        }
+#pragma unroll
+        for (int h = 0; h < GH; ++h) {
+            float lo = sums[h], hi = -128.f * lo;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) qb[nt][p][h] = split_pair(hi, lo);
         }
     }
     // ---- this lane's columns of scores: nt * 8 + 2 j + c
@@ -251,13 +276,16 @@ attn_kv4_kernel(const Kv4Args a) {
         }
     }
 
+    uint32_t magic;
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
     bool ok = true;
-    for (int k = 0; k < n_mine && ok; ++k) {
-        const int st = k % ST;
-        ok = mbar_wait(&full[warp][st], (uint32_t)((k / ST) & 1), &abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+    int st = 0;
+    uint32_t phase = 0;
+    for (int k = 0; k < n_mine; ++k) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag));
         if (!ok) break;
         const uint8_t* base = ring + st * C::SB;
+        if (++st == ST) { st = 0; phase ^= 1u; }
         const int key0 = tile_of(k) * C::US;
 
         // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
@@ -268,28 +296,44 @@ attn_kv4_kernel(const Kv4Args a) {
             uint32_t ka[W], kb[W], ga[W], gb[W];
             lds_words<W>(rb + r * (HD / 2) + j * (4 * W), ka);
             lds_words<W>(rb + (r + 8) * (HD / 2) + j * (4 * W), kb);
-            lds_words<W>(rb + kv4_key_groups(HD) + r * (4 * W), ga);
-            lds_words<W>(rb + kv4_key_groups(HD) + (r + 8) * (4 * W), gb);
+            const uint8_t* groups = rb + kv4_key_groups(HD) + r * (4 * W);
+            lds_words<W>(groups, ga);
+            lds_words<W>(groups + 32 * W, gb);
+            // what the lowest values, and the 128 that the codes have too much, add to the scores: a product with the queries' sums,
+            // whose operand the groups' words are as they lie
+            uint32_t wa[2] = {0u, 0u}, wb[2] = {0u, 0u};
+            if (W >= 4 || j < W) {
+                wa[0] = reinterpret_cast<const uint32_t*>(groups)[j];
+                wb[0] = reinterpret_cast<const uint32_t*>(groups + 32 * W)[j];
+            }
+            if (W == 8 || 4 + j < W) {
+                wa[1] = reinterpret_cast<const uint32_t*>(groups)[4 + j];
+                wb[1] = reinterpret_cast<const uint32_t*>(groups + 32 * W)[4 + j];
+            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[rec][nt][0] = s[rec][nt][1] = s[rec][nt][2] = s[rec][nt][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) {
+                mma16816_zero(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][0][0], GH > 1 ? qb[nt][0][GH - 1] : 0u);
+#pragma unroll
+                for (int p = 1; p < 3; ++p) mma16816(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][p][0], GH > 1 ? qb[nt][p][GH - 1] : 0u);
+            }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const uint32_t a0 = codes128<0>(ka[w]), a1 = codes128<0>(kb[w]), a2 = codes128<1>(ka[w]), a3 = codes128<1>(kb[w]);
-                const uint32_t b0 = codes128<2>(ka[w]), b1 = codes128<2>(kb[w]), b2 = codes128<3>(ka[w]), b3 = codes128<3>(kb[w]);
+                const uint32_t a0 = codes128<0>(ka[w], magic), a1 = codes128<0>(kb[w], magic), a2 = codes128<1>(ka[w], magic), a3 = codes128<1>(kb[w], magic);
+                const uint32_t b0 = codes128<2>(ka[w], magic), b1 = codes128<2>(kb[w], magic), b2 = codes128<3>(ka[w], magic), b3 = codes128<3>(kb[w], magic);
                 const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]);
-                const float za = fmaf(-128.f, sa, kv4_lowest(ga[w])), zb = fmaf(-128.f, sb, kv4_lowest(gb[w]));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float raw[4] = {0.f, 0.f, 0.f, 0.f};
+                    float raw[4];
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
-                        mma16816(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
+                        if (p == 0) mma16816_zero(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
+                        else mma16816(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
                         mma16816(raw, b0, b1, b2, b3, q[nt][w][p][2], q[nt][w][p][3]);
                     }
-                    s[rec][nt][0] = fmaf(sa, raw[0], fmaf(za, qs[nt][0][w], s[rec][nt][0]));
-                    s[rec][nt][1] = fmaf(sa, raw[1], fmaf(za, qs[nt][1][w], s[rec][nt][1]));
-                    s[rec][nt][2] = fmaf(sb, raw[2], fmaf(zb, qs[nt][0][w], s[rec][nt][2]));
-                    s[rec][nt][3] = fmaf(sb, raw[3], fmaf(zb, qs[nt][1][w], s[rec][nt][3]));
+                    s[rec][nt][0] = fmaf(sa, raw[0], s[rec][nt][0]);
+                    s[rec][nt][1] = fmaf(sa, raw[1], s[rec][nt][1]);
+                    s[rec][nt][2] = fmaf(sb, raw[2], s[rec][nt][2]);
+                    s[rec][nt][3] = fmaf(sb, raw[3], s[rec][nt][3]);
                 }
             }
         }
@@ -317,7 +361,8 @@ attn_kv4_kernel(const Kv4Args a) {
                         }
                 }
         }
-        const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1)) || n_tok < tpc || n_heads < hpc || hpc * tpc < C::BM;
+        // (columns that are no query see as much as the others, and nobody reads them)
+        const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
         if (edge) {
 #pragma unroll
             for (int rec = 0; rec < SR; ++rec)
@@ -361,7 +406,9 @@ attn_kv4_kernel(const Kv4Args a) {
                     for (int i = 0; i < 2 * W; ++i) { o[nt][i][c] *= f; o[nt][i][2 + c] *= f; }
                 }
         }
-        // ---- probabilities and values
+        // ---- probabilities and values.  On an edge (EDGE) what a column does not see does not count, whatever it holds: a value's
+        // step or lowest number may be NaN
+        auto values = [&](auto EDGE) {
 #pragma unroll
         for (int rec = 0; rec < SR; ++rec) {
             const uint8_t* rb = base + rec * kv4_record_bytes(HD);
@@ -396,25 +443,28 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int c = e & 1;
-                    p[nt][e] = exp2f(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
+                    p[nt][e] = exp2_ftz(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
                     l[nt][c] += p[nt][e];
                 }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]), za = kv4_lowest(ga[w]), zb = kv4_lowest(gb[w]);
-                const uint32_t a0 = codes0<0>(v01[w]), a1 = codes0<1>(v01[w]), a2 = codes0<0>(v89[w]), a3 = codes0<1>(v89[w]);
-                const uint32_t b0 = codes0<2>(v01[w]), b1 = codes0<3>(v01[w]), b2 = codes0<2>(v89[w]), b3 = codes0<3>(v89[w]);
+                const uint32_t a0 = codes0<0>(v01[w], magic), a1 = codes0<1>(v01[w], magic), a2 = codes0<0>(v89[w], magic), a3 = codes0<1>(v89[w], magic);
+                const uint32_t b0 = codes0<2>(v01[w], magic), b1 = codes0<3>(v01[w], magic), b2 = codes0<2>(v89[w], magic), b3 = codes0<3>(v89[w], magic);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float x[4] = {p[nt][0] * sa, p[nt][1] * sa, p[nt][2] * sb, p[nt][3] * sb};
-                    float z[4] = {p[nt][0] * za, p[nt][1] * za, p[nt][2] * zb, p[nt][3] * zb};
-                    if (edge) {                                // what a column does not see does not count, whatever it holds
+                    if constexpr (EDGE.value) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (s[rec][nt][e] == -INFINITY) x[e] = z[e] = 0.f;
+                        for (int e = 0; e < 4; ++e) {
+                            const bool seen = s[rec][nt][e] != -INFINITY;
+                            if (!seen) x[e] = 0.f;
+                            if (seen) zs[nt][e & 1][w] = fmaf(p[nt][e], e < 2 ? za : zb, zs[nt][e & 1][w]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) zs[nt][e & 1][w] = fmaf(p[nt][e], e < 2 ? za : zb, zs[nt][e & 1][w]);
                     }
-                    zs[nt][0][w] += z[0] + z[2];
-                    zs[nt][1][w] += z[1] + z[3];
 #pragma unroll
                     for (int part = 0; part < PARTS; ++part) {
                         const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
@@ -424,6 +474,9 @@ attn_kv4_kernel(const Kv4Args a) {
                 }
             }
         }
+        };
+        if (edge) values(std::true_type{});
+        else values(std::false_type{});
         __syncwarp();                                          // every lane has read the unit
         if (issued < n_mine) issue();
     }
