@@ -76,18 +76,25 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-// codes n and 4 + n of a word as the bfloat16 pair 128 + code, and as the codes themselves.  `magic` is 0x43004300 in a register: mask
-// and "or" are then one instruction (with two constants they are two: the one pass over a code is what bounds the kernel)
-template <int N> __device__ __forceinline__ uint32_t codes128(uint32_t x, uint32_t magic) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(y) : "r"(x >> (4 * N)), "r"(magic));
-    return y;
+// Codes n and 4 + n of a word as a bfloat16 pair.  FAST: the code's bits are left where they are and read as a bfloat16 number below
+// the normal ones (or just at their start): the lowest 8 bits of that format count in steps of 2^-133, so the pair is
+// the codes times 2^-133, or 2^-129 for odd n, in one instruction (and a shift for two of four).  The products' other operand is
+// scaled up by a power of two instead, and the results are scaled back.  (With 128 added to the code, the usual way, a code took 1.75
+// instructions and the 128 had to be taken off again: 64 requests of 8k 167 us.)  Otherwise: the codes themselves.
+#define KV4_UNIT 133
+template <bool FAST, int N> __device__ __forceinline__ uint32_t codes(uint32_t x) {
+    if constexpr (FAST) {
+        return (N & 2 ? x >> 8 : x) & (N & 1 ? 0x00f000f0u : 0x000f000fu);
+    } else {
+        const uint32_t y = ((x >> (4 * N)) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(128.f), __float2bfloat16(128.f)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
 }
-template <int N> __device__ __forceinline__ uint32_t codes0(uint32_t x, uint32_t magic) {
-    const uint32_t y = codes128<N>(x, magic);
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(128.f), __float2bfloat16(128.f)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
+// x * 2^e for any e
+__device__ __forceinline__ float scaled(float x, int e) { const int h = e / 2; return x * pow2(h) * pow2(e - h); }
 __device__ __forceinline__ float exp2_ftz(float x) {        // to 2 units of the last place; 0 below 2^-126
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -115,11 +122,11 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     return w;
 }
 
-template <int PARTS, int NT, int NW, int SR, int ST>
+template <int PARTS, int NT, int NW, int SR, int PU, int ST>
 struct Kv4Cfg {
     static constexpr int HD = BRAID_HD, W = HD / 32;
-    static constexpr int US = 16 * SR;                       // tokens a unit
-    static constexpr int SB = SR * kv4_record_bytes(HD);     // bytes a unit
+    static constexpr int US = 16 * SR * PU;                  // tokens a unit: PU turns of SR records
+    static constexpr int SB = SR * PU * kv4_record_bytes(HD);   // bytes a unit
     static constexpr int BM = 8 * NT;                        // columns a CTA
     static constexpr int RING = NW * ST * SB;
     static constexpr int MERGE = NW * BM * (HD + 4) * 4;
@@ -127,10 +134,10 @@ struct Kv4Cfg {
     static_assert(BRAID_PAGE_SIZE % US == 0, "a unit must not straddle a page");
 };
 
-template <int PARTS, int NT, int NW, int SR, int ST>
+template <int PARTS, int NT, int NW, int SR, int PU, int ST>
 __global__ void __launch_bounds__(NW * 32)
 attn_kv4_kernel(const Kv4Args a) {
-    using C = Kv4Cfg<PARTS, NT, NW, SR, ST>;
+    using C = Kv4Cfg<PARTS, NT, NW, SR, PU, ST>;
     using T = typename std::conditional<PARTS == 3, float, __nv_bfloat16>::type;
     constexpr int HD = C::HD, W = C::W;
     pdl_trigger();
@@ -206,46 +213,57 @@ attn_kv4_kernel(const Kv4Args a) {
     // ---- queries: column nt * 8 + r, numbers 32 w + 8 j .. + 7 of the head
     uint32_t q[NT][W][PARTS][4];
     constexpr int GH = W > 4 ? 2 : 1;
-    uint32_t qb[NT][3][GH];                                    // -128 and 1 times the sum of group j's (and 4 + j's) numbers, in three parts
+    uint32_t qb[NT][3][GH];                                    // the sum of group j's (and 4 + j's) numbers beside a zero, in three parts
+    int q_exp[NT];                                             // of columns nt * 8 + r: the queries are scaled by 2^q_exp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int col = nt * 8 + r, tl = col / hpc, hl = col - tl * hpc;
         const bool in = tl < n_tok && hl < n_heads;
         const T* src = (const T*)a.q + (size_t)(q_start + (in ? tok0 + tl : 0)) * a.q_stride + (size_t)(head0 + (in ? hl : 0)) * HD + 8 * j;
         const bool wide = !(((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) & 15);
+        float x[W][8], most = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (wide) {
+                constexpr int VW = 16 / sizeof(T);
+#pragma unroll
+                for (int i = 0; i < 8; i += VW) load_run<T, VW>(src + 32 * w + i, x[w] + i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[w][i] = to_f32(src[32 * w + i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!in) x[w][i] = 0.f;
+                most = fmaxf(most, fabsf(x[w][i]));
+            }
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        q_exp[nt] = 120 - exponent(most);                      // the column's largest number becomes one of 2^120
         float sums[GH];
 #pragma unroll
         for (int h = 0; h < GH; ++h) sums[h] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            float x[8];
-            if (wide) {
-                constexpr int VW = 16 / sizeof(T);
-#pragma unroll
-                for (int i = 0; i < 8; i += VW) load_run<T, VW>(src + 32 * w + i, x + i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = to_f32(src[32 * w + i]);
-            }
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!in) x[i] = 0.f;
-                sum += x[i];
-            }
+            for (int i = 0; i < 8; ++i) sum += x[w][i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             if ((w & 3) == j) sums[w >> 2] = sum;
 #pragma unroll
+            for (int i = 0; i < 8; ++i) x[w][i] = scaled(x[w][i], q_exp[nt] - (i & 2 ? 4 : 0));       // numbers of odd n meet 16 times their code
+#pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) q[nt][w][p][n] = split_pair(x[2 * n], x[2 * n + 1]);
+                for (int n = 0; n < 4; ++n) q[nt][w][p][n] = split_pair(x[w][2 * n], x[w][2 * n + 1]);
         }
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
-            float lo = sums[h], hi = -128.f * lo;
+            float none = 0.f, sum = scaled(sums[h], q_exp[nt] - KV4_UNIT);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) qb[nt][p][h] = split_pair(hi, lo);
+            for (int p = 0; p < 3; ++p) qb[nt][p][h] = split_pair(none, sum);
         }
     }
     // ---- this lane's columns of scores: nt * 8 + 2 j + c
@@ -259,10 +277,18 @@ attn_kv4_kernel(const Kv4Args a) {
             const bool in = tl < n_tok && hl < n_heads;
             pos[nt][c] = in ? pos_min + tl : -1;               // -1: the column sees nothing
             lo[nt][c] = a.window > 0 ? pos[nt][c] - a.window + 1 : 0;
-            sc[nt][c] = (in && a.head_scale ? a.scale * a.head_scale[head0 + hl] : a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E);
+            sc[nt][c] = scaled((in && a.head_scale ? a.scale * a.head_scale[head0 + hl] : a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E),
+                               KV4_UNIT - __shfl_sync(0xffffffffu, q_exp[nt], 8 * j + 4 * c));
         }
 
     float o[NT][2 * W][4], zs[NT][2][W], m[NT][2], l[NT][2];
+    bool ok = true;
+    int st = 0, p_exp = 0;                                     // the probabilities are scaled by 2^p_exp
+    uint32_t phase = 0;
+    // Probabilities that are scaled up may pass the range of float32 where later values are much larger than the first unit's: the results
+    // are then not finite, and the warp walks once more with the codes as whole numbers and nothing scaled.
+    auto walk = [&](auto FAST) {
+    constexpr bool fast = decltype(FAST)::value;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -275,20 +301,35 @@ attn_kv4_kernel(const Kv4Args a) {
             for (int w = 0; w < W; ++w) zs[nt][c][w] = 0.f;
         }
     }
-
-    uint32_t magic;
-    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic));
-    bool ok = true;
-    int st = 0;
-    uint32_t phase = 0;
     for (int k = 0; k < n_mine; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag));
         if (!ok) break;
-        const uint8_t* base = ring + st * C::SB;
+        const uint8_t* unit_base = ring + st * C::SB;
         if (++st == ST) { st = 0; phase ^= 1u; }
-        const int key0 = tile_of(k) * C::US;
+        const int unit_key0 = tile_of(k) * C::US;
+        if (fast && k == 0) {
+            // the scale: values of the first unit's largest size, times the largest probability and the most keys, stay in range
+            float most = 0.f;
+#pragma unroll
+            for (int rec = 0; rec < SR * PU; ++rec)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = unit_key0 + 16 * rec + 8 * h + r;
+                    const uint32_t* g = reinterpret_cast<const uint32_t*>(unit_base + rec * kv4_record_bytes(HD) + kv4_value_groups(HD)) + (8 * h + r) * W;
+                    if (key <= pos_max && (key >= k_lo || key < a.keep_first))
+                        for (int w = j; w < W; w += 4) most = fmaxf(most, fmaxf(fabsf(kv4_lowest(g[w])), 16.f * kv4_step(g[w])));
+                }
+            const int e = exponent(warp_max(most));
+            p_exp = min(90 - e, 100);
+            if (e < -40) { p_exp = 1000; return; }             // very small values: walk with nothing scaled
+        }
 
-        // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
+#pragma unroll 1
+        for (int turn = 0; turn < PU; ++turn) {
+        const uint8_t* base = unit_base + turn * (SR * kv4_record_bytes(HD));
+        const int key0 = unit_key0 + turn * (16 * SR);
+        if (PU > 1 && (key0 > pos_max || (key0 + 16 * SR <= k_lo && key0 >= a.keep_first))) continue;
+        // ---- scores of the turn's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
         float s[SR][NT][4];
 #pragma unroll
         for (int rec = 0; rec < SR; ++rec) {
@@ -299,8 +340,7 @@ attn_kv4_kernel(const Kv4Args a) {
             const uint8_t* groups = rb + kv4_key_groups(HD) + r * (4 * W);
             lds_words<W>(groups, ga);
             lds_words<W>(groups + 32 * W, gb);
-            // what the lowest values, and the 128 that the codes have too much, add to the scores: a product with the queries' sums,
-            // whose operand the groups' words are as they lie
+            // what the lowest values add to the scores: a product with the queries' sums, whose operand the groups' words are as they lie
             uint32_t wa[2] = {0u, 0u}, wb[2] = {0u, 0u};
             if (W >= 4 || j < W) {
                 wa[0] = reinterpret_cast<const uint32_t*>(groups)[j];
@@ -318,8 +358,8 @@ attn_kv4_kernel(const Kv4Args a) {
             }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const uint32_t a0 = codes128<0>(ka[w], magic), a1 = codes128<0>(kb[w], magic), a2 = codes128<1>(ka[w], magic), a3 = codes128<1>(kb[w], magic);
-                const uint32_t b0 = codes128<2>(ka[w], magic), b1 = codes128<2>(kb[w], magic), b2 = codes128<3>(ka[w], magic), b3 = codes128<3>(kb[w], magic);
+                const uint32_t a0 = codes<true, 0>(ka[w]), a1 = codes<true, 0>(kb[w]), a2 = codes<true, 1>(ka[w]), a3 = codes<true, 1>(kb[w]);
+                const uint32_t b0 = codes<true, 2>(ka[w]), b1 = codes<true, 2>(kb[w]), b2 = codes<true, 3>(ka[w]), b3 = codes<true, 3>(kb[w]);
                 const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -362,7 +402,7 @@ attn_kv4_kernel(const Kv4Args a) {
                 }
         }
         // (columns that are no query see as much as the others, and nobody reads them)
-        const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
+        const bool edge = !(key0 + 16 * SR - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
         if (edge) {
 #pragma unroll
             for (int rec = 0; rec < SR; ++rec)
@@ -443,14 +483,14 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int c = e & 1;
-                    p[nt][e] = exp2_ftz(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
+                    p[nt][e] = exp2_ftz(s[rec][nt][e] - ((m[nt][c] == -INFINITY ? 0.f : m[nt][c]) - (float)p_exp));
                     l[nt][c] += p[nt][e];
                 }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]), za = kv4_lowest(ga[w]), zb = kv4_lowest(gb[w]);
-                const uint32_t a0 = codes0<0>(v01[w], magic), a1 = codes0<1>(v01[w], magic), a2 = codes0<0>(v89[w], magic), a3 = codes0<1>(v89[w], magic);
-                const uint32_t b0 = codes0<2>(v01[w], magic), b1 = codes0<3>(v01[w], magic), b2 = codes0<2>(v89[w], magic), b3 = codes0<3>(v89[w], magic);
+                const uint32_t a0 = codes<fast, 0>(v01[w]), a1 = codes<fast, 1>(v01[w]), a2 = codes<fast, 0>(v89[w]), a3 = codes<fast, 1>(v89[w]);
+                const uint32_t b0 = codes<fast, 2>(v01[w]), b1 = codes<fast, 3>(v01[w]), b2 = codes<fast, 2>(v89[w]), b3 = codes<fast, 3>(v89[w]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float x[4] = {p[nt][0] * sa, p[nt][1] * sa, p[nt][2] * sb, p[nt][3] * sb};
@@ -475,10 +515,36 @@ attn_kv4_kernel(const Kv4Args a) {
             }
         }
         };
-        if (edge) values(std::true_type{});
+        if (edge || !fast) values(std::true_type{});
         else values(std::false_type{});
+        }
         __syncwarp();                                          // every lane has read the unit
         if (issued < n_mine) issue();
+    }
+    };
+    walk(std::true_type{});
+    int even = KV4_UNIT, odd = KV4_UNIT - 4;                   // codes counted in steps of 2^-133, numbers of odd n in steps 16 times that
+    {
+        float t = p_exp > 100 ? INFINITY : 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) t = fmaf(0.f, o[nt][i][0], fmaf(0.f, o[nt][i][1], fmaf(0.f, o[nt][i][2], fmaf(0.f, o[nt][i][3], t))));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                t = fmaf(0.f, l[nt][c], t);
+#pragma unroll
+                for (int w = 0; w < W; ++w) t = fmaf(0.f, zs[nt][c][w], t);
+            }
+        }
+        if (__any_sync(0xffffffffu, ok && t != 0.f)) {
+            for (; st != istage; phase ^= (st == ST - 1), st = st == ST - 1 ? 0 : st + 1)        // (units asked for and not walked)
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag)) && ok;
+            issued = p_exp = 0;
+            while (issued < min(ST, n_mine)) issue();
+            walk(std::false_type{});
+            even = odd = 0;
+        }
     }
     if (!ok) {
         // a copy did not arrive in time: wait for the others (bounded too), so that none lands after the CTA has ended
@@ -501,6 +567,7 @@ attn_kv4_kernel(const Kv4Args a) {
                 for (int w = 0; w < W; ++w) zs[nt][c][w] += __shfl_xor_sync(0xffffffffu, zs[nt][c][w], x);
             }
     __syncthreads();                                           // every warp is done with its ring
+    const float back = pow2(-p_exp);
     float* mo = reinterpret_cast<float*>(smem);                // [warp][column][HD]
     float* ml = mo + NW * C::BM * HD;                          // [warp][column][2]
 #pragma unroll
@@ -511,9 +578,10 @@ attn_kv4_kernel(const Kv4Args a) {
             float* dst = mo + (warp * C::BM + col) * HD + 4 * r;
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(o[nt][2 * w][c] + zs[nt][c][w], o[nt][2 * w][2 + c] + zs[nt][c][w],
-                                                                       o[nt][2 * w + 1][c] + zs[nt][c][w], o[nt][2 * w + 1][2 + c] + zs[nt][c][w]);
-            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c]; }
+                *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(
+                    (scaled(o[nt][2 * w][c], even) + zs[nt][c][w]) * back, (scaled(o[nt][2 * w][2 + c], odd) + zs[nt][c][w]) * back,
+                    (scaled(o[nt][2 * w + 1][c], even) + zs[nt][c][w]) * back, (scaled(o[nt][2 * w + 1][2 + c], odd) + zs[nt][c][w]) * back);
+            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c] * back; }
         }
     __syncthreads();
     const bool out_wide = !(((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) & (4 * sizeof(T) - 1));
@@ -615,19 +683,22 @@ attn_kv4_merge_kernel(const Kv4Args a) {
 }
 
 // ------------------------------------------------------------------ host side
-// Warps, records a unit and stages a ring: what fits 227 KB with several CTAs an SM.
+// Four warps a CTA.  A turn takes SR records of 16 tokens: four of them give a warp enough independent products to work on (one request of
+// 128k, heads of 128: 53 us with two records a turn and 12 warps an SM, 45 with four and 8); two where the registers hold no more: 16
+// columns, float32, heads above 128.
 #define KV4_NW 4
-#define KV4_SR 2
-#define KV4_ST (BRAID_HD > 128 ? 2 : 3)
-// Columns a CTA: 8, or 16 where a step has that many and the registers hold their results.
+#define KV4_PU 1
 #define KV4_NT_MAX (BRAID_HD > 128 ? 1 : 2)
+constexpr int kv4_sr(int parts, int nt) { return BRAID_HD <= 128 && parts == 1 && nt == 1 ? 4 : 2; }
+constexpr int kv4_st(int parts, int nt) { return kv4_sr(parts, nt) == 4 || BRAID_HD > 128 ? 2 : 3; }
+template <int PARTS, int NT> using Kv4C = Kv4Cfg<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>;
 
 template <int PARTS, int NT>
-static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>; }
+static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>; }
 
 template <int PARTS, int NT>
 static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
-    using C = Kv4Cfg<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>;
+    using C = Kv4C<PARTS, NT>;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kv4_kernel<PARTS, NT>(), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
@@ -639,7 +710,7 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
     if (gz > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld tiles, %d heads, %d sequences)", gz, a.nkh * hchunks, a.n_seqs);
     if (gz == 0) return BRAID_OK;
-    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, KV4_SR, KV4_ST>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
+    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
     BRAID_LAUNCH_CHECK();
 }
 
@@ -652,9 +723,8 @@ extern "C" int braid_attn_kv4_slots(int f32, int columns) {
     int dev = 0, sms = 0, per_sm = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int smem = Kv4Cfg<1, 1, KV4_NW, KV4_SR, KV4_ST>::SMEM, smem2 = Kv4Cfg<1, KV4_NT_MAX, KV4_NW, KV4_SR, KV4_ST>::SMEM;
     const void* f = columns <= 8 ? (f32 ? kv4_kernel<3, 1>() : kv4_kernel<1, 1>()) : (f32 ? kv4_kernel<3, KV4_NT_MAX>() : kv4_kernel<1, KV4_NT_MAX>());
-    const int bytes = columns <= 8 ? smem : smem2;
+    const int bytes = columns <= 8 ? (f32 ? Kv4C<3, 1>::SMEM : Kv4C<1, 1>::SMEM) : (f32 ? Kv4C<3, KV4_NT_MAX>::SMEM : Kv4C<1, KV4_NT_MAX>::SMEM);
     cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, f, KV4_NW * 32, bytes);
     if (e != cudaSuccess || per_sm <= 0 || sms <= 0) return 148 * 2;
