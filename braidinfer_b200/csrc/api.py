@@ -183,6 +183,9 @@ class Kernels:
         self.pending_partial = None     # the open PartialProduct, if any (it owns the GEMM workspace)
         self.workspace_generation = 0   # grows when a scratch buffer moves (captured graphs are stale then)
         self._attn_partial: Optional[torch.Tensor] = None
+        self._kv4_pages: Optional[torch.Tensor] = None
+        self._kv4_numbers: Optional[torch.Tensor] = None
+        self._kv4_repair: Optional[torch.Tensor] = None
         self._verbose = verbose
 
     # ------------------------------------------------------------------ plumbing
@@ -800,9 +803,9 @@ class Kernels:
     def kv4_expand(self, cache: torch.Tensor, out: torch.Tensor, page_table: torch.Tensor, q_len: torch.Tensor, kv_before: torch.Tensor,
                    window: Optional[int] = None, keep_first: int = 0) -> None:
         """Read the pages that a step's queries see back into ordinary ones, out [pages, 2, kv_heads, page size, hd] (float32 or
-        bfloat16), page for page: with a window, from the first block that a sequence's first new token sees, and its kept first
-        blocks.  Places of those pages behind the sequence's end come out zero; other pages stay as they were.  A page belongs to one
-        sequence."""
+        bfloat16), page for page: with a window, from the first position that a sequence's first new token sees, and its kept first
+        ones.  Other places of those pages, behind the sequence's end too, come out zero; other pages stay as they were.  A page belongs
+        to one sequence."""
         lib = self.part_library("kv4")
         if out.dim() != 5 or out.shape[0] != cache.shape[0] or out.shape[1] != 2 or out.shape[3] != build.page_size() or not out.is_contiguous():
             raise KernelError(f"kv4_expand: the pages must be contiguous [{cache.shape[0]}, 2, kv_heads, {build.page_size()}, head_dim], got "
@@ -817,8 +820,8 @@ class Kernels:
         self.launches += 1
         self._check_lib(lib, lib.braid_kv4_expand(cache.data_ptr(), out.data_ptr(), dtype_code(out.dtype), page_table.data_ptr(), q_len.data_ptr(),
                                                   kv_before.data_ptr(), n, page_table.shape[1], cache.shape[1], hd, cache.shape[0],
-                                                  int(window or 0), int(keep_first or 0), self._error_flag.data_ptr() + 16, self._stream()),
-                        "kv4_expand")
+                                                  int(window or 0), int(keep_first or 0), 0, None, 0, self._error_flag.data_ptr() + 16,
+                                                  self._stream()), "kv4_expand")
 
     def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
                  q_len: torch.Tensor, kv_before: torch.Tensor, token_seq: torch.Tensor, n_seqs: int, max_q_len: int, max_kv_len: int,
@@ -858,19 +861,30 @@ class Kernels:
                         *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
+        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, n_seqs, nqh, nkh):
+            self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
+                                 int(window or 0), scale, int(keep_first or 0), head_scale, dict(
+                                     sink=sink, out_scale=out_scale, head_sinks=head_sinks, head_gate=head_gate, distance_bias=distance_bias,
+                                     softcap=softcap))
+            return
         if backend == "auto":
             self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                int(window or 0), scale, sink, out_scale, head_sinks, head_gate, int(keep_first or 0), head_scale, distance_bias,
                                softcap, settled)
             return
+        self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, int(window or 0), scale, int(keep_first or 0),
+                             head_scale, sink, out_scale, head_sinks, head_gate, distance_bias, softcap)
+
+    def _attn_kv4_plain(self, q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale, sink,
+                        out_scale, head_sinks, head_gate, distance_bias, softcap, repair=None, n_seqs=0) -> None:
         lib = self.part_library("kv4")
         self.launches += 1
         self._check_lib(lib, lib.braid_attn_kv4_simple(
             q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype_code(out.dtype), cache.data_ptr(), page_table.data_ptr(),
-            token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(), rows, nqh, nkh, hd, page_table.shape[1], cache.shape[0],
-            int(window or 0), int(keep_first or 0), float(scale), int(sink is not None), float(sink or 0.0), float(out_scale),
-            _ptr(head_sinks), _ptr(head_gate), head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale),
-            *self._bias_args(distance_bias), float(softcap or 0.0), self._error_flag.data_ptr() + 16, self._stream()), what)
+            token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(), out.shape[0], nqh, nkh, hd, page_table.shape[1], cache.shape[0],
+            window, keep_first, float(scale), int(sink is not None), float(sink or 0.0), float(out_scale), _ptr(head_sinks), _ptr(head_gate),
+            head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale), *self._bias_args(distance_bias), float(softcap or 0.0),
+            _ptr(repair), n_seqs, self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
 
     def kv4_attention_library(self, head_dim: int):
         """The attention over a 4-bit cache for one head size, compiled at first use."""
@@ -886,6 +900,63 @@ class Kernels:
             lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once)
             self._attn_libs[("kv4", head_dim)] = lib
         return lib
+
+    # The most that the pages of a step's prompts, read back for attention, may take at once: more sequences go one group after another.
+    KV4_PAGES_BYTES = 1 << 30
+
+    # Prompts of at least so many (16 columns of queries, kv head, sequence) have their pages read back once for all of them.  The kernel
+    # over 4 bits reads them for every 16 columns, sliced over the machine; the one over ordinary pages takes 128 columns a CTA, which
+    # walks the context alone.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: 32 tokens of 4 sequences
+    # behind 8,000 (256 of them) 187 / 120, 64 tokens (512) 193 / 200, 512 tokens (4,096) 317 / 1,198; of one behind 32,000: 128 tokens (256)
+    # 646 / 450, 512 tokens (1,024) 667 / 1,782; without a context, 128 tokens 13.7 / 11.2, 512 tokens 21 / 48.
+    KV4_PAGES_FROM = 400
+
+    @staticmethod
+    def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, n_seqs: int, nqh: int, nkh: int) -> bool:
+        """Whether attention reads the step's pages back and runs over ordinary ones."""
+        g = nqh // nkh
+        tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
+        return (max_q_len > 8 and tiles * nkh * n_seqs >= Kernels.KV4_PAGES_FROM and out.dtype == torch.bfloat16 and q.stride(0) % 8 == 0
+                and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0)
+
+    def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
+                        scale, keep_first, head_scale, options) -> None:
+        """Prompts, bfloat16: the pages that the queries see are read back, block c of sequence i as page i * cols + c of a workspace,
+        and the attention of ordinary pages runs over them.  Values that are NaN are read back as zero, and the sequences that hold some
+        are computed by the plain kernel (which otherwise ends at once)."""
+        lib = self.part_library("kv4")
+        if self._kv4_repair is None or self._kv4_repair.numel() < n_seqs + 2:
+            self._kv4_repair = torch.zeros(max(n_seqs, 1022) + 2, dtype=torch.int32, device="cuda")
+            self.workspace_generation += 1
+        cols = min(page_table.shape[1], max(1, -(-max_kv_len // build.page_size())))
+        page = 2 * nkh * build.page_size() * hd
+        group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
+        need = group * cols
+        if self._kv4_pages is None or self._kv4_pages.numel() < need * page:
+            self._kv4_pages = torch.empty(need * page, dtype=torch.bfloat16, device="cuda")
+            self.workspace_generation += 1
+        if self._kv4_numbers is None or self._kv4_numbers.numel() < need:
+            self._kv4_numbers = torch.arange(max(need, 1 << 14), dtype=torch.int32, device="cuda")
+            self.workspace_generation += 1
+        pages = self._kv4_pages[:need * page].view(need, 2, nkh, build.page_size(), hd)
+        table = self._kv4_numbers[:need].view(group, cols)
+        tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(options["softcap"])
+                                                                                     or options["distance_bias"] is not None)
+        for i in range(0, n_seqs, group):
+            n = min(group, n_seqs - i)
+            part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
+            own = page_table[i:i + n]
+            self.launches += 1
+            self._check_lib(lib, lib.braid_kv4_expand(cache.data_ptr(), pages.data_ptr(), BF16, own.data_ptr(), part[1].data_ptr(), part[2].data_ptr(),
+                                                      n, page_table.shape[1], nkh, hd, cache.shape[0], window, keep_first, cols,
+                                                      self._kv4_repair.data_ptr(), i, self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
+            if tc:
+                self.attn_tc(q, out, pages, table, *part, n, max_q_len, nqh, nkh, hd, window, scale, **options)
+            else:
+                self.attn_mma(q, out, pages, table, *part, token_seq, n, max_q_len, nqh, nkh, hd, window, scale, keep_first=keep_first,
+                              head_scale=head_scale, **options)
+        self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale,
+                             **options, repair=self._kv4_repair, n_seqs=n_seqs)
 
     def _attn_kv4_mma(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                       scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled) -> None:
@@ -1041,10 +1112,10 @@ class Kernels:
             elif name == "kv4":
                 lib.braid_step_tables.argtypes = [c_void_p] * 8 + [c_int] * 5 + [c_void_p, c_void_p]
                 lib.braid_kv4_store.argtypes = [c_void_p, c_longlong] * 2 + [c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_void_p]
-                lib.braid_kv4_expand.argtypes = [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 7 + [c_void_p, c_void_p]
+                lib.braid_kv4_expand.argtypes = [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_void_p, c_int, c_void_p, c_void_p]
                 lib.braid_attn_kv4_simple.argtypes = [c_void_p, c_longlong] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 8 + \
                                                      [c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_longlong] + [c_void_p] * 3 + \
-                                                     [c_float, c_void_p, c_void_p]
+                                                     [c_float, c_void_p, c_int, c_void_p, c_void_p]
                 names = ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand", "braid_attn_kv4_simple")
             elif name == "streams":
                 lib.braid_streams.argtypes = [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,

@@ -244,17 +244,20 @@ extern "C" int braid_kv4_store(const void* k, long long k_stride, const void* v,
 }
 
 // ------------------------------------------------------------------ reading back
-// The pages of a step's sequences as values, into pages [page][2][kv head][64][hd] of the same numbering: what a sequence's
-// queries see (from its window's first position, and its kept first ones, up to its new tokens); places of those pages behind the
-// sequence's end come out zero.  A CTA takes one page of one kv head.  A page belongs to one sequence.
+// The pages of a step's sequences as values, into pages [page][2][kv head][64][hd]: what a sequence's queries see (from its window's first
+// position, and its kept first ones, up to its new tokens); other places of those pages come out zero.  The
+// pages are numbered as the cache's, or (out_cols > 0) block c of sequence i is page i * out_cols + c.  A CTA takes one page of one kv
+// head.  A page belongs to one sequence.
 struct ExpandArgs {
     const uint8_t* cache;
     void* out;
     const int* page_table;
     const int* q_len;
     const int* kv_before;
-    int nkh, hd, cols, num_pages, window, keep_first;
+    int nkh, hd, cols, num_pages, window, keep_first, out_cols;
     int* error_flag;
+    int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [2 + seq0 + sequence] become 1
+    int seq0;
 };
 
 template <typename T>
@@ -273,6 +276,7 @@ kv4_expand_kernel(ExpandArgs a) {
         if (threadIdx.x == 0) atomicExch(a.error_flag, 1);
         return;
     }
+    const size_t out_page = a.out_cols > 0 ? (size_t)seq * a.out_cols + c : (size_t)page;
     const int hd = a.hd, W = hd / KV4_GROUP, per = hd / 8;
     const uint8_t* src = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(hd);
     const int n_here = min(BRAID_PAGE_SIZE, end - key0);
@@ -280,11 +284,16 @@ kv4_expand_kernel(ExpandArgs a) {
         const int c8 = it % per, tp = it / per, t = tp % BRAID_PAGE_SIZE, value = tp / BRAID_PAGE_SIZE;
         const int w = c8 >> 2, j = c8 & 3;
         float x[8];
-        if (t < n_here) {
+        if (t < n_here && (key0 + t >= lo || key0 + t < a.keep_first)) {
             const uint8_t* rec = src + (t / KV4_REC) * kv4_record_bytes(hd);
             const int tr = t % KV4_REC;
             const uint32_t group = reinterpret_cast<const uint32_t*>(rec + (value ? kv4_value_groups(hd) : kv4_key_groups(hd)))[tr * W + w];
-            const float step = kv4_step(group), low = kv4_lowest(group);
+            float step = kv4_step(group), low = kv4_lowest(group);
+            if (value && a.repair && !(fabsf(step) + fabsf(low) < INFINITY)) {
+                step = low = 0.f;
+                a.repair[2 + a.seq0 + seq] = 1;
+                a.repair[0] = 1;
+            }
             if (!value) {
                 const uint32_t word = reinterpret_cast<const uint32_t*>(rec + tr * (hd / 2))[j * W + w];
 #pragma unroll
@@ -302,7 +311,7 @@ kv4_expand_kernel(ExpandArgs a) {
 #pragma unroll
             for (int n = 0; n < 8; ++n) x[n] = 0.f;
         }
-        T* dst = (T*)a.out + ((((size_t)page * 2 + value) * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * hd + 8 * c8;
+        T* dst = (T*)a.out + (((out_page * 2 + value) * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * hd + 8 * c8;
         constexpr int VW = 16 / sizeof(T);
 #pragma unroll
         for (int i = 0; i < 8; i += VW) store_run<T, VW>(dst + i, x + i);
@@ -310,13 +319,14 @@ kv4_expand_kernel(ExpandArgs a) {
 }
 
 extern "C" int braid_kv4_expand(const void* cache, void* out, int dtype, const int* page_table, const int* q_len, const int* kv_before,
-                                int n_seqs, int cols, int nkh, int hd, int num_pages, int window, int keep_first, int* error_flag, void* stream) {
+                                int n_seqs, int cols, int nkh, int hd, int num_pages, int window, int keep_first, int out_cols, int* repair,
+                                int seq0, int* error_flag, void* stream) {
     if (n_seqs <= 0 || cols <= 0) return BRAID_OK;
     if (int rc = kv4_check("kv4_expand", nkh, hd, cache)) return rc;
     if ((uintptr_t)out & 15) BRAID_REFUSE("kv4_expand: the pages must start on 16 bytes");
     if (nkh > 65535 || n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", nkh, n_seqs);
-    ExpandArgs a{(const uint8_t*)cache, out, page_table, q_len, kv_before, nkh, hd, cols, num_pages, window, window > 0 ? keep_first : 0, error_flag};
-    const dim3 grid(cols, nkh, n_seqs);
+    ExpandArgs a{(const uint8_t*)cache, out, page_table, q_len, kv_before, nkh, hd, cols, num_pages, window, window > 0 ? keep_first : 0, out_cols, error_flag, repair, seq0};
+    const dim3 grid(out_cols > 0 ? min(cols, out_cols) : cols, nkh, n_seqs);
     if (dtype == BRAID_F32) braid_launch(kv4_expand_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, a);
     else if (dtype == BRAID_BF16) braid_launch(kv4_expand_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
     else BRAID_REFUSE("kv4_expand: unknown dtype code %d", dtype);
@@ -326,6 +336,9 @@ extern "C" int braid_kv4_expand(const void* cache, void* out, int dtype, const i
 // ------------------------------------------------------------------ plain attention
 // One warp per (row, query head), 32 keys at a time: a lane a key for the scores, a lane a number of the head for the values.  All
 // arithmetic float32.  Options as in attn_simple.cu.  Rows of padding (token_seq < 0) are left as they were.
+// With `repair` ([0]: whether to work at all, [1]: CTAs that are done, [2 + i]: whether for sequence i; all 0 before) it goes over the
+// result of a product that multiplies masked values by 0 (the attention of ordinary pages): a NaN among them would make all of it NaN, so
+// they were taken out, and the rows of those sequences are computed here.  The last CTA to end leaves all numbers 0 again.
 struct Kv4SimpleArgs {
     const void* q;
     void* out;
@@ -347,22 +360,17 @@ struct Kv4SimpleArgs {
     const float* bias_rate;
     float softcap;
     int* error_flag;
+    int* repair;
+    int n_seqs;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(128)
-attn_kv4_simple_kernel(Kv4SimpleArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    __shared__ float qs_all[4][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + warp;
-    if (item >= (long long)a.rows * a.nqh) return;
+__device__ void attn_kv4_item(const Kv4SimpleArgs& a, long long item, float* qs, int lane) {
     const int row = (int)(item / a.nqh), head = (int)(item - (long long)row * a.nqh);
     const int seq = a.token_seq[row];
-    if (seq < 0) return;
-    float* qs = qs_all[warp];
+    if (seq < 0 || (a.repair && !a.repair[2 + seq])) return;
     const int hd = a.hd, W = hd / KV4_GROUP, kvh = head / (a.nqh / a.nkh);
+    __syncwarp();
     const T* q = (const T*)a.q + (size_t)row * a.q_stride + (size_t)head * hd;
     for (int d = lane; d < hd; d += 32) qs[d] = to_f32(q[d]);
     __syncwarp();
@@ -437,20 +445,39 @@ attn_kv4_simple_kernel(Kv4SimpleArgs a) {
         if (w < W) o[32 * w + lane] = from_f32<T>(acc[w] * inv);
 }
 
+template <typename T>
+__global__ void __launch_bounds__(128)
+attn_kv4_simple_kernel(const Kv4SimpleArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float qs_all[4][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (a.repair && *(volatile int*)a.repair == 0) return;
+    for (long long item = (long long)blockIdx.x * 4 + warp; item < (long long)a.rows * a.nqh; item += (long long)gridDim.x * 4)
+        attn_kv4_item<T>(a, item, qs_all[warp], lane);
+    if (a.repair) {
+        __syncthreads();
+        if (threadIdx.x == 0 && atomicAdd(a.repair + 1, 1) == (int)gridDim.x - 1) {      // every CTA has looked at the flag
+            for (int i = 0; i < a.n_seqs + 2; ++i) a.repair[i] = 0;
+        }
+    }
+}
+
 extern "C" int braid_attn_kv4_simple(const void* q, long long q_stride, void* out, long long out_stride, int dtype, const void* cache,
                                      const int* page_table, const int* token_seq, const int* q_start, const int* kv_before, int rows, int nqh,
                                      int nkh, int hd, int cols, int num_pages, int window, int keep_first, float scale, int has_sink, float sink,
                                      float out_scale, const float* head_sinks, const void* head_gate, long long gate_stride, const float* head_scale,
-                                     const float* bias_slope, const float* bias_rate, float softcap, int* error_flag, void* stream) {
+                                     const float* bias_slope, const float* bias_rate, float softcap, int* repair, int n_seqs, int* error_flag, void* stream) {
     if (rows <= 0) return BRAID_OK;
     if (int rc = kv4_check("attn_kv4", nkh, hd, cache)) return rc;
     if (nqh <= 0 || nqh % nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", nqh, nkh);
     if (num_pages <= 0 || cols <= 0) BRAID_REFUSE("attn_kv4: the cache has no pages (pages=%d, table columns=%d)", num_pages, cols);
-    const long long ctas = ((long long)rows * nqh + 3) / 4;
+    long long ctas = ((long long)rows * nqh + 3) / 4;
+    if (repair) ctas = min(ctas, 148LL);                      // one an SM: they hardly ever have anything to do
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
     Kv4SimpleArgs a{q, out, (const uint8_t*)cache, page_table, token_seq, q_start, kv_before, q_stride, out_stride, rows, nqh, nkh, hd, cols, num_pages,
                     window, window > 0 ? keep_first : 0, scale, has_sink || head_sinks, sink, out_scale, head_sinks, head_gate, gate_stride, head_scale,
-                    bias_slope, bias_rate, softcap, error_flag};
+                    bias_slope, bias_rate, softcap, error_flag, repair, n_seqs};
     if (dtype == BRAID_F32) braid_launch(attn_kv4_simple_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
     else if (dtype == BRAID_BF16) braid_launch(attn_kv4_simple_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
     else BRAID_REFUSE("attn_kv4: unknown dtype code %d", dtype);

@@ -114,7 +114,7 @@ def test_entry_points_refuse(K):
     assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 2, 4, -1, 4, 9, p, None) == -1
     assert lib.braid_kv4_store(p, 128, p, 128, 0, p, p - p % 16 + 4, 3, 2, 64, 5, p, None) == -1          # a cache off its 16 bytes
     assert lib.braid_kv4_store(p, 128, p, 128, 7, p, p - p % 16, 3, 2, 64, 5, p, None) == -1
-    assert lib.braid_kv4_expand(p - p % 16, p - p % 16, 0, p, p, p, 70000, 3, 2, 64, 5, 0, 0, p, None) == -1
+    assert lib.braid_kv4_expand(p - p % 16, p - p % 16, 0, p, p, p, 70000, 3, 2, 64, 5, 0, 0, 0, None, 0, p, None) == -1
     assert b"grid" in lib.braid_last_error()
     # nothing to do is no error
     assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 0, 0, 0, 4, 9, p, None) == 0
