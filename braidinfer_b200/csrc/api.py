@@ -139,10 +139,13 @@ class RowScale:
         return torch.rsqrt(self.shares.sum(0) / self.width + self.eps)
 
 
-_KV4_ARGS = struct.Struct("<15Q3q12i4f2i")      # Kv4Args of attn_kv4.cu
+# The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
+_KV4_ARGS = struct.Struct("<15Q3q12i4f2i")
+_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<7Q10i")
 
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # torch's own quick way to the stream handle
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _scale_args(scale: Optional["RowScale"]):
@@ -729,15 +732,16 @@ class Kernels:
     # ------------------------------------------------------------------ a cache held in 4 bits
     def _on_device(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
         """Refuse tensors that are not on the device these kernels launch on, and launches while another one is current."""
+        here = self._device_index
         for t in tensors:
-            if t is not None and (t.device.type != "cuda" or t.device.index != self._device_index):
-                raise KernelError(f"{what}: a tensor on {t.device}; these kernels run on cuda:{self._device_index}")
-        if torch.cuda.current_device() != self._device_index:
-            raise KernelError(f"{what}: the current device is not cuda:{self._device_index}")
+            if t is not None and t.get_device() != here:
+                raise KernelError(f"{what}: a tensor on {t.device}; these kernels run on cuda:{here}")
+        if _CURRENT_DEVICE() != here:
+            raise KernelError(f"{what}: the current device is not cuda:{here}")
 
     @staticmethod
     def _i32(what: str, name: str, t: Optional[torch.Tensor], least: int) -> None:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < least):
             raise KernelError(f"{what}: {name} must be contiguous int32 with at least {least} numbers")
 
     @staticmethod
@@ -766,21 +770,22 @@ class Kernels:
         of every new token; -1 for rows past the tokens) and, where given, positions and token_seq [rows] (0 and -1 past the tokens)
         and q_start [n].  Lengths that fit neither the rows, the list nor the table, and pages outside [0, num_pages), raise a device error
         (`check_device_errors`); what does not fit is not written anywhere else."""
+        what, i32 = "step_tables", self._i32
         lib = self.part_library("kv4")
-        n = q_len.numel()
+        n, rows = q_len.numel(), place.numel()
         if page_table.dim() != 2 or page_table.shape[0] != n or kv_before.numel() != n:
             raise KernelError(f"step_tables: {n} requests want as many kv_before and rows of the page table, got {kv_before.numel()} and "
                               f"{tuple(page_table.shape)}")
-        rows, cols = place.numel(), page_table.shape[1]
-        for name, t, size in (("q_len", q_len, n), ("kv_before", kv_before, n), ("pages", pages, 0), ("page_table", page_table, n * cols),
-                              ("place", place, rows), ("positions", positions, rows), ("token_seq", token_seq, rows), ("q_start", q_start, n)):
-            self._i32("step_tables", name, t, size)
-        self._on_device("step_tables", q_len, kv_before, pages, page_table, place, positions, token_seq, q_start)
+        cols = page_table.shape[1]
+        i32(what, "q_len", q_len, n), i32(what, "kv_before", kv_before, n), i32(what, "pages", pages, 0), i32(what, "page_table", page_table, 0)
+        i32(what, "place", place, rows), i32(what, "positions", positions, rows), i32(what, "token_seq", token_seq, rows)
+        i32(what, "q_start", q_start, n)
+        self._on_device(what, q_len, kv_before, pages, page_table, place, positions, token_seq, q_start)
         self.launches += 1
-        self._check_lib(lib, lib.braid_step_tables(
-            q_len.data_ptr(), kv_before.data_ptr(), pages.data_ptr(), page_table.data_ptr(), place.data_ptr(), _ptr(positions),
-            _ptr(token_seq), _ptr(q_start), n, pages.numel(), rows, cols, int(num_pages), self._error_flag.data_ptr() + 24, self._stream()),
-            "step_tables")
+        args = _TABLES_ARGS.pack(
+            q_len.data_ptr(), kv_before.data_ptr(), pages.data_ptr(), page_table.data_ptr(), place.data_ptr(), _ptr(positions) or 0,
+            _ptr(token_seq) or 0, _ptr(q_start) or 0, n, pages.numel(), rows, cols, num_pages, self._error_flag.data_ptr() + 24)
+        self._check_lib(lib, lib.braid_step_tables(args, self._stream()), what)
 
     def kv4_store(self, k: torch.Tensor, v: torch.Tensor, place: torch.Tensor, cache: torch.Tensor, hd: int) -> None:
         """Write keys and values [rows, kv_heads * hd] (rows of any stride, float32 or bfloat16) into a 4-bit cache at the rows'
@@ -796,9 +801,9 @@ class Kernels:
         self._i32("kv4_store", "place", place, rows)
         self._on_device("kv4_store", k, v, place, cache)
         self.launches += 1
-        self._check_lib(lib, lib.braid_kv4_store(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), dtype_code(k.dtype), place.data_ptr(),
-                                                 cache.data_ptr(), rows, nkh, hd, cache.shape[0], self._error_flag.data_ptr(),
-                                                 self._stream()), "kv4_store")
+        args = _STORE_ARGS.pack(k.data_ptr(), v.data_ptr(), place.data_ptr(), cache.data_ptr(), self._error_flag.data_ptr(), k.stride(0), v.stride(0),
+                                rows, nkh, hd, cache.shape[0], dtype_code(k.dtype))
+        self._check_lib(lib, lib.braid_kv4_store(args, self._stream()), "kv4_store")
 
     def kv4_expand(self, cache: torch.Tensor, out: torch.Tensor, page_table: torch.Tensor, q_len: torch.Tensor, kv_before: torch.Tensor,
                    window: Optional[int] = None, keep_first: int = 0) -> None:
@@ -817,11 +822,14 @@ class Kernels:
         for name, t, size in (("page_table", page_table, 0), ("q_len", q_len, n), ("kv_before", kv_before, n)):
             self._i32("kv4_expand", name, t, size)
         self._on_device("kv4_expand", cache, out, page_table, q_len, kv_before)
+        self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
+
+    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_cols=0, repair=None, seq0=0) -> None:
         self.launches += 1
-        self._check_lib(lib, lib.braid_kv4_expand(cache.data_ptr(), out.data_ptr(), dtype_code(out.dtype), page_table.data_ptr(), q_len.data_ptr(),
-                                                  kv_before.data_ptr(), n, page_table.shape[1], cache.shape[1], hd, cache.shape[0],
-                                                  int(window or 0), int(keep_first or 0), 0, None, 0, self._error_flag.data_ptr() + 16,
-                                                  self._stream()), "kv4_expand")
+        args = _EXPAND_ARGS.pack(cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), q_len.data_ptr(), kv_before.data_ptr(),
+                                 self._error_flag.data_ptr() + 16, _ptr(repair) or 0, n, cache.shape[1], hd, page_table.shape[1], cache.shape[0],
+                                 window, keep_first, out_cols, seq0, dtype_code(out.dtype))
+        self._check_lib(lib, lib.braid_kv4_expand(args, self._stream()), "kv4_expand")
 
     def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
                  q_len: torch.Tensor, kv_before: torch.Tensor, token_seq: torch.Tensor, n_seqs: int, max_q_len: int, max_kv_len: int,
@@ -945,11 +953,7 @@ class Kernels:
         for i in range(0, n_seqs, group):
             n = min(group, n_seqs - i)
             part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
-            own = page_table[i:i + n]
-            self.launches += 1
-            self._check_lib(lib, lib.braid_kv4_expand(cache.data_ptr(), pages.data_ptr(), BF16, own.data_ptr(), part[1].data_ptr(), part[2].data_ptr(),
-                                                      n, page_table.shape[1], nkh, hd, cache.shape[0], window, keep_first, cols,
-                                                      self._kv4_repair.data_ptr(), i, self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
+            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, cols, self._kv4_repair, i)
             if tc:
                 self.attn_tc(q, out, pages, table, *part, n, max_q_len, nqh, nkh, hd, window, scale, **options)
             else:
@@ -1110,9 +1114,10 @@ class Kernels:
                 lib.braid_delta_work_floats.restype = c_longlong
                 names = ("braid_delta_rule", "braid_delta_gated_norm")
             elif name == "kv4":
-                lib.braid_step_tables.argtypes = [c_void_p] * 8 + [c_int] * 5 + [c_void_p, c_void_p]
-                lib.braid_kv4_store.argtypes = [c_void_p, c_longlong] * 2 + [c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_void_p]
-                lib.braid_kv4_expand.argtypes = [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_void_p, c_int, c_void_p, c_void_p]
+                for n in ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand"):
+                    getattr(lib, n).argtypes = [c_char_p, c_void_p]
+                if [lib.braid_kv4_args_bytes(i) for i in range(3)] != [_TABLES_ARGS.size, _STORE_ARGS.size, _EXPAND_ARGS.size]:
+                    raise KernelError("the library of the 4-bit cache has other arguments than these bindings")
                 lib.braid_attn_kv4_simple.argtypes = [c_void_p, c_longlong] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 8 + \
                                                      [c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_longlong] + [c_void_p] * 3 + \
                                                      [c_float, c_void_p, c_int, c_void_p, c_void_p]

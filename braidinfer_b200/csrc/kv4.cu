@@ -114,21 +114,21 @@ step_tables_kernel(TablesArgs a) {
     }
 }
 
-extern "C" int braid_step_tables(const int* q_len, const int* kv_before, const int* pages, int* page_table, int* place, int* positions,
-                                 int* token_seq, int* q_start, int n, int n_pages_listed, int rows, int cols, int num_pages,
-                                 int* error_flag, void* stream) {
-    if (n < 0 || rows < 0 || cols < 0 || n_pages_listed < 0) BRAID_REFUSE("step_tables: negative sizes");
-    if (n > TABLES_MAX_REQUESTS) BRAID_REFUSE("step_tables: %d requests exceed %d", n, TABLES_MAX_REQUESTS);
-    if ((long long)num_pages * BRAID_PAGE_SIZE > 0x7fffffffLL) BRAID_REFUSE("step_tables: places in %d pages pass 32 bits", num_pages);
-    const long long items = (long long)rows + (long long)n * cols;
+// The entry points take their arguments as one structure that the caller fills in (csrc/api.py has the layouts): a call with one pointer
+// costs the host a fraction of one with twenty arguments.
+extern "C" int braid_step_tables(const TablesArgs* args, void* stream) {
+    const TablesArgs& a = *args;
+    if (a.n < 0 || a.rows < 0 || a.cols < 0 || a.n_pages_listed < 0) BRAID_REFUSE("step_tables: negative sizes");
+    if (a.n > TABLES_MAX_REQUESTS) BRAID_REFUSE("step_tables: %d requests exceed %d", a.n, TABLES_MAX_REQUESTS);
+    if ((long long)a.num_pages * BRAID_PAGE_SIZE > 0x7fffffffLL) BRAID_REFUSE("step_tables: places in %d pages pass 32 bits", a.num_pages);
+    const long long items = (long long)a.rows + (long long)a.n * a.cols;
     if (items == 0) return BRAID_OK;
     const long long ctas = (items + TABLES_THREADS * TABLES_PER_THREAD - 1) / (TABLES_THREADS * TABLES_PER_THREAD);
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("step_tables: the tables exceed the grid limit");
-    const size_t smem = 2 * ((size_t)n + 1) * sizeof(int);
+    const size_t smem = 2 * ((size_t)a.n + 1) * sizeof(int);
     cudaError_t e = cudaSuccess;
     if (smem > 40 * 1024) e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * (TABLES_MAX_REQUESTS + 1) * sizeof(int)));
     if (e != cudaSuccess) { braid_set_error("step_tables: cannot reserve shared memory: %s", cudaGetErrorString(e)); return (int)e; }
-    TablesArgs a{q_len, kv_before, pages, page_table, place, positions, token_seq, q_start, n, n_pages_listed, rows, cols, num_pages, error_flag};
     braid_launch(step_tables_kernel, dim3((unsigned)ctas), dim3(TABLES_THREADS), smem, (cudaStream_t)stream, a);
     BRAID_LAUNCH_CHECK();
 }
@@ -136,6 +136,21 @@ extern "C" int braid_step_tables(const int* q_len, const int* kv_before, const i
 // ------------------------------------------------------------------ write
 // Four lanes a group: lane j takes its numbers 8 j .. 8 j + 7, which are one word of key codes, or two 16-bit words of value
 // codes.  `place` < 0: a row of padding, nothing is written.  Places must differ from one another.
+//
+// A code is the quotient (x - lo) / step rounded to the nearest whole number, ties to even.  The quotient is taken as a product with 1 / step,
+// which may miss a number next to a tie, and then put right by the remainder x - lo - code step: that is exact (the code has
+// 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  (6,400 rows of 8 heads of 128, keys and values: 17 us
+// with a division a number, FIGURE us so; what is read and written takes 5 us.)
+struct StoreArgs {
+    const void* k;
+    const void* v;
+    const int* place;
+    uint8_t* cache;
+    int* error_flag;
+    long long k_stride, v_stride;
+    int rows, nkh, hd, num_pages, dtype;
+};
+
 template <typename T, bool WIDE>
 __device__ __forceinline__ void load8(const T* p, float* x) {
     if constexpr (WIDE) {
@@ -150,11 +165,10 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
-kv4_store_kernel(const T* __restrict__ k, long long k_stride, const T* __restrict__ v, long long v_stride, const int* __restrict__ place,
-                 uint8_t* __restrict__ cache, int rows, int nkh, int hd, long long places, int* error_flag) {
+kv4_store_kernel(const StoreArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int per = hd / 8, W = hd / KV4_GROUP;               // lanes a (row, plane, kv head)
+    const int hd = a.hd, nkh = a.nkh, per = hd / 8, W = hd / KV4_GROUP;        // lanes a (row, plane, kv head)
     const long long it = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long heads = it / per;
     const int c8 = (int)(it - heads * per);                   // numbers 8 c8 .. 8 c8 + 7
@@ -163,19 +177,21 @@ kv4_store_kernel(const T* __restrict__ k, long long k_stride, const T* __restric
     const bool value = ph >= nkh;
     const int kvh = value ? ph - nkh : ph;
     const int w = c8 >> 2, j = c8 & 3;
-    long long at = -1;
-    if (row < rows) {
-        at = place[row];
-        if (at >= places) { if (c8 == 0) atomicExch(error_flag, 1); at = -1; }
-    }
+    int at = -1;
     float x[8];
     bool bad = false;
     float lo = INFINITY, hi = -INFINITY;
+    if (row < a.rows) {
+        at = a.place[row];
+        if (at >= 0) {
+            load8<T, WIDE>((value ? (const T*)a.v + row * a.v_stride : (const T*)a.k + row * a.k_stride) + (long long)kvh * hd + 8 * c8, x);
+            if (at / BRAID_PAGE_SIZE >= a.num_pages) { if (c8 == 0) atomicExch(a.error_flag, 1); at = -1; }
+        }
+    }
     if (at >= 0) {
-        load8<T, WIDE>((value ? v + row * v_stride : k + row * k_stride) + (long long)kvh * hd + 8 * c8, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = __bfloat162float(__float2bfloat16_rn(x[i]));
+            if (sizeof(T) == 4) x[i] = __bfloat162float(__float2bfloat16_rn(x[i]));
             bad |= x[i] != x[i];
             lo = fminf(lo, x[i]);
             hi = fmaxf(hi, x[i]);
@@ -194,13 +210,25 @@ kv4_store_kernel(const T* __restrict__ k, long long k_stride, const T* __restric
     const __nv_bfloat16 step16 = bad ? nan : __float2bfloat16_rn(span / 15.f);
     const float step = __bfloat162float(step16);
     uint32_t code[8];
+    if (step >= 1e-36f) {
+        const float inv = 1.f / step;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)                               // the quotient is rounded as IEEE has it: ties are ties in every form
-        code[i] = step > 0.f ? (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) : 0u;
+        for (int i = 0; i < 8; ++i) {
+            const float t = x[i] - lo;
+            const float u = fminf(t * inv, 15.f) + 12582912.f;                 // 1.5 2^23: the sum is a whole number, in its lowest bits
+            const float rem = fmaf(12582912.f - u, step, t);                   // t - code step
+            const int c = (int)(__float_as_uint(u) & 15u);
+            const float two = 2.f * fabsf(rem);
+            const int off = (two > step || (two == step && (c & 1))) ? (rem > 0.f ? 1 : -1) : 0;
+            code[i] = (uint32_t)min(c + off, 15);
+        }
+    } else {                                                   // no range (or NaN): code 0; or one that 1 / step would leave float32's with
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = step > 0.f ? (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) : 0u;
+    }
     const uint32_t group = (uint32_t)__bfloat16_as_ushort(step16) | ((uint32_t)__bfloat16_as_ushort(bad ? nan : __float2bfloat16_rn(lo)) << 16);
-    const long long page = at / BRAID_PAGE_SIZE;
-    const int off = (int)(at - page * BRAID_PAGE_SIZE), t = off % KV4_REC;
-    uint8_t* rec = cache + (page * nkh + kvh) * kv4_page_bytes(hd) + (off / KV4_REC) * kv4_record_bytes(hd);
+    const int page = at / BRAID_PAGE_SIZE, off = at % BRAID_PAGE_SIZE, t = off % KV4_REC;
+    uint8_t* rec = a.cache + ((long long)page * nkh + kvh) * kv4_page_bytes(hd) + (off / KV4_REC) * kv4_record_bytes(hd);
     if (!value) {
         uint32_t word = 0;
 #pragma unroll
@@ -215,17 +243,6 @@ kv4_store_kernel(const T* __restrict__ k, long long k_stride, const T* __restric
     if (j == 0) reinterpret_cast<uint32_t*>(rec + (value ? kv4_value_groups(hd) : kv4_key_groups(hd)))[t * W + w] = group;
 }
 
-template <typename T>
-static int launch_store(const void* k, long long ks, const void* v, long long vs, const int* place, void* cache, int rows, int nkh, int hd,
-                        long long places, int* flag, cudaStream_t s) {
-    const long long items = (long long)rows * 2 * nkh * (hd / 8), ctas = (items + 255) / 256;
-    if (ctas > 0x7fffffffLL) BRAID_REFUSE("kv4_store: the rows exceed the grid limit");
-    const bool wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)(ks * sizeof(T)) | (uintptr_t)(vs * sizeof(T))) & 15);
-    braid_launch(wide ? kv4_store_kernel<T, true> : kv4_store_kernel<T, false>, dim3((unsigned)ctas), dim3(256), 0, s, (const T*)k, ks, (const T*)v, vs,
-                 place, (uint8_t*)cache, rows, nkh, hd, places, flag);
-    BRAID_LAUNCH_CHECK();
-}
-
 static int kv4_check(const char* what, int nkh, int hd, const void* cache) {
     if (nkh <= 0) BRAID_REFUSE("%s: %d kv heads", what, nkh);
     if (hd <= 0 || hd % KV4_GROUP || hd > 256) BRAID_REFUSE("%s: heads of %d numbers; groups of %d up to 256 are taken", what, hd, KV4_GROUP);
@@ -233,38 +250,100 @@ static int kv4_check(const char* what, int nkh, int hd, const void* cache) {
     return BRAID_OK;
 }
 
-extern "C" int braid_kv4_store(const void* k, long long k_stride, const void* v, long long v_stride, int dtype, const int* place, void* cache,
-                               int rows, int nkh, int hd, int num_pages, int* error_flag, void* stream) {
-    if (rows <= 0) return BRAID_OK;
-    if (int rc = kv4_check("kv4_store", nkh, hd, cache)) return rc;
-    const long long places = (long long)num_pages * BRAID_PAGE_SIZE;
-    if (dtype == BRAID_F32) return launch_store<float>(k, k_stride, v, v_stride, place, cache, rows, nkh, hd, places, error_flag, (cudaStream_t)stream);
-    if (dtype == BRAID_BF16) return launch_store<__nv_bfloat16>(k, k_stride, v, v_stride, place, cache, rows, nkh, hd, places, error_flag, (cudaStream_t)stream);
-    BRAID_REFUSE("kv4_store: unknown dtype code %d", dtype);
+template <typename T>
+static int launch_store(const StoreArgs& a, cudaStream_t s) {
+    const long long items = (long long)a.rows * 2 * a.nkh * (a.hd / 8), ctas = (items + 255) / 256;
+    if (ctas > 0x7fffffffLL) BRAID_REFUSE("kv4_store: the rows exceed the grid limit");
+    const bool wide = !(((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)(a.k_stride * sizeof(T)) | (uintptr_t)(a.v_stride * sizeof(T))) & 15);
+    braid_launch(wide ? kv4_store_kernel<T, true> : kv4_store_kernel<T, false>, dim3((unsigned)ctas), dim3(256), 0, s, a);
+    BRAID_LAUNCH_CHECK();
+}
+
+extern "C" int braid_kv4_store(const StoreArgs* a, void* stream) {
+    if (a->rows <= 0) return BRAID_OK;
+    if (int rc = kv4_check("kv4_store", a->nkh, a->hd, a->cache)) return rc;
+    if (a->dtype == BRAID_F32) return launch_store<float>(*a, (cudaStream_t)stream);
+    if (a->dtype == BRAID_BF16) return launch_store<__nv_bfloat16>(*a, (cudaStream_t)stream);
+    BRAID_REFUSE("kv4_store: unknown dtype code %d", a->dtype);
 }
 
 // ------------------------------------------------------------------ reading back
 // The pages of a step's sequences as values, into pages [page][2][kv head][64][hd]: what a sequence's queries see (from its window's first
 // position, and its kept first ones, up to its new tokens); other places of those pages come out zero.  The
-// pages are numbered as the cache's, or (out_cols > 0) block c of sequence i is page i * out_cols + c.  A CTA takes one page of one kv
-// head.  A page belongs to one sequence.
+// pages are numbered as the cache's, or (out_cols > 0) block c of sequence i is page i * out_cols + c.  A page belongs to one sequence.
+//
+// A CTA takes one page of one kv head, four lanes a token: lane j reads the W neighbouring words that hold its numbers 32 w + 8 j .. + 7
+// (of a value: the two 16-bit words a group that do), so that codes and groups come in one wide load each and the values leave 16
+// bytes at a time.  Bytes bound it: the values that it writes are 3.2 times (bfloat16) the codes that it reads.
 struct ExpandArgs {
     const uint8_t* cache;
     void* out;
     const int* page_table;
     const int* q_len;
     const int* kv_before;
-    int nkh, hd, cols, num_pages, window, keep_first, out_cols;
     int* error_flag;
     int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [2 + seq0 + sequence] become 1
-    int seq0;
+    int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
 };
 
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, uint32_t* x) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(x + i) = reinterpret_cast<const uint4*>(p)[i / 4];
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint2*>(x + i) = reinterpret_cast<const uint2*>(p)[i / 2];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+
+// lowest + step * code of codes n (first) and 4 + n (second) of a word, n 0 .. 3
 template <typename T>
+struct Kv4Pairs;
+template <>
+struct Kv4Pairs<__nv_bfloat16> {
+    using Pair = uint32_t;
+    // one multiply-add of the pair in bfloat16: the code and 128 + code are exact, the sum is rounded once
+    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, uint32_t* y) {
+        const uint32_t s2 = __byte_perm(group, group, 0x1010), l2 = __byte_perm(group, group, 0x3232);
+        const __nv_bfloat162 base(__float2bfloat16(128.f), __float2bfloat16(128.f));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t c = ((word >> (4 * n)) & 0x000f000fu) | 0x43004300u;
+            const __nv_bfloat162 v = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), base), *reinterpret_cast<const __nv_bfloat162*>(&s2),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&l2));
+            y[n] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    static __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+    static __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+};
+template <>
+struct Kv4Pairs<float> {
+    using Pair = float2;
+    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, float2* y) {
+        const float step = kv4_step(group), low = kv4_lowest(group);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {                          // a code under the lowest bits of 2^23 is 2^23 + code
+            const float a = __uint_as_float(((word >> (4 * n)) & 15u) | 0x4b000000u) - 8388608.f;
+            const float b = __uint_as_float(((word >> (16 + 4 * n)) & 15u) | 0x4b000000u) - 8388608.f;
+            y[n] = make_float2(fmaf(step, a, low), fmaf(step, b, low));
+        }
+    }
+    static __device__ __forceinline__ float2 lows(float2 a, float2 b) { return make_float2(a.x, b.x); }
+    static __device__ __forceinline__ float2 highs(float2 a, float2 b) { return make_float2(a.y, b.y); }
+};
+
+template <typename T, int W>
 __global__ void __launch_bounds__(256)
-kv4_expand_kernel(ExpandArgs a) {
+kv4_expand_kernel(const ExpandArgs a) {
     pdl_trigger();
     pdl_wait();
+    constexpr int HD = 32 * W;
+    using P = typename Kv4Pairs<T>::Pair;
     const int c = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
     const int before = a.kv_before[seq], end = before + a.q_len[seq];
     const int key0 = c * BRAID_PAGE_SIZE;
@@ -277,61 +356,66 @@ kv4_expand_kernel(ExpandArgs a) {
         return;
     }
     const size_t out_page = a.out_cols > 0 ? (size_t)seq * a.out_cols + c : (size_t)page;
-    const int hd = a.hd, W = hd / KV4_GROUP, per = hd / 8;
-    const uint8_t* src = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(hd);
-    const int n_here = min(BRAID_PAGE_SIZE, end - key0);
-    for (int it = threadIdx.x; it < 2 * BRAID_PAGE_SIZE * per; it += 256) {
-        const int c8 = it % per, tp = it / per, t = tp % BRAID_PAGE_SIZE, value = tp / BRAID_PAGE_SIZE;
-        const int w = c8 >> 2, j = c8 & 3;
-        float x[8];
-        if (t < n_here && (key0 + t >= lo || key0 + t < a.keep_first)) {
-            const uint8_t* rec = src + (t / KV4_REC) * kv4_record_bytes(hd);
-            const int tr = t % KV4_REC;
-            const uint32_t group = reinterpret_cast<const uint32_t*>(rec + (value ? kv4_value_groups(hd) : kv4_key_groups(hd)))[tr * W + w];
-            float step = kv4_step(group), low = kv4_lowest(group);
-            if (value && a.repair && !(fabsf(step) + fabsf(low) < INFINITY)) {
-                step = low = 0.f;
-                a.repair[2 + a.seq0 + seq] = 1;
-                a.repair[0] = 1;
-            }
-            if (!value) {
-                const uint32_t word = reinterpret_cast<const uint32_t*>(rec + tr * (hd / 2))[j * W + w];
+    const int t = threadIdx.x >> 2, j = threadIdx.x & 3, tr = t % KV4_REC;
+    const uint8_t* rec = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t / KV4_REC) * kv4_record_bytes(HD);
+    const bool in = key0 + t < end && (key0 + t >= lo || key0 + t < a.keep_first);
+    T* dst = (T*)a.out + ((out_page * 2 * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * HD + 8 * j;
+    const size_t plane = (size_t)a.nkh * BRAID_PAGE_SIZE * HD;
+    uint32_t kc[W], kg[W], vc[W], vg[W];
+    load_words<W>(rec + tr * (HD / 2) + 4 * W * j, kc);
+    load_words<W>(rec + kv4_key_groups(HD) + 4 * W * tr, kg);
+    load_words<W>(rec + kv4_value_codes(HD) + tr * (HD / 2) + 4 * W * j, vc);
+    load_words<W>(rec + kv4_value_groups(HD) + 4 * W * tr, vg);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    x[2 * n] = fmaf(step, (float)((word >> (4 * n)) & 15u), low);
-                    x[2 * n + 1] = fmaf(step, (float)((word >> (16 + 4 * n)) & 15u), low);
-                }
-            } else {
-                const uint16_t* codes = reinterpret_cast<const uint16_t*>(rec + kv4_value_codes(hd) + tr * (hd / 2));
-                const uint32_t word = codes[2 * j * W + w] | ((uint32_t)codes[(2 * j + 1) * W + w] << 16);
-#pragma unroll
-                for (int n = 0; n < 8; ++n) x[n] = fmaf(step, (float)((word >> (4 * n)) & 15u), low);
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = 0.f;
+    for (int w = 0; w < W; ++w) {
+        if (!in) kc[w] = kg[w] = vg[w] = 0u;                   // a group of step 0 and lowest value 0
+        // the 16 bits of group w in the lane's first and second half of value words
+        const int h0 = w, h1 = W + w;
+        const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
+        const uint32_t both = in ? v0 | (v1 << 16) : 0u;
+        if (a.repair && ((vg[w] & 0x7f80u) == 0x7f80u || (vg[w] & 0x7f800000u) == 0x7f800000u)) {
+            vg[w] = 0u;
+            a.repair[2 + a.seq0 + seq] = 1;
+            a.repair[0] = 1;
         }
-        T* dst = (T*)a.out + (((out_page * 2 + value) * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * hd + 8 * c8;
-        constexpr int VW = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 8; i += VW) store_run<T, VW>(dst + i, x + i);
+        __align__(16) P y[4];
+        P z[4];
+        Kv4Pairs<T>::make(kc[w], kg[w], y);                    // pairs of neighbours, in order
+        *reinterpret_cast<uint4*>(dst + 32 * w) = *reinterpret_cast<const uint4*>(y);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
+        Kv4Pairs<T>::make(both, vg[w], z);                     // numbers n and 4 + n
+        y[0] = Kv4Pairs<T>::lows(z[0], z[1]);
+        y[1] = Kv4Pairs<T>::lows(z[2], z[3]);
+        y[2] = Kv4Pairs<T>::highs(z[0], z[1]);
+        y[3] = Kv4Pairs<T>::highs(z[2], z[3]);
+        *reinterpret_cast<uint4*>(dst + plane + 32 * w) = *reinterpret_cast<const uint4*>(y);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + plane + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
     }
 }
 
-extern "C" int braid_kv4_expand(const void* cache, void* out, int dtype, const int* page_table, const int* q_len, const int* kv_before,
-                                int n_seqs, int cols, int nkh, int hd, int num_pages, int window, int keep_first, int out_cols, int* repair,
-                                int seq0, int* error_flag, void* stream) {
-    if (n_seqs <= 0 || cols <= 0) return BRAID_OK;
-    if (int rc = kv4_check("kv4_expand", nkh, hd, cache)) return rc;
-    if ((uintptr_t)out & 15) BRAID_REFUSE("kv4_expand: the pages must start on 16 bytes");
-    if (nkh > 65535 || n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", nkh, n_seqs);
-    ExpandArgs a{(const uint8_t*)cache, out, page_table, q_len, kv_before, nkh, hd, cols, num_pages, window, window > 0 ? keep_first : 0, out_cols, error_flag, repair, seq0};
-    const dim3 grid(out_cols > 0 ? min(cols, out_cols) : cols, nkh, n_seqs);
-    if (dtype == BRAID_F32) braid_launch(kv4_expand_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, a);
-    else if (dtype == BRAID_BF16) braid_launch(kv4_expand_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
-    else BRAID_REFUSE("kv4_expand: unknown dtype code %d", dtype);
+template <typename T>
+static int launch_expand(const ExpandArgs& a, cudaStream_t s) {
+    const dim3 grid(a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols, a.nkh, a.n_seqs);
+    void (*const kernels[8])(const ExpandArgs) = {kv4_expand_kernel<T, 1>, kv4_expand_kernel<T, 2>, kv4_expand_kernel<T, 3>, kv4_expand_kernel<T, 4>,
+                                                  kv4_expand_kernel<T, 5>, kv4_expand_kernel<T, 6>, kv4_expand_kernel<T, 7>, kv4_expand_kernel<T, 8>};
+    braid_launch(kernels[a.hd / KV4_GROUP - 1], grid, dim3(256), 0, s, a);
     BRAID_LAUNCH_CHECK();
 }
+
+extern "C" int braid_kv4_expand(const ExpandArgs* args, void* stream) {
+    ExpandArgs a = *args;
+    if (a.n_seqs <= 0 || a.cols <= 0) return BRAID_OK;
+    if (int rc = kv4_check("kv4_expand", a.nkh, a.hd, a.cache)) return rc;
+    if ((uintptr_t)a.out & 15) BRAID_REFUSE("kv4_expand: the pages must start on 16 bytes");
+    if (a.nkh > 65535 || a.n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", a.nkh, a.n_seqs);
+    if (a.window <= 0) a.window = a.keep_first = 0;
+    if (a.dtype == BRAID_F32) return launch_expand<float>(a, (cudaStream_t)stream);
+    if (a.dtype == BRAID_BF16) return launch_expand<__nv_bfloat16>(a, (cudaStream_t)stream);
+    BRAID_REFUSE("kv4_expand: unknown dtype code %d", a.dtype);
+}
+
+// Bytes of the argument structures: tables, write, reading back.
+extern "C" int braid_kv4_args_bytes(int which) { return which == 0 ? (int)sizeof(TablesArgs) : which == 1 ? (int)sizeof(StoreArgs) : (int)sizeof(ExpandArgs); }
 
 // ------------------------------------------------------------------ plain attention
 // One warp per (row, query head), 32 keys at a time: a lane a key for the scores, a lane a number of the head for the values.  All

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import plain_kv4 as P
-from braidinfer_b200.csrc.api import KernelError, get_kernels
+from braidinfer_b200.csrc.api import KernelError, Kernels, get_kernels
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -23,6 +23,13 @@ U = 2.0 ** -24
 @pytest.fixture(scope="module")
 def K():
     return get_kernels(verbose=False)
+
+
+@pytest.fixture(params=["auto", "pages"])
+def route(request, monkeypatch):
+    """Prompts as the sizes have it (here: over 4 bits), and over pages read back."""
+    if request.param == "pages":
+        monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
 
 
 def gen(seed):
@@ -270,20 +277,20 @@ def test_options(K, name, dt, backend):
 @pytest.mark.parametrize("seqs, nqh, nkh, hd", [
     ([(9, 0)], 4, 2, 64), ([(130, 0), (17, 200)], 8, 2, 128), ([(64, 64), (1, 500), (0, 9), (33, 31)], 3, 1, 32), ([(70, 5)], 20, 1, 96), ([(40, 100)], 2, 2, 256),
     ([(12, 1000)], 6, 1, 160)])
-def test_prompts(K, seqs, nqh, nkh, hd, dt):
+def test_prompts(K, route, seqs, nqh, nkh, hd, dt):
     Case(K, seqs, nqh, nkh, hd, dt).check(K)
 
 
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("name", OPTIONS)
-def test_options_of_prompts(K, name, dt):
+def test_options_of_prompts(K, route, name, dt):
     c = Case(K, [(50, 100), (90, 0), (1, 300)], 4, 2, 64, dt)
     c.check(K, **options(name, c.rows, c.nqh, dt))
 
 
 @pytest.mark.parametrize("new", [1, 6, 40])
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
-def test_what_is_not_seen_does_not_count(K, dt, new):
+def test_what_is_not_seen_does_not_count(K, route, dt, new):
     """NaN in places behind the sequence's end and before its window, and in pages that no sequence holds; the values of a sequence
     whose own keys hold a NaN are NaN, and its neighbour's are not."""
     c = Case(K, [(new, 150), (new, 90)], 4, 2, 64, dt)
@@ -319,7 +326,7 @@ def test_what_is_not_seen_does_not_count(K, dt, new):
 
 @pytest.mark.parametrize("backend", ["plain", "auto"])
 @pytest.mark.parametrize("new", [1, 30])
-def test_absent_pages_are_flagged(K, new, backend):
+def test_absent_pages_are_flagged(K, route, new, backend):
     c = Case(K, [(new, 100)], 4, 2, 64, BF)
     for page in (-1, c.num, 1 << 30):
         c.table[0, 0] = page
@@ -374,7 +381,7 @@ def test_values_of_all_sizes(K, name, dt):
 
 @pytest.mark.parametrize("seqs", [[(1, 9000), (1, 10), (1, 4000)], [(4, 5000)], [(33, 3000)]])
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
-def test_long_contexts_slices_and_repeats(K, seqs, dt):
+def test_long_contexts_slices_and_repeats(K, route, seqs, dt):
     c = Case(K, seqs, 8, 2, 64, dt)
     out = c.check(K)
     assert torch.equal(c.run(K), out)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import plain_kv4 as P
-from braidinfer_b200.csrc import build
+from braidinfer_b200.csrc import api, build
 from braidinfer_b200.csrc.api import KernelError, Kernels
 
 
@@ -108,15 +108,15 @@ def test_entry_points_refuse(K):
     lib = K.part_library("kv4")
     b = (ctypes.c_int * 64)()
     p = ctypes.addressof(b)
+    even = p - p % 16
+    tables = lambda n=2, listed=4, rows=4, cols=4, pages=9: lib.braid_step_tables(api._TABLES_ARGS.pack(*[p] * 5, 0, 0, 0, n, listed, rows, cols, pages, p), None)
     # more requests than the tables' shared memory holds; places past 32 bits
-    assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 20000, 4, 4, 4, 9, p, None) == -1
-    assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 2, 4, 4, 4, 1 << 26, p, None) == -1
-    assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 2, 4, -1, 4, 9, p, None) == -1
-    assert lib.braid_kv4_store(p, 128, p, 128, 0, p, p - p % 16 + 4, 3, 2, 64, 5, p, None) == -1          # a cache off its 16 bytes
-    assert lib.braid_kv4_store(p, 128, p, 128, 7, p, p - p % 16, 3, 2, 64, 5, p, None) == -1
-    assert lib.braid_kv4_expand(p - p % 16, p - p % 16, 0, p, p, p, 70000, 3, 2, 64, 5, 0, 0, 0, None, 0, p, None) == -1
+    assert tables(n=20000) == tables(pages=1 << 26) == tables(rows=-1) == -1
+    store = lambda at=even, rows=3, kind=0, hd=64, kv=2: lib.braid_kv4_store(api._STORE_ARGS.pack(p, p, p, at, p, 128, 128, rows, kv, hd, 5, kind), None)
+    assert store(at=even + 4) == store(kind=7) == store(hd=48) == store(hd=288) == store(kv=0) == -1
+    expand = lambda at=even, n=2, kind=0: lib.braid_kv4_expand(api._EXPAND_ARGS.pack(even, at, p, p, p, p, 0, n, 2, 64, 3, 5, 0, 0, 0, 0, kind), None)
+    assert expand(at=even + 8) == expand(kind=5) == -1 and expand(n=70000) == -1
     assert b"grid" in lib.braid_last_error()
     # nothing to do is no error
-    assert lib.braid_step_tables(p, p, p, p, p, None, None, None, 0, 0, 0, 4, 9, p, None) == 0
-    assert lib.braid_kv4_store(p, 128, p, 128, 0, p, p, 0, 2, 64, 5, p, None) == 0
+    assert tables(n=0, listed=0, rows=0) == store(rows=0) == expand(n=0) == 0
     assert build.page_size() == P.PAGE
