@@ -2,18 +2,19 @@
 //
 // softmax over the visible keys of scale * q . k_j, with k_j = lowest + step * code a group of 32 numbers, so that
 //   q . k_j = sum over groups g of  step_jg (q_g . code_jg) + lowest_jg sum(q_g)
-//   out     = sum over keys of  (p_j step_jg) code_jg + sum over keys of p_j lowest_jg        (for the numbers of group g)
-// The codes themselves are the tensor cores' operand (mma.sync m16n8k16, bfloat16, float32 sums): a mask and an "or" turn
-// two of them into the bfloat16 pair 128 + code, exact, straight from the bytes as they are stored; the 128 comes off through
-// sum(q_g) for the keys and by a subtraction for the values.  So neither keys nor values are ever rounded, and what scales them is applied
-// to a group's sums (keys) or to the probabilities (values).  Keys and value columns are the 16 rows of a product and the
+//   out     = sum over keys of  (p_j step_jg) (code_jg - 8) + sum over keys of p_j (lowest_jg + 8 step_jg)     (for the numbers of group g)
+// (codes less 8: both sums are then about as small as the result.  With the codes as they are, each was some 2 standard deviations of the values
+// and the result what was left of them: errors of 0.0046 of the result in bfloat16 and 7e-6 in float32 behind 128k and 3k tokens.)
+// The codes themselves are the tensor cores' operand (mma.sync m16n8k16, float32 sums): a mask makes two of them a pair of 16-bit
+// numbers, exact, straight from the bytes as they are stored (`codes`).  So neither keys nor values are ever rounded, and what scales
+// them is applied to a group's sums (keys) or to the probabilities (values).  Keys and value columns are the 16 rows of a product and the
 // queries its 8 columns (query heads of one kv head, of up to 8 tokens), so that few queries waste little.
 //
 // What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
 // shifts are half.  Every warp walks units of 32 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
 // (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
 // and results; a context longer than that is sliced over CTAs, whose results a second kernel merges.
-// The running maximum of a column is raised only when a unit's scores exceed it by more than 8 (in powers of two): a vote instead
+// The running maximum of a column is raised only when a unit's scores exceed it by more than 4 (in powers of two): a vote instead
 // of a reduction over the warp; sums are taken against the same maximum, so nothing is lost.
 //
 // float32 runs (PARTS 3): queries and scaled probabilities are three bfloat16 numbers each, whose products with the codes are exact, so
@@ -21,6 +22,7 @@
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 #include "softcap.cuh"
+#include <cuda_fp16.h>
 #include <type_traits>
 
 #ifndef BRAID_HD
@@ -51,7 +53,7 @@ struct Kv4Args {
 };
 
 #define LOG2E 1.4426950408889634f
-#define KV4_RAISE 8.f
+#define KV4_RAISE 4.f
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -59,6 +61,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -76,18 +83,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-// Codes n and 4 + n of a word as a bfloat16 pair.  FAST: the code's bits are left where they are and read as a bfloat16 number below
-// the normal ones (or just at their start): the lowest 8 bits of that format count in steps of 2^-133, so the pair is
-// the codes times 2^-133, or 2^-129 for odd n, in one instruction (and a shift for two of four).  The products' other operand is
-// scaled up by a power of two instead, and the results are scaled back.  (With 128 added to the code, the usual way, a code took 1.75
-// instructions and the 128 had to be taken off again: 64 requests of 8k 167 us.)  Otherwise: the codes themselves.
+// Codes n and 4 + n of a word as a pair of 16-bit numbers.  FAST: the code's bits are left where they are and read as a number below
+// the normal ones (or just at their start): the lowest 8 bits of bfloat16 count in steps of 2^-133, the lowest 11 of float16 in
+// steps of 2^-24, so the pair is the codes times that, or 16 times that for odd n, in one instruction (and a shift for two of four).
+// The products' other operand is scaled up by a power of two instead, and the results are scaled back.  (With 128 added to the code, the usual
+// way, a code took 1.75 instructions and the 128 had to be taken off again: 64 requests of 8k 167 us instead of 140.)  Otherwise: the
+// codes less 8, as they are, in bfloat16.
 #define KV4_UNIT 133
 template <bool FAST, int N> __device__ __forceinline__ uint32_t codes(uint32_t x) {
     if constexpr (FAST) {
         return (N & 2 ? x >> 8 : x) & (N & 1 ? 0x00f000f0u : 0x000f000fu);
     } else {
         const uint32_t y = ((x >> (4 * N)) & 0x000f000fu) | 0x43004300u;
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(128.f), __float2bfloat16(128.f)));
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), __nv_bfloat162(__float2bfloat16(136.f), __float2bfloat16(136.f)));
         return *reinterpret_cast<const uint32_t*>(&r);
     }
 }
@@ -113,6 +121,10 @@ __device__ __forceinline__ void lds_words(const void* p, uint32_t* x) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = reinterpret_cast<const uint32_t*>(p)[i];
     }
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 // a bfloat16 pair from two float32 numbers, and what the rounding leaves
 __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
@@ -283,10 +295,15 @@ attn_kv4_kernel(const Kv4Args a) {
 
     float o[NT][2 * W][4], zs[NT][2][W], m[NT][2], l[NT][2];
     bool ok = true;
-    int st = 0, p_exp = 0;                                     // the probabilities are scaled by 2^p_exp
+    bool walked = PARTS == 1;
+    int st = 0, step_exp[W];                                   // FAST: the steps of a group are scaled by 2^step_exp
     uint32_t phase = 0;
-    // Probabilities that are scaled up may pass the range of float32 where later values are much larger than the first unit's: the results
-    // are then not finite, and the warp walks once more with the codes as whole numbers and nothing scaled.
+#pragma unroll
+    for (int w = 0; w < W; ++w) step_exp[w] = 0;
+    // FAST takes the scaled probabilities as float16 numbers: they are rounded by 2^-11 (a code counts up to 15 steps, which with the 2^-8 of
+    // bfloat16 made errors of 0.0046 of the result), and pass the type's range where a group's later steps are much larger than its
+    // first ones (2^7 times, at a probability of 1; at the other end, steps of down to 2^-23 of those keep all 11 bits): the results are
+    // then not finite, and the warp walks once more in bfloat16, codes less 8 and nothing scaled.
     auto walk = [&](auto FAST) {
     constexpr bool fast = decltype(FAST)::value;
 #pragma unroll
@@ -308,8 +325,10 @@ attn_kv4_kernel(const Kv4Args a) {
         if (++st == ST) { st = 0; phase ^= 1u; }
         const int unit_key0 = tile_of(k) * C::US;
         if (fast && k == 0) {
-            // the scale: values of the first unit's largest size, times the largest probability and the most keys, stay in range
-            float most = 0.f;
+            // a group's scale: its largest step in the first unit, times a probability of 1, becomes one of 2^9
+            float most[GH];
+#pragma unroll
+            for (int h = 0; h < GH; ++h) most[h] = 0.f;
 #pragma unroll
             for (int rec = 0; rec < SR * PU; ++rec)
 #pragma unroll
@@ -317,11 +336,21 @@ attn_kv4_kernel(const Kv4Args a) {
                     const int key = unit_key0 + 16 * rec + 8 * h + r;
                     const uint32_t* g = reinterpret_cast<const uint32_t*>(unit_base + rec * kv4_record_bytes(HD) + kv4_value_groups(HD)) + (8 * h + r) * W;
                     if (key <= pos_max && (key >= k_lo || key < a.keep_first))
-                        for (int w = j; w < W; w += 4) most = fmaxf(most, fmaxf(fabsf(kv4_lowest(g[w])), 16.f * kv4_step(g[w])));
+#pragma unroll
+                        for (int i = 0; i < GH; ++i)
+                            if (4 * i + j < W) most[i] = fmaxf(most[i], kv4_step(g[4 * i + j]));
                 }
-            const int e = exponent(warp_max(most));
-            p_exp = min(90 - e, 100);
-            if (e < -40) { p_exp = 1000; return; }             // very small values: walk with nothing scaled
+            bool in = true;
+#pragma unroll
+            for (int i = 0; i < GH; ++i) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], x));
+                const int e = most[i] == 0.f ? 100 : 9 - exponent(most[i]);
+                in &= e >= 0 && e <= 100;
+#pragma unroll
+                for (int w = 4 * i; w < W && w < 4 * i + 4; ++w) step_exp[w] = __shfl_sync(0xffffffffu, e, w & 3);
+            }
+            if (!__all_sync(0xffffffffu, in)) { walked = false; return; }
         }
 
 #pragma unroll 1
@@ -483,12 +512,15 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int c = e & 1;
-                    p[nt][e] = exp2_ftz(s[rec][nt][e] - ((m[nt][c] == -INFINITY ? 0.f : m[nt][c]) - (float)p_exp));
+                    p[nt][e] = exp2_ftz(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
                     l[nt][c] += p[nt][e];
                 }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]), za = kv4_lowest(ga[w]), zb = kv4_lowest(gb[w]);
+                // (a step of 0 becomes some number below the codes' reach; its codes are 0)
+                const float sa = __uint_as_float(ga[w] * 65536u + (fast ? (uint32_t)step_exp[w] << 23 : 0u));
+                const float sb = __uint_as_float(gb[w] * 65536u + (fast ? (uint32_t)step_exp[w] << 23 : 0u));
+                const float za = fast ? kv4_lowest(ga[w]) : fmaf(8.f, sa, kv4_lowest(ga[w])), zb = fast ? kv4_lowest(gb[w]) : fmaf(8.f, sb, kv4_lowest(gb[w]));
                 const uint32_t a0 = codes<fast, 0>(v01[w]), a1 = codes<fast, 1>(v01[w]), a2 = codes<fast, 0>(v89[w]), a3 = codes<fast, 1>(v89[w]);
                 const uint32_t b0 = codes<fast, 2>(v01[w]), b1 = codes<fast, 3>(v01[w]), b2 = codes<fast, 2>(v89[w]), b3 = codes<fast, 3>(v89[w]);
 #pragma unroll
@@ -505,11 +537,17 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) zs[nt][e & 1][w] = fmaf(p[nt][e], e < 2 ? za : zb, zs[nt][e & 1][w]);
                     }
+                    if constexpr (fast) {
+                        const uint32_t p0 = transpose8x8(pack_half(x[0], x[1])), p1 = transpose8x8(pack_half(x[2], x[3]));
+                        mma16816_f16(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
+                        mma16816_f16(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
+                    } else {
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
-                        const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
-                        mma16816(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
-                        mma16816(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
+                        for (int part = 0; part < PARTS; ++part) {
+                            const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
+                            mma16816(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
+                            mma16816(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
+                        }
                     }
                 }
             }
@@ -522,10 +560,9 @@ attn_kv4_kernel(const Kv4Args a) {
         if (issued < n_mine) issue();
     }
     };
-    walk(std::true_type{});
-    int even = KV4_UNIT, odd = KV4_UNIT - 4;                   // codes counted in steps of 2^-133, numbers of odd n in steps 16 times that
+    if constexpr (PARTS == 1) walk(std::true_type{});
     {
-        float t = p_exp > 100 ? INFINITY : 0.f;
+        float t = walked ? 0.f : INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -538,12 +575,14 @@ attn_kv4_kernel(const Kv4Args a) {
             }
         }
         if (__any_sync(0xffffffffu, ok && t != 0.f)) {
-            for (; st != istage; phase ^= (st == ST - 1), st = st == ST - 1 ? 0 : st + 1)        // (units asked for and not walked)
+            if constexpr (PARTS == 1) for (; st != istage; phase ^= (st == ST - 1), st = st == ST - 1 ? 0 : st + 1)        // (units asked for and not walked)
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag)) && ok;
-            issued = p_exp = 0;
-            while (issued < min(ST, n_mine)) issue();
+            if constexpr (PARTS == 1) {
+                issued = 0;
+                while (issued < min(ST, n_mine)) issue();
+            }
             walk(std::false_type{});
-            even = odd = 0;
+            walked = false;
         }
     }
     if (!ok) {
@@ -567,7 +606,6 @@ attn_kv4_kernel(const Kv4Args a) {
                 for (int w = 0; w < W; ++w) zs[nt][c][w] += __shfl_xor_sync(0xffffffffu, zs[nt][c][w], x);
             }
     __syncthreads();                                           // every warp is done with its ring
-    const float back = pow2(-p_exp);
     float* mo = reinterpret_cast<float*>(smem);                // [warp][column][HD]
     float* ml = mo + NW * C::BM * HD;                          // [warp][column][2]
 #pragma unroll
@@ -578,10 +616,14 @@ attn_kv4_kernel(const Kv4Args a) {
             float* dst = mo + (warp * C::BM + col) * HD + 4 * r;
 #pragma unroll
             for (int w = 0; w < W; ++w)
+            {
+                // FAST: codes counted in steps of 2^-24, those of odd n in steps 16 times that
+                const int even = walked ? 24 - step_exp[w] : 0, odd = walked ? even - 4 : 0;
                 *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(
-                    (scaled(o[nt][2 * w][c], even) + zs[nt][c][w]) * back, (scaled(o[nt][2 * w][2 + c], odd) + zs[nt][c][w]) * back,
-                    (scaled(o[nt][2 * w + 1][c], even) + zs[nt][c][w]) * back, (scaled(o[nt][2 * w + 1][2 + c], odd) + zs[nt][c][w]) * back);
-            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c] * back; }
+                    fmaf(o[nt][2 * w][c], pow2(even), zs[nt][c][w]), fmaf(o[nt][2 * w][2 + c], pow2(odd), zs[nt][c][w]),
+                    fmaf(o[nt][2 * w + 1][c], pow2(even), zs[nt][c][w]), fmaf(o[nt][2 * w + 1][2 + c], pow2(odd), zs[nt][c][w]));
+            }
+            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c]; }
         }
     __syncthreads();
     const bool out_wide = !(((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) & (4 * sizeof(T) - 1));
