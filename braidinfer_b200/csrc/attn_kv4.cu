@@ -11,7 +11,7 @@
 // queries its 8 columns (query heads of one kv head, of up to 8 tokens), so that few queries waste little.
 //
 // What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
-// shifts are half.  Every warp walks units of 32 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
+// shifts are half.  Every warp walks units of 32 or 64 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
 // (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
 // and results; a context longer than that is sliced over CTAs, whose results a second kernel merges.
 // The running maximum of a column is raised only when a unit's scores exceed it by more than 4 (in powers of two): a vote instead
@@ -134,11 +134,11 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     return w;
 }
 
-template <int PARTS, int NT, int NW, int SR, int PU, int ST>
+template <int PARTS, int NT, int NW, int SR, int ST>
 struct Kv4Cfg {
     static constexpr int HD = BRAID_HD, W = HD / 32;
-    static constexpr int US = 16 * SR * PU;                  // tokens a unit: PU turns of SR records
-    static constexpr int SB = SR * PU * kv4_record_bytes(HD);   // bytes a unit
+    static constexpr int US = 16 * SR;                       // tokens a unit
+    static constexpr int SB = SR * kv4_record_bytes(HD);     // bytes a unit
     static constexpr int BM = 8 * NT;                        // columns a CTA
     static constexpr int RING = NW * ST * SB;
     static constexpr int MERGE = NW * BM * (HD + 4) * 4;
@@ -146,10 +146,10 @@ struct Kv4Cfg {
     static_assert(BRAID_PAGE_SIZE % US == 0, "a unit must not straddle a page");
 };
 
-template <int PARTS, int NT, int NW, int SR, int PU, int ST>
-__global__ void __launch_bounds__(NW * 32)
+template <int PARTS, int NT, int NW, int SR, int ST>
+__global__ void __launch_bounds__(NW * 32, SR == 4 ? 2 : 1)
 attn_kv4_kernel(const Kv4Args a) {
-    using C = Kv4Cfg<PARTS, NT, NW, SR, PU, ST>;
+    using C = Kv4Cfg<PARTS, NT, NW, SR, ST>;
     using T = typename std::conditional<PARTS == 3, float, __nv_bfloat16>::type;
     constexpr int HD = C::HD, W = C::W;
     pdl_trigger();
@@ -225,7 +225,8 @@ attn_kv4_kernel(const Kv4Args a) {
     // ---- queries: column nt * 8 + r, numbers 32 w + 8 j .. + 7 of the head
     uint32_t q[NT][W][PARTS][4];
     constexpr int GH = W > 4 ? 2 : 1;
-    uint32_t qb[NT][3][GH];                                    // the sum of group j's (and 4 + j's) numbers beside a zero, in three parts
+    constexpr int QP = PARTS > 1 ? 3 : 2;                      // 16 bits of it, or all
+    uint32_t qb[NT][QP][GH];                                   // the sum of group j's (and 4 + j's) numbers beside a zero, in parts
     int q_exp[NT];                                             // of columns nt * 8 + r: the queries are scaled by 2^q_exp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -275,7 +276,7 @@ attn_kv4_kernel(const Kv4Args a) {
         for (int h = 0; h < GH; ++h) {
             float none = 0.f, sum = scaled(sums[h], q_exp[nt] - KV4_UNIT);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) qb[nt][p][h] = split_pair(none, sum);
+            for (int p = 0; p < QP; ++p) qb[nt][p][h] = split_pair(none, sum);
         }
     }
     // ---- this lane's columns of scores: nt * 8 + 2 j + c
@@ -293,6 +294,14 @@ attn_kv4_kernel(const Kv4Args a) {
                                KV4_UNIT - __shfl_sync(0xffffffffu, q_exp[nt], 8 * j + 4 * c));
         }
 
+    // a factor that is positive commutes with the maximum, and leaves -infinity as it is
+    bool late = !(a.softcap > 0.f) && !a.bias_slope;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) late = late && sc[nt][0] > 0.f && sc[nt][1] > 0.f;
+    late = __all_sync(0xffffffffu, late);
+    float lf[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { lf[nt][0] = late ? sc[nt][0] : 1.f; lf[nt][1] = late ? sc[nt][1] : 1.f; }
     float o[NT][2 * W][4], zs[NT][2][W], m[NT][2], l[NT][2];
     bool ok = true;
     bool walked = PARTS == 1;
@@ -321,20 +330,20 @@ attn_kv4_kernel(const Kv4Args a) {
     for (int k = 0; k < n_mine; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag));
         if (!ok) break;
-        const uint8_t* unit_base = ring + st * C::SB;
+        const uint8_t* base = ring + st * C::SB;
         if (++st == ST) { st = 0; phase ^= 1u; }
-        const int unit_key0 = tile_of(k) * C::US;
+        const int key0 = tile_of(k) * C::US;
         if (fast && k == 0) {
             // a group's scale: its largest step in the first unit, times a probability of 1, becomes one of 2^9
             float most[GH];
 #pragma unroll
             for (int h = 0; h < GH; ++h) most[h] = 0.f;
 #pragma unroll
-            for (int rec = 0; rec < SR * PU; ++rec)
+            for (int rec = 0; rec < SR; ++rec)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int key = unit_key0 + 16 * rec + 8 * h + r;
-                    const uint32_t* g = reinterpret_cast<const uint32_t*>(unit_base + rec * kv4_record_bytes(HD) + kv4_value_groups(HD)) + (8 * h + r) * W;
+                    const int key = key0 + 16 * rec + 8 * h + r;
+                    const uint32_t* g = reinterpret_cast<const uint32_t*>(base + rec * kv4_record_bytes(HD) + kv4_value_groups(HD)) + (8 * h + r) * W;
                     if (key <= pos_max && (key >= k_lo || key < a.keep_first))
 #pragma unroll
                         for (int i = 0; i < GH; ++i)
@@ -353,12 +362,7 @@ attn_kv4_kernel(const Kv4Args a) {
             if (!__all_sync(0xffffffffu, in)) { walked = false; return; }
         }
 
-#pragma unroll 1
-        for (int turn = 0; turn < PU; ++turn) {
-        const uint8_t* base = unit_base + turn * (SR * kv4_record_bytes(HD));
-        const int key0 = unit_key0 + turn * (16 * SR);
-        if (PU > 1 && (key0 > pos_max || (key0 + 16 * SR <= k_lo && key0 >= a.keep_first))) continue;
-        // ---- scores of the turn's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
+        // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
         float s[SR][NT][4];
 #pragma unroll
         for (int rec = 0; rec < SR; ++rec) {
@@ -383,7 +387,7 @@ attn_kv4_kernel(const Kv4Args a) {
             for (int nt = 0; nt < NT; ++nt) {
                 mma16816_zero(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][0][0], GH > 1 ? qb[nt][0][GH - 1] : 0u);
 #pragma unroll
-                for (int p = 1; p < 3; ++p) mma16816(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][p][0], GH > 1 ? qb[nt][p][GH - 1] : 0u);
+                for (int p = 1; p < QP; ++p) mma16816(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][p][0], GH > 1 ? qb[nt][p][GH - 1] : 0u);
             }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -406,13 +410,14 @@ attn_kv4_kernel(const Kv4Args a) {
                 }
             }
         }
-        // ---- factors, cap, bias; mask
+        // ---- factors, cap, bias; mask.  Plain scores are left as they are: their factor is applied where the exponential is taken
+        if (!late)
 #pragma unroll
-        for (int rec = 0; rec < SR; ++rec)
+            for (int rec = 0; rec < SR; ++rec)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[rec][nt][e] *= sc[nt][e & 1];
+                    for (int e = 0; e < 4; ++e) s[rec][nt][e] *= sc[nt][e & 1];
         if (a.softcap > 0.f) softcap_scores<SR * NT * 4>(&s[0][0][0], 1.f, a.softcap * LOG2E);
         if (a.bias_slope) {
 #pragma unroll
@@ -431,7 +436,7 @@ attn_kv4_kernel(const Kv4Args a) {
                 }
         }
         // (columns that are no query see as much as the others, and nobody reads them)
-        const bool edge = !(key0 + 16 * SR - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
+        const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
         if (edge) {
 #pragma unroll
             for (int rec = 0; rec < SR; ++rec)
@@ -453,6 +458,7 @@ attn_kv4_kernel(const Kv4Args a) {
                 float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
 #pragma unroll
                 for (int rec = 1; rec < SR; ++rec) x = fmaxf(x, fmaxf(s[rec][nt][c], s[rec][nt][2 + c]));
+                x *= lf[nt][c];
                 top[nt][c] = x;
                 raise |= x > m[nt][c] + KV4_RAISE;
             }
@@ -512,7 +518,7 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int c = e & 1;
-                    p[nt][e] = exp2_ftz(s[rec][nt][e] - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));
+                    p[nt][e] = exp2_ftz(fmaf(s[rec][nt][e], lf[nt][c], m[nt][c] == -INFINITY ? 0.f : -m[nt][c]));
                     l[nt][c] += p[nt][e];
                 }
 #pragma unroll
@@ -555,7 +561,6 @@ attn_kv4_kernel(const Kv4Args a) {
         };
         if (edge || !fast) values(std::true_type{});
         else values(std::false_type{});
-        }
         __syncwarp();                                          // every lane has read the unit
         if (issued < n_mine) issue();
     }
@@ -725,18 +730,18 @@ attn_kv4_merge_kernel(const Kv4Args a) {
 }
 
 // ------------------------------------------------------------------ host side
-// Four warps a CTA.  A turn takes SR records of 16 tokens: four of them give a warp enough independent products to work on (one request of
-// 128k, heads of 128: 53 us with two records a turn and 12 warps an SM, 45 with four and 8); two where the registers hold no more: 16
-// columns, float32, heads above 128.
+// Four warps a CTA.  A unit is SR records of 16 tokens: four of them give a warp enough independent products to work on (one request of
+// 128k, heads of 128: 53 us with two records a unit and 12 warps an SM, 45 with four and 8, which may take 255 registers then; 54 with
+// 12 warps of four records in parts that come and go by themselves); two where the registers hold no more: 16 columns, float32, heads
+// above 128.
 #define KV4_NW 4
-#define KV4_PU 1
 #define KV4_NT_MAX (BRAID_HD > 128 ? 1 : 2)
 constexpr int kv4_sr(int parts, int nt) { return BRAID_HD <= 128 && parts == 1 && nt == 1 ? 4 : 2; }
 constexpr int kv4_st(int parts, int nt) { return kv4_sr(parts, nt) == 4 || BRAID_HD > 128 ? 2 : 3; }
-template <int PARTS, int NT> using Kv4C = Kv4Cfg<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>;
+template <int PARTS, int NT> using Kv4C = Kv4Cfg<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>;
 
 template <int PARTS, int NT>
-static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>; }
+static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>; }
 
 template <int PARTS, int NT>
 static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
@@ -752,7 +757,7 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
     if (gz > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld tiles, %d heads, %d sequences)", gz, a.nkh * hchunks, a.n_seqs);
     if (gz == 0) return BRAID_OK;
-    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), KV4_PU, kv4_st(PARTS, NT)>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
+    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
     BRAID_LAUNCH_CHECK();
 }
 
