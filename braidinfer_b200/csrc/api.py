@@ -140,7 +140,7 @@ class RowScale:
 
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
-_KV4_ARGS = struct.Struct("<15Q3q12i4f2i")
+_KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<7Q10i")
 
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
@@ -905,7 +905,7 @@ class Kernels:
             lib.braid_attn_kv4.restype = c_int
             if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
                 raise KernelError("the attention library over a 4-bit cache is another than was asked for")
-            lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once)
+            lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once, clusters by their size)
             self._attn_libs[("kv4", head_dim)] = lib
         return lib
 
@@ -970,15 +970,19 @@ class Kernels:
         plan = lib.plans.get(key)
         if plan is None:
             columns = lib.braid_attn_kv4_columns(key[0], f32)
-            plan = lib.plans[key] = (columns, lib.braid_attn_kv4_slots(f32, columns))
-        columns, slots = plan
+            plan = lib.plans[key] = (columns, lib.braid_attn_kv4_slots(f32, columns),
+                                     [0, 0] + [lib.braid_attn_kv4_clusters(f32, columns, n) for n in range(2, 9)])
+        columns, slots, clusters = plan
         hpc = min(g, columns)
         ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (columns // hpc))
         span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
         # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
         n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
+        # the slices are a cluster where the device holds all clusters at once (a second round would double the time: 6 sequences of 5 tokens
+        # in a window of 4,096, 96 clusters of 3, 57 us against 33 with a kernel that merges)
+        cluster = 1 < n_splits <= 8 and ctas <= clusters[n_splits]
         partial = None
-        if n_splits > 1:
+        if n_splits > 1 and not cluster:
             need = rows * nqh * n_splits * (hd + 2)
             if self._attn_partial is None or self._attn_partial.numel() < need:
                 self._attn_partial = torch.empty(max(need, 1 << 22), dtype=torch.float32, device="cuda")
@@ -990,8 +994,8 @@ class Kernels:
             kv_before.data_ptr(), token_seq.data_ptr(), _ptr(head_sinks) or 0, _ptr(head_gate) or 0, _ptr(head_scale) or 0, _ptr(bias[0]) or 0,
             _ptr(bias[1]) or 0, self._error_flag.data_ptr() + 16, q.stride(0), out.stride(0), head_gate.stride(0) if head_gate is not None else 0,
             rows, n_seqs, max_q_len, nqh, nkh, page_table.shape[1], cache.shape[0], window, keep_first, n_splits, int(sink is not None),
-            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns)
-        self.launches += 1 + (n_splits > 1)
+            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns, int(cluster), 0)
+        self.launches += 1 + (partial is not None)
         self._check_lib(lib, lib.braid_attn_kv4(args, self._stream()), "attn_kv4")
 
     # ------------------------------------------------------------------ element-wise kernels of other models

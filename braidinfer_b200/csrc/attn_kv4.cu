@@ -13,7 +13,8 @@
 // What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
 // shifts are half.  Every warp walks units of 32 or 64 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
 // (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
-// and results; a context longer than that is sliced over CTAs, whose results a second kernel merges.
+// and results.  A context is sliced over CTAs where few would work on it: up to 8 slices are a cluster, whose CTAs read one another's
+// results and end together; those of more are merged by a second kernel.
 // The running maximum of a column is raised only when a unit's scores exceed it by more than 4 (in powers of two): a vote instead
 // of a reduction over the warp; sums are taken against the same maximum, so nothing is lost.
 //
@@ -50,6 +51,7 @@ struct Kv4Args {
     int rows, n_seqs, max_q_len, nqh, nkh, cols, num_pages, window, keep_first, n_splits, has_sink, settled;
     float scale, sink, out_scale, softcap;
     int f32, columns;            // float32 rows; columns a CTA
+    int cluster, unused;         // the slices (up to 8) are CTAs of a cluster, which merges them
 };
 
 #define LOG2E 1.4426950408889634f
@@ -103,6 +105,33 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e,
 __device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
 // x * 2^e for any e
 __device__ __forceinline__ float scaled(float x, int e) { const int h = e / 2; return x * pow2(h) * pow2(e - h); }
+// The CTAs of a cluster: all have come here, and see what the others wrote before.
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Shared memory at the address `at` of CTA `rank` of the cluster (`cluster` false: of this CTA).
+__device__ __forceinline__ float2 ld_cluster2(uint32_t at, int rank, int cluster) {
+    float2 v;
+    if (cluster) {
+        uint32_t p;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p) : "memory");
+    } else {
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    }
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at, int rank, int cluster) {
+    float4 v;
+    if (cluster) {
+        uint32_t p;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+    } else {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    }
+    return v;
+}
 __device__ __forceinline__ float exp2_ftz(float x) {        // to 2 units of the last place; 0 below 2^-126
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -632,24 +661,45 @@ attn_kv4_kernel(const Kv4Args a) {
         }
     __syncthreads();
     const bool out_wide = !(((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) & (4 * sizeof(T) - 1));
-    for (int i = tid; i < C::BM * (HD / 4); i += NW * 32) {
+    // a column's numbers d .. d + 3 from what `n` slices of this CTA's (or the cluster's) warps left
+    auto merge = [&](int col, int d, int n, float& M, float& L, float4& x) {
+        M = -INFINITY;
+        L = 0.f;
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint32_t at_ml = smem_u32(ml + col * 2), at_o = smem_u32(mo + col * HD + d);
+        for (int i = 0; i < n; ++i)
+#pragma unroll
+            for (int w = 0; w < NW; ++w) M = fmaxf(M, ld_cluster2(at_ml + w * (C::BM * 8), i, a.cluster).x);
+        const float ref = M == -INFINITY ? 0.f : M;
+        for (int i = 0; i < n; ++i) {
+            float2 sl[NW];
+            float4 y[NW];
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                sl[w] = ld_cluster2(at_ml + w * (C::BM * 8), i, a.cluster);
+                y[w] = ld_cluster4(at_o + w * (C::BM * HD * 4), i, a.cluster);
+            }
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                // a slice without a finite score has weight 0, which leaves nothing of its zeros and all of a NaN (weight 1 if none has one)
+                const float f = M == -INFINITY ? 1.f : exp2f(sl[w].x - ref);
+                L = fmaf(sl[w].y, f, L);
+                x.x = fmaf(y[w].x, f, x.x); x.y = fmaf(y[w].y, f, x.y); x.z = fmaf(y[w].z, f, x.z); x.w = fmaf(y[w].w, f, x.w);
+            }
+        }
+    };
+    if (a.cluster) cluster_barrier();                          // every CTA's results are in its shared memory
+    const int first = a.cluster ? split * (NW * 32) + tid : tid, turn = a.cluster ? a.n_splits * (NW * 32) : NW * 32;
+    for (int i = first; i < C::BM * (HD / 4); i += turn) {
         const int col = i / (HD / 4), d = (i - col * (HD / 4)) * 4;
         const int tl = col / hpc, hl = col - tl * hpc;
         if (!(tl < n_tok && hl < n_heads)) continue;
         const int head = head0 + hl;
         const size_t row = (size_t)(q_start + tok0 + tl);
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * C::BM + col) * 2]);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = M == -INFINITY ? 1.f : exp2f(ml[(w * C::BM + col) * 2] - M);     // nothing finite: zeros, or a NaN that stays
-            const float4 y = *reinterpret_cast<const float4*>(mo + (w * C::BM + col) * HD + d);
-            L = fmaf(ml[(w * C::BM + col) * 2 + 1], f, L);
-            x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-        }
-        if (a.n_splits > 1) {
+        float M, L;
+        float4 x;
+        merge(col, d, a.cluster ? a.n_splits : 1, M, L, x);
+        if (a.n_splits > 1 && !a.cluster) {
             const size_t at = (row * a.nqh + head) * a.n_splits + split;
             *reinterpret_cast<float4*>(a.partial + at * HD + d) = x;
             if (d == 0) *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(M, L);
@@ -671,50 +721,55 @@ attn_kv4_kernel(const Kv4Args a) {
         } else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
         else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
     }
+    if (a.cluster) cluster_barrier();                          // no CTA ends before the others have read its results
 }
 
-// The slices of a (row, head) made one: sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), four numbers a thread.
+// The slices of a (row, head) made one: sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A CTA a (row, head): HD / 4 threads take four numbers
+// each of every G-th slice (so that all loads of up to 8 G slices are on their way together), and the first of them join the shares.
 template <typename T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 attn_kv4_merge_kernel(const Kv4Args a) {
-    constexpr int HD = BRAID_HD;
+    constexpr int HD = BRAID_HD, Q = HD / 4, G = 256 / Q;
     pdl_trigger();
     pdl_wait();
-    const long long it = (long long)blockIdx.x * 128 + threadIdx.x;
-    const long long rh = it / (HD / 4);
-    const int d = (int)(it - rh * (HD / 4)) * 4;
-    if (rh >= (long long)a.rows * a.nqh) return;
-    const long long row = rh / a.nqh;
-    const int head = (int)(rh - row * a.nqh);
+    __shared__ float4 so[G][Q];
+    __shared__ float2 sm[G];
+    const int rh = blockIdx.x, row = rh / a.nqh, head = rh - row * a.nqh;
     if (a.token_seq[row] < 0) return;
-    const float* po = a.partial + (size_t)rh * a.n_splits * HD + d;
+    const int g = threadIdx.x / Q, q = threadIdx.x - g * Q;
+    const bool works = g < G;
+    const float* po = a.partial + (size_t)rh * a.n_splits * HD + q * 4;
     const float2* pm = reinterpret_cast<const float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD) + (size_t)rh * a.n_splits;
     float M = -INFINITY, L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int B = 8;                                       // slices in flight
-    for (int s0 = 0; s0 < a.n_splits; s0 += B) {
-        float2 ml[B];
-        float4 y[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const bool in = s0 + i < a.n_splits;
-            ml[i] = in ? pm[s0 + i] : make_float2(-INFINITY, 0.f);
-            y[i] = in ? *reinterpret_cast<const float4*>(po + (size_t)(s0 + i) * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float Mn = M;
-#pragma unroll
-        for (int i = 0; i < B; ++i) Mn = fmaxf(Mn, ml[i].x);
-        const float ref = Mn == -INFINITY ? 0.f : Mn, c = M == -INFINITY && Mn == -INFINITY ? 1.f : exp2f(M - ref);
-        L *= c; x.x *= c; x.y *= c; x.z *= c; x.w *= c;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            // a slice without a finite score has weight 0, which leaves nothing of its zeros and all of a NaN
-            const float f = exp2f(ml[i].x - ref);
-            L = fmaf(ml[i].y, f, L);
-            x.x = fmaf(y[i].x, f, x.x); x.y = fmaf(y[i].y, f, x.y); x.z = fmaf(y[i].z, f, x.z); x.w = fmaf(y[i].w, f, x.w);
-        }
+    auto join = [&](float m, float l, const float4& y) {       // a share without a finite score has weight 0: nothing of zeros, all of a NaN
+        const float Mn = fmaxf(M, m), ref = Mn == -INFINITY ? 0.f : Mn, c = Mn == -INFINITY ? 1.f : exp2f(M - ref), f = Mn == -INFINITY ? 1.f : exp2f(m - ref);
+        L = fmaf(L, c, l * f);
+        x.x = fmaf(x.x, c, y.x * f); x.y = fmaf(x.y, c, y.y * f); x.z = fmaf(x.z, c, y.z * f); x.w = fmaf(x.w, c, y.w * f);
         M = Mn;
+    };
+    constexpr int B = 8;
+    if (works)
+        for (int s0 = g; s0 < a.n_splits; s0 += B * G) {
+            float2 ml[B];
+            float4 y[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const bool in = s0 + i * G < a.n_splits;
+                ml[i] = in ? pm[s0 + i * G] : make_float2(-INFINITY, 0.f);
+                y[i] = in ? *reinterpret_cast<const float4*>(po + (size_t)(s0 + i * G) * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if (s0 + i * G < a.n_splits) join(ml[i].x, ml[i].y, y[i]);
+        }
+    if (works) {
+        so[g][q] = x;
+        if (q == 0) sm[g] = make_float2(M, L);
     }
+    __syncthreads();
+    if (threadIdx.x >= Q) return;
+    for (int i = 1; i < G; ++i) join(sm[i].x, sm[i].y, so[i][q]);
     float f = 1.f;
     if (a.has_sink) {
         const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
@@ -722,8 +777,8 @@ attn_kv4_merge_kernel(const Kv4Args a) {
         L = L * f + exp2f(sk - mn);
     }
     float inv = f * a.out_scale / L;
-    if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[row * a.gate_stride + head])));
-    T* dst = (T*)a.out + row * a.out_stride + (size_t)head * HD + d;
+    if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[(size_t)row * a.gate_stride + head])));
+    T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * HD + q * 4;
     const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
 #pragma unroll
     for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(y[e]);
@@ -757,7 +812,20 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
     if (gz > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld tiles, %d heads, %d sequences)", gz, a.nkh * hchunks, a.n_seqs);
     if (gz == 0) return BRAID_OK;
-    braid_launch(attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>, dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz), dim3(KV4_NW * 32), C::SMEM, s, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz);
+    cfg.blockDim = dim3(KV4_NW * 32);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = braid_pdl_enabled();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = a.n_splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>, a);
     BRAID_LAUNCH_CHECK();
 }
 
@@ -778,6 +846,26 @@ extern "C" int braid_attn_kv4_slots(int f32, int columns) {
     return per_sm * sms;
 }
 
+// Clusters of `size` CTAs that the device holds at once (0: none).
+extern "C" int braid_attn_kv4_clusters(int f32, int columns, int size) {
+    const void* f = columns <= 8 ? (f32 ? kv4_kernel<3, 1>() : kv4_kernel<1, 1>()) : (f32 ? kv4_kernel<3, KV4_NT_MAX>() : kv4_kernel<1, KV4_NT_MAX>());
+    const int bytes = columns <= 8 ? (f32 ? Kv4C<3, 1>::SMEM : Kv4C<1, 1>::SMEM) : (f32 ? Kv4C<3, KV4_NT_MAX>::SMEM : Kv4C<1, KV4_NT_MAX>::SMEM);
+    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, size);
+    cfg.blockDim = dim3(KV4_NW * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = size;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess) { cudaGetLastError(); return 0; }
+    return n;
+}
+
 // `args`: a Kv4Args, filled in by the caller (csrc/api.py has its layout).
 extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     Kv4Args a = *args;
@@ -792,15 +880,16 @@ extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     if (!a.bias_slope != !a.bias_rate) BRAID_REFUSE("attn_kv4: a distance bias has a slope and a rate a head");
     if (a.softcap > 0.f && a.bias_slope) BRAID_REFUSE("attn_kv4: a cap on the scores and a distance bias are not combined");
     if (a.n_splits < 1) a.n_splits = 1;
-    if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: n_splits > 1 needs the partial buffer");
+    if (a.n_splits <= 1 || a.n_splits > 8) a.cluster = 0;
+    if (a.n_splits > 1 && !a.cluster && !a.partial) BRAID_REFUSE("attn_kv4: slices that are no cluster need the partial buffer");
     cudaStream_t s = (cudaStream_t)stream;
     int rc;
     if (a.columns <= 8) rc = a.f32 ? launch_kv4<3, 1>(a, s) : launch_kv4<1, 1>(a, s);
     else rc = a.f32 ? launch_kv4<3, KV4_NT_MAX>(a, s) : launch_kv4<1, KV4_NT_MAX>(a, s);
-    if (rc || a.n_splits == 1) return rc;
-    const long long ctas = ((long long)a.rows * a.nqh * (BRAID_HD / 4) + 127) / 128;
+    if (rc || a.n_splits == 1 || a.cluster) return rc;
+    const long long ctas = (long long)a.rows * a.nqh;
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
-    if (a.f32) braid_launch(attn_kv4_merge_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, s, a);
-    else braid_launch(attn_kv4_merge_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, s, a);
+    if (a.f32) braid_launch(attn_kv4_merge_kernel<float>, dim3((unsigned)ctas), dim3(256), 0, s, a);
+    else braid_launch(attn_kv4_merge_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(256), 0, s, a);
     BRAID_LAUNCH_CHECK();
 }
