@@ -3,7 +3,8 @@ per sequence, and the per-step page tables that kernels read.
 
 Storage of a group: [layer_in_group][page][planes][kv_head][page_size][head_dim] in
 the run's element type; planes is 2 (K, V), or 1 where a mixer keeps one vector a token
-that is key and value at once (`CacheRequest.planes`).  A group collects the schedule entries whose mixers asked for
+that is key and value at once (`CacheRequest.planes`).  A group held in 4 bits (`CacheRequest.four_bit`) is
+[layer_in_group][page][kv_head][bytes of a page and kv head] instead (csrc/kv4.cuh).  A group collects the schedule entries whose mixers asked for
 the same thing (`CacheRequest.group_key`): all keys, or a window of them.  The
 reference's layout is one 64-token chunk holding all layers
 (crates/braidinfer-runtime/src/paged_kv.rs:17-21); per-layer pools make a layer's pages
@@ -27,11 +28,13 @@ PAGE_SIZE = _page_size()      # csrc/page.h holds the number
 @dataclass
 class LayerCache:
     """What a mixer sees of the cache during one step."""
-    storage: torch.Tensor            # [pages, planes, kv_heads, page_size, head_dim]
+    storage: torch.Tensor            # [pages, planes, kv_heads, page_size, head_dim], or uint8 [pages, kv_heads, bytes]
     page_size: int
     read_only: bool
     group: int
     page_table: Optional[torch.Tensor] = None    # [sequences of the step, blocks] int32, set per step
+    four_bit: bool = False
+    place: Optional[torch.Tensor] = None         # (four_bit) [rows] int32: page * page_size + position in it of every row, or -1, set per step
 
 
 class CacheGroup:
@@ -39,8 +42,11 @@ class CacheGroup:
         self.request = request
         self.entries = entries                   # schedule entries that own a layer here
         self.pages = GroupPages(num_pages, PAGE_SIZE, request.kind, request.window, request.keep_first)
-        self.storage = torch.zeros((len(entries), num_pages, request.planes, request.num_kv_heads, PAGE_SIZE, request.head_dim),
-                                   dtype=dtype, device=device)
+        shape = (len(entries), num_pages, request.planes, request.num_kv_heads, PAGE_SIZE, request.head_dim)
+        if request.four_bit:
+            # (codes, and a step and a lowest value for every 32 numbers: zeros read as zeros)
+            shape, dtype = (len(entries), num_pages, request.num_kv_heads, PAGE_SIZE * (request.head_dim + request.head_dim // 4)), torch.uint8
+        self.storage = torch.zeros(shape, dtype=dtype, device=device)
 
     def nbytes(self) -> int:
         return self.storage.numel() * self.storage.element_size()
@@ -102,11 +108,12 @@ class CacheManager:
         sees (a windowed owner gives pages back once its own window has passed them)."""
         if reader is None:
             return                            # a mixer that keeps nothing ignores the view it is handed
-        if (reader.num_kv_heads, reader.head_dim, reader.planes) != (owner.num_kv_heads, owner.head_dim, owner.planes):
+        if (reader.num_kv_heads, reader.head_dim, reader.planes, reader.four_bit) != (owner.num_kv_heads, owner.head_dim, owner.planes,
+                                                                                      owner.four_bit):
             raise CacheError(
                 f"schedule entry {e} reads the cache of entry {owner_entry}, but its mixer expects "
-                f"{reader.num_kv_heads} kv heads of {reader.head_dim} and that cache holds "
-                f"{owner.num_kv_heads} of {owner.head_dim}")
+                f"{reader.num_kv_heads} kv heads of {reader.head_dim}{' in 4 bits' if reader.four_bit else ''} and that cache holds "
+                f"{owner.num_kv_heads} of {owner.head_dim}{' in 4 bits' if owner.four_bit else ''}")
         if owner.kind == "window":
             if (reader.kind != "window" or reader.window is None or reader.window > owner.window
                     or reader.keep_first > owner.keep_first):
@@ -141,9 +148,15 @@ class CacheManager:
         return [g.pages.pool.in_use for g in self.groups]
 
     # ------------------------------------------------------------------ steps
-    def begin_step(self, slot_ids: Sequence[int], new_tokens: Sequence[int]) -> List[np.ndarray]:
+    @property
+    def four_bit(self) -> bool:
+        """Whether a group is held in 4 bits (its mixers want every row's place in the cache)."""
+        return any(g.request.four_bit for g in self.groups)
+
+    def begin_step(self, slot_ids: Sequence[int], new_tokens: Sequence[int], lists: bool = False) -> List:
         """Reserve pages for the tokens each sequence brings; return, per group, the page
-        table [sequences, blocks] (int32, -1 where a block is absent or released)."""
+        table [sequences, blocks] (int32, -1 where a block is absent or released), or with `lists` every sequence's
+        list of pages."""
         if len(set(slot_ids)) != len(slot_ids):
             raise CacheError("a slot appears twice in one step")
         for g in self.groups:
@@ -157,6 +170,9 @@ class CacheManager:
         for g in self.groups:
             for s, n in zip(slot_ids, new_tokens):
                 g.pages.grow(s, self.lengths[s] + n)
+            if lists:
+                tables.append([list(g.pages.blocks[s]) for s in slot_ids])
+                continue
             cols = max(1, max(len(g.pages.blocks[s]) for s in slot_ids))
             t = np.full((len(slot_ids), cols), -1, dtype=np.int32)
             for i, s in enumerate(slot_ids):
@@ -176,7 +192,7 @@ class CacheManager:
         if where is None:
             return None
         g, layer = where
-        return LayerCache(self.groups[g].storage[layer], PAGE_SIZE, self.entry_read_only[entry], g)
+        return LayerCache(self.groups[g].storage[layer], PAGE_SIZE, self.entry_read_only[entry], g, four_bit=self.groups[g].request.four_bit)
 
     def state_view(self, entry: int) -> Optional[torch.Tensor]:
         return self.state[entry]

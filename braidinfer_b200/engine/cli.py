@@ -13,8 +13,8 @@ environment, the prompt from the arguments.
   BRAIDINFER_LOGIT_TRACE=<file>      append `step= tok= logit_hash=` a chosen token, to find the step where
                                      two runs part (generate.rs:380-396; see engine/generate.py)
 This library's own: TEMPERATURE (default 0 = greedy, as the reference's binary is),
-TOP_K, TOP_P, MIN_P, REPETITION_PENALTY, SEED, DTYPE=bfloat16|float32, BATCH_FILE=<file
-with one prompt a line>.
+TOP_K, TOP_P, MIN_P, REPETITION_PENALTY, SEED, DTYPE=bfloat16|float32, CACHE_FORMAT=full|int4
+(keys and values in 4 bits a number), BATCH_FILE=<file with one prompt a line>.
 
 With a tokenizer.json in the model folder (and the `tokenizers` package) the prompt is
 text and so is the output; BOS is prepended unless it is there already or
@@ -124,7 +124,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
             prompts_text = [line.rstrip("\n") for line in f if line.strip()]
     t_load = time.perf_counter()
     m = load(model, dtype=dtype, max_seq_len=max_seq_len, max_batch=max(1, min(len(prompts_text), 64)),
-             seed=_env_int("WEIGHT_SEED", 0))
+             seed=_env_int("WEIGHT_SEED", 0), cache_format=os.environ.get("CACHE_FORMAT", "full"))
     print(f"LOAD PROFILE: load = {(time.perf_counter() - t_load) * 1000:.0f} ms", file=sys.stderr)
     spec = m.spec
     codec = TextCodec(None if model.startswith("random:") else model, spec.vocab_size, spec.bos_token_id)

@@ -40,13 +40,21 @@ def parse_dtype(name: Union[str, torch.dtype]) -> torch.dtype:
     return _DTYPES[name]
 
 
+def parse_cache_format(name: str) -> str:
+    if name not in ("full", "int4"):
+        raise ValueError(f"unknown cache format {name!r}; choose full or int4")
+    return name
+
+
 class Engine:
     def __init__(self, config_dict: Optional[Mapping], tensors_or_folder, *, dtype="bfloat16", max_tokens: int = 8192,
                  max_slots: Optional[int] = None, device: str = "cuda:0", gemm_backend: str = "auto",
                  attention_backend: str = "auto", row_multiple: int = 1, use_graphs: bool = True,
-                 fuse_reduce: bool = True, scaled_norm: bool = True, verbose: bool = True, spec=None) -> None:
+                 fuse_reduce: bool = True, scaled_norm: bool = True, verbose: bool = True, spec=None, cache_format: str = "full") -> None:
         """`config_dict` (config.json's content) picks the architecture and its description of
-        parts; or pass a `ModelSpec` as `spec` directly (then `config_dict` may be None)."""
+        parts; or pass a `ModelSpec` as `spec` directly (then `config_dict` may be None).  `cache_format` "int4": keys and values are
+        held in 4 bits a number, 1.25 bytes a key and value number together instead of 4 (bfloat16), in models whose caches are all
+        those of attention with rotated heads of 32, 64, ... 256 numbers."""
         from ..csrc.api import get_kernels
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
@@ -60,7 +68,7 @@ class Engine:
             self.arch, self.config, self.spec = None, None, spec
         self.rt = Runtime(act_dtype=self.dtype, device=self.device, kernels=self.kernels,
                           gemm_backend=gemm_backend, attention_backend=attention_backend, fuse_reduce=fuse_reduce,
-                          scaled_norm=scaled_norm)
+                          scaled_norm=scaled_norm, cache_format=parse_cache_format(cache_format))
         self.model = DecoderModel(self.spec, self.rt)
         specs = self.model.tensor_specs()
         if isinstance(tensors_or_folder, (str, os.PathLike)):
@@ -74,6 +82,11 @@ class Engine:
         self.weight_bytes = sum(t.numel() * t.element_size() for t in tensors.values())
         self.model.load(tensors)
         del tensors
+        if self.rt.cache_format == "int4":
+            for entry, (req, _, _) in zip(self.spec.schedule, self.model.cache_plan()):
+                if req is not None and not req.four_bit:
+                    raise ValueError(f"cache_format 'int4': layer {entry.layer}'s mixer ({self.spec.layers[entry.layer].mixer.kind}) keeps a "
+                                     "cache that is not held in 4 bits")
         self.max_tokens = int(max_tokens)
         n_pages = -(-self.max_tokens // PAGE_SIZE)
         self.max_slots = int(max_slots) if max_slots else max(1, min(n_pages, 1024))
@@ -200,7 +213,7 @@ class Engine:
                 raise ValueError("want must have one list per entry")
         before = [self.cache.length(s) for s in slots]
         n_new = [len(t) for t in tokens]
-        tables = self.cache.begin_step(slots, n_new)
+        tables = self.cache.begin_step(slots, n_new, lists=self.cache.four_bit)
         one_each = all(n == 1 for n in n_new)
         # Steps of few tokens are bound by the host when it launches them kernel by kernel (some 330
         # launches take it 6 ms, the device 3): they go through CUDA graphs, which can depend on a
@@ -215,9 +228,12 @@ class Engine:
         graphable = self.use_graphs and shaped and tap is None
         if device_tokens is not None and not one_each:
             raise ValueError("device_tokens needs a step of one token a sequence")
-        ctx = self.packer.pack(slots, tokens, before, want_l, tables, bucket_tables=shaped,
-                               token_source_rows=device_tokens[1] if device_tokens is not None else None,
-                               pad_rows_to=token_tile(sum(n_new)) if short_prompt else 0, upload=False)
+        layout = dict(bucket_tables=shaped, token_source_rows=device_tokens[1] if device_tokens is not None else None,
+                      pad_rows_to=token_tile(sum(n_new)) if short_prompt else 0)
+        if self.cache.four_bit:
+            ctx = self.packer.pack_lengths(slots, tokens, before, want_l, tables, [g.pages.pool.num_pages for g in self.cache.groups], **layout)
+        else:
+            ctx = self.packer.pack(slots, tokens, before, want_l, tables, upload=False, **layout)
         ctx.kernels = self.kernels
         ctx.may_be_captured = shaped
         # the step opens with a copy of its tables, or with their fetch and a graph's launch: both wait for all that runs, and every
@@ -231,7 +247,11 @@ class Engine:
             ctx.max_q_len = FEW_TOKENS if max(n_new) <= FEW_TOKENS else ctx.rows
         # a step that a graph will replay has its tables fetched by a kernel; one launched kernel by kernel, whose first kernels read
         # the tables before they wait for their predecessors, by a copy
-        self.packer.upload(self.kernels if graphable and self._graph_ready(ctx) else None)
+        replayed = graphable and self._graph_ready(ctx)
+        if self.cache.four_bit:
+            self.packer.upload_lengths(ctx, self.kernels, replayed)
+        else:
+            self.packer.upload(self.kernels if replayed else None)
         if device_tokens is not None:
             self.kernels.gather_i32(device_tokens[0], self.packer.token_source_view, ctx.token_ids)
         try:

@@ -74,6 +74,8 @@ class StepContext:
     # and owes it to its results; a scale that nobody took by the end of the block is an error.
     row_scales: dict = field(default_factory=dict)
     kernels: object = None
+    # Per cache group, where a group is held in 4 bits: every row's place in the cache (Kernels.step_tables).
+    places: List[torch.Tensor] = field(default_factory=list)
 
     def defer(self, tensor: torch.Tensor, handle, kind: str) -> None:
         self.deferred[tensor.data_ptr()] = (handle, kind)
@@ -147,6 +149,8 @@ class StepPacker:
         self._turn = 0
         self._dev: Optional[torch.Tensor] = None
         self._pending: Optional[Tuple[list, int]] = None
+        self._lengths: Optional[tuple] = None
+        self._fence: Optional[torch.Tensor] = None
         self.h2d_bytes_last = 0
         self.generation = 0          # grows when the device buffer moves (captured graphs are stale then)
 
@@ -287,6 +291,88 @@ class StepPacker:
         parts = [_Sized(sz) for sz in sizes]
         return self._context(dev, parts, offs, [_Shaped(s) for s in shapes], rows, n, n, [1] * n, kv_before, slots,
                              want_rows)
+
+    def pack_lengths(self, slots: Sequence[int], tokens: Sequence[Sequence[int]], kv_before: Sequence[int], want: Sequence[Sequence[int]],
+                     page_lists: Sequence[Sequence[Sequence[int]]], num_pages: Sequence[int], bucket_tables: bool = False,
+                     token_source_rows: Optional[Sequence[int]] = None, pad_rows_to: int = 0) -> StepContext:
+        """A step whose tables a kernel builds (`Kernels.step_tables`): the host moves the tokens, the lengths and, a cache group, the
+        sequences' lists of pages (`page_lists`; `num_pages` the pages of the group's cache), and `upload_lengths` has positions, sequence
+        numbers, first rows, page tables and the rows' places in the cache made of them.  The same tables as `pack` builds, and places;
+        options as there."""
+        n = len(slots)
+        if token_source_rows is not None and any(len(t) != 1 for t in tokens):
+            raise ValueError("tokens can be taken from the device only in steps of one token a sequence")
+        q_len = [len(t) for t in tokens]
+        n_tokens = sum(q_len)
+        rows = -(-max(n_tokens, int(pad_rows_to)) // self.row_multiple) * self.row_multiple
+        want_rows, r = [], 0
+        for i, m in enumerate(q_len):
+            for w in want[i]:
+                if not (0 <= w < m):
+                    raise IndexError(f"wanted place {w} is outside the {m} tokens that sequence {i} brings")
+                want_rows.append(r + w)
+            r += m
+        cols = [max(1, max(len(b) for b in lists)) for lists in page_lists]
+        if bucket_tables:
+            cols = [max(8, 1 << (c - 1).bit_length()) for c in cols]
+        groups = len(page_lists)
+        # what the kernel builds lies first, then what is moved; the lists of pages last: their size is no part of a step's shape, and
+        # no kernel of the step reads them
+        built = [rows, rows, n] + [n * c for c in cols] + [rows] * groups
+        moved = [rows, n, n, n, len(want_rows), n] + [sum(map(len, lists)) for lists in page_lists]
+        offs, at = [], 0
+        for size in built + moved:
+            offs.append(at)
+            at += -(-size // 4) * 4
+        base = offs[len(built)]
+        st, dev = self._buffers(max(at, 4))
+        pn = st[1]
+
+        def put(k: int, values) -> None:
+            o = offs[len(built) + k] - base
+            pn[o:o + len(values)] = values
+
+        ids = np.zeros(rows, dtype=np.int32)
+        ids[:n_tokens] = tokens[0] if n == 1 else [t for seq in tokens for t in seq]
+        for k, values in enumerate((ids, q_len, kv_before, slots, want_rows, token_source_rows if token_source_rows is not None else range(n))):
+            put(k, values)
+        for g, lists in enumerate(page_lists):
+            put(6 + g, [p for b in lists for p in b])
+
+        def view(k: int, *shape) -> torch.Tensor:
+            v = dev[offs[k]:offs[k] + (built + moved)[k]]
+            return v.view(*shape) if shape else v
+
+        b = len(built)
+        self._lengths = (st, base, at - base, num_pages, [view(b + 6 + g) for g in range(groups)])
+        self.h2d_bytes_last = (at - base) * 4
+        self.token_source_view = view(b + 5)
+        return StepContext(
+            rows=rows, n_tokens=n_tokens, n_seqs=n, positions=view(0), token_seq=view(1), q_start=view(2),
+            page_tables=[view(3 + g, n, cols[g]) for g in range(groups)], places=[view(3 + groups + g) for g in range(groups)],
+            token_ids=view(b), q_len=view(b + 1), kv_before=view(b + 2), slot_ids=view(b + 3), want_rows=view(b + 4) if want_rows else None,
+            n_want=len(want_rows), max_q_len=max(q_len), max_kv_len=max(x + m for x, m in zip(kv_before, q_len)),
+            all_decode=all(m == 1 for m in q_len), host_q_len=tuple(q_len), host_kv_before=tuple(kv_before), host_slots=tuple(slots))
+
+    def upload_lengths(self, ctx: StepContext, kernels, replayed: bool) -> None:
+        """Move what `pack_lengths` gathered and build the step's tables.  `replayed`: a graph is launched next, which waits for it all; a
+        step launched kernel by kernel has kernels that read tables before they wait for their predecessors, so something else
+        than these kernels has to stand between."""
+        st, base, size, num_pages, pages = self._lengths
+        if replayed and size <= self.FETCH_MOST:
+            kernels.fetch_i32(st[0][:size], self._dev[base:base + size])
+        else:
+            self._dev[base:base + size].copy_(st[0][:size], non_blocking=True)
+        if st[2] is None:
+            st[2] = torch.cuda.Event()
+        st[2].record()
+        for g, table in enumerate(ctx.page_tables):
+            first = dict(positions=ctx.positions, token_seq=ctx.token_seq, q_start=ctx.q_start) if g == 0 else {}
+            kernels.step_tables(ctx.q_len, ctx.kv_before, pages[g], table, ctx.places[g], num_pages=num_pages[g], **first)
+        if not replayed:
+            if self._fence is None:
+                self._fence = torch.zeros(1, dtype=torch.int32, device=self.device)
+            self._fence.zero_()
 
     def _context(self, dev, parts, offs, tables, rows, n_tokens, n_seqs, q_len, kv_before, slots, want_rows):
         def view(k: int, shape=None) -> torch.Tensor:

@@ -110,6 +110,8 @@ class DecoderModel:
             view = cache.layer_view(e)
             if view is not None:
                 view.page_table = ctx.page_tables[view.group]
+                if view.four_bit:
+                    view.place = ctx.places[view.group]
             ctx.reader_takes_sum, ctx.sum_rides = self._takes_sum[e], ""
             h = self.blocks[entry.layer].forward(h, ctx, view, cache.state_view(e))
             if tap is not None:

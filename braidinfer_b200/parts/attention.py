@@ -47,6 +47,8 @@ Options that other designs use, each off unless named:
                     and stores keys and values (csrc/conv_heads.cu)
     shared_kv       the layer makes no keys and values: it reads those that an earlier layer cached (the schedule's
                     `cache_of`), with its own queries, window and output; goes with `conv`
+    A run whose cache is held in 4 bits (Runtime.cache_format) has the rows' keys and values written by a kernel of their own after
+    the rotation, and attention over what they read as; that goes with rotated heads (plain or with head norms) of 32, 64, ... 256 numbers.
     cache_window    how far back the cache keeps keys where readers see further than this layer's own window
 unit_qk_eps, q_temp, qkv_bias, proj_norm, unit_v_eps and value_dim without rotation are for heads that are not rotated (position encoding "none"): one kernel norms, scales and
 stores.  Keys, values and queries are then padded with zeros to one head size that the attention kernels take
@@ -189,6 +191,13 @@ class GQAAttention(Mixer):
             self.qk_norm = (float(qn["eps"]), prefix + qn["q_name"], prefix + qn["k_name"])
         self.q_norm_w = self.k_norm_w = None
         self.conv_w = self.conv_b = None
+        self.four_bit = getattr(runtime, "cache_format", "full") == "int4"
+        if self.four_bit:
+            if self.taps or self.prep or self.value_from_key or self.talk_name:
+                raise ValueError("gqa_attention: a cache in 4 bits goes with rotated heads, not with a convolution, heads that are normed "
+                                 "without weights or not rotated, keys as values or a mix of the heads' probabilities")
+            if self.hd_pad % 32 or not 32 <= self.hd_pad <= 256:
+                raise ValueError(f"gqa_attention: a cache in 4 bits holds heads of 32, 64, ... 256 numbers, not {self.hd_pad}")
         if (self.qk_norm or self.value_from_key) and not hasattr(self.pe, "norm_encode_and_store"):
             raise ValueError(f"position encoding '{pe.kind}' cannot norm heads or store a key as the value")
 
@@ -257,7 +266,8 @@ class GQAAttention(Mixer):
 
     def cache_request(self) -> Optional[CacheRequest]:
         kind = "window" if self.window else "full"
-        return CacheRequest(kind, self.nkh, self.hd_pad, self.cache_window, keep_first=self.keep_first if self.window else 0)
+        return CacheRequest(kind, self.nkh, self.hd_pad, self.cache_window, keep_first=self.keep_first if self.window else 0,
+                            four_bit=self.four_bit)
 
     def state_bytes(self) -> int:
         return (self.taps - 1) * self.channels * 4 if self.taps > 1 else 0
@@ -278,13 +288,17 @@ class GQAAttention(Mixer):
             return self._forward_padded(qkv, gate, residual, ctx, cache)
         if self.taps:
             return self._forward_conv(qkv, residual, ctx, cache, state)
-        if self.qk_norm or self.value_from_key:
-            self.pe.norm_encode_and_store(qkv, self.nqh, self.nkh, ctx, cache, self.q_norm_w, self.k_norm_w,
-                                          self.qk_norm[0] if self.qk_norm else 0.0, self.value_from_key)
-        else:
-            self.pe.encode_and_store(qkv, self.nqh, self.nkh, ctx, cache)
         rows = x.shape[0]
         D = self.hd_pad
+        encoded = None if cache.four_bit else cache      # what the rotation writes into; 4 bits are written from the rotated rows
+        if self.qk_norm or self.value_from_key:
+            self.pe.norm_encode_and_store(qkv, self.nqh, self.nkh, ctx, encoded, self.q_norm_w, self.k_norm_w,
+                                          self.qk_norm[0] if self.qk_norm else 0.0, self.value_from_key)
+        else:
+            self.pe.encode_and_store(qkv, self.nqh, self.nkh, ctx, encoded)
+        if cache.four_bit and not cache.read_only:
+            k0, v0 = self.nqh * D, (self.nqh + self.nkh) * D
+            rt.kernels.kv4_store(qkv[:, k0:v0], qkv[:, v0:v0 + self.nkh * D], cache.place, cache.storage, D)
         if self.talk is not None:
             # every head's probabilities over the values of every kv head, then the mix of the heads
             wide = rt.empty(rows, self.nqh * self.nkh * D)
@@ -365,6 +379,13 @@ class GQAAttention(Mixer):
         so that a handful of sequences still fills the machine.  A factor on plain scores that is not positive goes to the
         mma.sync kernel too: the tcgen05 kernel masks before the factor."""
         K = self.rt.kernels
+        if cache.four_bit:
+            K.attn_kv4(qkv, out, cache.storage, cache.page_table, ctx.q_start, ctx.q_len, ctx.kv_before, ctx.token_seq, ctx.n_seqs,
+                       ctx.max_q_len, ctx.max_kv_len, self.nqh, self.nkh, hd, self.window, self.scale, sink=self.sink,
+                       out_scale=self.out_mult, head_sinks=self.head_sinks, head_gate=gate, keep_first=self.keep_first,
+                       head_scale=self.head_scale, distance_bias=self.distance_bias, softcap=self.softcap, settled=ctx.settled,
+                       backend="plain" if self.rt.attention_backend == "plain" else "auto")
+            return
         plain = (self.rt.is_f32 or self.rt.attention_backend == "plain" or not K.attn_mma_supports(hd))
         extras = bool(self.keep_first) or self.head_scale is not None or value_heads > 1
         scaled_late = self.distance_bias is None and not self.softcap and not self.scale > 0

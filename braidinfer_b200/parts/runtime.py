@@ -23,6 +23,8 @@ class Runtime:
     # In steps of up to 128 tokens, let an RMSNorm leave its scale to the product that reads its output
     # (csrc/rowscale.cuh), so that the kernel before it works on parts of rows instead of whole rows.
     scaled_norm: bool = True
+    # How keys and values are kept: "full" (the run's element type), or "int4" (4 bits a number, csrc/kv4.cuh).
+    cache_format: str = "full"
 
     @property
     def is_f32(self) -> bool:

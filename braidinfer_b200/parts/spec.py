@@ -108,7 +108,8 @@ class CacheRequest:
     `window` tokens only.  Layers whose requests are equal share one group of
     storage.  `planes` is how many vectors of `head_dim` a token and kv head keep:
     2 for a key and a value, 1 where one vector serves as both (a latent).  `keep_first` (kind "window"): the
-    sequence's first positions stay beside the window, for mixers whose queries see them at any distance.
+    sequence's first positions stay beside the window, for mixers whose queries see them at any distance.  `four_bit`: keys and
+    values are held in 4 bits a number (csrc/kv4.cuh).
     """
     kind: str
     num_kv_heads: int
@@ -116,6 +117,7 @@ class CacheRequest:
     window: Optional[int] = None
     planes: int = 2
     keep_first: int = 0
+    four_bit: bool = False
 
     def group_key(self) -> Tuple:
-        return (self.kind, self.num_kv_heads, self.head_dim, self.window, self.planes, self.keep_first)
+        return (self.kind, self.num_kv_heads, self.head_dim, self.window, self.planes, self.keep_first, self.four_bit)

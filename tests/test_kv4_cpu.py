@@ -120,3 +120,35 @@ def test_entry_points_refuse(K):
     # nothing to do is no error
     assert tables(n=0, listed=0, rows=0) == store(rows=0) == expand(n=0) == 0
     assert build.page_size() == P.PAGE
+
+
+def test_mixers_that_a_4_bit_cache_does_not_go_with():
+    from braidinfer_b200.cache import CacheError, CacheManager
+    from braidinfer_b200.engine.engine import parse_cache_format
+    from braidinfer_b200.parts.attention import GQAAttention
+    from braidinfer_b200.parts.runtime import Runtime
+    from braidinfer_b200.parts.spec import CacheRequest, PartSpec
+
+    def mixer(pe="rope", fmt="int4", **kw):
+        rope = PartSpec(pe, {"head_dim": kw.get("head_dim", 64), "theta": 1e4})
+        params = dict(hidden_size=64, num_heads=4, num_kv_heads=2, head_dim=64, position_encoding=rope)
+        return GQAAttention({**params, **kw}, "l.", Runtime(torch.bfloat16, torch.device("cpu"), None, cache_format=fmt))
+
+    req = mixer().cache_request()
+    assert req.four_bit and not mixer(fmt="full").cache_request().four_bit and req.group_key() != mixer(fmt="full").cache_request().group_key()
+    assert mixer(qk_norm={"eps": 1e-5, "q_name": "q", "k_name": "k"}).cache_request().four_bit and mixer("none").cache_request().four_bit
+    for bad in (dict(head_dim=48), dict(head_dim=288), dict(conv=4), dict(talk="t"), dict(value_from_key=True), dict(pe="none", unit_qk_eps=1e-5)):
+        with pytest.raises(ValueError):
+            mixer(**bad)
+        if "head_dim" not in bad:
+            assert mixer(fmt="full", **bad) is not None
+    with pytest.raises(ValueError):
+        parse_cache_format("int8")
+    assert parse_cache_format("int4") == "int4"
+    c = CacheManager([(req, None, 0), (req, 0, 0)], 64 * 5, 3, torch.bfloat16, "cpu")
+    assert c.four_bit and tuple(c.groups[0].storage.shape) == (1, 5, 2, 64 * 80) and c.groups[0].storage.dtype == torch.uint8
+    assert c.layer_view(1).four_bit and c.layer_view(1).read_only
+    a, b = c.alloc_slot(), c.alloc_slot()
+    assert c.begin_step([b, a], [65, 1], lists=True) == [[[0, 1], [2]]]
+    with pytest.raises(CacheError, match="in 4 bits"):
+        CacheManager([(req, None, 0), (CacheRequest("full", 2, 64), 0, 0)], 64, 1, torch.bfloat16, "cpu")
