@@ -141,7 +141,7 @@ class RowScale:
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
 _KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
-_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<7Q10i")
+_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q10i")
 
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # torch's own quick way to the stream handle
@@ -186,9 +186,6 @@ class Kernels:
         self.pending_partial = None     # the open PartialProduct, if any (it owns the GEMM workspace)
         self.workspace_generation = 0   # grows when a scratch buffer moves (captured graphs are stale then)
         self._attn_partial: Optional[torch.Tensor] = None
-        self._kv4_pages: Optional[torch.Tensor] = None
-        self._kv4_numbers: Optional[torch.Tensor] = None
-        self._kv4_repair: Optional[torch.Tensor] = None
         self._verbose = verbose
 
     # ------------------------------------------------------------------ plumbing
@@ -824,11 +821,12 @@ class Kernels:
         self._on_device("kv4_expand", cache, out, page_table, q_len, kv_before)
         self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
 
-    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_cols=0, repair=None, seq0=0) -> None:
+    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_table=None, repair=None, seq0=0) -> None:
         self.launches += 1
         args = _EXPAND_ARGS.pack(cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), q_len.data_ptr(), kv_before.data_ptr(),
-                                 self._error_flag.data_ptr() + 16, _ptr(repair) or 0, n, cache.shape[1], hd, page_table.shape[1], cache.shape[0],
-                                 window, keep_first, out_cols, seq0, dtype_code(out.dtype))
+                                 self._error_flag.data_ptr() + 16, _ptr(repair) or 0, _ptr(out_table) or 0, n, cache.shape[1], hd,
+                                 page_table.shape[1], cache.shape[0], window, keep_first, out_table.shape[1] if out_table is not None else 0,
+                                 seq0, dtype_code(out.dtype))
         self._check_lib(lib, lib.braid_kv4_expand(args, self._stream()), "kv4_expand")
 
     def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -884,7 +882,7 @@ class Kernels:
                              head_scale, sink, out_scale, head_sinks, head_gate, distance_bias, softcap)
 
     def _attn_kv4_plain(self, q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale, sink,
-                        out_scale, head_sinks, head_gate, distance_bias, softcap, repair=None, n_seqs=0) -> None:
+                        out_scale, head_sinks, head_gate, distance_bias, softcap, repair=None) -> None:
         lib = self.part_library("kv4")
         self.launches += 1
         self._check_lib(lib, lib.braid_attn_kv4_simple(
@@ -892,7 +890,7 @@ class Kernels:
             token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(), out.shape[0], nqh, nkh, hd, page_table.shape[1], cache.shape[0],
             window, keep_first, float(scale), int(sink is not None), float(sink or 0.0), float(out_scale), _ptr(head_sinks), _ptr(head_gate),
             head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale), *self._bias_args(distance_bias), float(softcap or 0.0),
-            _ptr(repair), n_seqs, self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
+            _ptr(repair), self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
 
     def kv4_attention_library(self, head_dim: int):
         """The attention over a 4-bit cache for one head size, compiled at first use."""
@@ -933,34 +931,28 @@ class Kernels:
         and the attention of ordinary pages runs over them.  Values that are NaN are read back as zero, and the sequences that hold some
         are computed by the plain kernel (which otherwise ends at once)."""
         lib = self.part_library("kv4")
-        if self._kv4_repair is None or self._kv4_repair.numel() < n_seqs + 2:
-            self._kv4_repair = torch.zeros(max(n_seqs, 1022) + 2, dtype=torch.int32, device="cuda")
-            self.workspace_generation += 1
         cols = min(page_table.shape[1], max(1, -(-max_kv_len // build.page_size())))
         page = 2 * nkh * build.page_size() * hd
         group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
-        need = group * cols
-        if self._kv4_pages is None or self._kv4_pages.numel() < need * page:
-            self._kv4_pages = torch.empty(need * page, dtype=torch.bfloat16, device="cuda")
-            self.workspace_generation += 1
-        if self._kv4_numbers is None or self._kv4_numbers.numel() < need:
-            self._kv4_numbers = torch.arange(max(need, 1 << 14), dtype=torch.int32, device="cuda")
-            self.workspace_generation += 1
-        pages = self._kv4_pages[:need * page].view(need, 2, nkh, build.page_size(), hd)
-        table = self._kv4_numbers[:need].view(group, cols)
+        # from torch's allocator at every call: calls on other streams, and other graphs, have their own
+        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.bfloat16, device=out.device)
+        table = torch.empty((group, cols), dtype=torch.int32, device=out.device)
+        repair = torch.zeros(n_seqs + 1, dtype=torch.int32, device=out.device)
+        fence = repair.new_empty(1)
         tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(options["softcap"])
                                                                                      or options["distance_bias"] is not None)
         for i in range(0, n_seqs, group):
             n = min(group, n_seqs - i)
             part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
-            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, cols, self._kv4_repair, i)
+            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, table, repair, i)
             if tc:
                 self.attn_tc(q, out, pages, table, *part, n, max_q_len, nqh, nkh, hd, window, scale, **options)
             else:
+                fence.zero_()        # that kernel reads pages of earlier tokens before its predecessor has ended; not before something else has
                 self.attn_mma(q, out, pages, table, *part, token_seq, n, max_q_len, nqh, nkh, hd, window, scale, keep_first=keep_first,
                               head_scale=head_scale, **options)
         self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale,
-                             **options, repair=self._kv4_repair, n_seqs=n_seqs)
+                             **options, repair=repair)
 
     def _attn_kv4_mma(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                       scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled) -> None:
@@ -983,11 +975,8 @@ class Kernels:
         cluster = 1 < n_splits <= 8 and ctas <= clusters[n_splits]
         partial = None
         if n_splits > 1 and not cluster:
-            need = rows * nqh * n_splits * (hd + 2)
-            if self._attn_partial is None or self._attn_partial.numel() < need:
-                self._attn_partial = torch.empty(max(need, 1 << 22), dtype=torch.float32, device="cuda")
-                self.workspace_generation += 1
-            partial = self._attn_partial
+            # from torch's allocator at every call: calls on other streams, and other graphs, have their own
+            partial = torch.empty(rows * nqh * n_splits * (hd + 2), dtype=torch.float32, device=out.device)
         bias = distance_bias or (None, None)
         args = _KV4_ARGS.pack(
             q.data_ptr(), out.data_ptr(), _ptr(partial) or 0, cache.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
@@ -1124,7 +1113,7 @@ class Kernels:
                     raise KernelError("the library of the 4-bit cache has other arguments than these bindings")
                 lib.braid_attn_kv4_simple.argtypes = [c_void_p, c_longlong] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 8 + \
                                                      [c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_longlong] + [c_void_p] * 3 + \
-                                                     [c_float, c_void_p, c_int, c_void_p, c_void_p]
+                                                     [c_float, c_void_p, c_void_p, c_void_p]
                 names = ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand", "braid_attn_kv4_simple")
             elif name == "streams":
                 lib.braid_streams.argtypes = [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,

@@ -282,7 +282,8 @@ struct ExpandArgs {
     const int* q_len;
     const int* kv_before;
     int* error_flag;
-    int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [2 + seq0 + sequence] become 1
+    int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [1 + seq0 + sequence] become 1
+    int* out_table;              // (out_cols > 0) [n_seqs, out_cols]: the numbers of the pages, for whoever reads them
     int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
 };
 
@@ -347,6 +348,7 @@ kv4_expand_kernel(const ExpandArgs a) {
     const int c = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
     const int before = a.kv_before[seq], end = before + a.q_len[seq];
     const int key0 = c * BRAID_PAGE_SIZE;
+    if (a.out_table && kvh == 0 && threadIdx.x == 0) a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
     if (key0 >= end) return;
     const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0;
     if (key0 + BRAID_PAGE_SIZE <= lo && key0 >= a.keep_first) return;
@@ -375,7 +377,7 @@ kv4_expand_kernel(const ExpandArgs a) {
         const uint32_t both = in ? v0 | (v1 << 16) : 0u;
         if (a.repair && ((vg[w] & 0x7f80u) == 0x7f80u || (vg[w] & 0x7f800000u) == 0x7f800000u)) {
             vg[w] = 0u;
-            a.repair[2 + a.seq0 + seq] = 1;
+            a.repair[1 + a.seq0 + seq] = 1;
             a.repair[0] = 1;
         }
         __align__(16) P y[4];
@@ -420,9 +422,9 @@ extern "C" int braid_kv4_args_bytes(int which) { return which == 0 ? (int)sizeof
 // ------------------------------------------------------------------ plain attention
 // One warp per (row, query head), 32 keys at a time: a lane a key for the scores, a lane a number of the head for the values.  All
 // arithmetic float32.  Options as in attn_simple.cu.  Rows of padding (token_seq < 0) are left as they were.
-// With `repair` ([0]: whether to work at all, [1]: CTAs that are done, [2 + i]: whether for sequence i; all 0 before) it goes over the
-// result of a product that multiplies masked values by 0 (the attention of ordinary pages): a NaN among them would make all of it NaN, so
-// they were taken out, and the rows of those sequences are computed here.  The last CTA to end leaves all numbers 0 again.
+// With `repair` ([0]: whether to work at all, [1 + i]: whether for sequence i) it goes over the result of a product that multiplies masked
+// values by 0 (the attention of ordinary pages): a NaN among them would make all of it NaN, so they were taken out, and the rows of
+// those sequences are computed here.
 struct Kv4SimpleArgs {
     const void* q;
     void* out;
@@ -444,15 +446,14 @@ struct Kv4SimpleArgs {
     const float* bias_rate;
     float softcap;
     int* error_flag;
-    int* repair;
-    int n_seqs;
+    const int* repair;
 };
 
 template <typename T>
 __device__ void attn_kv4_item(const Kv4SimpleArgs& a, long long item, float* qs, int lane) {
     const int row = (int)(item / a.nqh), head = (int)(item - (long long)row * a.nqh);
     const int seq = a.token_seq[row];
-    if (seq < 0 || (a.repair && !a.repair[2 + seq])) return;
+    if (seq < 0 || (a.repair && !a.repair[1 + seq])) return;
     const int hd = a.hd, W = hd / KV4_GROUP, kvh = head / (a.nqh / a.nkh);
     __syncwarp();
     const T* q = (const T*)a.q + (size_t)row * a.q_stride + (size_t)head * hd;
@@ -536,22 +537,16 @@ attn_kv4_simple_kernel(const Kv4SimpleArgs a) {
     pdl_wait();
     __shared__ float qs_all[4][256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.repair && *(volatile int*)a.repair == 0) return;
+    if (a.repair && a.repair[0] == 0) return;
     for (long long item = (long long)blockIdx.x * 4 + warp; item < (long long)a.rows * a.nqh; item += (long long)gridDim.x * 4)
         attn_kv4_item<T>(a, item, qs_all[warp], lane);
-    if (a.repair) {
-        __syncthreads();
-        if (threadIdx.x == 0 && atomicAdd(a.repair + 1, 1) == (int)gridDim.x - 1) {      // every CTA has looked at the flag
-            for (int i = 0; i < a.n_seqs + 2; ++i) a.repair[i] = 0;
-        }
-    }
 }
 
 extern "C" int braid_attn_kv4_simple(const void* q, long long q_stride, void* out, long long out_stride, int dtype, const void* cache,
                                      const int* page_table, const int* token_seq, const int* q_start, const int* kv_before, int rows, int nqh,
                                      int nkh, int hd, int cols, int num_pages, int window, int keep_first, float scale, int has_sink, float sink,
                                      float out_scale, const float* head_sinks, const void* head_gate, long long gate_stride, const float* head_scale,
-                                     const float* bias_slope, const float* bias_rate, float softcap, int* repair, int n_seqs, int* error_flag, void* stream) {
+                                     const float* bias_slope, const float* bias_rate, float softcap, const int* repair, int* error_flag, void* stream) {
     if (rows <= 0) return BRAID_OK;
     if (int rc = kv4_check("attn_kv4", nkh, hd, cache)) return rc;
     if (nqh <= 0 || nqh % nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", nqh, nkh);
@@ -561,7 +556,7 @@ extern "C" int braid_attn_kv4_simple(const void* q, long long q_stride, void* ou
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
     Kv4SimpleArgs a{q, out, (const uint8_t*)cache, page_table, token_seq, q_start, kv_before, q_stride, out_stride, rows, nqh, nkh, hd, cols, num_pages,
                     window, window > 0 ? keep_first : 0, scale, has_sink || head_sinks, sink, out_scale, head_sinks, head_gate, gate_stride, head_scale,
-                    bias_slope, bias_rate, softcap, error_flag, repair, n_seqs};
+                    bias_slope, bias_rate, softcap, error_flag, repair};
     if (dtype == BRAID_F32) braid_launch(attn_kv4_simple_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
     else if (dtype == BRAID_BF16) braid_launch(attn_kv4_simple_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
     else BRAID_REFUSE("attn_kv4: unknown dtype code %d", dtype);

@@ -424,3 +424,77 @@ def test_run_of_all_of_them(K):
         off = (out.cpu().double().view(want.shape) - want).abs()
         assert (off <= mag * (2.0 ** -7 + 2 * (2.0 ** -8 * smag[1] + 16 * U * smag[0])[..., None]) + 2.0 ** -8 * want.abs()).all()
         before = [n + b for n, b in zip(new, before)]
+
+
+KINDS = {"few": ([(1, 300), (2, 64)], 8, 2, 64), "slices": ([(1, 20000)], 4, 1, 128), "prompts": ([(130, 200), (90, 0)], 8, 4, 128),
+         "prompts of other heads": ([(130, 200), (90, 0)], 8, 4, 96)}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_graphs_and_streams_keep_apart(K, monkeypatch, kind):
+    """The same call on two inputs, captured into graphs that replay at the same time, and on two streams at once."""
+    if "prompts" in kind:
+        monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    seqs, nqh, nkh, hd = KINDS[kind]
+    cases = [Case(K, seqs, nqh, nkh, hd, BF, seed=s) for s in (1, 2)]
+    want = [c.run(K) for c in cases]
+    assert not torch.equal(*want)
+    args, outs = [], [torch.empty_like(w) for w in want]
+    for c, o in zip(cases, outs):
+        args.append((c.q, o, c.cache, c.table.to(DEV), c.start.to(DEV), dev(c.q_len), dev(c.before), c.seq.to(DEV), len(seqs), max(c.q_len),
+                     max(n + b for n, b in seqs), nqh, nkh, hd, None, hd ** -0.5))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    graphs = []
+    for a, s in zip(args, streams):
+        with torch.cuda.stream(s):
+            K.attn_kv4(*a)                                    # (libraries and attributes are set up outside of a capture)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                K.attn_kv4(*a)
+            graphs.append(g)
+    for how in ("graphs", "streams"):
+        for _ in range(20):
+            for o in outs:
+                o.fill_(9.0)
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for a, s, g in zip(args, streams, graphs):
+                    with torch.cuda.stream(s):
+                        g.replay() if how == "graphs" else K.attn_kv4(*a)
+            torch.cuda.synchronize()
+            for o, w in zip(outs, want):
+                assert torch.equal(o, w)
+    K.check_device_errors()
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("seqs", [[(1, 100)], [(3, 9000)], [(140, 30)]])
+def test_rows_that_start_anywhere(K, route, seqs, dt):
+    c = Case(K, seqs, 6, 2, 64, dt)
+    want = c.run(K)
+    wide = torch.zeros(c.rows, 6 * 64 + 5, dtype=dt, device=DEV)
+    wide[:, 3:3 + 6 * 64] = c.q
+    c.q = wide[:, 3:3 + 6 * 64]
+    out = torch.full((c.rows, 6 * 64 + 7), 9.0, dtype=dt, device=DEV)
+    c.run(K, out=out[:, 1:1 + 6 * 64])
+    off = (out[:, 1:1 + 6 * 64].double() - want.double()).abs().max()
+    # (prompts that start on no 16 bytes go over 4 bits, where keys and values are not rounded: two roundings of 2^-8, and the results')
+    assert (out[:, 0] == 9).all() and (out[:, 1 + 6 * 64:] == 9).all() and off <= (2.0 ** -6 if dt == BF else 2.0 ** -20) * want.abs().max()
+
+
+def test_places_of_one_step_in_any_order(K):
+    """Rows whose places are neighbours go through many threads at once: every byte is one row's."""
+    hd, kv, rows = 128, 4, 6000
+    g = gen(3)
+    x = torch.randn(2, rows, kv * hd, generator=g).to(BF)
+    place = torch.randperm(64 * 100, generator=g)[:rows]
+    cache = torch.zeros(100, kv, K.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+    K.kv4_store(x[0].to(DEV), x[1].to(DEV), dev(place), cache, hd)
+    K.check_device_errors()
+    code, step, lo = P.read(cache, hd)
+    for plane in (0, 1):
+        c, s, l = P.quantise(x[plane].double().view(rows, kv, hd))
+        p, t = place // 64, place % 64
+        assert torch.equal(code[p, plane, :, t], c) and torch.equal(step[p, plane, :, t], s) and torch.equal(lo[p, plane, :, t], l)
