@@ -134,13 +134,14 @@ extern "C" int braid_step_tables(const TablesArgs* args, void* stream) {
 }
 
 // ------------------------------------------------------------------ write
-// Four lanes a group: lane j takes its numbers 8 j .. 8 j + 7, which are one word of key codes, or two 16-bit words of value
+// Two lanes a group: lane h takes its numbers 16 h .. 16 h + 15, which are two words of key codes, or four 16-bit words of value
 // codes.  `place` < 0: a row of padding, nothing is written.  Places must differ from one another.
 //
 // A code is the quotient (x - lo) / step rounded to the nearest whole number, ties to even.  The quotient is taken as a product with 1 / step,
 // which may miss a number next to a tie, and then put right by the remainder x - lo - code step: that is exact (the code has
-// 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  (6,400 rows of 8 heads of 128, keys and values: 17 us
-// with a division a number, FIGURE us so; what is read and written takes 5 us.)
+// 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  Instructions bound it, some 15 a number.  (6,414 rows of 8
+// heads of 128, keys and values, bfloat16: 23 us with 8 numbers a thread and tests of each for NaN, TIME_STORE us so; what is read and
+// written takes 5 us.)
 struct StoreArgs {
     const void* k;
     const void* v;
@@ -163,84 +164,101 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
     }
 }
 
-template <typename T, bool WIDE>
+__device__ __forceinline__ float min_nan(float a, float b) { float y; asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
+__device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
+
+// A row takes 2 nkh hd / 16 threads: a CTA holds several rows, or a row passes through it 256 threads at a time.
+template <typename T, int W, bool WIDE>
 __global__ void __launch_bounds__(256)
-kv4_store_kernel(const StoreArgs a) {
+kv4_store_kernel(const StoreArgs a, int row_threads, int rows_cta) {
     pdl_trigger();
     pdl_wait();
-    const int hd = a.hd, nkh = a.nkh, per = hd / 8, W = hd / KV4_GROUP;        // lanes a (row, plane, kv head)
-    const long long it = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long heads = it / per;
-    const int c8 = (int)(it - heads * per);                   // numbers 8 c8 .. 8 c8 + 7
-    const long long row = heads / (2 * nkh);
-    const int ph = (int)(heads - row * (2 * nkh));
-    const bool value = ph >= nkh;
-    const int kvh = value ? ph - nkh : ph;
-    const int w = c8 >> 2, j = c8 & 3;
-    int at = -1;
-    float x[8];
-    bool bad = false;
-    float lo = INFINITY, hi = -INFINITY;
-    if (row < a.rows) {
-        at = a.place[row];
-        if (at >= 0) {
-            load8<T, WIDE>((value ? (const T*)a.v + row * a.v_stride : (const T*)a.k + row * a.k_stride) + (long long)kvh * hd + 8 * c8, x);
-            if (at / BRAID_PAGE_SIZE >= a.num_pages) { if (c8 == 0) atomicExch(a.error_flag, 1); at = -1; }
+    constexpr int hd = 32 * W, per = 2 * W;                   // lanes a (row, plane, kv head)
+    const int nkh = a.nkh;
+    const int r_cta = rows_cta > 1 ? threadIdx.x / row_threads : 0;
+    const long long row = (long long)blockIdx.x * rows_cta + r_cta;
+    const bool here = row < a.rows && r_cta < rows_cta;
+    const int at = here ? a.place[row] : -1;
+    for (int it0 = rows_cta > 1 ? threadIdx.x - r_cta * row_threads : threadIdx.x, turn = 0; turn < row_threads; it0 += 256, turn += rows_cta > 1 ? row_threads : 256) {
+        const bool live = here && it0 < row_threads;
+        const int it = live ? it0 : 0;
+        const int ph = it / per, c16 = it - ph * per;         // numbers 16 c16 .. 16 c16 + 15
+        const bool value = ph >= nkh;
+        const int kvh = value ? ph - nkh : ph, w = c16 >> 1, h = c16 & 1;
+        float x[16];
+        if (live) {                                           // (asked for beside the row's place, not after it)
+            const T* src = (value ? (const T*)a.v + row * a.v_stride : (const T*)a.k + row * a.k_stride) + (long long)kvh * hd + 16 * c16;
+            load8<T, WIDE>(src, x);
+            load8<T, WIDE>(src + 8, x + 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
         }
-    }
-    if (at >= 0) {
+        if (sizeof(T) == 4)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (sizeof(T) == 4) x[i] = __bfloat162float(__float2bfloat16_rn(x[i]));
-            bad |= x[i] != x[i];
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
+            for (int i = 0; i < 16; ++i) x[i] = __bfloat162float(__float2bfloat16_rn(x[i]));
+        float lo = x[0], hi = x[0];                           // NaN if one is
+#pragma unroll
+        for (int i = 1; i < 16; ++i) { lo = min_nan(lo, x[i]); hi = max_nan(hi, x[i]); }
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));                 // rows and heads take whole pairs of lanes
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+        if (!live || at < 0) continue;
+        const int page = at / BRAID_PAGE_SIZE, off = at % BRAID_PAGE_SIZE, t = off % KV4_REC;
+        if (page >= a.num_pages) {
+            if (it == 0) atomicExch(a.error_flag, 1);
+            continue;
         }
-    }
+        const float span = hi - lo;
+        const bool bad = !(span <= 3.4028234663852886e38f);
+        const __nv_bfloat16 nan = __ushort_as_bfloat16(0x7fff);
+        const __nv_bfloat16 step16 = bad ? nan : __float2bfloat16_rn(span / 15.f);
+        const float step = __bfloat162float(step16);
+        // codes in the lowest bits of 1.5 2^23 + code
+        uint32_t code[16];
+        constexpr float base = 12582912.f;
+        if (step >= 1e-36f) {
+            const float inv = 1.f / step;
+            const uint32_t half = __float_as_uint(0.5f * step);
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {                         // per is a multiple of 4: the four lanes are of one warp and one group
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-    }
-    if (at < 0) return;
-    const float span = hi - lo;
-    bad |= !(span <= 3.4028234663852886e38f);
-    const __nv_bfloat16 nan = __ushort_as_bfloat16(0x7fff);
-    const __nv_bfloat16 step16 = bad ? nan : __float2bfloat16_rn(span / 15.f);
-    const float step = __bfloat162float(step16);
-    uint32_t code[8];
-    if (step >= 1e-36f) {
-        const float inv = 1.f / step;
+            for (int i = 0; i < 16; ++i) {
+                const float d = x[i] - lo;
+                float u = fmaf(d, inv, base);
+                const float rem = fmaf(base - u, step, d);    // d - code step
+                // too far off, or a tie and an odd code: the next one (half a step less one unit is the bound for odd codes)
+                const float limit = __uint_as_float(half - (__float_as_uint(u) & 1u));
+                u += fabsf(rem) > limit ? copysignf(1.f, rem) : 0.f;
+                code[i] = __float_as_uint(fminf(u, base + 15.f));
+            }
+        } else {                                              // no range (or NaN): code 0; or one that 1 / step would leave float32's with
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = x[i] - lo;
-            const float u = fminf(t * inv, 15.f) + 12582912.f;                 // 1.5 2^23: the sum is a whole number, in its lowest bits
-            const float rem = fmaf(12582912.f - u, step, t);                   // t - code step
-            const int c = (int)(__float_as_uint(u) & 15u);
-            const float two = 2.f * fabsf(rem);
-            const int off = (two > step || (two == step && (c & 1))) ? (rem > 0.f ? 1 : -1) : 0;
-            code[i] = (uint32_t)min(c + off, 15);
+            for (int i = 0; i < 16; ++i) code[i] = __float_as_uint(base) + (step > 0.f ? (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) : 0u);
         }
-    } else {                                                   // no range (or NaN): code 0; or one that 1 / step would leave float32's with
+        uint8_t* rec = a.cache + ((long long)page * nkh + kvh) * kv4_page_bytes(hd) + (off / KV4_REC) * kv4_record_bytes(hd);
+        // sums of codes at their places, with what they have too much taken off at the end
+        constexpr uint32_t C = 0x4b400000u;
+        if (!value) {
+            uint32_t* words = reinterpret_cast<uint32_t*>(rec + t * (hd / 2)) + w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) code[i] = step > 0.f ? (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) : 0u;
+            for (int g = 0; g < 2; ++g) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) word += (code[8 * g + 2 * n] - C) * (1u << (4 * n)) + (code[8 * g + 2 * n + 1] - C) * (1u << (16 + 4 * n));
+                words[(2 * h + g) * W] = word;
+            }
+        } else {
+            uint16_t* codes = reinterpret_cast<uint16_t*>(rec + kv4_value_codes(hd) + t * (hd / 2)) + w;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) word += (code[4 * g + n] - C) * (1u << (4 * n));
+                codes[(4 * h + g) * W] = (uint16_t)word;
+            }
+        }
+        if (h == 0)
+            reinterpret_cast<uint32_t*>(rec + (value ? kv4_value_groups(hd) : kv4_key_groups(hd)))[t * W + w] =
+                (uint32_t)__bfloat16_as_ushort(step16) | ((uint32_t)__bfloat16_as_ushort(bad ? nan : __float2bfloat16_rn(lo)) << 16);
     }
-    const uint32_t group = (uint32_t)__bfloat16_as_ushort(step16) | ((uint32_t)__bfloat16_as_ushort(bad ? nan : __float2bfloat16_rn(lo)) << 16);
-    const int page = at / BRAID_PAGE_SIZE, off = at % BRAID_PAGE_SIZE, t = off % KV4_REC;
-    uint8_t* rec = a.cache + ((long long)page * nkh + kvh) * kv4_page_bytes(hd) + (off / KV4_REC) * kv4_record_bytes(hd);
-    if (!value) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) word |= (code[2 * n] << (4 * n)) | (code[2 * n + 1] << (16 + 4 * n));
-        reinterpret_cast<uint32_t*>(rec + t * (hd / 2))[j * W + w] = word;
-    } else {
-        uint16_t* codes = reinterpret_cast<uint16_t*>(rec + kv4_value_codes(hd) + t * (hd / 2));
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            codes[(2 * j + h) * W + w] = (uint16_t)(code[4 * h] | (code[4 * h + 1] << 4) | (code[4 * h + 2] << 8) | (code[4 * h + 3] << 12));
-    }
-    if (j == 0) reinterpret_cast<uint32_t*>(rec + (value ? kv4_value_groups(hd) : kv4_key_groups(hd)))[t * W + w] = group;
 }
 
 static int kv4_check(const char* what, int nkh, int hd, const void* cache) {
@@ -250,20 +268,27 @@ static int kv4_check(const char* what, int nkh, int hd, const void* cache) {
     return BRAID_OK;
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 static int launch_store(const StoreArgs& a, cudaStream_t s) {
-    const long long items = (long long)a.rows * 2 * a.nkh * (a.hd / 8), ctas = (items + 255) / 256;
-    if (ctas > 0x7fffffffLL) BRAID_REFUSE("kv4_store: the rows exceed the grid limit");
-    const bool wide = !(((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)(a.k_stride * sizeof(T)) | (uintptr_t)(a.v_stride * sizeof(T))) & 15);
-    braid_launch(wide ? kv4_store_kernel<T, true> : kv4_store_kernel<T, false>, dim3((unsigned)ctas), dim3(256), 0, s, a);
+    const long long threads = (long long)2 * a.nkh * (a.hd / 16);
+    if (threads > 0x3fffffffLL) BRAID_REFUSE("kv4_store: %d kv heads exceed the kernel's limit", a.nkh);
+    const int rows_cta = threads <= 128 ? (int)(256 / threads) : 1;
+    const int ctas = (a.rows + rows_cta - 1) / rows_cta;
+    void (*const kernels[8])(const StoreArgs, int, int) = {kv4_store_kernel<T, 1, WIDE>, kv4_store_kernel<T, 2, WIDE>, kv4_store_kernel<T, 3, WIDE>,
+                                                           kv4_store_kernel<T, 4, WIDE>, kv4_store_kernel<T, 5, WIDE>, kv4_store_kernel<T, 6, WIDE>,
+                                                           kv4_store_kernel<T, 7, WIDE>, kv4_store_kernel<T, 8, WIDE>};
+    braid_launch(kernels[a.hd / KV4_GROUP - 1], dim3(ctas), dim3(256), 0, s, a, (int)threads, rows_cta);
     BRAID_LAUNCH_CHECK();
 }
 
 extern "C" int braid_kv4_store(const StoreArgs* a, void* stream) {
     if (a->rows <= 0) return BRAID_OK;
     if (int rc = kv4_check("kv4_store", a->nkh, a->hd, a->cache)) return rc;
-    if (a->dtype == BRAID_F32) return launch_store<float>(*a, (cudaStream_t)stream);
-    if (a->dtype == BRAID_BF16) return launch_store<__nv_bfloat16>(*a, (cudaStream_t)stream);
+    const int size = a->dtype == BRAID_F32 ? 4 : 2;
+    const bool wide = !(((uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)(a->k_stride * size) | (uintptr_t)(a->v_stride * size)) & 15);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (a->dtype == BRAID_F32) return wide ? launch_store<float, true>(*a, s) : launch_store<float, false>(*a, s);
+    if (a->dtype == BRAID_BF16) return wide ? launch_store<__nv_bfloat16, true>(*a, s) : launch_store<__nv_bfloat16, false>(*a, s);
     BRAID_REFUSE("kv4_store: unknown dtype code %d", a->dtype);
 }
 
