@@ -143,6 +143,8 @@ class RowScale:
 _KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q10i")
 
+_KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
+
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # torch's own quick way to the stream handle
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -736,25 +738,31 @@ class Kernels:
         if _CURRENT_DEVICE() != here:
             raise KernelError(f"{what}: the current device is not cuda:{here}")
 
-    @staticmethod
-    def _i32(what: str, name: str, t: Optional[torch.Tensor], least: int) -> None:
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < least):
-            raise KernelError(f"{what}: {name} must be contiguous int32 with at least {least} numbers")
+    def _i32(self, what: str, *named) -> None:
+        """Refuse what is not contiguous int32 on the kernels' device with at least so many numbers: (name, tensor, numbers) each."""
+        here = self._device_index
+        for name, t, least in named:
+            if t is not None:
+                if t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < least:
+                    raise KernelError(f"{what}: {name} must be contiguous int32 with at least {least} numbers")
+                if t.get_device() != here:
+                    raise KernelError(f"{what}: {name} lies on {t.device}; these kernels run on cuda:{here}")
 
     @staticmethod
     def kv4_supports(head_dim: int) -> bool:
         """Head sizes that a 4-bit cache holds: whole groups of 32 numbers, up to 256."""
-        return head_dim % 32 == 0 and 32 <= head_dim <= 256
+        return head_dim in _KV4_PAGE_BYTES
 
     @staticmethod
     def kv4_page_bytes(head_dim: int) -> int:
         """Bytes that a page's tokens take of one kv head, keys and values: 1.25 a number pair (csrc/kv4.cuh has the layout)."""
-        if not Kernels.kv4_supports(head_dim):
+        n = _KV4_PAGE_BYTES.get(head_dim)
+        if n is None:
             raise KernelError(f"a 4-bit cache holds heads of 32, 64, ... 256 numbers, not {head_dim}")
-        return build.page_size() * (head_dim + head_dim // 4)
+        return n
 
     def _check_kv4(self, what: str, cache: torch.Tensor, hd: int) -> None:
-        if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[2] != self.kv4_page_bytes(hd):
+        if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[2] != self.kv4_page_bytes(hd):
             raise KernelError(f"{what}: the cache must be contiguous uint8 [pages, kv_heads, {self.kv4_page_bytes(hd)}], got {cache.dtype} "
                               f"{tuple(cache.shape)}")
 
@@ -767,17 +775,16 @@ class Kernels:
         of every new token; -1 for rows past the tokens) and, where given, positions and token_seq [rows] (0 and -1 past the tokens)
         and q_start [n].  Lengths that fit neither the rows, the list nor the table, and pages outside [0, num_pages), raise a device error
         (`check_device_errors`); what does not fit is not written anywhere else."""
-        what, i32 = "step_tables", self._i32
-        lib = self.part_library("kv4")
-        n, rows = q_len.numel(), place.numel()
-        if page_table.dim() != 2 or page_table.shape[0] != n or kv_before.numel() != n:
+        what = "step_tables"
+        lib = self._part_libs.get("kv4") or self.part_library("kv4")
+        n, rows, shape = q_len.numel(), place.numel(), page_table.shape
+        if len(shape) != 2 or shape[0] != n or kv_before.numel() != n:
             raise KernelError(f"step_tables: {n} requests want as many kv_before and rows of the page table, got {kv_before.numel()} and "
-                              f"{tuple(page_table.shape)}")
-        cols = page_table.shape[1]
-        i32(what, "q_len", q_len, n), i32(what, "kv_before", kv_before, n), i32(what, "pages", pages, 0), i32(what, "page_table", page_table, 0)
-        i32(what, "place", place, rows), i32(what, "positions", positions, rows), i32(what, "token_seq", token_seq, rows)
-        i32(what, "q_start", q_start, n)
-        self._on_device(what, q_len, kv_before, pages, page_table, place, positions, token_seq, q_start)
+                              f"{tuple(shape)}")
+        cols = shape[1]
+        self._i32(what, ("q_len", q_len, n), ("kv_before", kv_before, n), ("pages", pages, 0), ("page_table", page_table, 0), ("place", place, rows),
+                  ("positions", positions, rows), ("token_seq", token_seq, rows), ("q_start", q_start, n))
+        self._on_device(what)
         self.launches += 1
         args = _TABLES_ARGS.pack(
             q_len.data_ptr(), kv_before.data_ptr(), pages.data_ptr(), page_table.data_ptr(), place.data_ptr(), _ptr(positions) or 0,
@@ -788,18 +795,19 @@ class Kernels:
         """Write keys and values [rows, kv_heads * hd] (rows of any stride, float32 or bfloat16) into a 4-bit cache at the rows'
         places (`step_tables`; -1: a row of padding, not written; no place twice).  They are rounded to bfloat16 first, as an
         ordinary cache of a bfloat16 run holds them."""
-        lib = self.part_library("kv4")
-        self._check_kv4("kv4_store", cache, hd)
-        nkh, rows = cache.shape[1], k.shape[0]
-        for x in (k, v):
-            if x.dim() != 2 or x.shape != (rows, nkh * hd) or x.stride(1) != 1 or x.dtype != k.dtype:
-                raise KernelError(f"kv4_store: keys and values are rows of {nkh * hd} numbers of one element type, got {tuple(k.shape)} and "
-                                  f"{tuple(v.shape)}")
-        self._i32("kv4_store", "place", place, rows)
-        self._on_device("kv4_store", k, v, place, cache)
+        what = "kv4_store"
+        lib = self._part_libs.get("kv4") or self.part_library("kv4")
+        self._check_kv4(what, cache, hd)
+        (num_pages, nkh, _), shape = cache.shape, k.shape
+        if len(shape) != 2 or shape[1] != nkh * hd or v.shape != shape or k.dtype is not v.dtype or k.stride(1) != 1 or v.stride(1) != 1:
+            raise KernelError(f"kv4_store: keys and values are rows of {nkh * hd} numbers of one element type, got {tuple(shape)} and "
+                              f"{tuple(v.shape)}")
+        rows = shape[0]
+        self._i32(what, ("place", place, rows))
+        self._on_device(what, k, v, cache)
         self.launches += 1
         args = _STORE_ARGS.pack(k.data_ptr(), v.data_ptr(), place.data_ptr(), cache.data_ptr(), self._error_flag.data_ptr(), k.stride(0), v.stride(0),
-                                rows, nkh, hd, cache.shape[0], dtype_code(k.dtype))
+                                rows, nkh, hd, num_pages, dtype_code(k.dtype))
         self._check_lib(lib, lib.braid_kv4_store(args, self._stream()), "kv4_store")
 
     def kv4_expand(self, cache: torch.Tensor, out: torch.Tensor, page_table: torch.Tensor, q_len: torch.Tensor, kv_before: torch.Tensor,
@@ -816,9 +824,8 @@ class Kernels:
         self._check_kv4("kv4_expand", cache, hd)
         if out.shape[2] != cache.shape[1]:
             raise KernelError(f"kv4_expand: the cache holds {cache.shape[1]} kv heads, the pages {out.shape[2]}")
-        for name, t, size in (("page_table", page_table, 0), ("q_len", q_len, n), ("kv_before", kv_before, n)):
-            self._i32("kv4_expand", name, t, size)
-        self._on_device("kv4_expand", cache, out, page_table, q_len, kv_before)
+        self._i32("kv4_expand", ("page_table", page_table, 0), ("q_len", q_len, n), ("kv_before", kv_before, n))
+        self._on_device("kv4_expand", cache, out)
         self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
 
     def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_table=None, repair=None, seq0=0) -> None:
@@ -860,11 +867,9 @@ class Kernels:
             raise KernelError(f"attn_kv4: a page table of {n_seqs} sequences is wanted, got {tuple(page_table.shape)}")
         if int(keep_first or 0) < 0 or int(window or 0) < 0 or max_q_len < 0 or max_kv_len < 0:
             raise KernelError("attn_kv4: window, keep_first and lengths must not be negative")
-        for name, t, size in (("page_table", page_table, 0), ("q_start", q_start, n_seqs), ("q_len", q_len, n_seqs),
-                              ("kv_before", kv_before, n_seqs), ("token_seq", token_seq, rows)):
-            self._i32(what, name, t, size)
-        self._on_device(what, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, head_sinks, head_gate, head_scale,
-                        *(distance_bias or ()))
+        self._i32(what, ("page_table", page_table, 0), ("q_start", q_start, n_seqs), ("q_len", q_len, n_seqs), ("kv_before", kv_before, n_seqs),
+                  ("token_seq", token_seq, rows))
+        self._on_device(what, q, out, cache, head_sinks, head_gate, head_scale, *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
         if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, n_seqs, nqh, nkh):
@@ -970,6 +975,8 @@ class Kernels:
         span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
         # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
         n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
+        if 8 < n_splits <= 32 and -(-span // 128) <= 32 and ctas <= clusters[8]:
+            n_splits = 8                 # up to four units a warp: one launch instead of two costs the device no more (3k tokens: 8.7 and 8.5 us)
         # the slices are a cluster where the device holds all clusters at once (a second round would double the time: 6 sequences of 5 tokens
         # in a window of 4,096, 96 clusters of 3, 57 us against 33 with a kernel that merges)
         cluster = 1 < n_splits <= 8 and ctas <= clusters[n_splits]
