@@ -968,18 +968,18 @@ class Kernels:
         if plan is None:
             columns = lib.braid_attn_kv4_columns(key[0], f32)
             plan = lib.plans[key] = (columns, lib.braid_attn_kv4_slots(f32, columns),
-                                     [0, 0] + [lib.braid_attn_kv4_clusters(f32, columns, n) for n in range(2, 9)])
+                                     [0, 0] + [lib.braid_attn_kv4_clusters(f32, columns, n) for n in range(2, 5)])
         columns, slots, clusters = plan
         hpc = min(g, columns)
         ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (columns // hpc))
         span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
         # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
         n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
-        if 8 < n_splits <= 32 and -(-span // 128) <= 32 and ctas <= clusters[8]:
-            n_splits = 8                 # up to four units a warp: one launch instead of two costs the device no more (3k tokens: 8.7 and 8.5 us)
-        # the slices are a cluster where the device holds all clusters at once (a second round would double the time: 6 sequences of 5 tokens
-        # in a window of 4,096, 96 clusters of 3, 57 us against 33 with a kernel that merges)
-        cluster = 1 < n_splits <= 8 and ctas <= clusters[n_splits]
+        # Few slices are a cluster where the device holds all clusters at once: one launch instead of two.  Larger clusters wait for as many
+        # free places side by side (us as a cluster / with a kernel that merges, on the device: 4 requests of 3,000 tokens in float32, 4 slices
+        # 12.4 / 12.7, 8 slices 11.4 / 10.3, 16 slices 13.7 / 9.6; one request of 1,100, 4 slices 10.8 / 10.6, 8 slices 11.1 / 9.1), and a
+        # second round doubles the time (6 sequences of 5 tokens in a window of 4,096, 96 clusters of 3: 57 / 33).
+        cluster = 1 < n_splits <= 4 and ctas <= clusters[n_splits]
         partial = None
         if n_splits > 1 and not cluster:
             # from torch's allocator at every call: calls on other streams, and other graphs, have their own

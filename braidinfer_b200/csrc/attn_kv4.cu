@@ -13,7 +13,7 @@
 // What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
 // shifts are half.  Every warp walks units of 32 or 64 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
 // (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
-// and results.  A context is sliced over CTAs where few would work on it: up to 8 slices are a cluster, whose CTAs read one another's
+// and results.  A context is sliced over CTAs where few would work on it: a few slices are a cluster, whose CTAs read one another's
 // results and end together; those of more are merged by a second kernel.
 // The running maximum of a column is raised only when a unit's scores exceed it by more than 4 (in powers of two): a vote instead
 // of a reduction over the warp; sums are taken against the same maximum, so nothing is lost.
