@@ -141,6 +141,7 @@ class RowScale:
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
 _KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
+_KV4_PROMPT_ARGS = struct.Struct("<11Q3q8i7f4x")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q10i")
 
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
@@ -908,6 +909,11 @@ class Kernels:
             lib.braid_attn_kv4.restype = c_int
             if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
                 raise KernelError("the attention library over a 4-bit cache is another than was asked for")
+            if self.attn_tc_supports(head_dim):
+                lib.braid_attn_kv4_prompt.argtypes = [c_char_p, c_void_p]
+                lib.braid_attn_kv4_prompt.restype = c_int
+                if lib.braid_attn_kv4_prompt_args_bytes() != _KV4_PROMPT_ARGS.size:
+                    raise KernelError("the attention library over a 4-bit cache has other arguments than these bindings")
             lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once, clusters by their size)
             self._attn_libs[("kv4", head_dim)] = lib
         return lib
@@ -946,12 +952,20 @@ class Kernels:
         fence = repair.new_empty(1)
         tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(options["softcap"])
                                                                                      or options["distance_bias"] is not None)
+        prompt = self.kv4_attention_library(hd)
         for i in range(0, n_seqs, group):
             n = min(group, n_seqs - i)
             part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
             self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, table, repair, i)
             if tc:
-                self.attn_tc(q, out, pages, table, *part, n, max_q_len, nqh, nkh, hd, window, scale, **options)
+                gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
+                args = _KV4_PROMPT_ARGS.pack(
+                    q.data_ptr(), pages.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in part), self._error_flag.data_ptr() + 12,
+                    _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0),
+                    gate.stride(0) if gate is not None else 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
+                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0)
+                self.launches += 1
+                self._check_lib(prompt, prompt.braid_attn_kv4_prompt(args, self._stream()), "attn_kv4")
             else:
                 fence.zero_()        # that kernel reads pages of earlier tokens before its predecessor has ended; not before something else has
                 self.attn_mma(q, out, pages, table, *part, token_seq, n, max_q_len, nqh, nkh, hd, window, scale, keep_first=keep_first,

@@ -185,7 +185,7 @@ def latent_attention_library(rank: int, rot: int, verbose: bool = True) -> Path:
 
 def kv4_attention_library(head_dim: int, verbose: bool = True) -> Path:
     """The tensor-core attention over a cache held in 4 bits, compiled for one head size."""
-    return build_library(f"braidinfer_attn_kv4_hd{head_dim}", ["errors.cu", "attn_kv4.cu"], defines=[f"-DBRAID_HD={head_dim}"], verbose=verbose)
+    return build_library(f"braidinfer_attn_kv4_hd{head_dim}", ["errors.cu", "attn_kv4.cu", "attn_kv4_tc.cu"], defines=[f"-DBRAID_HD={head_dim}"], verbose=verbose)
 
 
 def attention_library(head_dim: int, verbose: bool = True, value_heads: int = 1) -> Path:
