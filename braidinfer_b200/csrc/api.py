@@ -141,7 +141,7 @@ class RowScale:
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
 _KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
-_KV4_PROMPT_ARGS = struct.Struct("<11Q3q8i7f4x")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
+_KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7fi")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q10i")
 
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
@@ -962,8 +962,8 @@ class Kernels:
                 args = _KV4_PROMPT_ARGS.pack(
                     q.data_ptr(), pages.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in part), self._error_flag.data_ptr() + 12,
                     _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0),
-                    gate.stride(0) if gate is not None else 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
-                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0)
+                    gate.stride(0) if gate is not None else 0, 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
+                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0, 1)
                 self.launches += 1
                 self._check_lib(prompt, prompt.braid_attn_kv4_prompt(args, self._stream()), "attn_kv4")
             else:

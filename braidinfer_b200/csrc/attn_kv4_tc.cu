@@ -21,17 +21,21 @@
 #define FA_BN 64                                 // keys per tile: one page
 #define FA_PAGE BRAID_PAGE_SIZE
 static_assert(FA_PAGE == 64, "a key tile of this kernel is one page of 64 positions");
-#define FA_THREADS 320                           // TMA warp, MMA warp, 8 softmax warps
+#define FA_SOFTMAX 4                             // warps before: TMA, S of either group, P V (20 warps in all: 5 a quarter of the SM)
+#define FA_THREADS ((FA_SOFTMAX + 16) * 32)      // two groups of 8 softmax warps
 #define FA_HB (BRAID_HD / 64)                    // 64-element blocks of the head dimension
 #define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] bf16, 128-byte rows
 #define FA_KBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]
 #define FA_Q_BYTES (FA_HB * FA_QBLOCK_BYTES)
 #define FA_KV_BYTES (FA_HB * FA_KBLOCK_BYTES)    // one K or one V tile
-#define FA_KST 2                                 // stages of the key ring
-#define FA_VST 2                                 // stages of the value ring
-#define FA_BAR_BYTES 192
-#define FA_SMEM (FA_Q_BYTES + (FA_KST + FA_VST) * FA_KV_BYTES + FA_BAR_BYTES)
-#define FA_TMEM_COLS 256                         // S0 [0,64) S1 [64,128) (P over their first 32 columns), O [128, 128 + HD)
+#define FA_KST 4                                 // stages of the key ring
+#define FA_VST 4                                 // stages of the value ring
+#define FA_BAR_BYTES 256
+#define FA_SMEM (2 * FA_Q_BYTES + (FA_KST + FA_VST) * FA_KV_BYTES + FA_BAR_BYTES)
+// tensor memory: O of the first 128 rows [0, 128), of the others [128, 256); scores of either [256, 384), P of either [448, 512)
+#define FA_TMEM_COLS 512
+#define FA_TMEM_S 256
+#define FA_TMEM_P 448
 
 // The two warps of a pair (64 threads): whether any of them says yes, and a plain meeting.
 __device__ __forceinline__ bool pair_any(int id, bool yes) {
@@ -62,18 +66,19 @@ struct Kv4PromptArgs {
     const float* bias_slope;     // BIAS: [nqh] float32 r1 and r2 of the distance bias r1 ln(1 + r2 (p - j))
     const float* bias_rate;
     long long q_stride, out_stride, gate_stride;
+    float* partial;              // n_splits > 1: what attn_kv4_merge_kernel (attn_kv4.cu) reads
     int rows, n_seqs, max_q_len, nqh, nkh, cols, window, has_sink;
     float scale, sink, out_scale, softcap;
     // filled in here: in units of log2(e); CAP: scale / cap, the tanh's argument
     float scale_log2, sink_log2, cap_log2;
-    int unused;
+    int n_splits;
 };
 
 #define FA_PLAIN 0
 #define FA_BIAS 1
 #define FA_CAP 2
 template <int FORM>
-__global__ void __launch_bounds__(FA_THREADS, 2)
+__global__ void __launch_bounds__(FA_THREADS, 1)
 attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Kv4PromptArgs a) {
     constexpr int HD = BRAID_HD;
     constexpr bool BIAS = FORM == FA_BIAS, CAP = FORM == FA_CAP;
@@ -86,7 +91,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         return;
     }
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + FA_Q_BYTES;                 // [FA_KST]
+    uint8_t* sK = sQ + 2 * FA_Q_BYTES;             // [FA_KST]
     uint8_t* sV = sK + FA_KST * FA_KV_BYTES;       // [FA_VST]
     uint64_t* bars = (uint64_t*)(sV + FA_VST * FA_KV_BYTES);
     uint64_t* q_full = bars;                       // [1]
@@ -94,16 +99,14 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint64_t* k_empty = k_full + FA_KST;           // [FA_KST]
     uint64_t* v_full = k_empty + FA_KST;           // [FA_VST]
     uint64_t* v_empty = v_full + FA_VST;           // [FA_VST]
-    uint64_t* s_full = v_empty + FA_VST;           // [2]
-    // two p_ready barriers take turns: the softmax warps may finish tile j + 1 before the MMA warp has
-    // looked at tile j's (it issues S of tile j + 1 first, and may then wait for a value tile), and a
-    // single barrier two phases ahead reads like one that has not moved
-    uint64_t* p_ready = s_full + 2;                // [2]
-    uint64_t* pv_done = p_ready + 2;               // [1]
-    uint32_t* tmem_slot = (uint32_t*)(pv_done + 1);
-    static_assert((1 + 2 * FA_KST + 2 * FA_VST + 5) * 8 + 8 <= FA_BAR_BYTES, "the barriers outgrow their bytes");
+    uint64_t* s_full = v_empty + FA_VST;           // [2] of the first, of the second 128 rows; the others alike
+    uint64_t* s_free = s_full + 2;                 // [2] the scores are in registers
+    uint64_t* p_ready = s_free + 2;                // [2]
+    uint64_t* pv_done = p_ready + 2;               // [2]
+    uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
+    static_assert((1 + 2 * FA_KST + 2 * FA_VST + 8) * 8 + 8 <= FA_BAR_BYTES, "the barriers outgrow their bytes");
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    __shared__ float share[2][2][FA_BM];           // what the two threads of a row tell one another
+    __shared__ float share[2][2][2][FA_BM];        // what the two threads of a row tell one another: [group][turn][half][row]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = a.nqh / a.nkh;
@@ -115,14 +118,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // short ones fill the gaps at the end
     const int seq = blockIdx.y;
     const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
-    const int tile = gridDim.z - 1 - blockIdx.z;
+    const int unit = gridDim.z - 1 - blockIdx.z, tile = unit / a.n_splits, split = unit - tile * a.n_splits;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 2); }
         for (int s = 0; s < FA_VST; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-        mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
-        mbar_init(&p_ready[0], 256); mbar_init(&p_ready[1], 256); mbar_init(pv_done, 1);
+        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -132,27 +134,32 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const uint32_t tmem_o = tmem_base + 128;
     pdl_wait();
 
     const int q_len = a.q_len[seq];
-    const int tok0 = tile * tpc;
+    const int tok0 = tile * (2 * tpc);
     const bool active = tok0 < q_len;             // uniform over the CTA
     const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
-    const int n_tok = active ? min(tpc, q_len - tok0) : 0;
-    const int pos_min = kv_before + tok0, pos_max = pos_min + n_tok - 1;
+    const int ng = q_len - tok0 > tpc ? 2 : 1;    // groups of 128 rows that hold tokens
+    const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + 2 * tpc, q_len) - 1;
     const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
-    const int t_lo = k_lo / FA_BN, t_hi = active ? pos_max / FA_BN + 1 : 0;
-    const int n_tiles = active ? t_hi - t_lo : 0;
+    int t_lo = k_lo / FA_BN, t_hi = active ? pos_max / FA_BN + 1 : t_lo;
+    if (a.n_splits > 1) {
+        const int per = (t_hi - t_lo + a.n_splits - 1) / a.n_splits;
+        t_lo = min(t_hi, t_lo + split * per);
+        t_hi = min(t_hi, t_lo + per);
+    }
+    const int n_tiles = t_hi - t_lo;
     const int head0 = kvh * g + hchunk * hpc;
     const int n_heads = min(hpc, g - hchunk * hpc);
 
     if (warp == 0) {
-        if (lane == 0 && active) {
-            mbar_expect_tx(q_full, (uint32_t)(hpc * tpc * 128 * FA_HB));      // the box is hpc x tpc rows of 128 bytes
+        if (lane == 0 && n_tiles > 0) {
+            mbar_expect_tx(q_full, (uint32_t)(ng * hpc * tpc * 128 * FA_HB));      // the box is hpc x tpc rows of 128 bytes
+            for (int gr = 0; gr < ng; ++gr)
 #pragma unroll
-            for (int hb = 0; hb < FA_HB; ++hb)
-                tma_load_3d(&map_q, q_full, sQ + hb * FA_QBLOCK_BYTES, hb * 64, head0, q_start + tok0);
+                for (int hb = 0; hb < FA_HB; ++hb)
+                    tma_load_3d(&map_q, q_full, sQ + gr * FA_Q_BYTES + hb * FA_QBLOCK_BYTES, hb * 64, head0, q_start + tok0 + gr * tpc);
             // key and value tiles go out independently, each as soon as its stage is free
             int jk = 0, jv = 0;
             uint32_t idle = 0;
@@ -188,70 +195,72 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0 && active) {
+    } else if (warp <= 2) {
+        // S of one group's rows.  Three warps issue products: one of 64 keys takes the tensor cores some 500 cycles, and one thread that issues
+        // S and P V of both groups in turn, with its waits and commits, some 1,900
+        const int group = warp - 1;
+        if (lane == 0 && n_tiles > 0 && group < ng) {
             constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN);
-            constexpr uint32_t idesc_pv = umma_idesc_bf16_b_mn(FA_BM, HD);
-            bool ok = mbar_wait(q_full, 0, abort_flag);
             // operand descriptors differ only in their start address (bits 0..13 of the low word, in 16-byte units)
-            const uint64_t dq = umma_desc_sw128(smem_u32(sQ));
-            const uint64_t dk = umma_desc_sw128(smem_u32(sK));
-            const uint64_t dv = umma_desc_sw128_mn(smem_u32(sV), FA_KBLOCK_BYTES);
-            const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, v_lo = (uint32_t)dv;
-            const uint32_t kq_hi = (uint32_t)(dq >> 32), v_hi = (uint32_t)(dv >> 32);
-            const uint32_t bar0 = smem_u32(bars);                        // barrier i lies at bar0 + 8 i
-            const uint32_t a_k_empty = bar0 + 8 * (uint32_t)(k_empty - bars), a_v_empty = bar0 + 8 * (uint32_t)(v_empty - bars);
-            const uint32_t a_s_full = bar0 + 8 * (uint32_t)(s_full - bars), a_pv_done = bar0 + 8 * (uint32_t)(pv_done - bars);
-            auto issue_pv = [&](int i, int st) -> bool {
-                if (!mbar_wait(&v_full[st], (uint32_t)((i / FA_VST) & 1), abort_flag)) return false;
-                if (!mbar_wait(&p_ready[i & 1], (uint32_t)((i >> 1) & 1), abort_flag)) return false;     // P written, O rescaled
-                tc_fence_after();
-                const uint32_t vs_lo = v_lo + (uint32_t)((st * FA_KV_BYTES) >> 4);
-                const uint32_t tp = tmem_base + (i & 1) * FA_BN;
-                umma_ts_lohi(tmem_o, tp, vs_lo, v_hi, idesc_pv, i > 0 ? 1u : 0u);
-#pragma unroll
-                for (int ks = 1; ks < FA_BN / 16; ++ks)
-                    umma_ts_lohi(tmem_o, tp + ks * 8, vs_lo + (uint32_t)((ks * 16 * 128) >> 4), v_hi, idesc_pv, 1u);
-                umma_commit_addr(a_pv_done);
-                umma_commit_addr(a_v_empty + 8 * st);
-                return true;
-            };
-            int kst = 0, vst = 0;                  // ring stages of key tile j and of value tile j - 1
+            const uint64_t dq = umma_desc_sw128(smem_u32(sQ + group * FA_Q_BYTES)), dk = umma_desc_sw128(smem_u32(sK));
+            const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, kq_hi = (uint32_t)(dq >> 32);
+            bool ok = mbar_wait(q_full, 0, abort_flag);
             for (int j = 0; j < n_tiles && ok; ++j) {
-                ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag);
-                // S of tile j goes where S and P of tile j - 2 were: the second product of tile j - 2,
-                // which reads that P, has to be complete (it was issued a tile ago, so this wait is short;
-                // issue order alone does not keep a product's writes behind its predecessor's reads)
-                if (ok && j >= 2) ok = mbar_wait(pv_done, (uint32_t)(j & 1), abort_flag);
+                const int kst = j % FA_KST;
+                ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag)
+                     && (j == 0 || mbar_wait(&s_free[group], (uint32_t)((j - 1) & 1), abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4);
-                const uint32_t ts = tmem_base + (j & 1) * FA_BN;
+                const uint32_t ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4), ts = tmem_base + FA_TMEM_S + group * FA_BN;
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint32_t qoff = ((ks >> 2) * FA_QBLOCK_BYTES + (ks & 3) * 32) >> 4, koff = ((ks >> 2) * FA_KBLOCK_BYTES + (ks & 3) * 32) >> 4;
                     umma_ss_lohi(ts, q_lo + qoff, kq_hi, ks_lo + koff, kq_hi, idesc_qk, ks > 0 ? 1u : 0u);
                 }
-                umma_commit_addr(a_s_full + 8 * (j & 1));
-                umma_commit_addr(a_k_empty + 8 * kst);
-                if (++kst == FA_KST) kst = 0;
-                if (j > 0) {
-                    ok = issue_pv(j - 1, vst);
-                    if (++vst == FA_VST) vst = 0;
-                }
+                umma_commit(&s_full[group]);
+                umma_commit(&k_empty[kst]);
+                if (ng == 1) umma_commit(&k_empty[kst]);       // for the group without tokens
             }
-            if (ok && n_tiles > 0) issue_pv(n_tiles - 1, vst);
         }
-    } else if (active) {
+    } else if (warp == 3) {
+        if (lane == 0 && n_tiles > 0) {
+            constexpr uint32_t idesc_pv = umma_idesc_bf16_b_mn(FA_BM, HD);
+            const uint64_t dv = umma_desc_sw128_mn(smem_u32(sV), FA_KBLOCK_BYTES);
+            const uint32_t v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
+            bool ok = true;
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const int vst = j % FA_VST;
+                const uint32_t vs_lo = v_lo + (uint32_t)((vst * FA_KV_BYTES) >> 4);
+                ok = mbar_wait(&v_full[vst], (uint32_t)((j / FA_VST) & 1), abort_flag);
+#pragma unroll
+                for (int group = 0; group < 2; ++group) {
+                    if (!ok || group >= ng) break;
+                    ok = mbar_wait(&p_ready[group], (uint32_t)(j & 1), abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t to = tmem_base + group * 128, tp = tmem_base + FA_TMEM_P + group * 32;
+#pragma unroll
+                    for (int ks = 0; ks < FA_BN / 16; ++ks)
+                        umma_ts_lohi(to, tp + ks * 8, vs_lo + (uint32_t)((ks * 16 * 128) >> 4), v_hi, idesc_pv, (ks > 0 || j > 0) ? 1u : 0u);
+                    umma_commit(&pv_done[group]);
+                }
+                if (ok) umma_commit(&v_empty[vst]);
+            }
+        }
+    } else if (active && (warp - FA_SOFTMAX) >> 3 < ng) {
+        const int group = (warp - FA_SOFTMAX) >> 3;                     // the first or the second 128 rows
+        const int tokg = tok0 + group * tpc, n_tok = min(tpc, q_len - tokg);
+        const int first = kv_before + tokg, last = first + n_tok - 1;             // the group's positions
         const int quarter = warp & 3;                          // tensor-memory lanes 32 * quarter ...
-        const int half = (warp - 2) >> 2;                      // this thread's half of a row's keys and result columns
-        const int pair = 1 + quarter;                          // the barrier of the two warps that share their rows
+        const int half = ((warp - FA_SOFTMAX) >> 2) & 1;                // this thread's half of a tile's keys
+        const int pair = 1 + group * 4 + quarter;              // the barrier of the two warps that share their rows
         const int r = quarter * 32 + lane;                     // this thread's row
         const int tl = r / hpc, hl = r - tl * hpc;
         const bool valid = tl < n_tok && hl < n_heads;
-        const int pos = valid ? pos_min + tl : -1;
+        const int pos = valid ? first + tl : -1;
         const int lo = (a.window > 0) ? pos - a.window + 1 : 0;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tmem_o = tmem_base + group * 128;
         float m = -INFINITY, l = 0.f;
         float r1 = 0.f, r2 = 0.f;                             // the row's distance bias
         if (BIAS && valid) { r1 = a.bias_slope[head0 + hl]; r2 = a.bias_rate[head0 + hl]; }
@@ -259,15 +268,17 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const float sc = BIAS || CAP ? 1.f : a.scale_log2;
         bool ok = true;
         for (int j = 0; j < n_tiles; ++j) {
-            const int st = j & 1;
             // (a warp whose wait ran out goes on to meet its partner at every barrier below, so that neither waits for the other for good)
-            const bool came = mbar_wait(&s_full[st], (uint32_t)((j >> 1) & 1), abort_flag);
+            const bool came = mbar_wait(&s_full[group], (uint32_t)(j & 1), abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
             tc_fence_after();
             float sv[32];
-            tmem_ld32(tmem_base + st * FA_BN + half * 32 + lane_addr, sv);
+            tmem_ld32(tmem_base + FA_TMEM_S + group * FA_BN + half * 32 + lane_addr, sv);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[group]);           // (one arrival a warp)
             const int key0 = (t_lo + j) * FA_BN + half * 32;
-            const bool all_visible = (key0 + 31 <= pos_min) && (a.window == 0 || key0 >= pos_max - a.window + 1);
+            const bool all_visible = (key0 + 31 <= first) && (a.window == 0 || key0 >= last - a.window + 1);
             if (BIAS) {                                       // keys after the query (a negative distance) are masked below
                 const float d0 = (float)(pos - key0);
 #pragma unroll
@@ -275,12 +286,12 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     sv[i] = fmaf(sv[i], a.scale_log2, -r1 * __log2f(fmaf(r2, d0 - (float)i, 1.f)));
             }
             if (CAP) softcap_scores<32>(sv, a.scale_log2, a.cap_log2);
-            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
             if (!all_visible) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     if (!(key0 + i <= pos && key0 + i >= lo)) sv[i] = -INFINITY;
             }
+            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 mx0 = fmaxf(mx0, sv[i]); mx1 = fmaxf(mx1, sv[i + 1]);
@@ -288,16 +299,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;     // scale > 0 commutes with the maximum
             if (!valid) mx = -INFINITY;
-            // raise m only when the tile towers over it; -inf + 8 = -inf, so the first finite maximum always does.  The barrier also says
-            // that both warps have their scores in registers: the probabilities go over them.
-            tc_fence_before();
+            // raise m only when the tile towers over it; -inf + 8 = -inf, so the first finite maximum always does
             const bool any = pair_any(pair, mx > m + FA_RAISE);
-            tc_fence_after();
             float factor = 1.f;
             if (any) {
-                share[j & 1][half][r] = mx;
+                share[group][j & 1][half][r] = mx;
                 pair_sync(pair);
-                mx = fmaxf(mx, share[j & 1][1 - half][r]);
+                mx = fmaxf(mx, share[group][j & 1][1 - half][r]);
                 if (mx > m + FA_RAISE) {
                     factor = fast_exp2(m - mx);                // exp2(-inf) = 0: nothing was summed yet
                     m = mx;
@@ -318,14 +326,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 pk[i] = *reinterpret_cast<uint32_t*>(&b);
             }
             l = l * factor + (sum0 + sum1);
-            tmem_st16_nowait(tmem_base + st * FA_BN + half * 16 + lane_addr, pk);      // over the first half of this row's scores
             if (j > 0) {
-                // every tile, the second product of the tile before is waited for: a parity wait only tells apart a barrier that is
-                // at most one phase off
-                const bool done = mbar_wait(pv_done, (uint32_t)((j - 1) & 1), abort_flag);
+                // the group's product before this one has read its probabilities and is in O (waited for at every turn: a parity only tells
+                // apart a barrier that is at most one phase off)
+                const bool done = mbar_wait(&pv_done[group], (uint32_t)((j - 1) & 1), abort_flag);
                 ok = __all_sync(0xffffffffu, done) && ok;
+                tc_fence_after();
                 if (ok && any) {                               // a half of the row's columns
-                    tc_fence_after();
 #pragma unroll
                     for (int h = 0; h < HD / 64; ++h) {
                         float ov[32];
@@ -336,44 +343,59 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                 }
             }
+            tmem_st16_nowait(tmem_base + FA_TMEM_P + group * 32 + half * 16 + lane_addr, pk);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&p_ready[st]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[group]);
         }
         if (n_tiles > 0) {
             pair_sync(pair);                                   // the last exchange has been read
-            share[0][half][r] = l;
+            share[group][0][half][r] = l;
             pair_sync(pair);
-            l += share[0][1 - half][r];
+            l += share[group][0][1 - half][r];
+            const bool done = mbar_wait(&pv_done[group], (uint32_t)((n_tiles - 1) & 1), abort_flag);
+            ok = __all_sync(0xffffffffu, done) && ok;
+            tc_fence_after();
         }
-        if (ok && n_tiles > 0) {
-            ok = mbar_wait(pv_done, (uint32_t)((n_tiles - 1) & 1), abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                tc_fence_after();
-                // the sink joins the sum where the row is finished: l counts in units of 2^m; a sink far above every
-                // score makes the sum infinite and the row zero, which is the limit
-                const float sk = (a.head_sinks && valid) ? a.head_sinks[head0 + hl] * 1.4426950408889634f : a.sink_log2;
-                float inv = a.out_scale / (a.has_sink ? l + exp2f(sk - m) : l);
-                if (a.head_gate && valid)
-                    inv *= 1.f / (1.f + __expf(-__bfloat162float(a.head_gate[(size_t)(q_start + tok0 + tl) * a.gate_stride + head0 + hl])));
-                __nv_bfloat16* dst = a.out + (size_t)(q_start + tok0 + tl) * a.out_stride + (size_t)(head0 + hl) * HD + half * (HD / 2);
+        const size_t row = (size_t)(q_start + tokg + tl);
+        const int head = head0 + hl;
+        float inv = 1.f;
+        if (a.n_splits == 1 && valid) {
+            // the sink joins the sum where the row is finished: l counts in units of 2^m; a sink far above every
+            // score makes the sum infinite and the row zero, which is the limit
+            const float sk = a.head_sinks ? a.head_sinks[head] * 1.4426950408889634f : a.sink_log2;
+            inv = a.out_scale / (a.has_sink ? l + exp2f(sk - m) : l);
+            if (a.head_gate) inv *= 1.f / (1.f + __expf(-__bfloat162float(a.head_gate[row * a.gate_stride + head])));
+        }
+        const size_t at = (row * a.nqh + head) * a.n_splits + split;
+        if (a.n_splits > 1 && valid && half == 0)
+            *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(m, l);
 #pragma unroll
-                for (int h = 0; h < HD / 64; ++h) {
-                    float ov[32];
-                    tmem_ld32(tmem_o + half * (HD / 2) + h * 32 + lane_addr, ov);
-                    if (valid) {
+        for (int h = 0; h < HD / 64; ++h) {                    // a half of the row's columns
+            const int c0 = half * (HD / 2) + h * 32;
+            float ov[32];
+            if (n_tiles > 0) {
+                tmem_ld32(tmem_o + c0 + lane_addr, ov);
+            } else {                                           // a slice without a key
 #pragma unroll
-                        for (int c = 0; c < 32; c += 8) {
-                            uint32_t w[4];
+                for (int i = 0; i < 32; ++i) ov[i] = 0.f;
+            }
+            if (ok && valid && a.n_splits > 1) {
+                float* dst = a.partial + at * HD + c0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                __nv_bfloat162 b = __floats2bfloat162_rn(ov[c + 2 * i] * inv, ov[c + 2 * i + 1] * inv);
-                                w[i] = *reinterpret_cast<uint32_t*>(&b);
-                            }
-                            *reinterpret_cast<uint4*>(dst + h * 32 + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
+            } else if (ok && valid) {
+                __nv_bfloat16* dst = a.out + row * a.out_stride + (size_t)head * HD + c0;
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __nv_bfloat162 b = __floats2bfloat162_rn(ov[c + 2 * i] * inv, ov[c + 2 * i + 1] * inv);
+                        w[i] = *reinterpret_cast<uint32_t*>(&b);
                     }
+                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
@@ -407,7 +429,9 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     if (!fn) BRAID_REFUSE("attn_kv4: the driver does not export cuTensorMapEncodeTiled");
     const int g = a.nqh / a.nkh;
     const int hpc = g < FA_BM ? g : FA_BM, tpc = FA_BM / hpc, hchunks = (g + hpc - 1) / hpc;
-    const long long gx = (a.max_q_len + tpc - 1) / tpc;
+    if (a.n_splits < 1) a.n_splits = 1;
+    if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: slices need the partial buffer");
+    const long long gx = (long long)((a.max_q_len + 2 * tpc - 1) / (2 * tpc)) * a.n_splits;
     if (gx > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld token tiles, %d sequences)", gx, a.n_seqs);
     if ((long long)a.n_seqs * a.cols * 2 * a.nkh * FA_PAGE > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the pages' rows pass 32 bits");
