@@ -18,33 +18,39 @@
 #if BRAID_HD == 64 || BRAID_HD == 128
 
 #define FA_BM 128
-#define FA_BN 64                                 // keys per tile: one page
+#define FA_BN 128                                // keys per tile: two pages
 #define FA_PAGE BRAID_PAGE_SIZE
-static_assert(FA_PAGE == 64, "a key tile of this kernel is one page of 64 positions");
-#define FA_SOFTMAX 4                             // warps before: TMA, S of either group, P V (20 warps in all: 5 a quarter of the SM)
+static_assert(FA_PAGE == 64, "a key tile of this kernel is two pages of 64 positions");
+#define FA_SOFTMAX 4                             // warps before: TMA, S, one that only waits for the end, P V
 #define FA_THREADS ((FA_SOFTMAX + 16) * 32)      // two groups of 8 softmax warps
 #define FA_HB (BRAID_HD / 64)                    // 64-element blocks of the head dimension
 #define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] bf16, 128-byte rows
-#define FA_KBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]
+#define FA_PBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]: what a copy brings
+#define FA_KBLOCK_BYTES (2 * FA_PBLOCK_BYTES)    // two pages on end
 #define FA_Q_BYTES (FA_HB * FA_QBLOCK_BYTES)
 #define FA_KV_BYTES (FA_HB * FA_KBLOCK_BYTES)    // one K or one V tile
-#define FA_KST 4                                 // stages of the key ring
-#define FA_VST 4                                 // stages of the value ring
+#define FA_KST 2                                 // stages of the key ring
+#define FA_VST 2                                 // stages of the value ring
 #define FA_BAR_BYTES 256
 #define FA_SMEM (2 * FA_Q_BYTES + (FA_KST + FA_VST) * FA_KV_BYTES + FA_BAR_BYTES)
-// tensor memory: O of the first 128 rows [0, 128), of the others [128, 256); scores of either [256, 384), P of either [448, 512)
+// tensor memory: O of the first 128 rows [0, 128), of the others [128, 256); the scores of both in turn [256, 384); P of either [384, 448), [448, 512)
 #define FA_TMEM_COLS 512
 #define FA_TMEM_S 256
-#define FA_TMEM_P 448
+#define FA_TMEM_P 384
 
-// The two warps of a pair (64 threads): whether any of them says yes, and a plain meeting.
+// The two warps of a pair (64 threads): whether any of them says yes, and a plain meeting.  These barriers leave a warp's lanes free to part,
+// and the accesses to tensor memory behind them want them together: hence the __syncwarp.
 __device__ __forceinline__ bool pair_any(int id, bool yes) {
     uint32_t any;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(any) : "r"((uint32_t)yes), "r"(id) : "memory");
+    __syncwarp();
     return any != 0;
 }
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void pair_sync(int id) {
+    asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
+    __syncwarp();
+}
 // 16 consecutive columns of this thread's lane written (no wait).
 __device__ __forceinline__ void tmem_st16_nowait(uint32_t taddr, const uint32_t* w) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -122,7 +128,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 2); }
+        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
         for (int s = 0; s < FA_VST; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
         *abort_flag = 0;
@@ -143,13 +149,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int ng = q_len - tok0 > tpc ? 2 : 1;    // groups of 128 rows that hold tokens
     const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + 2 * tpc, q_len) - 1;
     const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
-    int t_lo = k_lo / FA_BN, t_hi = active ? pos_max / FA_BN + 1 : t_lo;
-    if (a.n_splits > 1) {
-        const int per = (t_hi - t_lo + a.n_splits - 1) / a.n_splits;
-        t_lo = min(t_hi, t_lo + split * per);
-        t_hi = min(t_hi, t_lo + per);
+    int page_lo = k_lo / FA_PAGE, page_hi = active ? pos_max / FA_PAGE + 1 : page_lo;
+    if (a.n_splits > 1) {                         // slices of whole tiles
+        const int per = ((page_hi - page_lo + 1) / 2 + a.n_splits - 1) / a.n_splits * 2;
+        page_lo = min(page_hi, page_lo + split * per);
+        page_hi = min(page_hi, page_lo + per);
     }
-    const int n_tiles = t_hi - t_lo;
+    const int n_tiles = (page_hi - page_lo + 1) / 2;
     const int head0 = kvh * g + hchunk * hpc;
     const int n_heads = min(hpc, g - hchunk * hpc);
 
@@ -170,18 +176,23 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const bool v_turn = !k_turn && jv < n_tiles && mbar_try_wait(&v_empty[jv % FA_VST], (uint32_t)((jv / FA_VST) & 1) ^ 1u);
                 if (k_turn || v_turn) {
                     const int j = k_turn ? jk : jv;
-                    int page = seq * a.cols + t_lo + j;
-                    if (t_lo + j >= a.cols) {                       // more keys than the caller said
-                        atomicExch(a.error_flag, 1);
-                        page = 0;
-                    }
-                    const int row = ((page * 2 + (k_turn ? 0 : 1)) * a.nkh + kvh) * FA_PAGE;
                     const int st = k_turn ? jk % FA_KST : jv % FA_VST;
                     uint64_t* bar = k_turn ? &k_full[st] : &v_full[st];
                     uint8_t* dst = (k_turn ? sK : sV) + st * FA_KV_BYTES;
                     mbar_expect_tx(bar, FA_KV_BYTES);
 #pragma unroll
-                    for (int hb = 0; hb < FA_HB; ++hb) tma_load_2d(&map_kv, bar, dst + hb * FA_KBLOCK_BYTES, hb * 64, row);
+                    for (int b = 0; b < 2; ++b) {
+                        // behind an odd number of pages the last one again: masked, and multiplied by 0
+                        int c = min(page_lo + 2 * j + b, page_hi - 1);
+                        if (c >= a.cols) {                          // more keys than the caller said
+                            atomicExch(a.error_flag, 1);
+                            c = 0;
+                        }
+                        const int row = (((seq * a.cols + c) * 2 + (k_turn ? 0 : 1)) * a.nkh + kvh) * FA_PAGE;
+#pragma unroll
+                        for (int hb = 0; hb < FA_HB; ++hb)
+                            tma_load_2d(&map_kv, bar, dst + hb * FA_KBLOCK_BYTES + b * FA_PBLOCK_BYTES, hb * 64, row);
+                    }
                     if (k_turn) ++jk; else ++jv;
                     moved = true;
                 }
@@ -195,31 +206,32 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
             }
         }
-    } else if (warp <= 2) {
-        // S of one group's rows.  Three warps issue products: one of 64 keys takes the tensor cores some 500 cycles, and one thread that issues
-        // S and P V of both groups in turn, with its waits and commits, some 1,900
-        const int group = warp - 1;
-        if (lane == 0 && n_tiles > 0 && group < ng) {
+    } else if (warp == 1) {
+        // S of either group in turn, in one place: the next goes there when the one before is in registers
+        if (lane == 0 && n_tiles > 0) {
             constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN);
             // operand descriptors differ only in their start address (bits 0..13 of the low word, in 16-byte units)
-            const uint64_t dq = umma_desc_sw128(smem_u32(sQ + group * FA_Q_BYTES)), dk = umma_desc_sw128(smem_u32(sK));
-            const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, kq_hi = (uint32_t)(dq >> 32);
+            const uint64_t dq = umma_desc_sw128(smem_u32(sQ)), dk = umma_desc_sw128(smem_u32(sK));
+            const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, kq_hi = (uint32_t)(dq >> 32), ts = tmem_base + FA_TMEM_S;
             bool ok = mbar_wait(q_full, 0, abort_flag);
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const int kst = j % FA_KST;
-                ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag)
-                     && (j == 0 || mbar_wait(&s_free[group], (uint32_t)((j - 1) & 1), abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4), ts = tmem_base + FA_TMEM_S + group * FA_BN;
+                ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag);
+                for (int group = 0; group < ng && ok; ++group) {
+                    // the one before: the first group's of this tile, or the last group's of the tile before
+                    if (group) ok = mbar_wait(&s_free[0], (uint32_t)(j & 1), abort_flag);
+                    else if (j > 0) ok = mbar_wait(&s_free[ng - 1], (uint32_t)((j - 1) & 1), abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t qs_lo = q_lo + (uint32_t)((group * FA_Q_BYTES) >> 4), ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4);
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t qoff = ((ks >> 2) * FA_QBLOCK_BYTES + (ks & 3) * 32) >> 4, koff = ((ks >> 2) * FA_KBLOCK_BYTES + (ks & 3) * 32) >> 4;
-                    umma_ss_lohi(ts, q_lo + qoff, kq_hi, ks_lo + koff, kq_hi, idesc_qk, ks > 0 ? 1u : 0u);
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        const uint32_t qoff = ((ks >> 2) * FA_QBLOCK_BYTES + (ks & 3) * 32) >> 4, koff = ((ks >> 2) * FA_KBLOCK_BYTES + (ks & 3) * 32) >> 4;
+                        umma_ss_lohi(ts, qs_lo + qoff, kq_hi, ks_lo + koff, kq_hi, idesc_qk, ks > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[group]);
                 }
-                umma_commit(&s_full[group]);
-                umma_commit(&k_empty[kst]);
-                if (ng == 1) umma_commit(&k_empty[kst]);       // for the group without tokens
+                if (ok) umma_commit(&k_empty[kst]);
             }
         }
     } else if (warp == 3) {
@@ -232,13 +244,11 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const int vst = j % FA_VST;
                 const uint32_t vs_lo = v_lo + (uint32_t)((vst * FA_KV_BYTES) >> 4);
                 ok = mbar_wait(&v_full[vst], (uint32_t)((j / FA_VST) & 1), abort_flag);
-#pragma unroll
-                for (int group = 0; group < 2; ++group) {
-                    if (!ok || group >= ng) break;
+                for (int group = 0; group < ng && ok; ++group) {
                     ok = mbar_wait(&p_ready[group], (uint32_t)(j & 1), abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t to = tmem_base + group * 128, tp = tmem_base + FA_TMEM_P + group * 32;
+                    const uint32_t to = tmem_base + group * 128, tp = tmem_base + FA_TMEM_P + group * 64;
 #pragma unroll
                     for (int ks = 0; ks < FA_BN / 16; ++ks)
                         umma_ts_lohi(to, tp + ks * 8, vs_lo + (uint32_t)((ks * 16 * 128) >> 4), v_hi, idesc_pv, (ks > 0 || j > 0) ? 1u : 0u);
@@ -247,7 +257,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (ok) umma_commit(&v_empty[vst]);
             }
         }
-    } else if (active && (warp - FA_SOFTMAX) >> 3 < ng) {
+    } else if (warp >= FA_SOFTMAX && active && (warp - FA_SOFTMAX) >> 3 < ng) {
         const int group = (warp - FA_SOFTMAX) >> 3;                     // the first or the second 128 rows
         const int tokg = tok0 + group * tpc, n_tok = min(tpc, q_len - tokg);
         const int first = kv_before + tokg, last = first + n_tok - 1;             // the group's positions
@@ -272,28 +282,28 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const bool came = mbar_wait(&s_full[group], (uint32_t)(j & 1), abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
             tc_fence_after();
-            float sv[32];
-            tmem_ld32(tmem_base + FA_TMEM_S + group * FA_BN + half * 32 + lane_addr, sv);
+            float sv[64];
+            tmem_ld32x2(tmem_base + FA_TMEM_S + half * 64 + lane_addr, sv);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[group]);           // (one arrival a warp)
-            const int key0 = (t_lo + j) * FA_BN + half * 32;
-            const bool all_visible = (key0 + 31 <= first) && (a.window == 0 || key0 >= last - a.window + 1);
+            const int key0 = page_lo * FA_PAGE + j * FA_BN + half * 64;
+            const bool all_visible = (key0 + 63 <= first) && (a.window == 0 || key0 >= last - a.window + 1);
             if (BIAS) {                                       // keys after the query (a negative distance) are masked below
                 const float d0 = (float)(pos - key0);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 64; ++i)
                     sv[i] = fmaf(sv[i], a.scale_log2, -r1 * __log2f(fmaf(r2, d0 - (float)i, 1.f)));
             }
-            if (CAP) softcap_scores<32>(sv, a.scale_log2, a.cap_log2);
+            if (CAP) softcap_scores<64>(sv, a.scale_log2, a.cap_log2);
             if (!all_visible) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 64; ++i)
                     if (!(key0 + i <= pos && key0 + i >= lo)) sv[i] = -INFINITY;
             }
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+            for (int i = 0; i < 64; i += 4) {
                 mx0 = fmaxf(mx0, sv[i]); mx1 = fmaxf(mx1, sv[i + 1]);
                 mx2 = fmaxf(mx2, sv[i + 2]); mx3 = fmaxf(mx3, sv[i + 3]);
             }
@@ -313,37 +323,44 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             // a row that is no query (past the tile's tokens or heads) sums nothing: exp2(-inf) = 0
             const float ms = !valid ? INFINITY : ((m == -INFINITY) ? 0.f : m);
-            // probabilities, rounded to bfloat16
-            float sum0 = 0.f, sum1 = 0.f;
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p0 = fast_exp2(fmaf(sv[2 * i], sc, -ms));
-                const float p1 = fast_exp2(fmaf(sv[2 * i + 1], sc, -ms));
-                sum0 += p0;
-                sum1 += p1;
-                __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-                pk[i] = *reinterpret_cast<uint32_t*>(&b);
-            }
-            l = l * factor + (sum0 + sum1);
             if (j > 0) {
                 // the group's product before this one has read its probabilities and is in O (waited for at every turn: a parity only tells
                 // apart a barrier that is at most one phase off)
                 const bool done = mbar_wait(&pv_done[group], (uint32_t)((j - 1) & 1), abort_flag);
                 ok = __all_sync(0xffffffffu, done) && ok;
                 tc_fence_after();
-                if (ok && any) {                               // a half of the row's columns
+            }
+            // probabilities, rounded to bfloat16
+            float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-                    for (int h = 0; h < HD / 64; ++h) {
-                        float ov[32];
-                        tmem_ld32(tmem_o + half * (HD / 2) + h * 32 + lane_addr, ov);
+            for (int c = 0; c < 2; ++c) {
+                uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ov[i] *= factor;
-                        tmem_st32_nowait(tmem_o + half * (HD / 2) + h * 32 + lane_addr, reinterpret_cast<const uint32_t*>(ov));
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const float p0 = fast_exp2(fmaf(sv[c * 32 + 2 * i], sc, -ms));
+                    const float p1 = fast_exp2(fmaf(sv[c * 32 + 2 * i + 1], sc, -ms));
+                    sum0 += p0;
+                    sum1 += p1;
+                    __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
+                    pk[i] = *reinterpret_cast<uint32_t*>(&b);
+                }
+                __syncwarp();
+                tmem_st16_nowait(tmem_base + FA_TMEM_P + group * 64 + half * 32 + c * 16 + lane_addr, pk);
+            }
+            l = l * factor + (sum0 + sum1);
+            __syncwarp();
+            if (any && j > 0) {                                // (the same for every lane)
+                // a half of the row's columns
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h) {
+                    float ov[32];
+                    tmem_ld32(tmem_o + half * (HD / 2) + h * 32 + lane_addr, ov);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) ov[i] *= factor;
+                    __syncwarp();
+                    tmem_st32_nowait(tmem_o + half * (HD / 2) + h * 32 + lane_addr, reinterpret_cast<const uint32_t*>(ov));
                 }
             }
-            tmem_st16_nowait(tmem_base + FA_TMEM_P + group * 32 + half * 16 + lane_addr, pk);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -375,6 +392,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int h = 0; h < HD / 64; ++h) {                    // a half of the row's columns
             const int c0 = half * (HD / 2) + h * 32;
             float ov[32];
+            __syncwarp();
             if (n_tiles > 0) {
                 tmem_ld32(tmem_o + c0 + lane_addr, ov);
             } else {                                           // a slice without a key

@@ -400,7 +400,8 @@ kv4_expand_kernel(const ExpandArgs a) {
         const int h0 = w, h1 = W + w;
         const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
         const uint32_t both = in ? v0 | (v1 << 16) : 0u;
-        if (a.repair && ((vg[w] & 0x7f80u) == 0x7f80u || (vg[w] & 0x7f800000u) == 0x7f800000u)) {
+        // NaN, or a step of 2^122 or a lowest value of 2^127 or more, from which a number may round to infinity
+        if (a.repair && ((vg[w] & 0x7f80u) >= 0x7c80u || (vg[w] & 0x7f800000u) >= 0x7f000000u)) {
             vg[w] = 0u;
             a.repair[1 + a.seq0 + seq] = 1;
             a.repair[0] = 1;
