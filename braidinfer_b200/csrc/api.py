@@ -140,9 +140,9 @@ class RowScale:
 
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
-_KV4_ARGS = struct.Struct("<15Q3q12i4f4i")
-_KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7fi")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
-_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q10i")
+_KV4_ARGS = struct.Struct("<15Q3q12i4f6i")
+_KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7f3i")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
+_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q11i4x")
 
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
 
@@ -829,12 +829,12 @@ class Kernels:
         self._on_device("kv4_expand", cache, out)
         self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
 
-    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_table=None, repair=None, seq0=0) -> None:
+    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_table=None, repair=None, seq0=0, q_from=0) -> None:
         self.launches += 1
         args = _EXPAND_ARGS.pack(cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), q_len.data_ptr(), kv_before.data_ptr(),
                                  self._error_flag.data_ptr() + 16, _ptr(repair) or 0, _ptr(out_table) or 0, n, cache.shape[1], hd,
                                  page_table.shape[1], cache.shape[0], window, keep_first, out_table.shape[1] if out_table is not None else 0,
-                                 seq0, dtype_code(out.dtype))
+                                 seq0, dtype_code(out.dtype), q_from)
         self._check_lib(lib, lib.braid_kv4_expand(args, self._stream()), "kv4_expand")
 
     def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -873,11 +873,18 @@ class Kernels:
         self._on_device(what, q, out, cache, head_sinks, head_gate, head_scale, *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
-        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, n_seqs, nqh, nkh):
+        tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
+        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, n_seqs, nqh, nkh, tc):
+            # a step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are (where the others are short
+            # on average, and some may be so short)
+            few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 64 * (n_seqs - 1) else 0
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                  int(window or 0), scale, int(keep_first or 0), head_scale, dict(
                                      sink=sink, out_scale=out_scale, head_sinks=head_sinks, head_gate=head_gate, distance_bias=distance_bias,
-                                     softcap=softcap))
+                                     softcap=softcap), tc, few + 1 if few else 0)
+            if few:
+                self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, few, max_kv_len, nqh, nkh, hd,
+                                   int(window or 0), scale, sink, out_scale, head_sinks, head_gate, 0, None, distance_bias, softcap, settled, few)
             return
         if backend == "auto":
             self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
@@ -907,6 +914,8 @@ class Kernels:
             lib.braid_last_error.restype = c_char_p
             lib.braid_attn_kv4.argtypes = [c_char_p, c_void_p]
             lib.braid_attn_kv4.restype = c_int
+            lib.braid_attn_kv4_merge.argtypes = [c_char_p, c_void_p]
+            lib.braid_attn_kv4_merge.restype = c_int
             if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
                 raise KernelError("the attention library over a 4-bit cache is another than was asked for")
             if self.attn_tc_supports(head_dim):
@@ -921,23 +930,25 @@ class Kernels:
     # The most that the pages of a step's prompts, read back for attention, may take at once: more sequences go one group after another.
     KV4_PAGES_BYTES = 1 << 30
 
-    # Prompts of at least so many (16 columns of queries, kv head, sequence) have their pages read back once for all of them.  The kernel
-    # over 4 bits reads them for every 16 columns, sliced over the machine; the one over ordinary pages takes 128 columns a CTA, which
-    # walks the context alone.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: 32 tokens of 4 sequences
-    # behind 8,000 (256 of them) 187 / 120, 64 tokens (512) 193 / 200, 512 tokens (4,096) 317 / 1,198; of one behind 32,000: 128 tokens (256)
-    # 646 / 450, 512 tokens (1,024) 667 / 1,782; without a context, 128 tokens 13.7 / 11.2, 512 tokens 21 / 48.
-    KV4_PAGES_FROM = 400
+    # FIGURES_CROSS
+    KV4_PAGES_FROM, KV4_PAGES_WORK = 300, 200_000
 
     @staticmethod
-    def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, n_seqs: int, nqh: int, nkh: int) -> bool:
-        """Whether attention reads the step's pages back and runs over ordinary ones."""
+    def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, max_kv_len: int, n_seqs: int, nqh: int, nkh: int, tc: bool) -> bool:
+        """Whether attention reads the step's pages back and runs over those."""
+        if max_q_len <= 8 or out.dtype != torch.bfloat16:
+            return False
         g = nqh // nkh
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
-        return (max_q_len > 8 and tiles * nkh * n_seqs >= Kernels.KV4_PAGES_FROM and out.dtype == torch.bfloat16 and q.stride(0) % 8 == 0
-                and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0)
+        units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
+        if tc:
+            worth = units >= Kernels.KV4_PAGES_FROM or (units >= 64 and units * max_kv_len >= Kernels.KV4_PAGES_WORK)
+        else:
+            worth = 3 * units >= Kernels.KV4_PAGES_FROM * (4 if max_kv_len < 1000 else 10)
+        return worth and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
     def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
-                        scale, keep_first, head_scale, options) -> None:
+                        scale, keep_first, head_scale, options, tc, q_from) -> None:
         """Prompts, bfloat16: the pages that the queries see are read back, block c of sequence i as page i * cols + c of a workspace,
         and the attention of ordinary pages runs over them.  Values that are NaN are read back as zero, and the sequences that hold some
         are computed by the plain kernel (which otherwise ends at once)."""
@@ -950,31 +961,56 @@ class Kernels:
         table = torch.empty((group, cols), dtype=torch.int32, device=out.device)
         repair = torch.zeros(n_seqs + 1, dtype=torch.int32, device=out.device)
         fence = repair.new_empty(1)
-        tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(options["softcap"])
-                                                                                     or options["distance_bias"] is not None)
         prompt = self.kv4_attention_library(hd)
+        n_splits = self._kv4_prompt_slices(out.shape[0], group, max_q_len, max_kv_len, nqh, nkh, hd, window) if tc else 1
+        partial = None
+        if n_splits > 1:
+            partial = torch.empty(out.shape[0] * nqh * n_splits * (hd + 2), dtype=torch.float32, device=out.device)
+        gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
         for i in range(0, n_seqs, group):
             n = min(group, n_seqs - i)
             part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
-            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, table, repair, i)
+            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, table, repair, i, q_from)
             if tc:
-                gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
                 args = _KV4_PROMPT_ARGS.pack(
                     q.data_ptr(), pages.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in part), self._error_flag.data_ptr() + 12,
                     _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0),
-                    gate.stride(0) if gate is not None else 0, 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
-                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0, 1)
+                    gate.stride(0) if gate is not None else 0, _ptr(partial) or 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
+                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0)
                 self.launches += 1
                 self._check_lib(prompt, prompt.braid_attn_kv4_prompt(args, self._stream()), "attn_kv4")
             else:
                 fence.zero_()        # that kernel reads pages of earlier tokens before its predecessor has ended; not before something else has
                 self.attn_mma(q, out, pages, table, *part, token_seq, n, max_q_len, nqh, nkh, hd, window, scale, keep_first=keep_first,
                               head_scale=head_scale, **options)
+        if partial is not None:
+            args = _KV4_ARGS.pack(
+                0, out.data_ptr(), partial.data_ptr(), 0, 0, 0, q_len.data_ptr(), 0, token_seq.data_ptr(), _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, 0, 0, 0,
+                self._error_flag.data_ptr() + 16, 0, out.stride(0), gate.stride(0) if gate is not None else 0, out.shape[0], n_seqs, max_q_len,
+                nqh, nkh, 0, 0, 0, 0, n_splits, int(options["sink"] is not None), 0, scale, options["sink"] or 0.0, options["out_scale"], 0.0, 0, 0, 0, q_from, 0, 0)
+            self.launches += 1
+            self._check_lib(prompt, prompt.braid_attn_kv4_merge(args, self._stream()), "attn_kv4")
         self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale,
                              **options, repair=repair)
 
+    def _kv4_prompt_slices(self, rows: int, n_seqs: int, max_q_len: int, max_kv_len: int, nqh: int, nkh: int, hd: int, window: int) -> int:
+        """Slices of the context for prompts over pages that were read back: a CTA takes 256 columns of queries, one an SM."""
+        g = nqh // nkh
+        tokens = 2 * (128 // min(g, 128))
+        ctas = nkh * -(-g // 128) * min(n_seqs * -(-max_q_len // tokens), rows // tokens + n_seqs)
+        most = min(max_kv_len, window + tokens) if window else max_kv_len
+        mean = most if window else max(1, max_kv_len - max_q_len // 2)
+        sms = torch.cuda.get_device_properties(self._device_index).multi_processor_count
+
+        def cost(n: int) -> float:
+            """us: 1.55 for 128 keys of a CTA; 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
+            (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 226, 249, 190, 214, 197, 217)"""
+            rounds = -(-ctas * n // sms)
+            return max(most, rounds * mean) / 128 / n * 1.55 + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
+        return min(range(1, max(1, min(8, most // 512)) + 1), key=cost)
+
     def _attn_kv4_mma(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
-                      scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled) -> None:
+                      scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled, q_to=0) -> None:
         lib = self.kv4_attention_library(hd)
         f32, g, rows = int(out.dtype == torch.float32), nqh // nkh, out.shape[0]
         key = (min(g * max_q_len, 9), f32)
@@ -997,14 +1033,14 @@ class Kernels:
         partial = None
         if n_splits > 1 and not cluster:
             # from torch's allocator at every call: calls on other streams, and other graphs, have their own
-            partial = torch.empty(rows * nqh * n_splits * (hd + 2), dtype=torch.float32, device=out.device)
+            partial = torch.empty((n_seqs * q_to if q_to else rows) * nqh * n_splits * (hd + 2), dtype=torch.float32, device=out.device)
         bias = distance_bias or (None, None)
         args = _KV4_ARGS.pack(
             q.data_ptr(), out.data_ptr(), _ptr(partial) or 0, cache.data_ptr(), page_table.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
             kv_before.data_ptr(), token_seq.data_ptr(), _ptr(head_sinks) or 0, _ptr(head_gate) or 0, _ptr(head_scale) or 0, _ptr(bias[0]) or 0,
             _ptr(bias[1]) or 0, self._error_flag.data_ptr() + 16, q.stride(0), out.stride(0), head_gate.stride(0) if head_gate is not None else 0,
             rows, n_seqs, max_q_len, nqh, nkh, page_table.shape[1], cache.shape[0], window, keep_first, n_splits, int(sink is not None),
-            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns, int(cluster), 0)
+            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns, int(cluster), 0, q_to, 0)
         self.launches += 1 + (partial is not None)
         self._check_lib(lib, lib.braid_attn_kv4(args, self._stream()), "attn_kv4")
 

@@ -51,11 +51,37 @@ struct Kv4Args {
     int rows, n_seqs, max_q_len, nqh, nkh, cols, num_pages, window, keep_first, n_splits, has_sink, settled;
     float scale, sink, out_scale, softcap;
     int f32, columns;            // float32 rows; columns a CTA
-    int cluster, unused;         // the slices (up to 8) are CTAs of a cluster, which merges them
+    int cluster;                 // the slices are CTAs of a cluster, which merges them
+    int q_from, q_to;            // (0: no bound) only sequences that bring at least, at most so many tokens
+    int partial_rows;            // rows of `partial`: `rows`, or with q_to n_seqs * q_to (sequence, token)
 };
 
 #define LOG2E 1.4426950408889634f
 #define KV4_RAISE 4.f
+
+// What a merged row is multiplied by: 1 / its sum, the sink's share in it, and the head's gate.
+template <typename T>
+__device__ __forceinline__ float kv4_finish(const Kv4Args& a, float M, float L, int row, int head, const T*) {
+    float f = 1.f;
+    if (a.has_sink) {                                          // one more score, with no value
+        const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
+        f = exp2f(M - mn);
+        L = L * f + exp2f(sk - mn);
+    }
+    float inv = f * a.out_scale / L;
+    if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[(size_t)row * a.gate_stride + head])));
+    return inv;
+}
+
+// The row whose slices are row `prow` of `partial`, or -1: none.
+__device__ __forceinline__ int kv4_merged_row(const Kv4Args& a, int prow) {
+    if (a.q_to > 0) {
+        const int seq = prow / a.q_to, t = prow - seq * a.q_to, n = a.q_len[seq];
+        return n <= a.q_to && t < n ? a.q_start[seq] + t : -1;
+    }
+    const int seq = a.token_seq[prow];
+    return seq < 0 || (a.q_from > 0 && a.q_len[seq] < a.q_from) ? -1 : prow;
+}
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -196,7 +222,7 @@ attn_kv4_kernel(const Kv4Args a) {
     const int unit = gridDim.z - 1 - blockIdx.z;              // late tokens, which see the most, first
     const int tile = unit / a.n_splits, split = unit - tile * a.n_splits;
     const int q_len = a.q_len[seq], tok0 = tile * tpc;
-    if (tok0 >= q_len) return;
+    if (tok0 >= q_len || (a.q_to > 0 && q_len > a.q_to)) return;
     const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
     const int n_tok = min(tpc, q_len - tok0);
     const int head0 = kvh * g + hchunk * hpc, n_heads = min(hpc, g - hchunk * hpc);
@@ -700,19 +726,12 @@ attn_kv4_kernel(const Kv4Args a) {
         float4 x;
         merge(col, d, a.cluster ? a.n_splits : 1, M, L, x);
         if (a.n_splits > 1 && !a.cluster) {
-            const size_t at = (row * a.nqh + head) * a.n_splits + split;
+            const size_t prow = a.q_to > 0 ? (size_t)seq * a.q_to + tok0 + tl : row, at = (prow * a.nqh + head) * a.n_splits + split;
             *reinterpret_cast<float4*>(a.partial + at * HD + d) = x;
-            if (d == 0) *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(M, L);
+            if (d == 0) *reinterpret_cast<float2*>(a.partial + (size_t)a.partial_rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(M, L);
             continue;
         }
-        float f = 1.f;
-        if (a.has_sink) {                                      // one more score, with no value
-            const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
-            f = exp2f(M - mn);
-            L = L * f + exp2f(sk - mn);
-        }
-        float inv = f * a.out_scale / L;
-        if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[row * a.gate_stride + head])));
+        const float inv = kv4_finish(a, M, L, (int)row, head, (T*)nullptr);
         T* dst = (T*)a.out + row * a.out_stride + (size_t)head * HD + d;
         __align__(16) T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
         if (!out_wide) {
@@ -734,12 +753,12 @@ attn_kv4_merge_kernel(const Kv4Args a) {
     pdl_wait();
     __shared__ float4 so[G][Q];
     __shared__ float2 sm[G];
-    const int rh = blockIdx.x, row = rh / a.nqh, head = rh - row * a.nqh;
-    if (a.token_seq[row] < 0) return;
+    const int rh = blockIdx.x, head = rh % a.nqh, row = kv4_merged_row(a, rh / a.nqh);
+    if (row < 0) return;
     const int g = threadIdx.x / Q, q = threadIdx.x - g * Q;
     const bool works = g < G;
     const float* po = a.partial + (size_t)rh * a.n_splits * HD + q * 4;
-    const float2* pm = reinterpret_cast<const float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD) + (size_t)rh * a.n_splits;
+    const float2* pm = reinterpret_cast<const float2*>(a.partial + (size_t)a.partial_rows * a.nqh * a.n_splits * HD) + (size_t)rh * a.n_splits;
     float M = -INFINITY, L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     auto join = [&](float m, float l, const float4& y) {       // a share without a finite score has weight 0: nothing of zeros, all of a NaN
@@ -770,18 +789,63 @@ attn_kv4_merge_kernel(const Kv4Args a) {
     __syncthreads();
     if (threadIdx.x >= Q) return;
     for (int i = 1; i < G; ++i) join(sm[i].x, sm[i].y, so[i][q]);
-    float f = 1.f;
-    if (a.has_sink) {
-        const float sk = (a.head_sinks ? a.head_sinks[head] : a.sink) * LOG2E, mn = fmaxf(M, sk);
-        f = exp2f(M - mn);
-        L = L * f + exp2f(sk - mn);
-    }
-    float inv = f * a.out_scale / L;
-    if (a.head_gate) inv *= 1.f / (1.f + expf(-to_f32(((const T*)a.head_gate)[(size_t)row * a.gate_stride + head])));
+    const float inv = kv4_finish(a, M, L, row, head, (T*)nullptr);
     T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * HD + q * 4;
     const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
 #pragma unroll
     for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(y[e]);
+}
+
+// The same for up to 8 slices, a warp a (row, head): prompts have thousands of those, and a CTA for each was bound by its start (22,400 of 128
+// numbers and 3 slices: FIGURE_MERGE).
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_kv4_merge_few_kernel(const Kv4Args a) {
+    constexpr int HD = BRAID_HD, W = HD / 32, V = W % 4 == 0 ? 4 : W % 2 == 0 ? 2 : 1, B = 8;
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rh = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (rh >= (long long)a.partial_rows * a.nqh) return;
+    const int head = (int)(rh % a.nqh), row = kv4_merged_row(a, (int)(rh / a.nqh)), n = a.n_splits;
+    if (row < 0) return;
+    const float2* pm = reinterpret_cast<const float2*>(a.partial + (size_t)a.partial_rows * a.nqh * n * HD) + (size_t)rh * n;
+    const float* po = a.partial + (size_t)rh * n * HD + lane * V;
+    const float2 ml = lane < n ? pm[lane] : make_float2(-INFINITY, 0.f);
+    float y[B][W];                                             // numbers 32 V i + V lane + 0 .. V - 1 in y[][V i ...]
+#pragma unroll
+    for (int s = 0; s < B; ++s)
+#pragma unroll
+        for (int i = 0; i < W; i += V) {
+            if (s >= n) break;
+            const float* src = po + (size_t)s * HD + 32 * i;
+            if constexpr (V == 4) *reinterpret_cast<float4*>(&y[s][i]) = *reinterpret_cast<const float4*>(src);
+            else if constexpr (V == 2) *reinterpret_cast<float2*>(&y[s][i]) = *reinterpret_cast<const float2*>(src);
+            else y[s][i] = *src;
+        }
+    float M = ml.x;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    // a share without a finite score has weight 0: nothing of zeros, all of a NaN
+    const float weight = M == -INFINITY ? 1.f : exp2f(ml.x - M);
+    float L = 0.f, x[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < B; ++s) {
+        const float w = __shfl_sync(0xffffffffu, weight, s), l = __shfl_sync(0xffffffffu, ml.y, s);
+        if (s >= n) break;
+        L = fmaf(l, w, L);
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[i] = fmaf(y[s][i], w, x[i]);
+    }
+    const float inv = kv4_finish(a, M, L, row, head, (T*)nullptr);
+    T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * HD + lane * V;
+#pragma unroll
+    for (int i = 0; i < W; i += V)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dst[32 * i + e] = from_f32<T>(x[i + e] * inv);
 }
 
 // ------------------------------------------------------------------ host side
@@ -866,6 +930,22 @@ extern "C" int braid_attn_kv4_clusters(int f32, int columns, int size) {
     return n;
 }
 
+// The slices' shares made one: also those of attn_kv4_prompt_kernel (attn_kv4_tc.cu).
+extern "C" int braid_attn_kv4_merge(const Kv4Args* args, void* stream) {
+    Kv4Args a = *args;
+    a.partial_rows = a.q_to > 0 ? a.n_seqs * a.q_to : a.rows;
+    const long long ctas = (long long)a.partial_rows * a.nqh;
+    if (ctas <= 0 || a.n_splits < 1) return BRAID_OK;
+    if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
+    if (!a.partial) BRAID_REFUSE("attn_kv4: slices that are no cluster need the partial buffer");
+    if (a.head_sinks) a.has_sink = 1;
+    const bool few = a.n_splits <= 8;
+    const dim3 grid((unsigned)(few ? (ctas + 7) / 8 : ctas));
+    if (a.f32) braid_launch(few ? attn_kv4_merge_few_kernel<float> : attn_kv4_merge_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, a);
+    else braid_launch(few ? attn_kv4_merge_few_kernel<__nv_bfloat16> : attn_kv4_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
+    BRAID_LAUNCH_CHECK();
+}
+
 // `args`: a Kv4Args, filled in by the caller (csrc/api.py has its layout).
 extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     Kv4Args a = *args;
@@ -879,6 +959,9 @@ extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     if (a.keep_first < 0 || a.max_q_len < 0) BRAID_REFUSE("attn_kv4: keep_first=%d, max_q_len=%d must not be negative", a.keep_first, a.max_q_len);
     if (!a.bias_slope != !a.bias_rate) BRAID_REFUSE("attn_kv4: a distance bias has a slope and a rate a head");
     if (a.softcap > 0.f && a.bias_slope) BRAID_REFUSE("attn_kv4: a cap on the scores and a distance bias are not combined");
+    if (a.q_to > 0 && (a.q_to < a.max_q_len || (long long)a.n_seqs * a.q_to > 0x7fffffffLL))
+        BRAID_REFUSE("attn_kv4: sequences of up to %d tokens do not go with a longest one of %d, or are too many", a.q_to, a.max_q_len);
+    a.partial_rows = a.q_to > 0 ? a.n_seqs * a.q_to : a.rows;
     if (a.n_splits < 1) a.n_splits = 1;
     if (a.n_splits <= 1 || a.n_splits > 8) a.cluster = 0;
     if (a.n_splits > 1 && !a.cluster && !a.partial) BRAID_REFUSE("attn_kv4: slices that are no cluster need the partial buffer");
@@ -886,10 +969,5 @@ extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     int rc;
     if (a.columns <= 8) rc = a.f32 ? launch_kv4<3, 1>(a, s) : launch_kv4<1, 1>(a, s);
     else rc = a.f32 ? launch_kv4<3, KV4_NT_MAX>(a, s) : launch_kv4<1, KV4_NT_MAX>(a, s);
-    if (rc || a.n_splits == 1 || a.cluster) return rc;
-    const long long ctas = (long long)a.rows * a.nqh;
-    if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
-    if (a.f32) braid_launch(attn_kv4_merge_kernel<float>, dim3((unsigned)ctas), dim3(256), 0, s, a);
-    else braid_launch(attn_kv4_merge_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(256), 0, s, a);
-    BRAID_LAUNCH_CHECK();
+    return rc || a.n_splits == 1 || a.cluster ? rc : braid_attn_kv4_merge(&a, stream);
 }

@@ -78,6 +78,8 @@ struct Kv4PromptArgs {
     // filled in here: in units of log2(e); CAP: scale / cap, the tanh's argument
     float scale_log2, sink_log2, cap_log2;
     int n_splits;
+    int q_from;                  // only sequences that bring at least so many tokens
+    int tiles;                   // > 0: the grid has so many token tiles of whatever sequences, in order; 0: as many for every sequence
 };
 
 #define FA_PLAIN 0
@@ -122,9 +124,47 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // CTAs start in the order x, y, z: all kv heads and sequences of the last token tile first, then
     // the tile before, ...: late tokens see the most keys, so the longest CTAs start first and the
     // short ones fill the gaps at the end
-    const int seq = blockIdx.y;
     const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
-    const int unit = gridDim.z - 1 - blockIdx.z, tile = unit / a.n_splits, split = unit - tile * a.n_splits;
+    const int unit = gridDim.z - 1 - blockIdx.z, split = unit % a.n_splits;
+    int seq = blockIdx.y, tile = unit / a.n_splits;
+    pdl_wait();
+    if (a.tiles > 0) {
+        // the grid's tile number `tile`: whose it is, and which of its tiles
+        __shared__ int found[2];
+        int before = 0;                           // tiles of the sequences before this round's
+        if (threadIdx.x == 0) found[0] = -1;
+        for (int s0 = 0; s0 < a.n_seqs && before <= tile; s0 += FA_THREADS) {
+            const int s = s0 + threadIdx.x, n = s < a.n_seqs ? max(a.q_len[s], 0) : 0;
+            const int mine = n >= a.q_from ? (n + 2 * tpc - 1) / (2 * tpc) : 0;
+            int upto = mine;                      // tiles of this warp's sequences up to this one
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            __shared__ int sums[FA_THREADS / 32];
+            __syncthreads();
+            if (lane == 31) sums[warp] = upto;
+            __syncthreads();
+            int all = 0, base = before;
+            for (int w = 0; w < FA_THREADS / 32; ++w) {
+                if (w < warp) base += sums[w];
+                all += sums[w];
+            }
+            if (mine > 0 && tile >= base + upto - mine && tile < base + upto) {
+                found[0] = s;
+                found[1] = base + upto - 1 - tile;             // late tokens, which see the most, first
+            }
+            before += all;
+        }
+        __syncthreads();
+        seq = found[0];
+        tile = found[1];
+        if (seq < 0) return;
+    }
+    const int q_len = a.q_len[seq];
+    const int tok0 = tile * (2 * tpc);
+    if (tok0 >= q_len || q_len < a.q_from) return;             // uniform over the CTA
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -140,16 +180,11 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    pdl_wait();
-
-    const int q_len = a.q_len[seq];
-    const int tok0 = tile * (2 * tpc);
-    const bool active = tok0 < q_len;             // uniform over the CTA
     const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
     const int ng = q_len - tok0 > tpc ? 2 : 1;    // groups of 128 rows that hold tokens
     const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + 2 * tpc, q_len) - 1;
     const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
-    int page_lo = k_lo / FA_PAGE, page_hi = active ? pos_max / FA_PAGE + 1 : page_lo;
+    int page_lo = k_lo / FA_PAGE, page_hi = pos_max / FA_PAGE + 1;
     if (a.n_splits > 1) {                         // slices of whole tiles
         const int per = ((page_hi - page_lo + 1) / 2 + a.n_splits - 1) / a.n_splits * 2;
         page_lo = min(page_hi, page_lo + split * per);
@@ -257,7 +292,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (ok) umma_commit(&v_empty[vst]);
             }
         }
-    } else if (warp >= FA_SOFTMAX && active && (warp - FA_SOFTMAX) >> 3 < ng) {
+    } else if (warp >= FA_SOFTMAX && (warp - FA_SOFTMAX) >> 3 < ng) {
         const int group = (warp - FA_SOFTMAX) >> 3;                     // the first or the second 128 rows
         const int tokg = tok0 + group * tpc, n_tok = min(tpc, q_len - tokg);
         const int first = kv_before + tokg, last = first + n_tok - 1;             // the group's positions
@@ -449,7 +484,12 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     const int hpc = g < FA_BM ? g : FA_BM, tpc = FA_BM / hpc, hchunks = (g + hpc - 1) / hpc;
     if (a.n_splits < 1) a.n_splits = 1;
     if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: slices need the partial buffer");
-    const long long gx = (long long)((a.max_q_len + 2 * tpc - 1) / (2 * tpc)) * a.n_splits;
+    // A tile a CTA for every sequence, or (where the rows are too few for that) so many CTAs as there may be tiles, which look up theirs: of
+    // FIGURES_TILES
+    const long long every = (a.max_q_len + 2 * tpc - 1) / (2 * tpc);
+    const long long most = a.rows / (2 * tpc) + (a.q_from > 1 ? (a.rows / a.q_from < a.n_seqs ? a.rows / a.q_from : a.n_seqs) : a.n_seqs);
+    a.tiles = 2 * most <= every * a.n_seqs ? (int)most : 0;
+    const long long gx = (a.tiles ? most : every) * a.n_splits;
     if (gx > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld token tiles, %d sequences)", gx, a.n_seqs);
     if ((long long)a.n_seqs * a.cols * 2 * a.nkh * FA_PAGE > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the pages' rows pass 32 bits");
@@ -487,7 +527,7 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     a.sink_log2 = a.sink * log2e;
     a.cap_log2 = a.softcap * log2e;
     braid_launch(a.softcap > 0.f ? attn_kv4_prompt_kernel<FA_CAP> : a.bias_slope ? attn_kv4_prompt_kernel<FA_BIAS> : attn_kv4_prompt_kernel<FA_PLAIN>,
-                 dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gx), dim3(FA_THREADS), FA_SMEM, (cudaStream_t)stream, mq, mkv, a);
+                 dim3(a.nkh * hchunks, a.tiles ? 1 : a.n_seqs, (unsigned)gx), dim3(FA_THREADS), FA_SMEM, (cudaStream_t)stream, mq, mkv, a);
     BRAID_LAUNCH_CHECK();
 }
 

@@ -310,6 +310,7 @@ struct ExpandArgs {
     int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [1 + seq0 + sequence] become 1
     int* out_table;              // (out_cols > 0) [n_seqs, out_cols]: the numbers of the pages, for whoever reads them
     int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
+    int q_from;                  // only the pages of sequences that bring at least so many tokens
 };
 
 template <int N>
@@ -370,60 +371,68 @@ kv4_expand_kernel(const ExpandArgs a) {
     pdl_wait();
     constexpr int HD = 32 * W;
     using P = typename Kv4Pairs<T>::Pair;
-    const int c = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+    const int kvh = blockIdx.y, seq = blockIdx.z;
     const int before = a.kv_before[seq], end = before + a.q_len[seq];
-    const int key0 = c * BRAID_PAGE_SIZE;
-    if (a.out_table && kvh == 0 && threadIdx.x == 0) a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
-    if (key0 >= end) return;
-    const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0;
-    if (key0 + BRAID_PAGE_SIZE <= lo && key0 >= a.keep_first) return;
-    const int page = a.page_table[(size_t)seq * a.cols + c];
-    if (page < 0 || page >= a.num_pages) {
-        if (threadIdx.x == 0) atomicExch(a.error_flag, 1);
-        return;
-    }
-    const size_t out_page = a.out_cols > 0 ? (size_t)seq * a.out_cols + c : (size_t)page;
-    const int t = threadIdx.x >> 2, j = threadIdx.x & 3, tr = t % KV4_REC;
-    const uint8_t* rec = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t / KV4_REC) * kv4_record_bytes(HD);
-    const bool in = key0 + t < end && (key0 + t >= lo || key0 + t < a.keep_first);
-    T* dst = (T*)a.out + ((out_page * 2 * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * HD + 8 * j;
-    const size_t plane = (size_t)a.nkh * BRAID_PAGE_SIZE * HD;
-    uint32_t kc[W], kg[W], vc[W], vg[W];
-    load_words<W>(rec + tr * (HD / 2) + 4 * W * j, kc);
-    load_words<W>(rec + kv4_key_groups(HD) + 4 * W * tr, kg);
-    load_words<W>(rec + kv4_value_codes(HD) + tr * (HD / 2) + 4 * W * j, vc);
-    load_words<W>(rec + kv4_value_groups(HD) + 4 * W * tr, vg);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        if (!in) kc[w] = kg[w] = vg[w] = 0u;                   // a group of step 0 and lowest value 0
-        // the 16 bits of group w in the lane's first and second half of value words
-        const int h0 = w, h1 = W + w;
-        const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
-        const uint32_t both = in ? v0 | (v1 << 16) : 0u;
-        // NaN, or a step of 2^122 or a lowest value of 2^127 or more, from which a number may round to infinity
-        if (a.repair && ((vg[w] & 0x7f80u) >= 0x7c80u || (vg[w] & 0x7f800000u) >= 0x7f000000u)) {
-            vg[w] = 0u;
-            a.repair[1 + a.seq0 + seq] = 1;
-            a.repair[0] = 1;
+    if (a.out_table && kvh == 0)
+        for (int c = blockIdx.x + gridDim.x * threadIdx.x; c < a.out_cols; c += gridDim.x * blockDim.x)
+            a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
+    if (end - before < a.q_from) return;
+    const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0, cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
+    for (int c = blockIdx.x; c < cols; c += gridDim.x) {
+        const int key0 = c * BRAID_PAGE_SIZE;
+        if (key0 >= end) return;
+        if (key0 + BRAID_PAGE_SIZE <= lo && key0 >= a.keep_first) continue;
+        const int page = a.page_table[(size_t)seq * a.cols + c];
+        if (page < 0 || page >= a.num_pages) {
+            if (threadIdx.x == 0) atomicExch(a.error_flag, 1);
+            continue;
         }
-        __align__(16) P y[4];
-        P z[4];
-        Kv4Pairs<T>::make(kc[w], kg[w], y);                    // pairs of neighbours, in order
-        *reinterpret_cast<uint4*>(dst + 32 * w) = *reinterpret_cast<const uint4*>(y);
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
-        Kv4Pairs<T>::make(both, vg[w], z);                     // numbers n and 4 + n
-        y[0] = Kv4Pairs<T>::lows(z[0], z[1]);
-        y[1] = Kv4Pairs<T>::lows(z[2], z[3]);
-        y[2] = Kv4Pairs<T>::highs(z[0], z[1]);
-        y[3] = Kv4Pairs<T>::highs(z[2], z[3]);
-        *reinterpret_cast<uint4*>(dst + plane + 32 * w) = *reinterpret_cast<const uint4*>(y);
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + plane + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
+        const size_t out_page = a.out_cols > 0 ? (size_t)seq * a.out_cols + c : (size_t)page;
+        const int t = threadIdx.x >> 2, j = threadIdx.x & 3, tr = t % KV4_REC;
+        const uint8_t* rec = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t / KV4_REC) * kv4_record_bytes(HD);
+        const bool in = key0 + t < end && (key0 + t >= lo || key0 + t < a.keep_first);
+        T* dst = (T*)a.out + ((out_page * 2 * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * HD + 8 * j;
+        const size_t plane = (size_t)a.nkh * BRAID_PAGE_SIZE * HD;
+        uint32_t kc[W], kg[W], vc[W], vg[W];
+        load_words<W>(rec + tr * (HD / 2) + 4 * W * j, kc);
+        load_words<W>(rec + kv4_key_groups(HD) + 4 * W * tr, kg);
+        load_words<W>(rec + kv4_value_codes(HD) + tr * (HD / 2) + 4 * W * j, vc);
+        load_words<W>(rec + kv4_value_groups(HD) + 4 * W * tr, vg);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (!in) kc[w] = kg[w] = vg[w] = 0u;                   // a group of step 0 and lowest value 0
+            // the 16 bits of group w in the lane's first and second half of value words
+            const int h0 = w, h1 = W + w;
+            const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
+            const uint32_t both = in ? v0 | (v1 << 16) : 0u;
+            // NaN, or a step of 2^122 or a lowest value of 2^127 or more, from which a number may round to infinity
+            if (a.repair && ((vg[w] & 0x7f80u) >= 0x7c80u || (vg[w] & 0x7f800000u) >= 0x7f000000u)) {
+                vg[w] = 0u;
+                a.repair[1 + a.seq0 + seq] = 1;
+                a.repair[0] = 1;
+            }
+            __align__(16) P y[4];
+            P z[4];
+            Kv4Pairs<T>::make(kc[w], kg[w], y);                    // pairs of neighbours, in order
+            *reinterpret_cast<uint4*>(dst + 32 * w) = *reinterpret_cast<const uint4*>(y);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
+            Kv4Pairs<T>::make(both, vg[w], z);                     // numbers n and 4 + n
+            y[0] = Kv4Pairs<T>::lows(z[0], z[1]);
+            y[1] = Kv4Pairs<T>::lows(z[2], z[3]);
+            y[2] = Kv4Pairs<T>::highs(z[0], z[1]);
+            y[3] = Kv4Pairs<T>::highs(z[2], z[3]);
+            *reinterpret_cast<uint4*>(dst + plane + 32 * w) = *reinterpret_cast<const uint4*>(y);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + plane + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
+        }
     }
 }
 
 template <typename T>
 static int launch_expand(const ExpandArgs& a, cudaStream_t s) {
-    const dim3 grid(a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols, a.nkh, a.n_seqs);
+    const int cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
+    // a CTA a page; where most sequences may be passed over, some of them a CTA
+    const int x = a.q_from > 1 ? min(cols, max(1, 32768 / (a.nkh * a.n_seqs))) : cols;
+    const dim3 grid(x, a.nkh, a.n_seqs);
     void (*const kernels[8])(const ExpandArgs) = {kv4_expand_kernel<T, 1>, kv4_expand_kernel<T, 2>, kv4_expand_kernel<T, 3>, kv4_expand_kernel<T, 4>,
                                                   kv4_expand_kernel<T, 5>, kv4_expand_kernel<T, 6>, kv4_expand_kernel<T, 7>, kv4_expand_kernel<T, 8>};
     braid_launch(kernels[a.hd / KV4_GROUP - 1], grid, dim3(256), 0, s, a);

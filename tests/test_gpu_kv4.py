@@ -281,6 +281,37 @@ def test_prompts(K, route, seqs, nqh, nkh, hd, dt):
     Case(K, seqs, nqh, nkh, hd, dt).check(K)
 
 
+@pytest.mark.parametrize("slices", [2, 3, 8])
+@pytest.mark.parametrize("name, hd", [("window", 64), ("sink", 128), ("sinks", 64), ("gate", 128), ("bias", 64), ("cap", 128)])
+def test_prompts_in_slices(K, monkeypatch, name, hd, slices):
+    """The context cut into slices, some of them without a key that a row sees, or without any."""
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    monkeypatch.setattr(Kernels, "_kv4_prompt_slices", lambda *a: slices)
+    c = Case(K, [(70, 900), (150, 0), (1, 100), (9, 333)], 8, 2, hd, BF)
+    c.check(K, **options(name, c.rows, c.nqh, BF))
+
+
+@pytest.mark.parametrize("slices", [None, 3])
+@pytest.mark.parametrize("room", [1 << 30, 1])
+@pytest.mark.parametrize("name, hd", [("window", 128), ("sinks", 64)])
+def test_prompts_beside_single_tokens(K, monkeypatch, name, hd, room, slices):
+    """Sequences of up to 2 tokens (8 columns of queries) are computed over 4 bits, the others over pages, a few sequences at a time."""
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    monkeypatch.setattr(Kernels, "KV4_PAGES_BYTES", room)
+    if slices:
+        monkeypatch.setattr(Kernels, "_kv4_prompt_slices", lambda *a: slices)
+    c = Case(K, [(1, 3000), (200, 100), (8, 64), (9, 10), (0, 5), (1, 0), (3, 700), (1, 500), (40, 0)], 8, 2, hd, BF)
+    ran = []
+    mma = K._attn_kv4_mma
+    monkeypatch.setattr(K, "_attn_kv4_mma", lambda *a: (ran.append(a[-1]), mma(*a)))
+    c.check(K, **options(name, c.rows, c.nqh, BF))
+    assert ran == [2]
+    # one prompt of many tokens beside another: all of them over pages
+    c = Case(K, [(200, 100), (150, 30), (1, 64)], 8, 2, hd, BF)
+    c.check(K, **options(name, c.rows, c.nqh, BF))
+    assert ran == [2]
+
+
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("name", OPTIONS)
 def test_options_of_prompts(K, route, name, dt):
