@@ -875,8 +875,9 @@ class Kernels:
             return
         tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
         if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, n_seqs, nqh, nkh, tc):
-            # a step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are (where the others are short
-            # on average, and some may be so short)
+            # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
+            # longest is short on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 393 / 848 / 226;
+            # 2,000 tokens beside one behind 30,000, 673 / 367 / 76.)
             few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 64 * (n_seqs - 1) else 0
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                  int(window or 0), scale, int(keep_first or 0), head_scale, dict(
@@ -930,7 +931,14 @@ class Kernels:
     # The most that the pages of a step's prompts, read back for attention, may take at once: more sequences go one group after another.
     KV4_PAGES_BYTES = 1 << 30
 
-    # FIGURES_CROSS
+    # Steps of at least so many units (16 columns of queries, kv head, sequence), or of 64 whose units times the longest context are so many, have
+    # their prompts' pages read back once for all of them.  The kernel over 4 bits reads them for every 16 columns; the one over ordinary pages
+    # takes 256 columns a CTA.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: a prompt alone, 128 tokens (256 units)
+    # 13.1 / 11.9, 256 tokens 14.7 / 23; four of 32 (256) 11.1 / 11.3; behind 1,000, 64 tokens (128) 25.6 / 20.4, 96 tokens (192) 25.8 / 26.2; behind
+    # 8,000, 16 tokens (32) 26 / 27.5, 64 tokens 34.5 / 69; behind 32,000, 16 tokens 76 / 66, 32 tokens 78 / 126, 128 tokens 96 / 457.
+    # Other head sizes and options go through the older kernel for ordinary pages, of which a CTA walks its context alone, from 4/3 of those units, or
+    # 10/3 behind 1,000 and more: heads of 96, a prompt alone, 256 tokens (512) 18.5 / 19.2, 512 tokens 29 / 42; behind 1,000, 256 tokens 51 / 43,
+    # 512 tokens (1,024) 68 / 88; behind 8,000, 256 tokens 269 / 200, 512 tokens 332 / 402; heads of 256 alike.
     KV4_PAGES_FROM, KV4_PAGES_WORK = 300, 200_000
 
     @staticmethod
@@ -994,7 +1002,7 @@ class Kernels:
                              **options, repair=repair)
 
     def _kv4_prompt_slices(self, rows: int, n_seqs: int, max_q_len: int, max_kv_len: int, nqh: int, nkh: int, hd: int, window: int) -> int:
-        """Slices of the context for prompts over pages that were read back: a CTA takes 256 columns of queries, one an SM."""
+        """Slices of the context for prompts over pages that were read back: a CTA takes 256 columns of queries, and an SM one CTA."""
         g = nqh // nkh
         tokens = 2 * (128 // min(g, 128))
         ctas = nkh * -(-g // 128) * min(n_seqs * -(-max_q_len // tokens), rows // tokens + n_seqs)

@@ -1,12 +1,20 @@
 // Attention of prompts over a cache held in 4 bits, on the 5th-generation tensor cores (tcgen05): over the pages that kv4_expand_kernel
 // (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size: -DBRAID_HD=64 or 128.
 //
-// The arrangement is that of attn_tc.cu (a CTA of 128 rows walks the visible keys a page at a time, two CTAs an SM; TMA into two rings,
-// S = Q K^T and O += P V in tensor memory, the running maximum raised when a tile exceeds it by more than 8), but for the softmax:
-// TWO threads share a row, each with half of the keys of a tile and half of the result's columns, in two warps that meet at a barrier of their own
-// once a tile.  The barrier carries the question whether any row's maximum has to be raised (barrier.red.or), so that the two exchange numbers
-// only then.  What bounds attn_tc.cu is the chain of a tile through one thread a row (load 64 scores, maximum, exponentials, round, store): it
-// reaches 42% of the tensor cores' rate.  FIGURES_PROMPT
+// A CTA takes two groups of 128 columns of queries (tokens x the query heads of a kv head) and walks the keys that they see, 128 at a time:
+//   S = Q K^T  (tensor memory, float32),   p = 2^(scale log2(e) S - m),   O += p V  (p bfloat16 in tensor memory)
+// with the running maximum m of a row raised only when a tile exceeds it by more than 8 powers of two.  Warp 0 brings pages into two rings by
+// TMA, warp 1 issues S, warp 3 P V, and 16 warps are the softmax: TWO threads share a row, each with half of a tile's keys and half of the
+// result's columns, in two warps that meet at a barrier of their own once a tile.  That barrier carries the question whether any row's
+// maximum has to be raised (barrier.red.or), so that the two exchange numbers only then.
+//
+// What bounds it: the exponentials of a tile take the SM 2,048 cycles, and so do its products.  So the two groups have ONE place for their
+// scores: S of one is computed while the other's exponentials run, which keeps the groups half a turn apart without a barrier between them.
+// A tile takes some 3,000 cycles.  Prompts of 6,414 tokens in all / 700 tokens behind 16,500 (88 of 148 SMs), 32 heads of 128 over 8, us with
+// the reading back: 83 / 344 by attn_tc.cu (a thread a row, tiles of 64 keys, two CTAs an SM); 89 / 331 the same with two threads a row; 90 / 332
+// with both groups in a CTA and scores of their own (96 / 376 with barriers that let their exponentials take turns); 104 / 393 with tiles of 128
+// keys whose probabilities lie over the scores, where all of a group's steps wait for one another; 78 / 237 so, and 78 / 224 with the
+// context in 3 slices.
 #include "kv4.cuh"
 #include "attn_tc.cuh"
 #include "softcap.cuh"
@@ -91,8 +99,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int HD = BRAID_HD;
     constexpr bool BIAS = FORM == FA_BIAS, CAP = FORM == FA_CAP;
     pdl_trigger();
-    // the swizzled tiles want 1024-byte alignment; two CTAs an SM leave no room for slack, so
-    // the start of dynamic shared memory is checked instead of rounded up
+    // the swizzled tiles want 1024-byte alignment; the start of dynamic shared memory is checked instead of rounded up
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) atomicExch(a.error_flag, 1);
@@ -153,7 +160,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             if (mine > 0 && tile >= base + upto - mine && tile < base + upto) {
                 found[0] = s;
-                found[1] = base + upto - 1 - tile;             // late tokens, which see the most, first
+                found[1] = tile - (base + upto - mine);
             }
             before += all;
         }
@@ -484,8 +491,9 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     const int hpc = g < FA_BM ? g : FA_BM, tpc = FA_BM / hpc, hchunks = (g + hpc - 1) / hpc;
     if (a.n_splits < 1) a.n_splits = 1;
     if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: slices need the partial buffer");
-    // A tile a CTA for every sequence, or (where the rows are too few for that) so many CTAs as there may be tiles, which look up theirs: of
-    // FIGURES_TILES
+    // A CTA for every tile that a sequence may have, or, where the rows are too few for that, for every tile that the step may have: those look up
+    // whose tile they are.  (A CTA that finds nothing to do still takes an SM for some us.  512 tokens beside 63 single ones, attention as a whole: 387
+    // us by sequence, 282 by step; 900 beside 100 sequences of up to 50: 246, 162; 3,000, 100, 200 and 1,500: 118, 114.)
     const long long every = (a.max_q_len + 2 * tpc - 1) / (2 * tpc);
     const long long most = a.rows / (2 * tpc) + (a.q_from > 1 ? (a.rows / a.q_from < a.n_seqs ? a.rows / a.q_from : a.n_seqs) : a.n_seqs);
     a.tiles = 2 * most <= every * a.n_seqs ? (int)most : 0;

@@ -140,7 +140,7 @@ extern "C" int braid_step_tables(const TablesArgs* args, void* stream) {
 // A code is the quotient (x - lo) / step rounded to the nearest whole number, ties to even.  The quotient is taken as a product with 1 / step,
 // which may miss a number next to a tie, and then put right by the remainder x - lo - code step: that is exact (the code has
 // 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  Instructions bound it, some 15 a number.  (6,414 rows of 8
-// heads of 128, keys and values, bfloat16: 23 us with 8 numbers a thread and tests of each for NaN, TIME_STORE us so; what is read and
+// heads of 128, keys and values, bfloat16: 23 us with 8 numbers a thread and tests of each for NaN, 15 us so; what is read and
 // written takes 5 us.)
 struct StoreArgs {
     const void* k;
@@ -430,8 +430,9 @@ kv4_expand_kernel(const ExpandArgs a) {
 template <typename T>
 static int launch_expand(const ExpandArgs& a, cudaStream_t s) {
     const int cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
-    // a CTA a page; where most sequences may be passed over, some of them a CTA
-    const int x = a.q_from > 1 ? min(cols, max(1, 32768 / (a.nkh * a.n_seqs))) : cols;
+    // A CTA a page; where most sequences may be passed over, some pages a CTA.  (512 tokens beside 63 single ones behind 8,000, attention as a
+    // whole: 285 us with a CTA a page, 225 with 4,096 CTAs; 512 behind 16,000 beside 15 behind 2,000: 210, 186.)
+    const int x = a.q_from > 1 ? min(cols, max(1, 4096 / (a.nkh * a.n_seqs))) : cols;
     const dim3 grid(x, a.nkh, a.n_seqs);
     void (*const kernels[8])(const ExpandArgs) = {kv4_expand_kernel<T, 1>, kv4_expand_kernel<T, 2>, kv4_expand_kernel<T, 3>, kv4_expand_kernel<T, 4>,
                                                   kv4_expand_kernel<T, 5>, kv4_expand_kernel<T, 6>, kv4_expand_kernel<T, 7>, kv4_expand_kernel<T, 8>};
