@@ -139,10 +139,11 @@ class RowScale:
         return torch.rsqrt(self.shares.sum(0) / self.width + self.eps)
 
 
-# The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs).
+# The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs, Kv4SimpleArgs).
 _KV4_ARGS = struct.Struct("<15Q3q12i4f6i")
 _KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7f3i")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q11i4x")
+_KV4_SIMPLE_ARGS = struct.Struct("<7Q2q8ifi2f2Qq3Qfi2Q")
 
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
 
@@ -829,11 +830,12 @@ class Kernels:
         self._on_device("kv4_expand", cache, out)
         self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
 
-    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_table=None, repair=None, seq0=0, q_from=0) -> None:
+    def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_cols=0, out_table=None, repair=None, seq0=0,
+                q_from=0) -> None:
         self.launches += 1
         args = _EXPAND_ARGS.pack(cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), q_len.data_ptr(), kv_before.data_ptr(),
                                  self._error_flag.data_ptr() + 16, _ptr(repair) or 0, _ptr(out_table) or 0, n, cache.shape[1], hd,
-                                 page_table.shape[1], cache.shape[0], window, keep_first, out_table.shape[1] if out_table is not None else 0,
+                                 page_table.shape[1], cache.shape[0], window, keep_first, out_cols,
                                  seq0, dtype_code(out.dtype), q_from)
         self._check_lib(lib, lib.braid_kv4_expand(args, self._stream()), "kv4_expand")
 
@@ -897,14 +899,15 @@ class Kernels:
 
     def _attn_kv4_plain(self, q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale, sink,
                         out_scale, head_sinks, head_gate, distance_bias, softcap, repair=None) -> None:
-        lib = self.part_library("kv4")
+        lib, bias = self.part_library("kv4"), distance_bias or (None, None)
+        args = _KV4_SIMPLE_ARGS.pack(
+            q.data_ptr(), out.data_ptr(), cache.data_ptr(), page_table.data_ptr(), token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(),
+            q.stride(0), out.stride(0), out.shape[0], nqh, nkh, hd, page_table.shape[1], cache.shape[0], window, keep_first, scale,
+            int(sink is not None), sink or 0.0, out_scale, _ptr(head_sinks) or 0, _ptr(head_gate) or 0,
+            head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, softcap or 0.0,
+            dtype_code(out.dtype), self._error_flag.data_ptr() + 16, _ptr(repair) or 0)
         self.launches += 1
-        self._check_lib(lib, lib.braid_attn_kv4_simple(
-            q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype_code(out.dtype), cache.data_ptr(), page_table.data_ptr(),
-            token_seq.data_ptr(), q_start.data_ptr(), kv_before.data_ptr(), out.shape[0], nqh, nkh, hd, page_table.shape[1], cache.shape[0],
-            window, keep_first, float(scale), int(sink is not None), float(sink or 0.0), float(out_scale), _ptr(head_sinks), _ptr(head_gate),
-            head_gate.stride(0) if head_gate is not None else 0, _ptr(head_scale), *self._bias_args(distance_bias), float(softcap or 0.0),
-            _ptr(repair), self._error_flag.data_ptr() + 16, self._stream()), "attn_kv4")
+        self._check_lib(lib, lib.braid_attn_kv4_simple(args, self._stream()), "attn_kv4")
 
     def kv4_attention_library(self, head_dim: int):
         """The attention over a 4-bit cache for one head size, compiled at first use."""
@@ -965,39 +968,45 @@ class Kernels:
         page = 2 * nkh * build.page_size() * hd
         group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
         # from torch's allocator at every call: calls on other streams, and other graphs, have their own
-        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.bfloat16, device=out.device)
-        table = torch.empty((group, cols), dtype=torch.int32, device=out.device)
-        repair = torch.zeros(n_seqs + 1, dtype=torch.int32, device=out.device)
-        fence = repair.new_empty(1)
-        prompt = self.kv4_attention_library(hd)
-        n_splits = self._kv4_prompt_slices(out.shape[0], group, max_q_len, max_kv_len, nqh, nkh, hd, window) if tc else 1
-        partial = None
-        if n_splits > 1:
-            partial = torch.empty(out.shape[0] * nqh * n_splits * (hd + 2), dtype=torch.float32, device=out.device)
-        gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
-        for i in range(0, n_seqs, group):
-            n = min(group, n_seqs - i)
-            part = (q_start[i:i + n], q_len[i:i + n], kv_before[i:i + n])
-            self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, table, repair, i, q_from)
-            if tc:
-                args = _KV4_PROMPT_ARGS.pack(
-                    q.data_ptr(), pages.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in part), self._error_flag.data_ptr() + 12,
-                    _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0),
-                    gate.stride(0) if gate is not None else 0, _ptr(partial) or 0, out.shape[0], n, max_q_len, nqh, nkh, cols, window, int(options["sink"] is not None),
-                    scale, options["sink"] or 0.0, options["out_scale"], options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0)
-                self.launches += 1
-                self._check_lib(prompt, prompt.braid_attn_kv4_prompt(args, self._stream()), "attn_kv4")
-            else:
-                fence.zero_()        # that kernel reads pages of earlier tokens before its predecessor has ended; not before something else has
+        device, stream = out.device, self._stream()
+        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.bfloat16, device=device)
+        repair = torch.zeros(n_seqs + 1, dtype=torch.int32, device=device)
+        lengths = (q_start, q_len, kv_before)
+        if not tc:
+            table, fence = torch.empty((group, cols), dtype=torch.int32, device=device), repair.new_empty(1)
+            for i in range(0, n_seqs, group):
+                n = min(group, n_seqs - i)
+                part = [t[i:i + n] for t in lengths]
+                self._expand(lib, cache, pages, page_table[i:i + n], *part[1:], n, hd, window, keep_first, cols, table, repair, i)
+                fence.zero_()    # that kernel reads pages of earlier tokens before its predecessor has ended; not before something else has
                 self.attn_mma(q, out, pages, table, *part, token_seq, n, max_q_len, nqh, nkh, hd, window, scale, keep_first=keep_first,
                               head_scale=head_scale, **options)
-        if partial is not None:
-            args = _KV4_ARGS.pack(
-                0, out.data_ptr(), partial.data_ptr(), 0, 0, 0, q_len.data_ptr(), 0, token_seq.data_ptr(), _ptr(options["head_sinks"]) or 0, _ptr(gate) or 0, 0, 0, 0,
-                self._error_flag.data_ptr() + 16, 0, out.stride(0), gate.stride(0) if gate is not None else 0, out.shape[0], n_seqs, max_q_len,
-                nqh, nkh, 0, 0, 0, 0, n_splits, int(options["sink"] is not None), 0, scale, options["sink"] or 0.0, options["out_scale"], 0.0, 0, 0, 0, q_from, 0, 0)
-            self.launches += 1
-            self._check_lib(prompt, prompt.braid_attn_kv4_merge(args, self._stream()), "attn_kv4")
+        else:
+            lib_tc, partial = self.kv4_attention_library(hd), None
+            gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
+            sinks, gate_stride, has_sink = _ptr(options["head_sinks"]) or 0, gate.stride(0) if gate is not None else 0, int(options["sink"] is not None)
+            sink, out_scale, rows = options["sink"] or 0.0, options["out_scale"], out.shape[0]
+            for i in range(0, n_seqs, group):
+                n = min(group, n_seqs - i)
+                part, part_table = (lengths, page_table) if n == n_seqs else ([t[i:i + n] for t in lengths], page_table[i:i + n])
+                self._expand(lib, cache, pages, part_table, *part[1:], n, hd, window, 0, cols, None, repair, i, q_from)
+                if i == 0:
+                    n_splits = self._kv4_prompt_slices(rows, group, max_q_len, max_kv_len, nqh, nkh, hd, window)
+                    if n_splits > 1:
+                        partial = torch.empty(rows * nqh * n_splits * (hd + 2), dtype=torch.float32, device=device)
+                args = _KV4_PROMPT_ARGS.pack(
+                    q.data_ptr(), pages.data_ptr(), out.data_ptr(), *[t.data_ptr() for t in part], self._error_flag.data_ptr() + 12, sinks,
+                    _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0), gate_stride, _ptr(partial) or 0, rows, n,
+                    max_q_len, nqh, nkh, cols, window, has_sink, scale, sink, out_scale, options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0)
+                self.launches += 1
+                self._check_lib(lib_tc, lib_tc.braid_attn_kv4_prompt(args, stream), "attn_kv4")
+            if partial is not None:
+                args = _KV4_ARGS.pack(
+                    0, out.data_ptr(), partial.data_ptr(), 0, 0, 0, q_len.data_ptr(), 0, token_seq.data_ptr(), sinks, _ptr(gate) or 0, 0, 0, 0,
+                    self._error_flag.data_ptr() + 16, 0, out.stride(0), gate_stride, rows, n_seqs, max_q_len, nqh, nkh, 0, 0, 0, 0, n_splits,
+                    has_sink, 0, scale, sink, out_scale, 0.0, 0, 0, 0, q_from, 0, 0)
+                self.launches += 1
+                self._check_lib(lib_tc, lib_tc.braid_attn_kv4_merge(args, stream), "attn_kv4")
         self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale,
                              **options, repair=repair)
 
@@ -1172,13 +1181,10 @@ class Kernels:
                 lib.braid_delta_work_floats.restype = c_longlong
                 names = ("braid_delta_rule", "braid_delta_gated_norm")
             elif name == "kv4":
-                for n in ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand"):
+                for n in ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand", "braid_attn_kv4_simple"):
                     getattr(lib, n).argtypes = [c_char_p, c_void_p]
-                if [lib.braid_kv4_args_bytes(i) for i in range(3)] != [_TABLES_ARGS.size, _STORE_ARGS.size, _EXPAND_ARGS.size]:
+                if [lib.braid_kv4_args_bytes(i) for i in range(4)] != [x.size for x in (_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS, _KV4_SIMPLE_ARGS)]:
                     raise KernelError("the library of the 4-bit cache has other arguments than these bindings")
-                lib.braid_attn_kv4_simple.argtypes = [c_void_p, c_longlong] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 8 + \
-                                                     [c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_longlong] + [c_void_p] * 3 + \
-                                                     [c_float, c_void_p, c_void_p, c_void_p]
                 names = ("braid_step_tables", "braid_kv4_store", "braid_kv4_expand", "braid_attn_kv4_simple")
             elif name == "streams":
                 lib.braid_streams.argtypes = [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,

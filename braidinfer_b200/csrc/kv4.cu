@@ -452,9 +452,6 @@ extern "C" int braid_kv4_expand(const ExpandArgs* args, void* stream) {
     BRAID_REFUSE("kv4_expand: unknown dtype code %d", a.dtype);
 }
 
-// Bytes of the argument structures: tables, write, reading back.
-extern "C" int braid_kv4_args_bytes(int which) { return which == 0 ? (int)sizeof(TablesArgs) : which == 1 ? (int)sizeof(StoreArgs) : (int)sizeof(ExpandArgs); }
-
 // ------------------------------------------------------------------ plain attention
 // One warp per (row, query head), 32 keys at a time: a lane a key for the scores, a lane a number of the head for the values.  All
 // arithmetic float32.  Options as in attn_simple.cu.  Rows of padding (token_seq < 0) are left as they were.
@@ -481,6 +478,7 @@ struct Kv4SimpleArgs {
     const float* bias_slope;
     const float* bias_rate;
     float softcap;
+    int dtype;
     int* error_flag;
     const int* repair;
 };
@@ -578,23 +576,25 @@ attn_kv4_simple_kernel(const Kv4SimpleArgs a) {
         attn_kv4_item<T>(a, item, qs_all[warp], lane);
 }
 
-extern "C" int braid_attn_kv4_simple(const void* q, long long q_stride, void* out, long long out_stride, int dtype, const void* cache,
-                                     const int* page_table, const int* token_seq, const int* q_start, const int* kv_before, int rows, int nqh,
-                                     int nkh, int hd, int cols, int num_pages, int window, int keep_first, float scale, int has_sink, float sink,
-                                     float out_scale, const float* head_sinks, const void* head_gate, long long gate_stride, const float* head_scale,
-                                     const float* bias_slope, const float* bias_rate, float softcap, const int* repair, int* error_flag, void* stream) {
-    if (rows <= 0) return BRAID_OK;
-    if (int rc = kv4_check("attn_kv4", nkh, hd, cache)) return rc;
-    if (nqh <= 0 || nqh % nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", nqh, nkh);
-    if (num_pages <= 0 || cols <= 0) BRAID_REFUSE("attn_kv4: the cache has no pages (pages=%d, table columns=%d)", num_pages, cols);
-    long long ctas = ((long long)rows * nqh + 3) / 4;
-    if (repair) ctas = min(ctas, 148LL);                      // one an SM: they hardly ever have anything to do
+// `args`: a Kv4SimpleArgs, filled in by the caller (csrc/api.py has its layout).
+extern "C" int braid_attn_kv4_simple(const Kv4SimpleArgs* args, void* stream) {
+    Kv4SimpleArgs a = *args;
+    if (a.rows <= 0) return BRAID_OK;
+    if (int rc = kv4_check("attn_kv4", a.nkh, a.hd, a.cache)) return rc;
+    if (a.nqh <= 0 || a.nqh % a.nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", a.nqh, a.nkh);
+    if (a.num_pages <= 0 || a.cols <= 0) BRAID_REFUSE("attn_kv4: the cache has no pages (pages=%d, table columns=%d)", a.num_pages, a.cols);
+    long long ctas = ((long long)a.rows * a.nqh + 3) / 4;
+    if (a.repair) ctas = min(ctas, 148LL);                    // one an SM: they hardly ever have anything to do
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the rows exceed the grid limit");
-    Kv4SimpleArgs a{q, out, (const uint8_t*)cache, page_table, token_seq, q_start, kv_before, q_stride, out_stride, rows, nqh, nkh, hd, cols, num_pages,
-                    window, window > 0 ? keep_first : 0, scale, has_sink || head_sinks, sink, out_scale, head_sinks, head_gate, gate_stride, head_scale,
-                    bias_slope, bias_rate, softcap, error_flag, repair};
-    if (dtype == BRAID_F32) braid_launch(attn_kv4_simple_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
-    else if (dtype == BRAID_BF16) braid_launch(attn_kv4_simple_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
-    else BRAID_REFUSE("attn_kv4: unknown dtype code %d", dtype);
+    if (a.window <= 0) a.window = a.keep_first = 0;
+    if (a.head_sinks) a.has_sink = 1;
+    if (a.dtype == BRAID_F32) braid_launch(attn_kv4_simple_kernel<float>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
+    else if (a.dtype == BRAID_BF16) braid_launch(attn_kv4_simple_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(128), 0, (cudaStream_t)stream, a);
+    else BRAID_REFUSE("attn_kv4: unknown dtype code %d", a.dtype);
     BRAID_LAUNCH_CHECK();
+}
+
+// Bytes of the argument structures: tables, write, reading back, plain attention.
+extern "C" int braid_kv4_args_bytes(int which) {
+    return which == 0 ? (int)sizeof(TablesArgs) : which == 1 ? (int)sizeof(StoreArgs) : which == 2 ? (int)sizeof(ExpandArgs) : (int)sizeof(Kv4SimpleArgs);
 }
