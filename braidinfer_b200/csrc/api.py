@@ -140,7 +140,7 @@ class RowScale:
 
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs, Kv4SimpleArgs).
-_KV4_ARGS = struct.Struct("<15Q3q12i4f6i")
+_KV4_ARGS = struct.Struct("<15Q3q12i4f5i4x")
 _KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7f3i")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q11i4x")
 _KV4_SIMPLE_ARGS = struct.Struct("<7Q2q8ifi2f2Qq3Qfi2Q")
@@ -878,8 +878,8 @@ class Kernels:
         tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
         if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, n_seqs, nqh, nkh, tc):
             # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
-            # longest is short on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 393 / 848 / 226;
-            # 2,000 tokens beside one behind 30,000, 673 / 367 / 76.)
+            # longest is short on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 409 / 848 / 224;
+            # 2,000 tokens beside one behind 30,000, 635 / 366 / 77.)
             few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 64 * (n_seqs - 1) else 0
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                  int(window or 0), scale, int(keep_first or 0), head_scale, dict(
@@ -927,22 +927,23 @@ class Kernels:
                 lib.braid_attn_kv4_prompt.restype = c_int
                 if lib.braid_attn_kv4_prompt_args_bytes() != _KV4_PROMPT_ARGS.size:
                     raise KernelError("the attention library over a 4-bit cache has other arguments than these bindings")
-            lib.plans = {}                                    # (query columns wanted, float32) -> (columns a CTA, CTAs held at once, clusters by their size)
+            lib.plans = {}                                    # float32 -> (CTAs held at once, clusters by their size)
             self._attn_libs[("kv4", head_dim)] = lib
         return lib
 
     # The most that the pages of a step's prompts, read back for attention, may take at once: more sequences go one group after another.
     KV4_PAGES_BYTES = 1 << 30
 
-    # Steps of at least so many units (16 columns of queries, kv head, sequence), or of 64 whose units times the longest context are so many, have
-    # their prompts' pages read back once for all of them.  The kernel over 4 bits reads them for every 16 columns; the one over ordinary pages
-    # takes 256 columns a CTA.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: a prompt alone, 128 tokens (256 units)
-    # 13.1 / 11.9, 256 tokens 14.7 / 23; four of 32 (256) 11.1 / 11.3; behind 1,000, 64 tokens (128) 25.6 / 20.4, 96 tokens (192) 25.8 / 26.2; behind
-    # 8,000, 16 tokens (32) 26 / 27.5, 64 tokens 34.5 / 69; behind 32,000, 16 tokens 76 / 66, 32 tokens 78 / 126, 128 tokens 96 / 457.
+    # Steps of at least so many units (16 columns of queries, kv head, sequence), or of 40 whose units times the longest context are so many, have
+    # their prompts' pages read back once for all of them.  The kernel over 4 bits reads them for every 8 columns; the one over ordinary pages
+    # takes 256 columns a CTA.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: a prompt alone, 64 tokens (128 units)
+    # 13.9 / 8.3, 96 tokens (192) 14.1 / 14.7, 256 tokens 15.5 / 29; four of 32 (256) 14.3 / 13.9; behind 1,000, 64 tokens 26.5 / 16.9, 96 tokens 26.3 /
+    # 30, four of 32 27.4 / 27.0; behind 8,000, 12 tokens (24) 26.6 / 21.7, 16 tokens (32) 26.8 / 26.0, 32 tokens 28.7 / 41.6; behind 32,000, 12
+    # tokens 77 / 53, 32 tokens 80 / 136, 128 tokens 98 / 519.
     # Other head sizes and options go through the older kernel for ordinary pages, of which a CTA walks its context alone, from 4/3 of those units, or
-    # 10/3 behind 1,000 and more: heads of 96, a prompt alone, 256 tokens (512) 18.5 / 19.2, 512 tokens 29 / 42; behind 1,000, 256 tokens 51 / 43,
-    # 512 tokens (1,024) 68 / 88; behind 8,000, 256 tokens 269 / 200, 512 tokens 332 / 402; heads of 256 alike.
-    KV4_PAGES_FROM, KV4_PAGES_WORK = 300, 200_000
+    # 8/3 behind 1,000 and more: heads of 96, a prompt alone, 128 tokens (256) 14.2 / 14.5, 512 tokens 29 / 54; behind 1,000, 256 tokens (512) 50.5 / 54,
+    # four of 64 (512) 46 / 37; behind 8,000, 256 tokens 269 / 236, 512 tokens 331 / 426; heads of 256 alike.
+    KV4_PAGES_FROM, KV4_PAGES_WORK = 190, 250_000
 
     @staticmethod
     def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, max_kv_len: int, n_seqs: int, nqh: int, nkh: int, tc: bool) -> bool:
@@ -953,9 +954,9 @@ class Kernels:
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
         units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
         if tc:
-            worth = units >= Kernels.KV4_PAGES_FROM or (units >= 64 and units * max_kv_len >= Kernels.KV4_PAGES_WORK)
+            worth = units >= Kernels.KV4_PAGES_FROM or (units >= 40 and units * max_kv_len >= Kernels.KV4_PAGES_WORK)
         else:
-            worth = 3 * units >= Kernels.KV4_PAGES_FROM * (4 if max_kv_len < 1000 else 10)
+            worth = 3 * units >= Kernels.KV4_PAGES_FROM * (4 if max_kv_len < 1000 else 8)
         return worth and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
     def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
@@ -1004,7 +1005,7 @@ class Kernels:
                 args = _KV4_ARGS.pack(
                     0, out.data_ptr(), partial.data_ptr(), 0, 0, 0, q_len.data_ptr(), 0, token_seq.data_ptr(), sinks, _ptr(gate) or 0, 0, 0, 0,
                     self._error_flag.data_ptr() + 16, 0, out.stride(0), gate_stride, rows, n_seqs, max_q_len, nqh, nkh, 0, 0, 0, 0, n_splits,
-                    has_sink, 0, scale, sink, out_scale, 0.0, 0, 0, 0, q_from, 0, 0)
+                    has_sink, 0, scale, sink, out_scale, 0.0, 0, 0, q_from, 0, 0)
                 self.launches += 1
                 self._check_lib(lib_tc, lib_tc.braid_attn_kv4_merge(args, stream), "attn_kv4")
         self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale,
@@ -1030,15 +1031,12 @@ class Kernels:
                       scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled, q_to=0) -> None:
         lib = self.kv4_attention_library(hd)
         f32, g, rows = int(out.dtype == torch.float32), nqh // nkh, out.shape[0]
-        key = (min(g * max_q_len, 9), f32)
-        plan = lib.plans.get(key)
+        plan = lib.plans.get(f32)
         if plan is None:
-            columns = lib.braid_attn_kv4_columns(key[0], f32)
-            plan = lib.plans[key] = (columns, lib.braid_attn_kv4_slots(f32, columns),
-                                     [0, 0] + [lib.braid_attn_kv4_clusters(f32, columns, n) for n in range(2, 5)])
-        columns, slots, clusters = plan
-        hpc = min(g, columns)
-        ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (columns // hpc))
+            plan = lib.plans[f32] = (lib.braid_attn_kv4_slots(f32), [0, 0] + [lib.braid_attn_kv4_clusters(f32, n) for n in range(2, 5)])
+        slots, clusters = plan
+        hpc = min(g, 8)
+        ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (8 // hpc))
         span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
         # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
         n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
@@ -1057,7 +1055,7 @@ class Kernels:
             kv_before.data_ptr(), token_seq.data_ptr(), _ptr(head_sinks) or 0, _ptr(head_gate) or 0, _ptr(head_scale) or 0, _ptr(bias[0]) or 0,
             _ptr(bias[1]) or 0, self._error_flag.data_ptr() + 16, q.stride(0), out.stride(0), head_gate.stride(0) if head_gate is not None else 0,
             rows, n_seqs, max_q_len, nqh, nkh, page_table.shape[1], cache.shape[0], window, keep_first, n_splits, int(sink is not None),
-            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, columns, int(cluster), 0, q_to, 0)
+            int(settled), scale, sink or 0.0, out_scale, softcap or 0.0, f32, int(cluster), 0, q_to, 0)
         self.launches += 1 + (partial is not None)
         self._check_lib(lib, lib.braid_attn_kv4(args, self._stream()), "attn_kv4")
 

@@ -50,7 +50,7 @@ struct Kv4Args {
     long long q_stride, out_stride, gate_stride;
     int rows, n_seqs, max_q_len, nqh, nkh, cols, num_pages, window, keep_first, n_splits, has_sink, settled;
     float scale, sink, out_scale, softcap;
-    int f32, columns;            // float32 rows; columns a CTA
+    int f32;                     // float32 rows
     int cluster;                 // the slices are CTAs of a cluster, which merges them
     int q_from, q_to;            // (0: no bound) only sequences that bring at least, at most so many tokens
     int partial_rows;            // rows of `partial`: `rows`, or with q_to n_seqs * q_to (sequence, token)
@@ -189,22 +189,22 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     return w;
 }
 
-template <int PARTS, int NT, int NW, int SR, int ST>
+template <int PARTS, int NW, int SR, int ST>
 struct Kv4Cfg {
     static constexpr int HD = BRAID_HD, W = HD / 32;
     static constexpr int US = 16 * SR;                       // tokens a unit
     static constexpr int SB = SR * kv4_record_bytes(HD);     // bytes a unit
-    static constexpr int BM = 8 * NT;                        // columns a CTA
+    static constexpr int BM = 8;                             // columns a CTA
     static constexpr int RING = NW * ST * SB;
     static constexpr int MERGE = NW * BM * (HD + 4) * 4;
     static constexpr int SMEM = RING > MERGE ? RING : MERGE;
     static_assert(BRAID_PAGE_SIZE % US == 0, "a unit must not straddle a page");
 };
 
-template <int PARTS, int NT, int NW, int SR, int ST>
+template <int PARTS, int NW, int SR, int ST>
 __global__ void __launch_bounds__(NW * 32, SR == 4 ? 2 : 1)
 attn_kv4_kernel(const Kv4Args a) {
-    using C = Kv4Cfg<PARTS, NT, NW, SR, ST>;
+    using C = Kv4Cfg<PARTS, NW, SR, ST>;
     using T = typename std::conditional<PARTS == 3, float, __nv_bfloat16>::type;
     constexpr int HD = C::HD, W = C::W;
     pdl_trigger();
@@ -277,87 +277,81 @@ attn_kv4_kernel(const Kv4Args a) {
     }
     while (issued < min(ST, n_mine)) issue();
 
-    // ---- queries: column nt * 8 + r, numbers 32 w + 8 j .. + 7 of the head
-    uint32_t q[NT][W][PARTS][4];
+    // ---- queries: column r, numbers 32 w + 8 j .. + 7 of the head
+    uint32_t q[W][PARTS][4];
     constexpr int GH = W > 4 ? 2 : 1;
     constexpr int QP = PARTS > 1 ? 3 : 2;                      // 16 bits of it, or all
-    uint32_t qb[NT][QP][GH];                                   // the sum of group j's (and 4 + j's) numbers beside a zero, in parts
-    int q_exp[NT];                                             // of columns nt * 8 + r: the queries are scaled by 2^q_exp
+    uint32_t qb[QP][GH];                                       // the sum of group j's (and 4 + j's) numbers beside a zero, in parts
+    int q_exp;                                                 // of column r: the queries are scaled by 2^q_exp
+    const int col = r, tl = col / hpc, hl = col - tl * hpc;
+    const bool in = tl < n_tok && hl < n_heads;
+    const T* src = (const T*)a.q + (size_t)(q_start + (in ? tok0 + tl : 0)) * a.q_stride + (size_t)(head0 + (in ? hl : 0)) * HD + 8 * j;
+    const bool wide = !(((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) & 15);
+    float x[W][8], most = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int col = nt * 8 + r, tl = col / hpc, hl = col - tl * hpc;
-        const bool in = tl < n_tok && hl < n_heads;
-        const T* src = (const T*)a.q + (size_t)(q_start + (in ? tok0 + tl : 0)) * a.q_stride + (size_t)(head0 + (in ? hl : 0)) * HD + 8 * j;
-        const bool wide = !(((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) & 15);
-        float x[W][8], most = 0.f;
+    for (int w = 0; w < W; ++w) {
+        if (wide) {
+            constexpr int VW = 16 / sizeof(T);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (wide) {
-                constexpr int VW = 16 / sizeof(T);
+            for (int i = 0; i < 8; i += VW) load_run<T, VW>(src + 32 * w + i, x[w] + i);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; i += VW) load_run<T, VW>(src + 32 * w + i, x[w] + i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[w][i] = to_f32(src[32 * w + i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!in) x[w][i] = 0.f;
-                most = fmaxf(most, fabsf(x[w][i]));
-            }
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        q_exp[nt] = 120 - exponent(most);                      // the column's largest number becomes one of 2^120
-        float sums[GH];
-#pragma unroll
-        for (int h = 0; h < GH; ++h) sums[h] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += x[w][i];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if ((w & 3) == j) sums[w >> 2] = sum;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[w][i] = scaled(x[w][i], q_exp[nt] - (i & 2 ? 4 : 0));       // numbers of odd n meet 16 times their code
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) q[nt][w][p][n] = split_pair(x[w][2 * n], x[w][2 * n + 1]);
+            for (int i = 0; i < 8; ++i) x[w][i] = to_f32(src[32 * w + i]);
         }
 #pragma unroll
-        for (int h = 0; h < GH; ++h) {
-            float none = 0.f, sum = scaled(sums[h], q_exp[nt] - KV4_UNIT);
-#pragma unroll
-            for (int p = 0; p < QP; ++p) qb[nt][p][h] = split_pair(none, sum);
+        for (int i = 0; i < 8; ++i) {
+            if (!in) x[w][i] = 0.f;
+            most = fmaxf(most, fabsf(x[w][i]));
         }
     }
-    // ---- this lane's columns of scores: nt * 8 + 2 j + c
-    int pos[NT][2], lo[NT][2];
-    float sc[NT][2];
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    q_exp = 120 - exponent(most);                      // the column's largest number becomes one of 2^120
+    float sums[GH];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < GH; ++h) sums[h] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int col = nt * 8 + 2 * j + c, tl = col / hpc, hl = col - tl * hpc;
-            const bool in = tl < n_tok && hl < n_heads;
-            pos[nt][c] = in ? pos_min + tl : -1;               // -1: the column sees nothing
-            lo[nt][c] = a.window > 0 ? pos[nt][c] - a.window + 1 : 0;
-            sc[nt][c] = scaled((in && a.head_scale ? a.scale * a.head_scale[head0 + hl] : a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E),
-                               KV4_UNIT - __shfl_sync(0xffffffffu, q_exp[nt], 8 * j + 4 * c));
-        }
+    for (int w = 0; w < W; ++w) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += x[w][i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((w & 3) == j) sums[w >> 2] = sum;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[w][i] = scaled(x[w][i], q_exp - (i & 2 ? 4 : 0));       // numbers of odd n meet 16 times their code
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) q[w][p][n] = split_pair(x[w][2 * n], x[w][2 * n + 1]);
+    }
+#pragma unroll
+    for (int h = 0; h < GH; ++h) {
+        float none = 0.f, sum = scaled(sums[h], q_exp - KV4_UNIT);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) qb[p][h] = split_pair(none, sum);
+    }
+    // ---- this lane's columns of scores: 2 j + c
+    int pos[2], lo[2];
+    float sc[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int col = 2 * j + c, tl = col / hpc, hl = col - tl * hpc;
+        const bool in = tl < n_tok && hl < n_heads;
+        pos[c] = in ? pos_min + tl : -1;                       // -1: the column sees nothing
+        lo[c] = a.window > 0 ? pos[c] - a.window + 1 : 0;
+        sc[c] = scaled((in && a.head_scale ? a.scale * a.head_scale[head0 + hl] : a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E),
+                       KV4_UNIT - __shfl_sync(0xffffffffu, q_exp, 8 * j + 4 * c));
+    }
 
     // a factor that is positive commutes with the maximum, and leaves -infinity as it is
     bool late = !(a.softcap > 0.f) && !a.bias_slope;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) late = late && sc[nt][0] > 0.f && sc[nt][1] > 0.f;
+    late = late && sc[0] > 0.f && sc[1] > 0.f;
     late = __all_sync(0xffffffffu, late);
-    float lf[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) { lf[nt][0] = late ? sc[nt][0] : 1.f; lf[nt][1] = late ? sc[nt][1] : 1.f; }
-    float o[NT][2 * W][4], zs[NT][2][W], m[NT][2], l[NT][2];
+    float lf[2];
+    lf[0] = late ? sc[0] : 1.f;
+    lf[1] = late ? sc[1] : 1.f;
+    float o[2 * W][4], zs[2][W], m[2], l[2];
     bool ok = true;
     bool walked = PARTS == 1;
     int st = 0, step_exp[W];                                   // FAST: the steps of a group are scaled by 2^step_exp
@@ -371,16 +365,13 @@ attn_kv4_kernel(const Kv4Args a) {
     auto walk = [&](auto FAST) {
     constexpr bool fast = decltype(FAST)::value;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int i = 0; i < 2 * W; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2 * W; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    for (int c = 0; c < 2; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            m[nt][c] = -INFINITY;
-            l[nt][c] = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) zs[nt][c][w] = 0.f;
-        }
+        for (int w = 0; w < W; ++w) zs[c][w] = 0.f;
     }
     for (int k = 0; k < n_mine; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag));
@@ -417,8 +408,8 @@ attn_kv4_kernel(const Kv4Args a) {
             if (!__all_sync(0xffffffffu, in)) { walked = false; return; }
         }
 
-        // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][nt][0, 1]: columns of row r, [2, 3]: of row r + 8
-        float s[SR][NT][4];
+        // ---- scores of the unit's tokens: rows 16 rec + r, + 8; s[rec][0, 1]: columns of row r, [2, 3]: of row r + 8
+        float s[SR][4];
 #pragma unroll
         for (int rec = 0; rec < SR; ++rec) {
             const uint8_t* rb = base + rec * kv4_record_bytes(HD);
@@ -438,31 +429,25 @@ attn_kv4_kernel(const Kv4Args a) {
                 wa[1] = reinterpret_cast<const uint32_t*>(groups)[4 + j];
                 wb[1] = reinterpret_cast<const uint32_t*>(groups + 32 * W)[4 + j];
             }
+            mma16816_zero(s[rec], wa[0], wb[0], wa[1], wb[1], qb[0][0], GH > 1 ? qb[0][GH - 1] : 0u);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma16816_zero(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][0][0], GH > 1 ? qb[nt][0][GH - 1] : 0u);
-#pragma unroll
-                for (int p = 1; p < QP; ++p) mma16816(s[rec][nt], wa[0], wb[0], wa[1], wb[1], qb[nt][p][0], GH > 1 ? qb[nt][p][GH - 1] : 0u);
-            }
+            for (int p = 1; p < QP; ++p) mma16816(s[rec], wa[0], wb[0], wa[1], wb[1], qb[p][0], GH > 1 ? qb[p][GH - 1] : 0u);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 const uint32_t a0 = codes<true, 0>(ka[w]), a1 = codes<true, 0>(kb[w]), a2 = codes<true, 1>(ka[w]), a3 = codes<true, 1>(kb[w]);
                 const uint32_t b0 = codes<true, 2>(ka[w]), b1 = codes<true, 2>(kb[w]), b2 = codes<true, 3>(ka[w]), b3 = codes<true, 3>(kb[w]);
                 const float sa = kv4_step(ga[w]), sb = kv4_step(gb[w]);
+                float raw[4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float raw[4];
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        if (p == 0) mma16816_zero(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
-                        else mma16816(raw, a0, a1, a2, a3, q[nt][w][p][0], q[nt][w][p][1]);
-                        mma16816(raw, b0, b1, b2, b3, q[nt][w][p][2], q[nt][w][p][3]);
-                    }
-                    s[rec][nt][0] = fmaf(sa, raw[0], s[rec][nt][0]);
-                    s[rec][nt][1] = fmaf(sa, raw[1], s[rec][nt][1]);
-                    s[rec][nt][2] = fmaf(sb, raw[2], s[rec][nt][2]);
-                    s[rec][nt][3] = fmaf(sb, raw[3], s[rec][nt][3]);
+                for (int p = 0; p < PARTS; ++p) {
+                    if (p == 0) mma16816_zero(raw, a0, a1, a2, a3, q[w][p][0], q[w][p][1]);
+                    else mma16816(raw, a0, a1, a2, a3, q[w][p][0], q[w][p][1]);
+                    mma16816(raw, b0, b1, b2, b3, q[w][p][2], q[w][p][3]);
                 }
+                s[rec][0] = fmaf(sa, raw[0], s[rec][0]);
+                s[rec][1] = fmaf(sa, raw[1], s[rec][1]);
+                s[rec][2] = fmaf(sb, raw[2], s[rec][2]);
+                s[rec][3] = fmaf(sb, raw[3], s[rec][3]);
             }
         }
         // ---- factors, cap, bias; mask.  Plain scores are left as they are: their factor is applied where the exponential is taken
@@ -470,25 +455,21 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
             for (int rec = 0; rec < SR; ++rec)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[rec][nt][e] *= sc[nt][e & 1];
-        if (a.softcap > 0.f) softcap_scores<SR * NT * 4>(&s[0][0][0], 1.f, a.softcap * LOG2E);
+                for (int e = 0; e < 4; ++e) s[rec][e] *= sc[e & 1];
+        if (a.softcap > 0.f) softcap_scores<SR * 4>(&s[0][0], 1.f, a.softcap * LOG2E);
         if (a.bias_slope) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < 2; ++c) {
+                const int col = 2 * j + c, hl = col % hpc;
+                const float r1 = hl < n_heads ? a.bias_slope[head0 + hl] : 0.f, r2 = hl < n_heads ? a.bias_rate[head0 + hl] : 0.f;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int col = nt * 8 + 2 * j + c, hl = col % hpc;
-                    const float r1 = hl < n_heads ? a.bias_slope[head0 + hl] : 0.f, r2 = hl < n_heads ? a.bias_rate[head0 + hl] : 0.f;
+                for (int rec = 0; rec < SR; ++rec)
 #pragma unroll
-                    for (int rec = 0; rec < SR; ++rec)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {          // (keys after the query are masked below)
-                            const float d = (float)(pos[nt][c] - (key0 + 16 * rec + 8 * h + r));
-                            s[rec][nt][2 * h + c] -= r1 * LOG2E * log1pf(r2 * fmaxf(d, 0.f));
-                        }
-                }
+                    for (int h = 0; h < 2; ++h) {          // (keys after the query are masked below)
+                        const float d = (float)(pos[c] - (key0 + 16 * rec + 8 * h + r));
+                        s[rec][2 * h + c] -= r1 * LOG2E * log1pf(r2 * fmaxf(d, 0.f));
+                    }
+            }
         }
         // (columns that are no query see as much as the others, and nobody reads them)
         const bool edge = !(key0 + C::US - 1 <= pos_min && (a.window == 0 || key0 >= pos_max - a.window + 1));
@@ -496,45 +477,39 @@ attn_kv4_kernel(const Kv4Args a) {
 #pragma unroll
             for (int rec = 0; rec < SR; ++rec)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 16 * rec + 8 * (e >> 1) + r, c = e & 1;
-                        if (!(key <= pos[nt][c] && (key >= lo[nt][c] || key < a.keep_first))) s[rec][nt][e] = -INFINITY;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + 16 * rec + 8 * (e >> 1) + r, c = e & 1;
+                    if (!(key <= pos[c] && (key >= lo[c] || key < a.keep_first))) s[rec][e] = -INFINITY;
+                }
         }
         // ---- running maximum
-        float top[NT][2];
+        float top[2];
         bool raise = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < 2; ++c) {
+            float x = fmaxf(s[0][c], s[0][2 + c]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
-#pragma unroll
-                for (int rec = 1; rec < SR; ++rec) x = fmaxf(x, fmaxf(s[rec][nt][c], s[rec][nt][2 + c]));
-                x *= lf[nt][c];
-                top[nt][c] = x;
-                raise |= x > m[nt][c] + KV4_RAISE;
-            }
+            for (int rec = 1; rec < SR; ++rec) x = fmaxf(x, fmaxf(s[rec][c], s[rec][2 + c]));
+            x *= lf[c];
+            top[c] = x;
+            raise |= x > m[c] + KV4_RAISE;
+        }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < 2; ++c) {
+                float x = top[c];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(x, m[c]);
+                const float f = x == -INFINITY ? 1.f : exp2f(m[c] - x);      // exp2(-inf) = 0
+                m[c] = x;
+                l[c] *= f;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float x = top[nt][c];
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(x, m[nt][c]);
-                    const float f = x == -INFINITY ? 1.f : exp2f(m[nt][c] - x);      // exp2(-inf) = 0
-                    m[nt][c] = x;
-                    l[nt][c] *= f;
+                for (int w = 0; w < W; ++w) zs[c][w] *= f;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) zs[nt][c][w] *= f;
-#pragma unroll
-                    for (int i = 0; i < 2 * W; ++i) { o[nt][i][c] *= f; o[nt][i][2 + c] *= f; }
-                }
+                for (int i = 0; i < 2 * W; ++i) { o[i][c] *= f; o[i][2 + c] *= f; }
+            }
         }
         // ---- probabilities and values.  On an edge (EDGE) what a column does not see does not count, whatever it holds: a value's
         // step or lowest number may be NaN
@@ -567,15 +542,13 @@ attn_kv4_kernel(const Kv4Args a) {
                     v89[w] = u[8 * (HD / 4)] | ((uint32_t)u[9 * (HD / 4)] << 16);
                 }
             }
-            float p[NT][4];
+            float p[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = e & 1;
-                    p[nt][e] = exp2_ftz(fmaf(s[rec][nt][e], lf[nt][c], m[nt][c] == -INFINITY ? 0.f : -m[nt][c]));
-                    l[nt][c] += p[nt][e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int c = e & 1;
+                p[e] = exp2_ftz(fmaf(s[rec][e], lf[c], m[c] == -INFINITY ? 0.f : -m[c]));
+                l[c] += p[e];
+            }
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 // (a step of 0 becomes some number below the codes' reach; its codes are 0)
@@ -584,31 +557,28 @@ attn_kv4_kernel(const Kv4Args a) {
                 const float za = fast ? kv4_lowest(ga[w]) : fmaf(8.f, sa, kv4_lowest(ga[w])), zb = fast ? kv4_lowest(gb[w]) : fmaf(8.f, sb, kv4_lowest(gb[w]));
                 const uint32_t a0 = codes<fast, 0>(v01[w]), a1 = codes<fast, 1>(v01[w]), a2 = codes<fast, 0>(v89[w]), a3 = codes<fast, 1>(v89[w]);
                 const uint32_t b0 = codes<fast, 2>(v01[w]), b1 = codes<fast, 3>(v01[w]), b2 = codes<fast, 2>(v89[w]), b3 = codes<fast, 3>(v89[w]);
+                float x[4] = {p[0] * sa, p[1] * sa, p[2] * sb, p[3] * sb};
+                if constexpr (EDGE.value) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float x[4] = {p[nt][0] * sa, p[nt][1] * sa, p[nt][2] * sb, p[nt][3] * sb};
-                    if constexpr (EDGE.value) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool seen = s[rec][nt][e] != -INFINITY;
-                            if (!seen) x[e] = 0.f;
-                            if (seen) zs[nt][e & 1][w] = fmaf(p[nt][e], e < 2 ? za : zb, zs[nt][e & 1][w]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) zs[nt][e & 1][w] = fmaf(p[nt][e], e < 2 ? za : zb, zs[nt][e & 1][w]);
+                    for (int e = 0; e < 4; ++e) {
+                        const bool seen = s[rec][e] != -INFINITY;
+                        if (!seen) x[e] = 0.f;
+                        if (seen) zs[e & 1][w] = fmaf(p[e], e < 2 ? za : zb, zs[e & 1][w]);
                     }
-                    if constexpr (fast) {
-                        const uint32_t p0 = transpose8x8(pack_half(x[0], x[1])), p1 = transpose8x8(pack_half(x[2], x[3]));
-                        mma16816_f16(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
-                        mma16816_f16(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
-                    } else {
+                } else {
 #pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
-                            const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
-                            mma16816(o[nt][2 * w], a0, a1, a2, a3, p0, p1);
-                            mma16816(o[nt][2 * w + 1], b0, b1, b2, b3, p0, p1);
-                        }
+                    for (int e = 0; e < 4; ++e) zs[e & 1][w] = fmaf(p[e], e < 2 ? za : zb, zs[e & 1][w]);
+                }
+                if constexpr (fast) {
+                    const uint32_t p0 = transpose8x8(pack_half(x[0], x[1])), p1 = transpose8x8(pack_half(x[2], x[3]));
+                    mma16816_f16(o[2 * w], a0, a1, a2, a3, p0, p1);
+                    mma16816_f16(o[2 * w + 1], b0, b1, b2, b3, p0, p1);
+                } else {
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
+                        mma16816(o[2 * w], a0, a1, a2, a3, p0, p1);
+                        mma16816(o[2 * w + 1], b0, b1, b2, b3, p0, p1);
                     }
                 }
             }
@@ -624,15 +594,12 @@ attn_kv4_kernel(const Kv4Args a) {
     {
         float t = walked ? 0.f : INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int i = 0; i < 2 * W; ++i) t = fmaf(0.f, o[i][0], fmaf(0.f, o[i][1], fmaf(0.f, o[i][2], fmaf(0.f, o[i][3], t))));
 #pragma unroll
-            for (int i = 0; i < 2 * W; ++i) t = fmaf(0.f, o[nt][i][0], fmaf(0.f, o[nt][i][1], fmaf(0.f, o[nt][i][2], fmaf(0.f, o[nt][i][3], t))));
+        for (int c = 0; c < 2; ++c) {
+            t = fmaf(0.f, l[c], t);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                t = fmaf(0.f, l[nt][c], t);
-#pragma unroll
-                for (int w = 0; w < W; ++w) t = fmaf(0.f, zs[nt][c][w], t);
-            }
+            for (int w = 0; w < W; ++w) t = fmaf(0.f, zs[c][w], t);
         }
         if (__any_sync(0xffffffffu, ok && t != 0.f)) {
             if constexpr (PARTS == 1) for (; st != istage; phase ^= (st == ST - 1), st = st == ST - 1 ? 0 : st + 1)        // (units asked for and not walked)
@@ -656,35 +623,31 @@ attn_kv4_kernel(const Kv4Args a) {
 
     // ---- the CTA's warps merge
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int x = 4; x < 32; x <<= 1) {
+            l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
-#pragma unroll
-                for (int w = 0; w < W; ++w) zs[nt][c][w] += __shfl_xor_sync(0xffffffffu, zs[nt][c][w], x);
-            }
+            for (int w = 0; w < W; ++w) zs[c][w] += __shfl_xor_sync(0xffffffffu, zs[c][w], x);
+        }
     __syncthreads();                                           // every warp is done with its ring
     float* mo = reinterpret_cast<float*>(smem);                // [warp][column][HD]
     float* ml = mo + NW * C::BM * HD;                          // [warp][column][2]
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int c = 0; c < 2; ++c) {
+        const int col = 2 * j + c;
+        float* dst = mo + (warp * C::BM + col) * HD + 4 * r;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int col = nt * 8 + 2 * j + c;
-            float* dst = mo + (warp * C::BM + col) * HD + 4 * r;
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-            {
-                // FAST: codes counted in steps of 2^-24, those of odd n in steps 16 times that
-                const int even = walked ? 24 - step_exp[w] : 0, odd = walked ? even - 4 : 0;
-                *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(
-                    fmaf(o[nt][2 * w][c], pow2(even), zs[nt][c][w]), fmaf(o[nt][2 * w][2 + c], pow2(odd), zs[nt][c][w]),
-                    fmaf(o[nt][2 * w + 1][c], pow2(even), zs[nt][c][w]), fmaf(o[nt][2 * w + 1][2 + c], pow2(odd), zs[nt][c][w]));
-            }
-            if (r == 0) { ml[(warp * C::BM + col) * 2] = m[nt][c]; ml[(warp * C::BM + col) * 2 + 1] = l[nt][c]; }
+        for (int w = 0; w < W; ++w)
+        {
+            // FAST: codes counted in steps of 2^-24, those of odd n in steps 16 times that
+            const int even = walked ? 24 - step_exp[w] : 0, odd = walked ? even - 4 : 0;
+            *reinterpret_cast<float4*>(dst + 32 * w) = make_float4(
+                fmaf(o[2 * w][c], pow2(even), zs[c][w]), fmaf(o[2 * w][2 + c], pow2(odd), zs[c][w]),
+                fmaf(o[2 * w + 1][c], pow2(even), zs[c][w]), fmaf(o[2 * w + 1][2 + c], pow2(odd), zs[c][w]));
         }
+        if (r == 0) { ml[(warp * C::BM + col) * 2] = m[c]; ml[(warp * C::BM + col) * 2 + 1] = l[c]; }
+    }
     __syncthreads();
     const bool out_wide = !(((uintptr_t)a.out | (uintptr_t)(a.out_stride * sizeof(T))) & (4 * sizeof(T) - 1));
     // a column's numbers d .. d + 3 from what `n` slices of this CTA's (or the cluster's) warps left
@@ -851,23 +814,23 @@ attn_kv4_merge_few_kernel(const Kv4Args a) {
 // ------------------------------------------------------------------ host side
 // Four warps a CTA.  A unit is SR records of 16 tokens: four of them give a warp enough independent products to work on (one request of
 // 128k, heads of 128: 53 us with two records a unit and 12 warps an SM, 45 with four and 8, which may take 255 registers then; 54 with
-// 12 warps of four records in parts that come and go by themselves); two where the registers hold no more: 16 columns, float32, heads
-// above 128.
+// 12 warps of four records in parts that come and go by themselves); two where the registers hold no more: float32, heads above 128.
+// More queries than 8 columns hold are more CTAs: 16 columns a CTA, which share the codes' way to the operands but leave room for two records, took
+// longer (us, 16 / 8 columns: 6 sequences of 5 tokens of 4 heads in a window of 4,096, 32 / 27; 64 of 5 behind 4,000, 214 / 179; heads of 64, 141 / 102).
 #define KV4_NW 4
-#define KV4_NT_MAX (BRAID_HD > 128 ? 1 : 2)
-constexpr int kv4_sr(int parts, int nt) { return BRAID_HD <= 128 && parts == 1 && nt == 1 ? 4 : 2; }
-constexpr int kv4_st(int parts, int nt) { return kv4_sr(parts, nt) == 4 || BRAID_HD > 128 ? 2 : 3; }
-template <int PARTS, int NT> using Kv4C = Kv4Cfg<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>;
+constexpr int kv4_sr(int parts) { return BRAID_HD <= 128 && parts == 1 ? 4 : 2; }
+constexpr int kv4_st(int parts) { return kv4_sr(parts) == 4 || BRAID_HD > 128 ? 2 : 3; }
+template <int PARTS> using Kv4C = Kv4Cfg<PARTS, KV4_NW, kv4_sr(PARTS), kv4_st(PARTS)>;
 
-template <int PARTS, int NT>
-static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>; }
+template <int PARTS>
+static const void* kv4_kernel() { return (const void*)attn_kv4_kernel<PARTS, KV4_NW, kv4_sr(PARTS), kv4_st(PARTS)>; }
 
-template <int PARTS, int NT>
+template <int PARTS>
 static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
-    using C = Kv4C<PARTS, NT>;
+    using C = Kv4C<PARTS>;
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(kv4_kernel<PARTS, NT>(), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kv4_kernel<PARTS>(), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) { braid_set_error("attn_kv4: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e)); return (int)e; }
         configured = true;
     }
@@ -889,21 +852,20 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
     attr[1].val.clusterDim.z = a.n_splits;
     cfg.attrs = attr;
     cfg.numAttrs = a.cluster ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, attn_kv4_kernel<PARTS, NT, KV4_NW, kv4_sr(PARTS, NT), kv4_st(PARTS, NT)>, a);
+    cudaLaunchKernelEx(&cfg, attn_kv4_kernel<PARTS, KV4_NW, kv4_sr(PARTS), kv4_st(PARTS)>, a);
     BRAID_LAUNCH_CHECK();
 }
 
 extern "C" int braid_attn_kv4_head_dim(void) { return BRAID_HD; }
 extern "C" int braid_attn_kv4_args_bytes(void) { return (int)sizeof(Kv4Args); }
-extern "C" int braid_attn_kv4_columns(int wanted, int f32) { return wanted <= 8 || KV4_NT_MAX == 1 || (f32 && BRAID_HD > 64) ? 8 : 16; }
 
 // CTAs that the device holds at once.
-extern "C" int braid_attn_kv4_slots(int f32, int columns) {
+extern "C" int braid_attn_kv4_slots(int f32) {
     int dev = 0, sms = 0, per_sm = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const void* f = columns <= 8 ? (f32 ? kv4_kernel<3, 1>() : kv4_kernel<1, 1>()) : (f32 ? kv4_kernel<3, KV4_NT_MAX>() : kv4_kernel<1, KV4_NT_MAX>());
-    const int bytes = columns <= 8 ? (f32 ? Kv4C<3, 1>::SMEM : Kv4C<1, 1>::SMEM) : (f32 ? Kv4C<3, KV4_NT_MAX>::SMEM : Kv4C<1, KV4_NT_MAX>::SMEM);
+    const void* f = f32 ? kv4_kernel<3>() : kv4_kernel<1>();
+    const int bytes = f32 ? Kv4C<3>::SMEM : Kv4C<1>::SMEM;
     cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, f, KV4_NW * 32, bytes);
     if (e != cudaSuccess || per_sm <= 0 || sms <= 0) return 148 * 2;
@@ -911,9 +873,9 @@ extern "C" int braid_attn_kv4_slots(int f32, int columns) {
 }
 
 // Clusters of `size` CTAs that the device holds at once (0: none).
-extern "C" int braid_attn_kv4_clusters(int f32, int columns, int size) {
-    const void* f = columns <= 8 ? (f32 ? kv4_kernel<3, 1>() : kv4_kernel<1, 1>()) : (f32 ? kv4_kernel<3, KV4_NT_MAX>() : kv4_kernel<1, KV4_NT_MAX>());
-    const int bytes = columns <= 8 ? (f32 ? Kv4C<3, 1>::SMEM : Kv4C<1, 1>::SMEM) : (f32 ? Kv4C<3, KV4_NT_MAX>::SMEM : Kv4C<1, KV4_NT_MAX>::SMEM);
+extern "C" int braid_attn_kv4_clusters(int f32, int size) {
+    const void* f = f32 ? kv4_kernel<3>() : kv4_kernel<1>();
+    const int bytes = f32 ? Kv4C<3>::SMEM : Kv4C<1>::SMEM;
     cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1, 1, size);
@@ -966,8 +928,6 @@ extern "C" int braid_attn_kv4(const Kv4Args* args, void* stream) {
     if (a.n_splits <= 1 || a.n_splits > 8) a.cluster = 0;
     if (a.n_splits > 1 && !a.cluster && !a.partial) BRAID_REFUSE("attn_kv4: slices that are no cluster need the partial buffer");
     cudaStream_t s = (cudaStream_t)stream;
-    int rc;
-    if (a.columns <= 8) rc = a.f32 ? launch_kv4<3, 1>(a, s) : launch_kv4<1, 1>(a, s);
-    else rc = a.f32 ? launch_kv4<3, KV4_NT_MAX>(a, s) : launch_kv4<1, KV4_NT_MAX>(a, s);
+    const int rc = a.f32 ? launch_kv4<3>(a, s) : launch_kv4<1>(a, s);
     return rc || a.n_splits == 1 || a.cluster ? rc : braid_attn_kv4_merge(&a, stream);
 }
