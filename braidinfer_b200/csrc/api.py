@@ -1027,6 +1027,16 @@ class Kernels:
             return max(most, rounds * mean) / 128 / n * 1.55 + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
         return min(range(1, max(1, min(8, most // 512)) + 1), key=cost)
 
+    @staticmethod
+    def _kv4_slices_cost(waves: float, n: int, us: float, least: bool) -> float:
+        """us of attention over 4 bits in n slices: `waves` CTAs a place for them without slices, which take 5 us and what they walk
+        (`us` all of a context).  Contexts differ in length, which fills the gaps of a wave.  (Heads of 128, 8 kv heads, requests of up to 8,000, 1 /
+        2 / 3 / 4 slices: 20 of them 71 / 59 / 55 / 58, 30 71 / 71 / 73 / 75, 40 104 / 92 / 93 / 94, 50 107 / 100 / 104 / 111, 64 126 / 128 / 133 / 140;
+        20 in float32 138 / 105 / 95 / 94.)"""
+        x = waves * n
+        rounds = 1 if x <= 1 else 0.75 * x + 0.6 if least else 0.85 * x + 0.5
+        return rounds * (5 + us / n) + (0 if n == 1 else 3)
+
     def _attn_kv4_mma(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                       scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias, softcap, settled, q_to=0) -> None:
         lib = self.kv4_attention_library(hd)
@@ -1038,8 +1048,12 @@ class Kernels:
         hpc = min(g, 8)
         ctas = n_seqs * nkh * -(-g // hpc) * -(-max_q_len // (8 // hpc))
         span = min(max_kv_len, window + keep_first + max_q_len) if window else max_kv_len
-        # one wave of CTAs over the device, and at least a unit of 32 tokens a warp
+        # one wave of CTAs over the device, and at least a unit of 32 tokens a warp ...
         n_splits = max(1, min(slots // max(ctas, 1), -(-span // 128)))
+        wave = span * (2 if f32 else 1) * max(hd, 100) / 16000            # us that a CTA walks
+        if 2 * ctas * n_splits > slots and wave >= 24 and ctas < 4 * slots:
+            # ... or, where CTAs leave much of a wave of long contexts empty, more and shorter ones
+            n_splits = min(range(n_splits, n_splits + 4), key=lambda n: self._kv4_slices_cost(ctas / slots, n, wave, n == n_splits))
         # Few slices are a cluster where the device holds all clusters at once: one launch instead of two.  Larger clusters wait for as many
         # free places side by side (us as a cluster / with a kernel that merges, on the device: 4 requests of 3,000 tokens in float32, 4 slices
         # 12.4 / 12.7, 8 slices 11.4 / 10.3, 16 slices 13.7 / 9.6; one request of 1,100, 4 slices 10.8 / 10.6, 8 slices 11.1 / 9.1), and a
