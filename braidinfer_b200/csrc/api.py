@@ -141,8 +141,8 @@ class RowScale:
 
 # The argument structures of csrc/attn_kv4.cu (Kv4Args) and csrc/kv4.cu (TablesArgs, StoreArgs, ExpandArgs, Kv4SimpleArgs).
 _KV4_ARGS = struct.Struct("<15Q3q12i4f5i4x")
-_KV4_PROMPT_ARGS = struct.Struct("<11Q3qQ8i7f3i")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
-_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<8Q11i4x")
+_KV4_PROMPT_ARGS = struct.Struct("<14Q3qQ8i7f4i4x")      # Kv4PromptArgs of csrc/attn_kv4_tc.cu
+_TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<10Q11i4x")
 _KV4_SIMPLE_ARGS = struct.Struct("<7Q2q8ifi2f2Qq3Qfi2Q")
 
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
@@ -831,12 +831,12 @@ class Kernels:
         self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
 
     def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_cols=0, out_table=None, repair=None, seq0=0,
-                q_from=0) -> None:
+                q_from=0, scales=None, top=0) -> None:
         self.launches += 1
         args = _EXPAND_ARGS.pack(cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), q_len.data_ptr(), kv_before.data_ptr(),
-                                 self._error_flag.data_ptr() + 16, _ptr(repair) or 0, _ptr(out_table) or 0, n, cache.shape[1], hd,
-                                 page_table.shape[1], cache.shape[0], window, keep_first, out_cols,
-                                 seq0, dtype_code(out.dtype), q_from)
+                                 self._error_flag.data_ptr() + 16, _ptr(repair) or 0, _ptr(out_table) or 0, _ptr(scales) or 0, top, n,
+                                 cache.shape[1], hd, page_table.shape[1], cache.shape[0], window, keep_first, out_cols, seq0,
+                                 0 if scales is not None else dtype_code(out.dtype), q_from)
         self._check_lib(lib, lib.braid_kv4_expand(args, self._stream()), "kv4_expand")
 
     def attn_kv4(self, q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -962,16 +962,17 @@ class Kernels:
     def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                         scale, keep_first, head_scale, options, tc, q_from) -> None:
         """Prompts, bfloat16: the pages that the queries see are read back, block c of sequence i as page i * cols + c of a workspace,
-        and the attention of ordinary pages runs over them.  Values that are NaN are read back as zero, and the sequences that hold some
-        are computed by the plain kernel (which otherwise ends at once)."""
+        and the attention of ordinary pages runs over them.  With `tc` they are float16 numbers, scaled a page and head.
+        Values that are NaN are read back as zero; the sequences that hold some, or whose values' sizes lie so far apart that float16 would not
+        hold them, are computed by the plain kernel (which otherwise ends at once)."""
         lib = self.part_library("kv4")
         cols = min(page_table.shape[1], max(1, -(-max_kv_len // build.page_size())))
         page = 2 * nkh * build.page_size() * hd
         group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
         # from torch's allocator at every call: calls on other streams, and other graphs, have their own
         device, stream = out.device, self._stream()
-        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.bfloat16, device=device)
-        repair = torch.zeros(n_seqs + 1, dtype=torch.int32, device=device)
+        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.float16 if tc else torch.bfloat16, device=device)
+        repair = torch.zeros(1 + n_seqs * (1 + nkh), dtype=torch.int32, device=device)     # and the sequences' largest exponents
         lengths = (q_start, q_len, kv_before)
         if not tc:
             table, fence = torch.empty((group, cols), dtype=torch.int32, device=device), repair.new_empty(1)
@@ -984,21 +985,23 @@ class Kernels:
                               head_scale=head_scale, **options)
         else:
             lib_tc, partial = self.kv4_attention_library(hd), None
+            scales = torch.empty(group * cols * nkh * 2, dtype=torch.int32, device=device)
+            flags, top = repair.data_ptr(), repair.data_ptr() + 4 * (1 + n_seqs)
             gate, bias = options["head_gate"], options["distance_bias"] or (None, None)
             sinks, gate_stride, has_sink = _ptr(options["head_sinks"]) or 0, gate.stride(0) if gate is not None else 0, int(options["sink"] is not None)
             sink, out_scale, rows = options["sink"] or 0.0, options["out_scale"], out.shape[0]
             for i in range(0, n_seqs, group):
                 n = min(group, n_seqs - i)
                 part, part_table = (lengths, page_table) if n == n_seqs else ([t[i:i + n] for t in lengths], page_table[i:i + n])
-                self._expand(lib, cache, pages, part_table, *part[1:], n, hd, window, 0, cols, None, repair, i, q_from)
+                self._expand(lib, cache, pages, part_table, *part[1:], n, hd, window, 0, cols, None, repair, i, q_from, scales, top)
                 if i == 0:
                     n_splits = self._kv4_prompt_slices(rows, group, max_q_len, max_kv_len, nqh, nkh, hd, window)
                     if n_splits > 1:
                         partial = torch.empty(rows * nqh * n_splits * (hd + 2), dtype=torch.float32, device=device)
                 args = _KV4_PROMPT_ARGS.pack(
                     q.data_ptr(), pages.data_ptr(), out.data_ptr(), *[t.data_ptr() for t in part], self._error_flag.data_ptr() + 12, sinks,
-                    _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, q.stride(0), out.stride(0), gate_stride, _ptr(partial) or 0, rows, n,
-                    max_q_len, nqh, nkh, cols, window, has_sink, scale, sink, out_scale, options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0)
+                    _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, scales.data_ptr(), top + 4 * i * nkh, flags, q.stride(0), out.stride(0),
+                    gate_stride, _ptr(partial) or 0, rows, n, max_q_len, nqh, nkh, cols, window, has_sink, scale, sink, out_scale, options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0, i)
                 self.launches += 1
                 self._check_lib(lib_tc, lib_tc.braid_attn_kv4_prompt(args, stream), "attn_kv4")
             if partial is not None:

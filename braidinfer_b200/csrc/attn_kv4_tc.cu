@@ -18,6 +18,8 @@
 #include "kv4.cuh"
 #include "attn_tc.cuh"
 #include "softcap.cuh"
+#include <cuda_fp16.h>
+#include <float.h>
 
 #ifndef BRAID_HD
 #error "compile with -DBRAID_HD=<head_dim>"
@@ -67,9 +69,12 @@ __device__ __forceinline__ void tmem_st16_nowait(uint32_t taddr, const uint32_t*
                  : "memory");
 }
 
+// An instruction descriptor with float16 operands instead of bfloat16 ones (bits 7 .. 9 of A, 10 .. 12 of B).
+__host__ __device__ constexpr uint32_t fa_idesc_f16(uint32_t idesc) { return idesc & ~((7u << 7) | (7u << 10)); }
+
 struct Kv4PromptArgs {
     const void* q;
-    const void* pages;           // block c of sequence i: page i * cols + c, [2][nkh][64][HD] bfloat16
+    const void* pages;           // block c of sequence i: page i * cols + c, [2][nkh][64][HD] float16, scaled
     __nv_bfloat16* out;
     const int* q_start;
     const int* q_len;
@@ -79,6 +84,9 @@ struct Kv4PromptArgs {
     const __nv_bfloat16* head_gate;  // [rows, gate_stride]: head h's result is multiplied by sigmoid(head_gate[row, h]); or null
     const float* bias_slope;     // BIAS: [nqh] float32 r1 and r2 of the distance bias r1 ln(1 + r2 (p - j))
     const float* bias_rate;
+    const int* scales;           // [pages, nkh, 2] exponents of the pages' keys and values, [n_seqs, nkh] of a sequence's largest values (kv4.cu)
+    const int* top;
+    int* repair;                 // [0] and [1 + seq0 + sequence] become 1 where pages' values differ too much
     long long q_stride, out_stride, gate_stride;
     float* partial;              // n_splits > 1: what attn_kv4_merge_kernel (attn_kv4.cu) reads
     int rows, n_seqs, max_q_len, nqh, nkh, cols, window, has_sink;
@@ -88,6 +96,7 @@ struct Kv4PromptArgs {
     int n_splits;
     int q_from;                  // only sequences that bring at least so many tokens
     int tiles;                   // > 0: the grid has so many token tiles of whatever sequences, in order; 0: as many for every sequence
+    int seq0;
 };
 
 #define FA_PLAIN 0
@@ -110,7 +119,8 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint8_t* sV = sK + FA_KST * FA_KV_BYTES;       // [FA_VST]
     uint64_t* bars = (uint64_t*)(sV + FA_VST * FA_KV_BYTES);
     uint64_t* q_full = bars;                       // [1]
-    uint64_t* k_full = q_full + 1;                 // [FA_KST]
+    uint64_t* q_ready = q_full + 1;                // [2] the queries of either group are float16
+    uint64_t* k_full = q_ready + 2;                // [FA_KST]
     uint64_t* k_empty = k_full + FA_KST;           // [FA_KST]
     uint64_t* v_full = k_empty + FA_KST;           // [FA_VST]
     uint64_t* v_empty = v_full + FA_VST;           // [FA_VST]
@@ -119,7 +129,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint64_t* p_ready = s_free + 2;                // [2]
     uint64_t* pv_done = p_ready + 2;               // [2]
     uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
-    static_assert((1 + 2 * FA_KST + 2 * FA_VST + 8) * 8 + 8 <= FA_BAR_BYTES, "the barriers outgrow their bytes");
+    static_assert((3 + 2 * FA_KST + 2 * FA_VST + 8) * 8 + 8 <= FA_BAR_BYTES, "the barriers outgrow their bytes");
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     __shared__ float share[2][2][2][FA_BM];        // what the two threads of a row tell one another: [group][turn][half][row]
 
@@ -177,7 +187,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         mbar_init(q_full, 1);
         for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
         for (int s = 0; s < FA_VST; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&q_ready[s], 8); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -251,16 +261,17 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp == 1) {
         // S of either group in turn, in one place: the next goes there when the one before is in registers
         if (lane == 0 && n_tiles > 0) {
-            constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN);
+            constexpr uint32_t idesc_qk = fa_idesc_f16(umma_idesc_bf16(FA_BM, FA_BN));
             // operand descriptors differ only in their start address (bits 0..13 of the low word, in 16-byte units)
             const uint64_t dq = umma_desc_sw128(smem_u32(sQ)), dk = umma_desc_sw128(smem_u32(sK));
             const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, kq_hi = (uint32_t)(dq >> 32), ts = tmem_base + FA_TMEM_S;
-            bool ok = mbar_wait(q_full, 0, abort_flag);
+            bool ok = true;
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const int kst = j % FA_KST;
                 ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag);
                 for (int group = 0; group < ng && ok; ++group) {
                     // the one before: the first group's of this tile, or the last group's of the tile before
+                    if (j == 0 && !mbar_wait(&q_ready[group], 0, abort_flag)) { ok = false; break; }
                     if (group) ok = mbar_wait(&s_free[0], (uint32_t)(j & 1), abort_flag);
                     else if (j > 0) ok = mbar_wait(&s_free[ng - 1], (uint32_t)((j - 1) & 1), abort_flag);
                     if (!ok) break;
@@ -278,7 +289,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
     } else if (warp == 3) {
         if (lane == 0 && n_tiles > 0) {
-            constexpr uint32_t idesc_pv = umma_idesc_bf16_b_mn(FA_BM, HD);
+            constexpr uint32_t idesc_pv = fa_idesc_f16(umma_idesc_bf16_b_mn(FA_BM, HD));
             const uint64_t dv = umma_desc_sw128_mn(smem_u32(sV), FA_KBLOCK_BYTES);
             const uint32_t v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
             bool ok = true;
@@ -316,10 +327,50 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         float m = -INFINITY, l = 0.f;
         float r1 = 0.f, r2 = 0.f;                             // the row's distance bias
         if (BIAS && valid) { r1 = a.bias_slope[head0 + hl]; r2 = a.bias_rate[head0 + hl]; }
-        // with the bias or the cap the scores are scaled there
-        const float sc = BIAS || CAP ? 1.f : a.scale_log2;
         bool ok = true;
+        // The queries become float16 numbers, a row's largest one of 2^8 .. 2^9: each of a row's threads takes a half of the 128 bytes or
+        // of the 128-byte blocks (in any order within: the tile's swizzle moves 16 bytes within them).
+        float row_factor = a.scale_log2;                      // of the scores: 2^(the row's exponent) in it, and below 2^(the page's)
+        if (n_tiles > 0) {
+            constexpr int CHUNKS = HD / 16;
+            uint8_t* src = sQ + group * FA_Q_BYTES + (HD == 128 ? half * FA_QBLOCK_BYTES : 0) + r * 128;
+            const int chunk0 = HD == 128 ? 0 : half * CHUNKS;
+            const bool came = mbar_wait(q_full, 0, abort_flag);
+            ok = __all_sync(0xffffffffu, came) && ok;
+            uint4 x[CHUNKS];
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                x[i] = *reinterpret_cast<const uint4*>(src + (chunk0 + ((i + lane) & (CHUNKS - 1))) * 16);
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+            }
+            share[group][1][half][r] = most;
+            pair_sync(pair);
+            most = fmaxf(most, share[group][1][1 - half][r]);
+            const int qe = most > 0.f ? min(max(kv4_exponent(most) - 8, -126), 119) : 0;
+            row_factor *= kv4_pow2(qe);
+            const float f = kv4_pow2(-qe);
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 y = __floats2half2_rn(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xffff0000u) * f);
+                    w[e] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                *reinterpret_cast<uint4*>(src + (chunk0 + ((i + lane) & (CHUNKS - 1))) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[group]);
+        }
+        const int top = a.top[(size_t)seq * a.nkh + kvh];     // the exponent that all of the result has
+        bool apart = false;
         for (int j = 0; j < n_tiles; ++j) {
+            const int page = min(min(page_lo + 2 * j + half, page_hi - 1), a.cols - 1);    // this thread's half of the keys is a page
+            const int2 exps = *reinterpret_cast<const int2*>(a.scales + (((size_t)seq * a.cols + page) * a.nkh + kvh) * 2);
             // (a warp whose wait ran out goes on to meet its partner at every barrier below, so that neither waits for the other for good)
             const bool came = mbar_wait(&s_full[group], (uint32_t)(j & 1), abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
@@ -329,15 +380,24 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[group]);           // (one arrival a warp)
+            // (finite, for products that are 0)
+            const float factor_s = fmaxf(fminf(exps.x ? row_factor * kv4_pow2(exps.x - KV4_EXPONENT) : row_factor, FLT_MAX), -FLT_MAX);
+            // with the bias or the cap the scores are scaled there
+            const float sc = BIAS || CAP ? 1.f : factor_s;
+            // The probabilities' exponent: values are scaled by their page's own, and the result has the sequence's largest.  2^7 makes a
+            // probability, up to 2^8 against a maximum that was not raised, one of up to 2^15, so that those down to 2^-21 keep 11 bits.
+            const int below = exps.y ? exps.y - top : 0;
+            apart |= below < -16;
+            const int pe = max(below, -40) + 7;
             const int key0 = page_lo * FA_PAGE + j * FA_BN + half * 64;
             const bool all_visible = (key0 + 63 <= first) && (a.window == 0 || key0 >= last - a.window + 1);
             if (BIAS) {                                       // keys after the query (a negative distance) are masked below
                 const float d0 = (float)(pos - key0);
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
-                    sv[i] = fmaf(sv[i], a.scale_log2, -r1 * __log2f(fmaf(r2, d0 - (float)i, 1.f)));
+                    sv[i] = fmaf(sv[i], factor_s, -r1 * __log2f(fmaf(r2, d0 - (float)i, 1.f)));
             }
-            if (CAP) softcap_scores<64>(sv, a.scale_log2, a.cap_log2);
+            if (CAP) softcap_scores<64>(sv, factor_s, a.cap_log2);
             if (!all_visible) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
@@ -372,24 +432,25 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 ok = __all_sync(0xffffffffu, done) && ok;
                 tc_fence_after();
             }
-            // probabilities, rounded to bfloat16
+            // probabilities times 2^pe, rounded to float16
+            const float shift = (float)pe - ms;
             float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p0 = fast_exp2(fmaf(sv[c * 32 + 2 * i], sc, -ms));
-                    const float p1 = fast_exp2(fmaf(sv[c * 32 + 2 * i + 1], sc, -ms));
+                    const float p0 = fast_exp2(fmaf(sv[c * 32 + 2 * i], sc, shift));
+                    const float p1 = fast_exp2(fmaf(sv[c * 32 + 2 * i + 1], sc, shift));
                     sum0 += p0;
                     sum1 += p1;
-                    __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-                    pk[i] = *reinterpret_cast<uint32_t*>(&b);
+                    const __half2 b = __floats2half2_rn(p0, p1);
+                    pk[i] = *reinterpret_cast<const uint32_t*>(&b);
                 }
                 __syncwarp();
                 tmem_st16_nowait(tmem_base + FA_TMEM_P + group * 64 + half * 32 + c * 16 + lane_addr, pk);
             }
-            l = l * factor + (sum0 + sum1);
+            l = fmaf(sum0 + sum1, kv4_pow2(-pe), l * factor);
             __syncwarp();
             if (any && j > 0) {                                // (the same for every lane)
                 // a half of the row's columns
@@ -417,14 +478,19 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             ok = __all_sync(0xffffffffu, done) && ok;
             tc_fence_after();
         }
+        if (apart) {
+            a.repair[1 + a.seq0 + seq] = 1;
+            a.repair[0] = 1;
+        }
+        const float o_factor = top ? kv4_pow2(top - KV4_EXPONENT - 7) : 1.f;
         const size_t row = (size_t)(q_start + tokg + tl);
         const int head = head0 + hl;
-        float inv = 1.f;
+        float inv = o_factor;
         if (a.n_splits == 1 && valid) {
             // the sink joins the sum where the row is finished: l counts in units of 2^m; a sink far above every
             // score makes the sum infinite and the row zero, which is the limit
             const float sk = a.head_sinks ? a.head_sinks[head] * 1.4426950408889634f : a.sink_log2;
-            inv = a.out_scale / (a.has_sink ? l + exp2f(sk - m) : l);
+            inv *= a.out_scale / (a.has_sink ? l + exp2f(sk - m) : l);
             if (a.head_gate) inv *= 1.f / (1.f + __expf(-__bfloat162float(a.head_gate[row * a.gate_stride + head])));
         }
         const size_t at = (row * a.nqh + head) * a.n_splits + split;
@@ -444,7 +510,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (ok && valid && a.n_splits > 1) {
                 float* dst = a.partial + at * HD + c0;
 #pragma unroll
-                for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
+                for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(ov[c] * inv, ov[c + 1] * inv, ov[c + 2] * inv, ov[c + 3] * inv);
             } else if (ok && valid) {
                 __nv_bfloat16* dst = a.out + row * a.out_stride + (size_t)head * HD + c0;
 #pragma unroll
@@ -480,7 +546,7 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     if (a.nqh <= 0 || a.nkh <= 0 || a.nqh % a.nkh) BRAID_REFUSE("attn_kv4: %d query heads do not divide into %d kv heads", a.nqh, a.nkh);
     if ((a.q_stride % 8) || (a.out_stride % 8) || (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.pages) & 15))
         BRAID_REFUSE("attn_kv4: prompts' queries, results and pages must be 16-byte aligned");
-    if (!a.error_flag) BRAID_REFUSE("attn_kv4: error_flag is required");
+    if (!a.error_flag || !a.scales || !a.top || !a.repair) BRAID_REFUSE("attn_kv4: the error flag, the pages' exponents and the flags are required");
     if (!a.bias_slope != !a.bias_rate) BRAID_REFUSE("attn_kv4: a distance bias has a slope and a rate a head");
     if (a.softcap > 0.f && a.bias_slope) BRAID_REFUSE("attn_kv4: a cap on the scores and a distance bias are not combined");
     // without a bias or a cap the maximum is taken, and keys are masked, before the factor
@@ -517,7 +583,7 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
         cuuint64_t strides[1] = {(cuuint64_t)BRAID_HD * 2};
         cuuint32_t box[2] = {64, FA_PAGE};
         cuuint32_t estr[2] = {1, 1};
-        CUresult r = fn(&mkv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.pages), dims, strides, box, estr,
+        CUresult r = fn(&mkv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.pages), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) BRAID_REFUSE("attn_kv4: cuTensorMapEncodeTiled(pages) failed with %d", (int)r);

@@ -1,6 +1,8 @@
 // A cache held in 4 bits (kv4.cuh has the format): the tables of a step, the write of new keys and values, their reading
 // back, and the plain attention that the tensor-core kernel (attn_kv4.cu) is checked against.
 #include "kv4.cuh"
+#include <cuda_fp16.h>
+#include <type_traits>
 
 // ------------------------------------------------------------------ tables of a step
 // From the lengths of n requests (q_len new tokens behind kv_before cached ones) and their pages, packed one request after
@@ -309,6 +311,8 @@ struct ExpandArgs {
     int* error_flag;
     int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [1 + seq0 + sequence] become 1
     int* out_table;              // (out_cols > 0) [n_seqs, out_cols]: the numbers of the pages, for whoever reads them
+    int* scales;                 // given: float16 numbers, scaled a page and kv head: [pages, nkh, 2] exponents + KV4_EXPONENT of keys, values (0: all zero)
+    int* top;                    // (scales) [n_seqs, nkh] from sequence seq0 on: the largest of a sequence's values' exponents; zeros before
     int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
     int q_from;                  // only the pages of sequences that bring at least so many tokens
 };
@@ -334,7 +338,7 @@ template <>
 struct Kv4Pairs<__nv_bfloat16> {
     using Pair = uint32_t;
     // one multiply-add of the pair in bfloat16: the code and 128 + code are exact, the sum is rounded once
-    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, uint32_t* y) {
+    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, uint32_t* y, float) {
         const uint32_t s2 = __byte_perm(group, group, 0x1010), l2 = __byte_perm(group, group, 0x3232);
         const __nv_bfloat162 base(__float2bfloat16(128.f), __float2bfloat16(128.f));
 #pragma unroll
@@ -349,9 +353,26 @@ struct Kv4Pairs<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 };
 template <>
+struct Kv4Pairs<__half> {
+    using Pair = uint32_t;
+    // the same in float16, step and lowest value times a power of two: they keep their 8 bits but for what is below 2^-24
+    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, uint32_t* y, float factor) {
+        const __half2 s2 = __float2half2_rn(kv4_step(group) * factor), l2 = __float2half2_rn(kv4_lowest(group) * factor);
+        const __half2 base = __float2half2_rn(1024.f);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t c = ((word >> (4 * n)) & 0x000f000fu) | 0x64006400u;
+            const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s2, l2);
+            y[n] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    static __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+    static __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+};
+template <>
 struct Kv4Pairs<float> {
     using Pair = float2;
-    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, float2* y) {
+    static __device__ __forceinline__ void make(uint32_t word, uint32_t group, float2* y, float) {
         const float step = kv4_step(group), low = kv4_lowest(group);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {                          // a code under the lowest bits of 2^23 is 2^23 + code
@@ -377,6 +398,9 @@ kv4_expand_kernel(const ExpandArgs a) {
         for (int c = blockIdx.x + gridDim.x * threadIdx.x; c < a.out_cols; c += gridDim.x * blockDim.x)
             a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
     if (end - before < a.q_from) return;
+    constexpr bool SCALED = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
+    __shared__ float3 sizes[2][8];
+    int turn = 0;
     const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0, cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
     for (int c = blockIdx.x; c < cols; c += gridDim.x) {
         const int key0 = c * BRAID_PAGE_SIZE;
@@ -401,22 +425,64 @@ kv4_expand_kernel(const ExpandArgs a) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             if (!in) kc[w] = kg[w] = vg[w] = 0u;                   // a group of step 0 and lowest value 0
-            // the 16 bits of group w in the lane's first and second half of value words
-            const int h0 = w, h1 = W + w;
-            const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
-            const uint32_t both = in ? v0 | (v1 << 16) : 0u;
-            // NaN, or a step of 2^122 or a lowest value of 2^127 or more, from which a number may round to infinity
-            if (a.repair && ((vg[w] & 0x7f80u) >= 0x7c80u || (vg[w] & 0x7f800000u) >= 0x7f000000u)) {
+            if (a.repair && ((vg[w] & 0x7f80u) == 0x7f80u || (vg[w] & 0x7f800000u) == 0x7f800000u)) {
                 vg[w] = 0u;
                 a.repair[1 + a.seq0 + seq] = 1;
                 a.repair[0] = 1;
             }
+        }
+        float kf = 1.f, vf = 1.f;
+        if constexpr (SCALED) {
+            // the page's largest key and value become numbers of 2^14 .. 2^15
+            float k = 0.f, v = 0.f, least = INFINITY;              // (least: of a group's largest value)
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float a0 = fmaxf(fabsf(kv4_lowest(kg[w])), fabsf(fmaf(15.f, kv4_step(kg[w]), kv4_lowest(kg[w]))));
+                const float a1 = fmaxf(fabsf(kv4_lowest(vg[w])), fabsf(fmaf(15.f, kv4_step(vg[w]), kv4_lowest(vg[w]))));
+                if (a0 < INFINITY) k = fmaxf(k, a0);
+                v = fmaxf(v, a1);
+                if (a1 > 0.f) least = fminf(least, a1);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                k = fmaxf(k, __shfl_xor_sync(0xffffffffu, k, o));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+                least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+            }
+            if ((threadIdx.x & 31) == 0) sizes[turn][threadIdx.x >> 5] = make_float3(k, v, least);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float3 x = sizes[turn][i];
+                k = fmaxf(k, x.x); v = fmaxf(v, x.y); least = fminf(least, x.z);
+            }
+            turn ^= 1;
+            const int ke = max(kv4_exponent(k) - 14, -112), ve = max(kv4_exponent(v) - 14, -112);
+            if (k > 0.f) kf = kv4_pow2(-ke);
+            if (v > 0.f) vf = kv4_pow2(-ve);
+            if (threadIdx.x == 0) {
+                *reinterpret_cast<int2*>(a.scales + (out_page * a.nkh + kvh) * 2) =
+                    make_int2(k > 0.f ? ke + KV4_EXPONENT : 0, v > 0.f ? ve + KV4_EXPONENT : 0);
+                if (v > 0.f) atomicMax(&a.top[(size_t)(a.seq0 + seq) * a.nkh + kvh], ve + KV4_EXPONENT);
+                // a group whose largest value is so much smaller than the page's would lose bits
+                if (least * 67108864.f < v) {
+                    a.repair[1 + a.seq0 + seq] = 1;
+                    a.repair[0] = 1;
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            // the 16 bits of group w in the lane's first and second half of value words
+            const int h0 = w, h1 = W + w;
+            const uint32_t v0 = (vc[h0 / 2] >> (16 * (h0 & 1))) & 0xffffu, v1 = (vc[h1 / 2] >> (16 * (h1 & 1))) & 0xffffu;
+            const uint32_t both = in ? v0 | (v1 << 16) : 0u;
             __align__(16) P y[4];
             P z[4];
-            Kv4Pairs<T>::make(kc[w], kg[w], y);                    // pairs of neighbours, in order
+            Kv4Pairs<T>::make(kc[w], kg[w], y, kf);                  // pairs of neighbours, in order
             *reinterpret_cast<uint4*>(dst + 32 * w) = *reinterpret_cast<const uint4*>(y);
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
-            Kv4Pairs<T>::make(both, vg[w], z);                     // numbers n and 4 + n
+            Kv4Pairs<T>::make(both, vg[w], z, vf);                   // numbers n and 4 + n
             y[0] = Kv4Pairs<T>::lows(z[0], z[1]);
             y[1] = Kv4Pairs<T>::lows(z[2], z[3]);
             y[2] = Kv4Pairs<T>::highs(z[0], z[1]);
@@ -447,6 +513,10 @@ extern "C" int braid_kv4_expand(const ExpandArgs* args, void* stream) {
     if ((uintptr_t)a.out & 15) BRAID_REFUSE("kv4_expand: the pages must start on 16 bytes");
     if (a.nkh > 65535 || a.n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", a.nkh, a.n_seqs);
     if (a.window <= 0) a.window = a.keep_first = 0;
+    if (a.scales) {
+        if (!a.repair || !a.top || a.out_cols <= 0) BRAID_REFUSE("kv4_expand: scaled pages want pages of their own, the largest exponents and the flags");
+        return launch_expand<__half>(a, (cudaStream_t)stream);
+    }
     if (a.dtype == BRAID_F32) return launch_expand<float>(a, (cudaStream_t)stream);
     if (a.dtype == BRAID_BF16) return launch_expand<__nv_bfloat16>(a, (cudaStream_t)stream);
     BRAID_REFUSE("kv4_expand: unknown dtype code %d", a.dtype);

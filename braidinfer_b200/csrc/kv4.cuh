@@ -28,3 +28,8 @@ __host__ __device__ constexpr int kv4_value_groups(int hd) { return 18 * hd; }
 
 __device__ __forceinline__ float kv4_step(uint32_t group) { return __uint_as_float(group << 16); }
 __device__ __forceinline__ float kv4_lowest(uint32_t group) { return __uint_as_float(group & 0xffff0000u); }
+
+// Powers of two of float32's normal numbers, and the exponent of a number that is 0 or one of those (0: -127).
+#define KV4_EXPONENT 200                                      // added to exponents that are kept, so that 0 can say "all zero"
+__device__ __forceinline__ float kv4_pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int kv4_exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }

@@ -390,13 +390,15 @@ SIZES = {  # factors on the values by position, on the keys, on the queries
     "small keys": (lambda t: 1 + 0 * t, 1e-20, 1e20), "constant": (lambda t: 0 * t, 1.0, 1.0)}
 
 
+@pytest.mark.parametrize("seqs", [[(1, 700), (3, 90)], [(200, 500), (60, 0)]], ids=["few", "prompts"])
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("name", SIZES)
-def test_values_of_all_sizes(K, name, dt):
+def test_values_of_all_sizes(K, monkeypatch, name, dt, seqs):
     """Values whose sizes lie far apart within a sequence, and keys and queries that make up for each other: what is scaled on the way
     must not leave its range.  (Values grow before they shrink: a result then hangs on the largest ones that its probabilities keep.)"""
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
     grow, fk, fq = SIZES[name]
-    c = Case(K, [(1, 700), (3, 90)], 8, 2, 128, dt)
+    c = Case(K, seqs, 8, 2, 128, dt)
     g = gen(5)
     x = torch.randn(2, c.num * 64, 2, 128, generator=g)
     for i in (0, 1):
@@ -408,6 +410,22 @@ def test_values_of_all_sizes(K, name, dt):
     c.q = (c.q.float() * fq).to(dt)
     c.check(K)
     c.check(K, backend="plain")
+
+
+@pytest.mark.parametrize("slices", [1, 3])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompts_keep_the_bits_of_the_codes(K, monkeypatch, hd, slices):
+    """Queries, keys, values and probabilities of prompts are float16 numbers of 11 bits: half a step is 2^-12 of each (and what lies far below
+    the largest of its row or page is off by 2^-25 of that, here less than 2^-11 of a part in 2^12)."""
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    monkeypatch.setattr(Kernels, "_kv4_prompt_slices", lambda *a: slices)
+    c = Case(K, [(150, 1000), (70, 0)], 8, 2, hd, BF)
+    out = c.run(K)
+    want, mag, smag = c.want()
+    n = sum(c.q_len)
+    score = 2 * 2.0 ** -12 * smag[1] + 32 * U * smag[0]
+    most = mag * (2 * score[..., None] + 2 * 2.0 ** -12 + 2.0 ** -18) + 2.0 ** -8 * want.abs() + 1e-30
+    assert ((out.double().view(want.shape) - want).abs() <= most)[:n].all()
 
 
 @pytest.mark.parametrize("seqs", [[(1, 9000), (1, 10), (1, 4000)], [(4, 5000)], [(33, 3000)]])

@@ -114,7 +114,7 @@ def test_entry_points_refuse(K):
     assert tables(n=20000) == tables(pages=1 << 26) == tables(rows=-1) == -1
     store = lambda at=even, rows=3, kind=0, hd=64, kv=2: lib.braid_kv4_store(api._STORE_ARGS.pack(p, p, p, at, p, 128, 128, rows, kv, hd, 5, kind), None)
     assert store(at=even + 4) == store(kind=7) == store(hd=48) == store(hd=288) == store(kv=0) == -1
-    expand = lambda at=even, n=2, kind=0: lib.braid_kv4_expand(api._EXPAND_ARGS.pack(even, at, p, p, p, p, 0, 0, n, 2, 64, 3, 5, 0, 0, 0, 0, kind, 0), None)
+    expand = lambda at=even, n=2, kind=0: lib.braid_kv4_expand(api._EXPAND_ARGS.pack(even, at, p, p, p, p, 0, 0, 0, 0, n, 2, 64, 3, 5, 0, 0, 0, 0, kind, 0), None)
     assert expand(at=even + 8) == expand(kind=5) == -1 and expand(n=70000) == -1
     assert b"grid" in lib.braid_last_error()
     # nothing to do is no error
