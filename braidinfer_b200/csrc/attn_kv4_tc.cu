@@ -2,19 +2,25 @@
 // (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size: -DBRAID_HD=64 or 128.
 //
 // A CTA takes two groups of 128 columns of queries (tokens x the query heads of a kv head) and walks the keys that they see, 128 at a time:
-//   S = Q K^T  (tensor memory, float32),   p = 2^(scale log2(e) S - m),   O += p V  (p bfloat16 in tensor memory)
+//   S = Q K^T  (tensor memory, float32),   p = 2^(scale log2(e) S - m),   O += p V  (p in tensor memory)
 // with the running maximum m of a row raised only when a tile exceeds it by more than 8 powers of two.  Warp 0 brings pages into two rings by
-// TMA, warp 1 issues S, warp 3 P V, and 16 warps are the softmax: TWO threads share a row, each with half of a tile's keys and half of the
-// result's columns, in two warps that meet at a barrier of their own once a tile.  That barrier carries the question whether any row's
+// TMA, warp 1 issues S, warp 3 P V, and 16 warps are the softmax: TWO threads share a row, each with half of a tile's keys (a page) and half of
+// the result's columns, in two warps that meet at a barrier of their own once a tile.  That barrier carries the question whether any row's
 // maximum has to be raised (barrier.red.or), so that the two exchange numbers only then.
+//
+// All operands are float16 numbers: their 11 bits hold what the codes say, where bfloat16's 8 made errors of 0.0031 to 0.0035 of the result
+// instead of 0.0017, which is the rounding of the result.  For their range, kv4_expand_kernel scales the keys and the values of a page and kv head
+// by a power of two each, and a row's queries are scaled here; the scores' factor and the probabilities' exponent take that back.  The
+// values of a sequence share one exponent in O, so a page whose values are far smaller than the largest (2^16 times) marks its sequence
+// for the plain kernel, which computes it again.
 //
 // What bounds it: the exponentials of a tile take the SM 2,048 cycles, and so do its products.  So the two groups have ONE place for their
 // scores: S of one is computed while the other's exponentials run, which keeps the groups half a turn apart without a barrier between them.
 // A tile takes some 3,000 cycles.  Prompts of 6,414 tokens in all / 700 tokens behind 16,500 (88 of 148 SMs), 32 heads of 128 over 8, us with
-// the reading back: 83 / 344 by attn_tc.cu (a thread a row, tiles of 64 keys, two CTAs an SM); 89 / 331 the same with two threads a row; 90 / 332
-// with both groups in a CTA and scores of their own (96 / 376 with barriers that let their exponentials take turns); 104 / 393 with tiles of 128
-// keys whose probabilities lie over the scores, where all of a group's steps wait for one another; 78 / 237 so, and 78 / 224 with the
-// context in 3 slices.
+// the reading back, in bfloat16: 83 / 344 by attn_tc.cu (a thread a row, tiles of 64 keys, two CTAs an SM); 89 / 331 the same with two threads a
+// row; 90 / 332 with both groups in a CTA and scores of their own (96 / 376 with barriers that let their exponentials take turns); 104 / 393 with
+// tiles of 128 keys whose probabilities lie over the scores, where all of a group's steps wait for one another; 78 / 237 so, and 78 / 224 with
+// the context in 3 slices.  In float16 86 / 231 (more registers for the softmax by setmaxnreg, 112 and 32: 3 and 13 % slower).
 #include "kv4.cuh"
 #include "attn_tc.cuh"
 #include "softcap.cuh"
@@ -69,6 +75,20 @@ __device__ __forceinline__ void tmem_st16_nowait(uint32_t taddr, const uint32_t*
                  : "memory");
 }
 
+// Two numbers at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 // An instruction descriptor with float16 operands instead of bfloat16 ones (bits 7 .. 9 of A, 10 .. 12 of B).
 __host__ __device__ constexpr uint32_t fa_idesc_f16(uint32_t idesc) { return idesc & ~((7u << 7) | (7u << 10)); }
 
@@ -265,13 +285,14 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // operand descriptors differ only in their start address (bits 0..13 of the low word, in 16-byte units)
             const uint64_t dq = umma_desc_sw128(smem_u32(sQ)), dk = umma_desc_sw128(smem_u32(sK));
             const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, kq_hi = (uint32_t)(dq >> 32), ts = tmem_base + FA_TMEM_S;
-            bool ok = true;
+            bool ok = mbar_wait(&q_ready[0], 0, abort_flag) && (ng == 1 || mbar_wait(&q_ready[1], 0, abort_flag));
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const int kst = j % FA_KST;
                 ok = mbar_wait(&k_full[kst], (uint32_t)((j / FA_KST) & 1), abort_flag);
-                for (int group = 0; group < ng && ok; ++group) {
+#pragma unroll
+                for (int group = 0; group < 2; ++group) {
+                    if (group >= ng || !ok) break;
                     // the one before: the first group's of this tile, or the last group's of the tile before
-                    if (j == 0 && !mbar_wait(&q_ready[group], 0, abort_flag)) { ok = false; break; }
                     if (group) ok = mbar_wait(&s_free[0], (uint32_t)(j & 1), abort_flag);
                     else if (j > 0) ok = mbar_wait(&s_free[ng - 1], (uint32_t)((j - 1) & 1), abort_flag);
                     if (!ok) break;
@@ -368,9 +389,15 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         const int top = a.top[(size_t)seq * a.nkh + kvh];     // the exponent that all of the result has
         bool apart = false;
+        auto exps_of = [&](int j) {                           // this thread's half of a tile's keys is a page
+            const int page = min(min(page_lo + 2 * j + half, page_hi - 1), a.cols - 1);
+            return *reinterpret_cast<const int2*>(a.scales + (((size_t)seq * a.cols + page) * a.nkh + kvh) * 2);
+        };
+        int2 next_exps = make_int2(0, 0);
+        if (n_tiles > 0) next_exps = exps_of(0);
         for (int j = 0; j < n_tiles; ++j) {
-            const int page = min(min(page_lo + 2 * j + half, page_hi - 1), a.cols - 1);    // this thread's half of the keys is a page
-            const int2 exps = *reinterpret_cast<const int2*>(a.scales + (((size_t)seq * a.cols + page) * a.nkh + kvh) * 2);
+            const int2 exps = next_exps;
+            if (j + 1 < n_tiles) next_exps = exps_of(j + 1);  // (a trip to L2, a tile ahead)
             // (a warp whose wait ran out goes on to meet its partner at every barrier below, so that neither waits for the other for good)
             const bool came = mbar_wait(&s_full[group], (uint32_t)(j & 1), abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
@@ -434,23 +461,23 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             // probabilities times 2^pe, rounded to float16
             const float shift = (float)pe - ms;
-            float sum0 = 0.f, sum1 = 0.f;
+            const float2 sc2 = make_float2(sc, sc), shift2 = make_float2(shift, shift);
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p0 = fast_exp2(fmaf(sv[c * 32 + 2 * i], sc, shift));
-                    const float p1 = fast_exp2(fmaf(sv[c * 32 + 2 * i + 1], sc, shift));
-                    sum0 += p0;
-                    sum1 += p1;
+                    const float2 t = fma2(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sc2, shift2);
+                    const float p0 = fast_exp2(t.x), p1 = fast_exp2(t.y);
+                    sum = add2(sum, make_float2(p0, p1));
                     const __half2 b = __floats2half2_rn(p0, p1);
                     pk[i] = *reinterpret_cast<const uint32_t*>(&b);
                 }
                 __syncwarp();
                 tmem_st16_nowait(tmem_base + FA_TMEM_P + group * 64 + half * 32 + c * 16 + lane_addr, pk);
             }
-            l = fmaf(sum0 + sum1, kv4_pow2(-pe), l * factor);
+            l = fmaf(sum.x + sum.y, kv4_pow2(-pe), l * factor);
             __syncwarp();
             if (any && j > 0) {                                // (the same for every lane)
                 // a half of the row's columns
