@@ -876,11 +876,11 @@ class Kernels:
         if rows == 0 or n_seqs == 0:
             return
         tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
-        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, n_seqs, nqh, nkh, tc):
-            # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
-            # longest is short on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 409 / 848 / 224;
-            # 2,000 tokens beside one behind 30,000, 635 / 366 / 77.)
-            few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 64 * (n_seqs - 1) else 0
+        # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
+        # longest are a few tokens on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 411 / 883 / 230;
+        # 2,000 tokens beside one behind 30,000, 637 / 368 / 81.)
+        few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 8 * (n_seqs - 1) else 0
+        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, 1 if few else n_seqs, nqh, nkh, tc):
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                  int(window or 0), scale, int(keep_first or 0), head_scale, dict(
                                      sink=sink, out_scale=out_scale, head_sinks=head_sinks, head_gate=head_gate, distance_bias=distance_bias,
@@ -934,30 +934,29 @@ class Kernels:
     # The most that the pages of a step's prompts, read back for attention, may take at once: more sequences go one group after another.
     KV4_PAGES_BYTES = 1 << 30
 
-    # Steps of at least so many units (16 columns of queries, kv head, sequence), or of 40 whose units times the longest context are so many, have
-    # their prompts' pages read back once for all of them.  The kernel over 4 bits reads them for every 8 columns; the one over ordinary pages
-    # takes 256 columns a CTA.  Heads of 128, four queries a kv head, 8 kv heads, us over pages / over 4 bits: a prompt alone, 64 tokens (128 units)
-    # 13.9 / 8.3, 96 tokens (192) 14.1 / 14.7, 256 tokens 15.5 / 29; four of 32 (256) 14.3 / 13.9; behind 1,000, 64 tokens 26.5 / 16.9, 96 tokens 26.3 /
-    # 30, four of 32 27.4 / 27.0; behind 8,000, 12 tokens (24) 26.6 / 21.7, 16 tokens (32) 26.8 / 26.0, 32 tokens 28.7 / 41.6; behind 32,000, 12
-    # tokens 77 / 53, 32 tokens 80 / 136, 128 tokens 98 / 519.
-    # Other head sizes and options go through the older kernel for ordinary pages, of which a CTA walks its context alone, from 4/3 of those units, or
-    # 8/3 behind 1,000 and more: heads of 96, a prompt alone, 128 tokens (256) 14.2 / 14.5, 512 tokens 29 / 54; behind 1,000, 256 tokens (512) 50.5 / 54,
-    # four of 64 (512) 46 / 37; behind 8,000, 256 tokens 269 / 236, 512 tokens 331 / 426; heads of 256 alike.
-    KV4_PAGES_FROM, KV4_PAGES_WORK = 190, 250_000
+    # Steps of at least so many units (16 columns of queries, kv head, sequence) have their prompts' pages read back once for all of them; behind
+    # long contexts fewer, down to 27 a sequence, for the reading back grows with the sequences.  The kernel over 4 bits reads the pages for every 8
+    # columns; the one over those that were read back takes 256 columns a CTA.  Heads of 128, four queries a kv head, 8 kv heads, us over pages /
+    # over 4 bits: a prompt alone, 64 tokens (128 units) 15.1 / 8.2, 128 tokens (256) 15.3 / 15.5, 256 tokens 17.1 / 29.5; behind 1,000, 64 tokens 28.6 /
+    # 16.9, 128 tokens 28.6 / 31.6; behind 8,000, 16 tokens (32) 29.1 / 26.0, 32 tokens 30.9 / 41.7, four of 12 (96) 59 / 51, four of 16 (128) 60 /
+    # 73; behind 32,000, 16 tokens 82 / 74, 32 tokens 83 / 151, 128 tokens 101 / 484.
+    # Other head sizes and options go through the older kernel for ordinary pages, of which a CTA walks its context alone: twice the units behind 1,000
+    # and more (heads of 96, a prompt alone, 128 tokens (256) 14.2 / 14.5, 512 tokens 29 / 54; behind 1,000, 256 tokens (512) 50.5 / 54, four of 64 46 /
+    # 37; behind 8,000, 256 tokens 269 / 236, 512 tokens 331 / 426; heads of 256 alike).
+    KV4_PAGES_FROM = 250
 
     @staticmethod
     def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, max_kv_len: int, n_seqs: int, nqh: int, nkh: int, tc: bool) -> bool:
-        """Whether attention reads the step's pages back and runs over those."""
+        """Whether attention reads the pages of `n_seqs` sequences back and runs over those."""
         if max_q_len <= 8 or out.dtype != torch.bfloat16:
             return False
         g = nqh // nkh
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
         units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
-        if tc:
-            worth = units >= Kernels.KV4_PAGES_FROM or (units >= 40 and units * max_kv_len >= Kernels.KV4_PAGES_WORK)
-        else:
-            worth = 3 * units >= Kernels.KV4_PAGES_FROM * (4 if max_kv_len < 1000 else 8)
-        return worth and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
+        least = Kernels.KV4_PAGES_FROM
+        if max_kv_len >= 1000:
+            least *= max(0.11 * n_seqs, 1100 / max_kv_len) if tc else 2
+        return units >= least and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
     def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                         scale, keep_first, head_scale, options, tc, q_from) -> None:
@@ -1024,10 +1023,10 @@ class Kernels:
         sms = torch.cuda.get_device_properties(self._device_index).multi_processor_count
 
         def cost(n: int) -> float:
-            """us: 1.55 for 128 keys of a CTA; 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
-            (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 226, 249, 190, 214, 197, 217)"""
+            """us: 1.65 for 128 keys of a CTA; 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
+            (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 240, 263, 201, 227, 207, 231)"""
             rounds = -(-ctas * n // sms)
-            return max(most, rounds * mean) / 128 / n * 1.55 + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
+            return max(most, rounds * mean) / 128 / n * 1.65 + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
         return min(range(1, max(1, min(8, most // 512)) + 1), key=cost)
 
     @staticmethod

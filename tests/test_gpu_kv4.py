@@ -300,7 +300,7 @@ def test_prompts_beside_single_tokens(K, monkeypatch, name, hd, room, slices):
     monkeypatch.setattr(Kernels, "KV4_PAGES_BYTES", room)
     if slices:
         monkeypatch.setattr(Kernels, "_kv4_prompt_slices", lambda *a: slices)
-    c = Case(K, [(1, 3000), (200, 100), (8, 64), (9, 10), (0, 5), (1, 0), (3, 700), (1, 500), (40, 0)], 8, 2, hd, BF)
+    c = Case(K, [(1, 3000), (200, 100), (8, 64), (9, 10), (0, 5), (1, 0), (3, 700), (1, 500), (20, 0)], 8, 2, hd, BF)
     ran = []
     mma = K._attn_kv4_mma
     monkeypatch.setattr(K, "_attn_kv4_mma", lambda *a: (ran.append(a[-1]), mma(*a)))
