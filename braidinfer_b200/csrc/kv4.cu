@@ -141,7 +141,7 @@ extern "C" int braid_step_tables(const TablesArgs* args, void* stream) {
 //
 // A code is the quotient (x - lo) / step rounded to the nearest whole number, ties to even.  The quotient is taken as a product with 1 / step,
 // which may miss a number next to a tie, and then put right by the remainder x - lo - code step: that is exact (the code has
-// 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  Instructions bound it, some 15 a number.  (6,414 rows of 8
+// 4 bits, the step 8, and the remainder is at most about step), so ties are ties.  Instructions bound it, some 15 a number.  (5,845 rows of 8
 // heads of 128, keys and values, bfloat16: 23 us with 8 numbers a thread and tests of each for NaN, 15 us so; what is read and
 // written takes 5 us.)
 struct StoreArgs {
