@@ -218,8 +218,10 @@ attn_kv4_kernel(const Kv4Args a) {
     const int g = a.nqh / a.nkh;
     const int hpc = min(g, C::BM), tpc = C::BM / hpc, hchunks = (g + hpc - 1) / hpc;
     const int seq = blockIdx.y;
-    const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
-    const int unit = gridDim.z - 1 - blockIdx.z;              // late tokens, which see the most, first
+    const int heads = a.nkh * hchunks, part = blockIdx.x / heads, hx = blockIdx.x - part * heads;
+    const int kvh = hx / hchunks, hchunk = hx - kvh * hchunks;
+    // late tokens, which see the most, first (and more than 65,535 tiles in parts along x)
+    const int unit = (int)(gridDim.x / heads - part) * (int)gridDim.z - 1 - (int)blockIdx.z;
     const int tile = unit / a.n_splits, split = unit - tile * a.n_splits;
     const int q_len = a.q_len[seq], tok0 = tile * tpc;
     if (tok0 >= q_len || (a.q_to > 0 && q_len > a.q_to)) return;
@@ -836,11 +838,12 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
     }
     const int g = a.nqh / a.nkh, hpc = g < C::BM ? g : C::BM, tpc = C::BM / hpc, hchunks = (g + hpc - 1) / hpc;
     const long long gz = (long long)((a.max_q_len + tpc - 1) / tpc) * a.n_splits;
-    if (gz > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
+    const long long parts = a.cluster ? 1 : (gz + 65534) / 65535;
+    if (gz > (a.cluster ? 65535 : 0x7fffffffLL - 65535) || (long long)a.nkh * hchunks * parts > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld tiles, %d heads, %d sequences)", gz, a.nkh * hchunks, a.n_seqs);
     if (gz == 0) return BRAID_OK;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.nkh * hchunks, a.n_seqs, (unsigned)gz);
+    cfg.gridDim = dim3((unsigned)(a.nkh * hchunks * parts), a.n_seqs, (unsigned)((gz + parts - 1) / parts));
     cfg.blockDim = dim3(KV4_NW * 32);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;

@@ -464,8 +464,8 @@ kv4_expand_kernel(const ExpandArgs a) {
                 *reinterpret_cast<int2*>(a.scales + (out_page * a.nkh + kvh) * 2) =
                     make_int2(k > 0.f ? ke + KV4_EXPONENT : 0, v > 0.f ? ve + KV4_EXPONENT : 0);
                 if (v > 0.f) atomicMax(&a.top[(size_t)(a.seq0 + seq) * a.nkh + kvh], ve + KV4_EXPONENT);
-                // a group whose largest value is so much smaller than the page's would lose bits
-                if (least * 67108864.f < v) {
+                // a group whose largest value is 2^26 times smaller than the page's would lose bits
+                if (least * 67108864.f < v || !(v < INFINITY)) {
                     a.repair[1 + a.seq0 + seq] = 1;
                     a.repair[0] = 1;
                 }

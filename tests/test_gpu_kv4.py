@@ -412,6 +412,16 @@ def test_values_of_all_sizes(K, monkeypatch, name, dt, seqs):
     c.check(K, backend="plain")
 
 
+def test_more_tiles_than_a_grid_is_deep(K):
+    """A token a tile, 70,001 of them (a window keeps the plain kernel's share small): both are within their roundings of the exact result."""
+    c = Case(K, [(70001, 30)], 8, 1, 32, F32)
+    out, plain = c.run(K, window=40), c.run(K, window=40, backend="plain")
+    n = 70001
+    assert (out[n:] == 9).all()
+    # scores of 32 numbers below 2^6, sums of 40: 16 2^-24 of the scores' products and some 2^-19 of the weights, of values up to 8
+    assert (out[:n] - plain[:n]).abs().max() <= 2 * 8 * (2 * 16 * U * 64 + 2.0 ** -19)
+
+
 @pytest.mark.parametrize("slices", [1, 3])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompts_keep_the_bits_of_the_codes(K, monkeypatch, hd, slices):
