@@ -875,12 +875,12 @@ class Kernels:
         self._on_device(what, q, out, cache, head_sinks, head_gate, head_scale, *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
-        tc = self.attn_tc_supports(hd) and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
+        tc = hd <= 128 and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
         # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
         # longest are a few tokens on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 411 / 883 / 230;
         # 2,000 tokens beside one behind 30,000, 637 / 368 / 81.)
         few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 8 * (n_seqs - 1) else 0
-        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, 1 if few else n_seqs, nqh, nkh, tc):
+        if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, 1 if few else n_seqs, nqh, nkh, hd, tc):
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
                                  int(window or 0), scale, int(keep_first or 0), head_scale, dict(
                                      sink=sink, out_scale=out_scale, head_sinks=head_sinks, head_gate=head_gate, distance_bias=distance_bias,
@@ -922,7 +922,7 @@ class Kernels:
             lib.braid_attn_kv4_merge.restype = c_int
             if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
                 raise KernelError("the attention library over a 4-bit cache is another than was asked for")
-            if self.attn_tc_supports(head_dim):
+            if head_dim <= 128:
                 lib.braid_attn_kv4_prompt.argtypes = [c_char_p, c_void_p]
                 lib.braid_attn_kv4_prompt.restype = c_int
                 if lib.braid_attn_kv4_prompt_args_bytes() != _KV4_PROMPT_ARGS.size:
@@ -940,20 +940,21 @@ class Kernels:
     # over 4 bits: a prompt alone, 64 tokens (128 units) 15.1 / 8.2, 128 tokens (256) 15.3 / 15.5, 256 tokens 17.1 / 29.5; behind 1,000, 64 tokens 28.6 /
     # 16.9, 128 tokens 28.6 / 31.6; behind 8,000, 16 tokens (32) 29.1 / 26.0, 32 tokens 30.9 / 41.7, four of 12 (96) 59 / 51, four of 16 (128) 60 /
     # 73; behind 32,000, 16 tokens 82 / 74, 32 tokens 83 / 151, 128 tokens 101 / 484.
-    # Other head sizes and options go through the older kernel for ordinary pages, of which a CTA walks its context alone: twice the units behind 1,000
-    # and more (heads of 96, a prompt alone, 128 tokens (256) 14.2 / 14.5, 512 tokens 29 / 54; behind 1,000, 256 tokens (512) 50.5 / 54, four of 64 46 /
-    # 37; behind 8,000, 256 tokens 269 / 236, 512 tokens 331 / 426; heads of 256 alike).
+    # Smaller heads: more units, as the codes are fewer (heads of 64, a prompt alone, 128 tokens 13.2 / 11.2, 512 tokens (1,024) 18 / 33; behind 8,000, 32
+    # tokens (64) 25.8 / 27.0, 64 tokens 31 / 50).  Heads above 128 and some options go through the older kernel for ordinary pages, of which a CTA walks
+    # its context alone: twice the units behind 1,000 and more (heads of 256, two queries a kv head, a prompt alone, 256 tokens (256) 25 / 23, 512 tokens
+    # 35 / 52; behind 1,000, 256 tokens 70 / 59, 512 tokens 81 / 121; behind 8,000, four of 128 (512) 398 / 370, 512 tokens 388 / 554).
     KV4_PAGES_FROM = 250
 
     @staticmethod
-    def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, max_kv_len: int, n_seqs: int, nqh: int, nkh: int, tc: bool) -> bool:
+    def _kv4_as_pages(q: torch.Tensor, out: torch.Tensor, max_q_len: int, max_kv_len: int, n_seqs: int, nqh: int, nkh: int, hd: int, tc: bool) -> bool:
         """Whether attention reads the pages of `n_seqs` sequences back and runs over those."""
         if max_q_len <= 8 or out.dtype != torch.bfloat16:
             return False
         g = nqh // nkh
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
         units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
-        least = Kernels.KV4_PAGES_FROM
+        least = Kernels.KV4_PAGES_FROM * (min(3, 128 / hd) if tc else 1)
         if max_kv_len >= 1000:
             least *= max(0.11 * n_seqs, 1100 / max_kv_len) if tc else 2
         return units >= least and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
@@ -961,16 +962,18 @@ class Kernels:
     def _attn_kv4_pages(self, q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd, window,
                         scale, keep_first, head_scale, options, tc, q_from) -> None:
         """Prompts, bfloat16: the pages that the queries see are read back, block c of sequence i as page i * cols + c of a workspace,
-        and the attention of ordinary pages runs over them.  With `tc` they are float16 numbers, scaled a page and head.
+        and the attention of ordinary pages runs over them.  With `tc` they are float16 numbers, scaled a page and head,
+        and the tcgen05 kernel of heads of up to 128 runs over them.
         Values that are NaN are read back as zero; the sequences that hold some, or whose values' sizes lie so far apart that float16 would not
         hold them, are computed by the plain kernel (which otherwise ends at once)."""
         lib = self.part_library("kv4")
         cols = min(page_table.shape[1], max(1, -(-max_kv_len // build.page_size())))
-        page = 2 * nkh * build.page_size() * hd
+        width = hd if not tc else 64 if hd <= 64 else 128                 # (zeros behind heads of 32 and 96)
+        page = 2 * nkh * build.page_size() * width
         group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
         # from torch's allocator at every call: calls on other streams, and other graphs, have their own
         device, stream = out.device, self._stream()
-        pages = torch.empty((group * cols, 2, nkh, build.page_size(), hd), dtype=torch.float16 if tc else torch.bfloat16, device=device)
+        pages = torch.empty((group * cols, 2, nkh, build.page_size(), width), dtype=torch.float16 if tc else torch.bfloat16, device=device)
         repair = torch.zeros(1 + n_seqs * (1 + nkh), dtype=torch.int32, device=device)     # and the sequences' largest exponents
         lengths = (q_start, q_len, kv_before)
         if not tc:

@@ -1,5 +1,6 @@
 // Attention of prompts over a cache held in 4 bits, on the 5th-generation tensor cores (tcgen05): over the pages that kv4_expand_kernel
-// (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size: -DBRAID_HD=64 or 128.
+// (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size: -DBRAID_HD=32, 64, 96 or
+// 128; heads of 32 and 96 are computed as ones of 64 and 128, their further numbers zero (in the pages, and behind the queries' map).
 //
 // A CTA takes two groups of 128 columns of queries (tokens x the query heads of a kv head) and walks the keys that they see, 128 at a time:
 //   S = Q K^T  (tensor memory, float32),   p = 2^(scale log2(e) S - m),   O += p V  (p in tensor memory)
@@ -31,7 +32,7 @@
 #error "compile with -DBRAID_HD=<head_dim>"
 #endif
 
-#if BRAID_HD == 64 || BRAID_HD == 128
+#if BRAID_HD <= 128
 
 #define FA_BM 128
 #define FA_BN 128                                // keys per tile: two pages
@@ -39,7 +40,8 @@
 static_assert(FA_PAGE == 64, "a key tile of this kernel is two pages of 64 positions");
 #define FA_SOFTMAX 4                             // warps before: TMA, S, one that only waits for the end, P V
 #define FA_THREADS ((FA_SOFTMAX + 16) * 32)      // two groups of 8 softmax warps
-#define FA_HB (BRAID_HD / 64)                    // 64-element blocks of the head dimension
+#define FA_HD (BRAID_HD <= 64 ? 64 : 128)        // the head size computed with
+#define FA_HB (FA_HD / 64)                       // 64-element blocks of it
 #define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] bf16, 128-byte rows
 #define FA_PBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]: what a copy brings
 #define FA_KBLOCK_BYTES (2 * FA_PBLOCK_BYTES)    // two pages on end
@@ -94,7 +96,7 @@ __host__ __device__ constexpr uint32_t fa_idesc_f16(uint32_t idesc) { return ide
 
 struct Kv4PromptArgs {
     const void* q;
-    const void* pages;           // block c of sequence i: page i * cols + c, [2][nkh][64][HD] float16, scaled
+    const void* pages;           // block c of sequence i: page i * cols + c, [2][nkh][64][FA_HD] float16, scaled
     __nv_bfloat16* out;
     const int* q_start;
     const int* q_len;
@@ -125,7 +127,7 @@ struct Kv4PromptArgs {
 template <int FORM>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Kv4PromptArgs a) {
-    constexpr int HD = BRAID_HD;
+    constexpr int HD = FA_HD;
     constexpr bool BIAS = FORM == FA_BIAS, CAP = FORM == FA_CAP;
     pdl_trigger();
     // the swizzled tiles want 1024-byte alignment; the start of dynamic shared memory is checked instead of rounded up
@@ -299,7 +301,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     tc_fence_after();
                     const uint32_t qs_lo = q_lo + (uint32_t)((group * FA_Q_BYTES) >> 4), ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
+                    for (int ks = 0; ks < BRAID_HD / 16; ++ks) {
                         const uint32_t qoff = ((ks >> 2) * FA_QBLOCK_BYTES + (ks & 3) * 32) >> 4, koff = ((ks >> 2) * FA_KBLOCK_BYTES + (ks & 3) * 32) >> 4;
                         umma_ss_lohi(ts, qs_lo + qoff, kq_hi, ks_lo + koff, kq_hi, idesc_qk, ks > 0 ? 1u : 0u);
                     }
@@ -522,10 +524,11 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         const size_t at = (row * a.nqh + head) * a.n_splits + split;
         if (a.n_splits > 1 && valid && half == 0)
-            *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * HD + at * 2) = make_float2(m, l);
+            *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * BRAID_HD + at * 2) = make_float2(m, l);
 #pragma unroll
         for (int h = 0; h < HD / 64; ++h) {                    // a half of the row's columns
             const int c0 = half * (HD / 2) + h * 32;
+            if (c0 >= BRAID_HD) break;
             float ov[32];
             __syncwarp();
             if (n_tiles > 0) {
@@ -535,11 +538,11 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int i = 0; i < 32; ++i) ov[i] = 0.f;
             }
             if (ok && valid && a.n_splits > 1) {
-                float* dst = a.partial + at * HD + c0;
+                float* dst = a.partial + at * BRAID_HD + c0;
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(ov[c] * inv, ov[c + 1] * inv, ov[c + 2] * inv, ov[c + 3] * inv);
             } else if (ok && valid) {
-                __nv_bfloat16* dst = a.out + row * a.out_stride + (size_t)head * HD + c0;
+                __nv_bfloat16* dst = a.out + row * a.out_stride + (size_t)head * BRAID_HD + c0;
 #pragma unroll
                 for (int c = 0; c < 32; c += 8) {
                     uint32_t w[4];
@@ -606,8 +609,8 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
         if (r != CUDA_SUCCESS) BRAID_REFUSE("attn_kv4: cuTensorMapEncodeTiled(q) failed with %d", (int)r);
     }
     {
-        cuuint64_t dims[2] = {(cuuint64_t)BRAID_HD, (cuuint64_t)a.n_seqs * a.cols * 2 * a.nkh * FA_PAGE};
-        cuuint64_t strides[1] = {(cuuint64_t)BRAID_HD * 2};
+        cuuint64_t dims[2] = {(cuuint64_t)FA_HD, (cuuint64_t)a.n_seqs * a.cols * 2 * a.nkh * FA_PAGE};
+        cuuint64_t strides[1] = {(cuuint64_t)FA_HD * 2};
         cuuint32_t box[2] = {64, FA_PAGE};
         cuuint32_t estr[2] = {1, 1};
         CUresult r = fn(&mkv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.pages), dims, strides, box, estr,

@@ -311,7 +311,7 @@ struct ExpandArgs {
     int* error_flag;
     int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [1 + seq0 + sequence] become 1
     int* out_table;              // (out_cols > 0) [n_seqs, out_cols]: the numbers of the pages, for whoever reads them
-    int* scales;                 // given: float16 numbers, scaled a page and kv head: [pages, nkh, 2] exponents + KV4_EXPONENT of keys, values (0: all zero)
+    int* scales;                 // given: float16 numbers, rows of 64 or 128, scaled a page and kv head: [pages, nkh, 2] exponents + KV4_EXPONENT of keys, values (0: all zero)
     int* top;                    // (scales) [n_seqs, nkh] from sequence seq0 on: the largest of a sequence's values' exponents; zeros before
     int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
     int q_from;                  // only the pages of sequences that bring at least so many tokens
@@ -399,6 +399,7 @@ kv4_expand_kernel(const ExpandArgs a) {
             a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
     if (end - before < a.q_from) return;
     constexpr bool SCALED = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
+    constexpr int OUT = !SCALED || HD > 128 ? HD : HD <= 64 ? 64 : 128;       // numbers of a row that is written, zeros behind the head's
     __shared__ float3 sizes[2][8];
     int turn = 0;
     const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0, cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
@@ -415,8 +416,8 @@ kv4_expand_kernel(const ExpandArgs a) {
         const int t = threadIdx.x >> 2, j = threadIdx.x & 3, tr = t % KV4_REC;
         const uint8_t* rec = a.cache + ((size_t)page * a.nkh + kvh) * kv4_page_bytes(HD) + (t / KV4_REC) * kv4_record_bytes(HD);
         const bool in = key0 + t < end && (key0 + t >= lo || key0 + t < a.keep_first);
-        T* dst = (T*)a.out + ((out_page * 2 * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * HD + 8 * j;
-        const size_t plane = (size_t)a.nkh * BRAID_PAGE_SIZE * HD;
+        T* dst = (T*)a.out + ((out_page * 2 * a.nkh + kvh) * BRAID_PAGE_SIZE + t) * OUT + 8 * j;
+        const size_t plane = (size_t)a.nkh * BRAID_PAGE_SIZE * OUT;
         uint32_t kc[W], kg[W], vc[W], vg[W];
         load_words<W>(rec + tr * (HD / 2) + 4 * W * j, kc);
         load_words<W>(rec + kv4_key_groups(HD) + 4 * W * tr, kg);
@@ -490,6 +491,9 @@ kv4_expand_kernel(const ExpandArgs a) {
             *reinterpret_cast<uint4*>(dst + plane + 32 * w) = *reinterpret_cast<const uint4*>(y);
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + plane + 32 * w + 4) = *reinterpret_cast<const uint4*>(y + 2);
         }
+#pragma unroll
+        for (int w = W; w < OUT / 32; ++w)
+            *reinterpret_cast<uint4*>(dst + 32 * w) = *reinterpret_cast<uint4*>(dst + plane + 32 * w) = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -514,7 +518,8 @@ extern "C" int braid_kv4_expand(const ExpandArgs* args, void* stream) {
     if (a.nkh > 65535 || a.n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", a.nkh, a.n_seqs);
     if (a.window <= 0) a.window = a.keep_first = 0;
     if (a.scales) {
-        if (!a.repair || !a.top || a.out_cols <= 0) BRAID_REFUSE("kv4_expand: scaled pages want pages of their own, the largest exponents and the flags");
+        if (!a.repair || !a.top || a.out_cols <= 0 || a.hd > 128)
+            BRAID_REFUSE("kv4_expand: scaled pages are of heads of up to 128, and want pages of their own, the largest exponents and the flags");
         return launch_expand<__half>(a, (cudaStream_t)stream);
     }
     if (a.dtype == BRAID_F32) return launch_expand<float>(a, (cudaStream_t)stream);
