@@ -875,7 +875,7 @@ class Kernels:
         self._on_device(what, q, out, cache, head_sinks, head_gate, head_scale, *(distance_bias or ()))
         if rows == 0 or n_seqs == 0:
             return
-        tc = hd <= 128 and not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
+        tc = not keep_first and head_scale is None and (scale > 0 or bool(softcap) or distance_bias is not None)
         # A step of prompts and of sequences that bring what 8 columns of queries hold: the latter as they are, where what stands beside the
         # longest are a few tokens on average.  (us, all over 4 bits / all over pages / so: 512 tokens beside 63 single ones behind 8,000, 411 / 883 / 230;
         # 2,000 tokens beside one behind 30,000, 637 / 368 / 81.)
@@ -922,11 +922,10 @@ class Kernels:
             lib.braid_attn_kv4_merge.restype = c_int
             if lib.braid_attn_kv4_args_bytes() != _KV4_ARGS.size or lib.braid_attn_kv4_head_dim() != head_dim:
                 raise KernelError("the attention library over a 4-bit cache is another than was asked for")
-            if head_dim <= 128:
-                lib.braid_attn_kv4_prompt.argtypes = [c_char_p, c_void_p]
-                lib.braid_attn_kv4_prompt.restype = c_int
-                if lib.braid_attn_kv4_prompt_args_bytes() != _KV4_PROMPT_ARGS.size:
-                    raise KernelError("the attention library over a 4-bit cache has other arguments than these bindings")
+            lib.braid_attn_kv4_prompt.argtypes = [c_char_p, c_void_p]
+            lib.braid_attn_kv4_prompt.restype = c_int
+            if lib.braid_attn_kv4_prompt_args_bytes() != _KV4_PROMPT_ARGS.size:
+                raise KernelError("the attention library over a 4-bit cache has other arguments than these bindings")
             lib.plans = {}                                    # float32 -> (CTAs held at once, clusters by their size)
             self._attn_libs[("kv4", head_dim)] = lib
         return lib
@@ -954,7 +953,7 @@ class Kernels:
         g = nqh // nkh
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
         units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
-        least = Kernels.KV4_PAGES_FROM * (min(3, 128 / hd) if tc else 1)
+        least = Kernels.KV4_PAGES_FROM * (max(1, min(3, 128 / hd)) if tc else 1)
         if max_kv_len >= 1000:
             least *= max(0.11 * n_seqs, 1100 / max_kv_len) if tc else 2
         return units >= least and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
@@ -963,12 +962,12 @@ class Kernels:
                         scale, keep_first, head_scale, options, tc, q_from) -> None:
         """Prompts, bfloat16: the pages that the queries see are read back, block c of sequence i as page i * cols + c of a workspace,
         and the attention of ordinary pages runs over them.  With `tc` they are float16 numbers, scaled a page and head,
-        and the tcgen05 kernel of heads of up to 128 runs over them.
+        and the tcgen05 kernel runs over them.
         Values that are NaN are read back as zero; the sequences that hold some, or whose values' sizes lie so far apart that float16 would not
         hold them, are computed by the plain kernel (which otherwise ends at once)."""
         lib = self.part_library("kv4")
         cols = min(page_table.shape[1], max(1, -(-max_kv_len // build.page_size())))
-        width = hd if not tc else 64 if hd <= 64 else 128                 # (zeros behind heads of 32 and 96)
+        width = hd if not tc else 64 if hd <= 64 else 128 if hd <= 128 else 256       # (zeros behind a head)
         page = 2 * nkh * build.page_size() * width
         group = max(1, min(n_seqs, self.KV4_PAGES_BYTES // (2 * page * cols)))
         # from torch's allocator at every call: calls on other streams, and other graphs, have their own
@@ -1019,7 +1018,7 @@ class Kernels:
     def _kv4_prompt_slices(self, rows: int, n_seqs: int, max_q_len: int, max_kv_len: int, nqh: int, nkh: int, hd: int, window: int) -> int:
         """Slices of the context for prompts over pages that were read back: a CTA takes 256 columns of queries, and an SM one CTA."""
         g = nqh // nkh
-        tokens = 2 * (128 // min(g, 128))
+        tokens = (2 if hd <= 128 else 1) * (128 // min(g, 128))
         ctas = nkh * -(-g // 128) * min(n_seqs * -(-max_q_len // tokens), rows // tokens + n_seqs)
         most = min(max_kv_len, window + tokens) if window else max_kv_len
         mean = most if window else max(1, max_kv_len - max_q_len // 2)

@@ -1,6 +1,7 @@
 // Attention of prompts over a cache held in 4 bits, on the 5th-generation tensor cores (tcgen05): over the pages that kv4_expand_kernel
-// (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size: -DBRAID_HD=32, 64, 96 or
-// 128; heads of 32 and 96 are computed as ones of 64 and 128, their further numbers zero (in the pages, and behind the queries' map).
+// (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size:
+// -DBRAID_HD=<32, 64, ... 256>.  The sizes computed with are 64, 128 and 256; a head's further numbers are zero (in the pages, and behind the
+// queries' map).
 //
 // A CTA takes two groups of 128 columns of queries (tokens x the query heads of a kv head) and walks the keys that they see, 128 at a time:
 //   S = Q K^T  (tensor memory, float32),   p = 2^(scale log2(e) S - m),   O += p V  (p in tensor memory)
@@ -8,6 +9,9 @@
 // TMA, warp 1 issues S, warp 3 P V, and 16 warps are the softmax: TWO threads share a row, each with half of a tile's keys (a page) and half of
 // the result's columns, in two warps that meet at a barrier of their own once a tile.  That barrier carries the question whether any row's
 // maximum has to be raised (barrier.red.or), so that the two exchange numbers only then.
+//
+// Heads above 128: a result of 128 rows fills as much tensor memory as two of the others.  There the two groups are the same 128 rows, each with half
+// of the result's columns; both compute all scores and probabilities.  (The products of a tile are then 3,072 cycles, 1,024 of them twice.)
 //
 // All operands are float16 numbers: their 11 bits hold what the codes say, where bfloat16's 8 made errors of 0.0031 to 0.0035 of the result
 // instead of 0.0017, which is the rounding of the result.  For their range, kv4_expand_kernel scales the keys and the values of a page and kv head
@@ -32,7 +36,6 @@
 #error "compile with -DBRAID_HD=<head_dim>"
 #endif
 
-#if BRAID_HD <= 128
 
 #define FA_BM 128
 #define FA_BN 128                                // keys per tile: two pages
@@ -40,17 +43,20 @@
 static_assert(FA_PAGE == 64, "a key tile of this kernel is two pages of 64 positions");
 #define FA_SOFTMAX 4                             // warps before: TMA, S, one that only waits for the end, P V
 #define FA_THREADS ((FA_SOFTMAX + 16) * 32)      // two groups of 8 softmax warps
-#define FA_HD (BRAID_HD <= 64 ? 64 : 128)        // the head size computed with
+#define FA_WIDE (BRAID_HD > 128)                 // the groups are the same rows
+#define FA_HD (BRAID_HD <= 64 ? 64 : BRAID_HD <= 128 ? 128 : 256)              // the head size computed with
+#define FA_OD (FA_WIDE ? 128 : FA_HD)            // result columns of a group
+#define FA_QTILES (FA_WIDE ? 1 : 2)              // tiles of 128 rows a CTA
 #define FA_HB (FA_HD / 64)                       // 64-element blocks of it
 #define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] bf16, 128-byte rows
 #define FA_PBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]: what a copy brings
 #define FA_KBLOCK_BYTES (2 * FA_PBLOCK_BYTES)    // two pages on end
 #define FA_Q_BYTES (FA_HB * FA_QBLOCK_BYTES)
 #define FA_KV_BYTES (FA_HB * FA_KBLOCK_BYTES)    // one K or one V tile
-#define FA_KST 2                                 // stages of the key ring
-#define FA_VST 2                                 // stages of the value ring
+#define FA_KST (FA_WIDE ? 1 : 2)                                 // stages of the key ring
+#define FA_VST (FA_WIDE ? 1 : 2)                                 // stages of the value ring
 #define FA_BAR_BYTES 256
-#define FA_SMEM (2 * FA_Q_BYTES + (FA_KST + FA_VST) * FA_KV_BYTES + FA_BAR_BYTES)
+#define FA_SMEM (FA_QTILES * FA_Q_BYTES + (FA_KST + FA_VST) * FA_KV_BYTES + FA_BAR_BYTES)
 // tensor memory: O of the first 128 rows [0, 128), of the others [128, 256); the scores of both in turn [256, 384); P of either [384, 448), [448, 512)
 #define FA_TMEM_COLS 512
 #define FA_TMEM_S 256
@@ -137,7 +143,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         return;
     }
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + 2 * FA_Q_BYTES;             // [FA_KST]
+    uint8_t* sK = sQ + FA_QTILES * FA_Q_BYTES;     // [FA_KST]
     uint8_t* sV = sK + FA_KST * FA_KV_BYTES;       // [FA_VST]
     uint64_t* bars = (uint64_t*)(sV + FA_VST * FA_KV_BYTES);
     uint64_t* q_full = bars;                       // [1]
@@ -146,7 +152,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint64_t* k_empty = k_full + FA_KST;           // [FA_KST]
     uint64_t* v_full = k_empty + FA_KST;           // [FA_VST]
     uint64_t* v_empty = v_full + FA_VST;           // [FA_VST]
-    uint64_t* s_full = v_empty + FA_VST;           // [2] of the first, of the second 128 rows; the others alike
+    uint64_t* s_full = v_empty + FA_VST;           // [2] of the first, of the second group; the others alike
     uint64_t* s_free = s_full + 2;                 // [2] the scores are in registers
     uint64_t* p_ready = s_free + 2;                // [2]
     uint64_t* pv_done = p_ready + 2;               // [2]
@@ -174,7 +180,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (threadIdx.x == 0) found[0] = -1;
         for (int s0 = 0; s0 < a.n_seqs && before <= tile; s0 += FA_THREADS) {
             const int s = s0 + threadIdx.x, n = s < a.n_seqs ? max(a.q_len[s], 0) : 0;
-            const int mine = n >= a.q_from ? (n + 2 * tpc - 1) / (2 * tpc) : 0;
+            const int mine = n >= a.q_from ? (n + FA_QTILES * tpc - 1) / (FA_QTILES * tpc) : 0;
             int upto = mine;                      // tiles of this warp's sequences up to this one
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -202,7 +208,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (seq < 0) return;
     }
     const int q_len = a.q_len[seq];
-    const int tok0 = tile * (2 * tpc);
+    const int tok0 = tile * (FA_QTILES * tpc);
     if (tok0 >= q_len || q_len < a.q_from) return;             // uniform over the CTA
 
     if (threadIdx.x == 0) {
@@ -220,8 +226,8 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
-    const int ng = q_len - tok0 > tpc ? 2 : 1;    // groups of 128 rows that hold tokens
-    const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + 2 * tpc, q_len) - 1;
+    const int ng = FA_WIDE || q_len - tok0 > tpc ? 2 : 1;    // groups that hold tokens
+    const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + FA_QTILES * tpc, q_len) - 1;
     const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
     int page_lo = k_lo / FA_PAGE, page_hi = pos_max / FA_PAGE + 1;
     if (a.n_splits > 1) {                         // slices of whole tiles
@@ -235,8 +241,8 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
     if (warp == 0) {
         if (lane == 0 && n_tiles > 0) {
-            mbar_expect_tx(q_full, (uint32_t)(ng * hpc * tpc * 128 * FA_HB));      // the box is hpc x tpc rows of 128 bytes
-            for (int gr = 0; gr < ng; ++gr)
+            mbar_expect_tx(q_full, (uint32_t)((FA_WIDE ? 1 : ng) * hpc * tpc * 128 * FA_HB));      // the box is hpc x tpc rows of 128 bytes
+            for (int gr = 0; gr < (FA_WIDE ? 1 : ng); ++gr)
 #pragma unroll
                 for (int hb = 0; hb < FA_HB; ++hb)
                     tma_load_3d(&map_q, q_full, sQ + gr * FA_Q_BYTES + hb * FA_QBLOCK_BYTES, hb * 64, head0, q_start + tok0 + gr * tpc);
@@ -299,7 +305,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     else if (j > 0) ok = mbar_wait(&s_free[ng - 1], (uint32_t)((j - 1) & 1), abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t qs_lo = q_lo + (uint32_t)((group * FA_Q_BYTES) >> 4), ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4);
+                    const uint32_t qs_lo = q_lo + (uint32_t)((FA_WIDE ? 0 : group * FA_Q_BYTES) >> 4), ks_lo = k_lo + (uint32_t)((kst * FA_KV_BYTES) >> 4);
 #pragma unroll
                     for (int ks = 0; ks < BRAID_HD / 16; ++ks) {
                         const uint32_t qoff = ((ks >> 2) * FA_QBLOCK_BYTES + (ks & 3) * 32) >> 4, koff = ((ks >> 2) * FA_KBLOCK_BYTES + (ks & 3) * 32) >> 4;
@@ -312,7 +318,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
     } else if (warp == 3) {
         if (lane == 0 && n_tiles > 0) {
-            constexpr uint32_t idesc_pv = fa_idesc_f16(umma_idesc_bf16_b_mn(FA_BM, HD));
+            constexpr uint32_t idesc_pv = fa_idesc_f16(umma_idesc_bf16_b_mn(FA_BM, FA_OD));
             const uint64_t dv = umma_desc_sw128_mn(smem_u32(sV), FA_KBLOCK_BYTES);
             const uint32_t v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
             bool ok = true;
@@ -324,18 +330,19 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     ok = mbar_wait(&p_ready[group], (uint32_t)(j & 1), abort_flag);
                     if (!ok) break;
                     tc_fence_after();
+                    const uint32_t vg_lo = vs_lo + (uint32_t)((FA_WIDE ? group * 2 * FA_KBLOCK_BYTES : 0) >> 4);
                     const uint32_t to = tmem_base + group * 128, tp = tmem_base + FA_TMEM_P + group * 64;
 #pragma unroll
                     for (int ks = 0; ks < FA_BN / 16; ++ks)
-                        umma_ts_lohi(to, tp + ks * 8, vs_lo + (uint32_t)((ks * 16 * 128) >> 4), v_hi, idesc_pv, (ks > 0 || j > 0) ? 1u : 0u);
+                        umma_ts_lohi(to, tp + ks * 8, vg_lo + (uint32_t)((ks * 16 * 128) >> 4), v_hi, idesc_pv, (ks > 0 || j > 0) ? 1u : 0u);
                     umma_commit(&pv_done[group]);
                 }
                 if (ok) umma_commit(&v_empty[vst]);
             }
         }
     } else if (warp >= FA_SOFTMAX && (warp - FA_SOFTMAX) >> 3 < ng) {
-        const int group = (warp - FA_SOFTMAX) >> 3;                     // the first or the second 128 rows
-        const int tokg = tok0 + group * tpc, n_tok = min(tpc, q_len - tokg);
+        const int group = (warp - FA_SOFTMAX) >> 3;            // the first or the second 128 rows, or 128 columns of the result
+        const int tokg = tok0 + (FA_WIDE ? 0 : group * tpc), n_tok = min(tpc, q_len - tokg);
         const int first = kv_before + tokg, last = first + n_tok - 1;             // the group's positions
         const int quarter = warp & 3;                          // tensor-memory lanes 32 * quarter ...
         const int half = ((warp - FA_SOFTMAX) >> 2) & 1;                // this thread's half of a tile's keys
@@ -355,9 +362,9 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // of the 128-byte blocks (in any order within: the tile's swizzle moves 16 bytes within them).
         float row_factor = a.scale_log2;                      // of the scores: 2^(the row's exponent) in it, and below 2^(the page's)
         if (n_tiles > 0) {
-            constexpr int CHUNKS = HD / 16;
-            uint8_t* src = sQ + group * FA_Q_BYTES + (HD == 128 ? half * FA_QBLOCK_BYTES : 0) + r * 128;
-            const int chunk0 = HD == 128 ? 0 : half * CHUNKS;
+            constexpr int CHUNKS = FA_OD / 16;                // of 8 numbers
+            uint8_t* src = sQ + (FA_WIDE ? 2 * group * FA_QBLOCK_BYTES : group * FA_Q_BYTES) + (HD > 64 ? half * FA_QBLOCK_BYTES : 0) + r * 128;
+            const int chunk0 = HD > 64 ? 0 : half * CHUNKS;
             const bool came = mbar_wait(q_full, 0, abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
             uint4 x[CHUNKS];
@@ -370,7 +377,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
             }
             share[group][1][half][r] = most;
-            pair_sync(pair);
+            if (FA_WIDE) {                                     // four threads have a row's numbers
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(9 + quarter) : "memory");
+                __syncwarp();
+                most = fmaxf(most, fmaxf(share[1 - group][1][half][r], share[1 - group][1][1 - half][r]));
+            } else {
+                pair_sync(pair);
+            }
             most = fmaxf(most, share[group][1][1 - half][r]);
             const int qe = most > 0.f ? min(max(kv4_exponent(most) - 8, -126), 119) : 0;
             row_factor *= kv4_pow2(qe);
@@ -484,13 +497,13 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (any && j > 0) {                                // (the same for every lane)
                 // a half of the row's columns
 #pragma unroll
-                for (int h = 0; h < HD / 64; ++h) {
+                for (int h = 0; h < FA_OD / 64; ++h) {
                     float ov[32];
-                    tmem_ld32(tmem_o + half * (HD / 2) + h * 32 + lane_addr, ov);
+                    tmem_ld32(tmem_o + half * (FA_OD / 2) + h * 32 + lane_addr, ov);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) ov[i] *= factor;
                     __syncwarp();
-                    tmem_st32_nowait(tmem_o + half * (HD / 2) + h * 32 + lane_addr, reinterpret_cast<const uint32_t*>(ov));
+                    tmem_st32_nowait(tmem_o + half * (FA_OD / 2) + h * 32 + lane_addr, reinterpret_cast<const uint32_t*>(ov));
                 }
             }
             tmem_st_wait();
@@ -523,16 +536,16 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (a.head_gate) inv *= 1.f / (1.f + __expf(-__bfloat162float(a.head_gate[row * a.gate_stride + head])));
         }
         const size_t at = (row * a.nqh + head) * a.n_splits + split;
-        if (a.n_splits > 1 && valid && half == 0)
+        if (a.n_splits > 1 && valid && half == 0 && !(FA_WIDE && group))
             *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * BRAID_HD + at * 2) = make_float2(m, l);
 #pragma unroll
-        for (int h = 0; h < HD / 64; ++h) {                    // a half of the row's columns
-            const int c0 = half * (HD / 2) + h * 32;
+        for (int h = 0; h < FA_OD / 64; ++h) {                 // a half of the row's columns
+            const int ct = half * (FA_OD / 2) + h * 32, c0 = ct + (FA_WIDE ? group * 128 : 0);
             if (c0 >= BRAID_HD) break;
             float ov[32];
             __syncwarp();
             if (n_tiles > 0) {
-                tmem_ld32(tmem_o + c0 + lane_addr, ov);
+                tmem_ld32(tmem_o + ct + lane_addr, ov);
             } else {                                           // a slice without a key
 #pragma unroll
                 for (int i = 0; i < 32; ++i) ov[i] = 0.f;
@@ -590,8 +603,8 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     // A CTA for every tile that a sequence may have, or, where the rows are too few for that, for every tile that the step may have: those look up
     // whose tile they are.  (A CTA that finds nothing to do still takes an SM for some us.  512 tokens beside 63 single ones, attention as a whole: 387
     // us by sequence, 282 by step; 900 beside 100 sequences of up to 50: 246, 162; 3,000, 100, 200 and 1,500: 118, 114.)
-    const long long every = (a.max_q_len + 2 * tpc - 1) / (2 * tpc);
-    const long long most = a.rows / (2 * tpc) + (a.q_from > 1 ? (a.rows / a.q_from < a.n_seqs ? a.rows / a.q_from : a.n_seqs) : a.n_seqs);
+    const long long every = (a.max_q_len + FA_QTILES * tpc - 1) / (FA_QTILES * tpc);
+    const long long most = a.rows / (FA_QTILES * tpc) + (a.q_from > 1 ? (a.rows / a.q_from < a.n_seqs ? a.rows / a.q_from : a.n_seqs) : a.n_seqs);
     a.tiles = 2 * most <= every * a.n_seqs ? (int)most : 0;
     const long long gx = (a.tiles ? most : every) * a.n_splits;
     if (gx > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
@@ -634,5 +647,3 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
                  dim3(a.nkh * hchunks, a.tiles ? 1 : a.n_seqs, (unsigned)gx), dim3(FA_THREADS), FA_SMEM, (cudaStream_t)stream, mq, mkv, a);
     BRAID_LAUNCH_CHECK();
 }
-
-#endif

@@ -311,7 +311,7 @@ struct ExpandArgs {
     int* error_flag;
     int* repair;                 // given: groups of values that are NaN come out zero, and repair[0] and [1 + seq0 + sequence] become 1
     int* out_table;              // (out_cols > 0) [n_seqs, out_cols]: the numbers of the pages, for whoever reads them
-    int* scales;                 // given: float16 numbers, rows of 64 or 128, scaled a page and kv head: [pages, nkh, 2] exponents + KV4_EXPONENT of keys, values (0: all zero)
+    int* scales;                 // given: float16 numbers, rows of 64, 128 or 256, scaled a page and kv head: [pages, nkh, 2] exponents + KV4_EXPONENT of keys, values (0: all zero)
     int* top;                    // (scales) [n_seqs, nkh] from sequence seq0 on: the largest of a sequence's values' exponents; zeros before
     int n_seqs, nkh, hd, cols, num_pages, window, keep_first, out_cols, seq0, dtype;
     int q_from;                  // only the pages of sequences that bring at least so many tokens
@@ -399,7 +399,7 @@ kv4_expand_kernel(const ExpandArgs a) {
             a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
     if (end - before < a.q_from) return;
     constexpr bool SCALED = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
-    constexpr int OUT = !SCALED || HD > 128 ? HD : HD <= 64 ? 64 : 128;       // numbers of a row that is written, zeros behind the head's
+    constexpr int OUT = !SCALED ? HD : HD <= 64 ? 64 : HD <= 128 ? 128 : 256;       // numbers of a row that is written, zeros behind the head's
     __shared__ float3 sizes[2][8];
     int turn = 0;
     const int lo = a.window > 0 ? max(0, before - a.window + 1) : 0, cols = a.out_cols > 0 ? min(a.cols, a.out_cols) : a.cols;
@@ -518,8 +518,7 @@ extern "C" int braid_kv4_expand(const ExpandArgs* args, void* stream) {
     if (a.nkh > 65535 || a.n_seqs > 65535) BRAID_REFUSE("kv4_expand: the step exceeds the grid limits (%d kv heads, %d sequences)", a.nkh, a.n_seqs);
     if (a.window <= 0) a.window = a.keep_first = 0;
     if (a.scales) {
-        if (!a.repair || !a.top || a.out_cols <= 0 || a.hd > 128)
-            BRAID_REFUSE("kv4_expand: scaled pages are of heads of up to 128, and want pages of their own, the largest exponents and the flags");
+        if (!a.repair || !a.top || a.out_cols <= 0) BRAID_REFUSE("kv4_expand: scaled pages want pages of their own, the largest exponents and the flags");
         return launch_expand<__half>(a, (cudaStream_t)stream);
     }
     if (a.dtype == BRAID_F32) return launch_expand<float>(a, (cudaStream_t)stream);

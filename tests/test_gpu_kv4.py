@@ -282,7 +282,7 @@ def test_prompts(K, route, seqs, nqh, nkh, hd, dt):
 
 
 @pytest.mark.parametrize("slices", [2, 3, 8])
-@pytest.mark.parametrize("name, hd", [("window", 64), ("sink", 128), ("sinks", 64), ("gate", 128), ("bias", 64), ("cap", 128), ("window", 96), ("gate", 32)])
+@pytest.mark.parametrize("name, hd", [("window", 64), ("sink", 128), ("sinks", 64), ("gate", 128), ("bias", 64), ("cap", 128), ("window", 96), ("gate", 32), ("window", 256), ("sinks", 160)])
 def test_prompts_in_slices(K, monkeypatch, name, hd, slices):
     """The context cut into slices, some of them without a key that a row sees, or without any."""
     monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
@@ -423,7 +423,7 @@ def test_more_tiles_than_a_grid_is_deep(K):
 
 
 @pytest.mark.parametrize("slices", [1, 3])
-@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("hd", range(32, 257, 32))
 def test_prompts_keep_the_bits_of_the_codes(K, monkeypatch, hd, slices):
     """Queries, keys, values and probabilities of prompts are float16 numbers of 11 bits: half a step is 2^-12 of each (and what lies far below
     the largest of its row or page is off by 2^-25 of that, here less than 2^-11 of a part in 2^12)."""
