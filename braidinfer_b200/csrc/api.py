@@ -939,10 +939,11 @@ class Kernels:
     # over 4 bits: a prompt alone, 64 tokens (128 units) 15.1 / 8.2, 128 tokens (256) 15.3 / 15.5, 256 tokens 17.1 / 29.5; behind 1,000, 64 tokens 28.6 /
     # 16.9, 128 tokens 28.6 / 31.6; behind 8,000, 16 tokens (32) 29.1 / 26.0, 32 tokens 30.9 / 41.7, four of 12 (96) 59 / 51, four of 16 (128) 60 /
     # 73; behind 32,000, 16 tokens 82 / 74, 32 tokens 83 / 151, 128 tokens 101 / 484.
-    # Smaller heads: more units, as the codes are fewer (heads of 64, a prompt alone, 128 tokens 13.2 / 11.2, 512 tokens (1,024) 18 / 33; behind 8,000, 32
-    # tokens (64) 25.8 / 27.0, 64 tokens 31 / 50).  Heads above 128 and some options go through the older kernel for ordinary pages, of which a CTA walks
-    # its context alone: twice the units behind 1,000 and more (heads of 256, two queries a kv head, a prompt alone, 256 tokens (256) 25 / 23, 512 tokens
-    # 35 / 52; behind 1,000, 256 tokens 70 / 59, 512 tokens 81 / 121; behind 8,000, four of 128 (512) 398 / 370, 512 tokens 388 / 554).
+    # Heads below 128: more units, as the codes are fewer (heads of 64, a prompt alone, 128 tokens 13.2 / 11.2, 512 tokens (1,024) 18 / 33; behind 8,000,
+    # 32 tokens (64) 25.8 / 27.0, 64 tokens 31 / 50); above as many (heads of 256, a prompt alone, 128 tokens (256) 17.2 / 20.8; behind 8,000, four of 32
+    # (128) 114 / 115).  Kept first tokens, a factor a head and a factor on scores that is not positive go through the older kernel for ordinary
+    # pages, of which a CTA walks its context alone: twice the units behind 1,000 and more (heads of 96, 256 tokens behind 1,000 (512) 50.5 / 54,
+    # four of 64 (512) 46 / 37; behind 8,000, 256 tokens 269 / 236, 512 tokens 331 / 426).
     KV4_PAGES_FROM = 250
 
     @staticmethod
@@ -1025,10 +1026,10 @@ class Kernels:
         sms = torch.cuda.get_device_properties(self._device_index).multi_processor_count
 
         def cost(n: int) -> float:
-            """us: 1.65 for 128 keys of a CTA; 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
+            """us: 1.65 for 128 keys of a CTA (3.1 of heads above 128); 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
             (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 240, 263, 201, 227, 207, 231)"""
             rounds = -(-ctas * n // sms)
-            return max(most, rounds * mean) / 128 / n * 1.65 + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
+            return max(most, rounds * mean) / 128 / n * (1.65 if hd <= 128 else 3.1) + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
         return min(range(1, max(1, min(8, most // 512)) + 1), key=cost)
 
     @staticmethod
