@@ -576,12 +576,23 @@ attn_kv4_kernel(const Kv4Args a) {
                     mma16816_f16(o[2 * w], a0, a1, a2, a3, p0, p1);
                     mma16816_f16(o[2 * w + 1], b0, b1, b2, b3, p0, p1);
                 } else {
+                    // The tensor cores cut sums off instead of rounding them, which over thousands of tokens is a bias: a record's products are
+                    // summed there, the records here.  (21 sequences of 7 tokens behind up to 11,614, heads of 32: errors of
+                    // 1.7e-5 of a float32 result before, 6.7e-7 so; 71 -> 78 us.)
+                    float t0[4], t1[4];
 #pragma unroll
                     for (int part = 0; part < PARTS; ++part) {
                         const uint32_t p0 = transpose8x8(split_pair(x[0], x[1])), p1 = transpose8x8(split_pair(x[2], x[3]));
-                        mma16816(o[2 * w], a0, a1, a2, a3, p0, p1);
-                        mma16816(o[2 * w + 1], b0, b1, b2, b3, p0, p1);
+                        if (part == 0) {
+                            mma16816_zero(t0, a0, a1, a2, a3, p0, p1);
+                            mma16816_zero(t1, b0, b1, b2, b3, p0, p1);
+                        } else {
+                            mma16816(t0, a0, a1, a2, a3, p0, p1);
+                            mma16816(t1, b0, b1, b2, b3, p0, p1);
+                        }
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { o[2 * w][i] += t0[i]; o[2 * w + 1][i] += t1[i]; }
                 }
             }
         }
