@@ -172,6 +172,10 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
     const int unit = gridDim.z - 1 - blockIdx.z, split = unit % a.n_splits;
     int seq = blockIdx.y, tile = unit / a.n_splits;
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
+    }
     pdl_wait();
     if (a.tiles > 0) {
         // the grid's tile number `tile`: whose it is, and which of its tiles
@@ -207,25 +211,10 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         tile = found[1];
         if (seq < 0) return;
     }
-    const int q_len = a.q_len[seq];
+    const int q_len = a.q_len[seq], q_start = a.q_start[seq], kv_before = a.kv_before[seq];
     const int tok0 = tile * (FA_QTILES * tpc);
     if (tok0 >= q_len || q_len < a.q_from) return;             // uniform over the CTA
 
-    if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
-        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
-        for (int s = 0; s < FA_VST; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&q_ready[s], 8); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 1) tmem_alloc(tmem_slot, FA_TMEM_COLS);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
     const int ng = FA_WIDE || q_len - tok0 > tpc ? 2 : 1;    // groups that hold tokens
     const int pos_min = kv_before + tok0, pos_max = kv_before + min(tok0 + FA_QTILES * tpc, q_len) - 1;
     const int k_lo = (a.window > 0 && pos_min - a.window + 1 > 0) ? pos_min - a.window + 1 : 0;
@@ -239,13 +228,29 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int head0 = kvh * g + hchunk * hpc;
     const int n_heads = min(hpc, g - hchunk * hpc);
 
-    if (warp == 0) {
-        if (lane == 0 && n_tiles > 0) {
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < FA_KST; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+        for (int s = 0; s < FA_VST; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&q_ready[s], 8); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); mbar_init(&p_ready[s], 8); mbar_init(&pv_done[s], 1); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (n_tiles > 0) {                        // (the queries are on their way while tensor memory is taken)
             mbar_expect_tx(q_full, (uint32_t)((FA_WIDE ? 1 : ng) * hpc * tpc * 128 * FA_HB));      // the box is hpc x tpc rows of 128 bytes
             for (int gr = 0; gr < (FA_WIDE ? 1 : ng); ++gr)
 #pragma unroll
                 for (int hb = 0; hb < FA_HB; ++hb)
                     tma_load_3d(&map_q, q_full, sQ + gr * FA_Q_BYTES + hb * FA_QBLOCK_BYTES, hb * 64, head0, q_start + tok0 + gr * tpc);
+        }
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, FA_TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (warp == 0) {
+        if (lane == 0 && n_tiles > 0) {
             // key and value tiles go out independently, each as soon as its stage is free
             int jk = 0, jv = 0;
             uint32_t idle = 0;
