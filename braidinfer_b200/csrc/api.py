@@ -1027,7 +1027,7 @@ class Kernels:
 
         def cost(n: int) -> float:
             """us: 1.65 for 128 keys of a CTA (3.1 of heads above 128); 7 for the kernel that merges, and the slices' float32 results written and read at 2.5 TB/s
-            (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 240, 263, 201, 227, 207, 231)"""
+            (700 tokens of 32 heads of 128 behind 16,500, 1 to 6 slices: 235, 256, 189, 218, 193, 213)"""
             rounds = -(-ctas * n // sms)
             return max(most, rounds * mean) / 128 / n * (1.65 if hd <= 128 else 3.1) + (7 + rows * nqh * n * hd * 8 / 2.5e6 if n > 1 else 0)
         return min(range(1, max(1, min(8, most // 512)) + 1), key=cost)

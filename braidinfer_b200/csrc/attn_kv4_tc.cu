@@ -25,7 +25,8 @@
 // the reading back, in bfloat16: 83 / 344 by attn_tc.cu (a thread a row, tiles of 64 keys, two CTAs an SM); 89 / 331 the same with two threads a
 // row; 90 / 332 with both groups in a CTA and scores of their own (96 / 376 with barriers that let their exponentials take turns); 104 / 393 with
 // tiles of 128 keys whose probabilities lie over the scores, where all of a group's steps wait for one another; 78 / 237 so, and 78 / 224 with
-// the context in 3 slices.  In float16 86 / 231 (more registers for the softmax by setmaxnreg, 112 and 32: 3 and 13 % slower).
+// the context in 3 slices.  In float16 86 / 231 (more registers for the softmax by setmaxnreg, 112 and 32: 3 and 13 % slower), 80 / 226
+// with queries asked for before tensor memory is taken and the result written 32 bytes a thread.
 #include "kv4.cuh"
 #include "attn_tc.cuh"
 #include "softcap.cuh"
@@ -96,6 +97,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+// 32 bytes on end, on 32: a whole sector of the cache, where 16 a thread are halves of two.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7]) : "memory");
 }
 // An instruction descriptor with float16 operands instead of bfloat16 ones (bits 7 .. 9 of A, 10 .. 12 of B).
 __host__ __device__ constexpr uint32_t fa_idesc_f16(uint32_t idesc) { return idesc & ~((7u << 7) | (7u << 10)); }
@@ -540,6 +546,7 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             inv *= a.out_scale / (a.has_sink ? l + exp2f(sk - m) : l);
             if (a.head_gate) inv *= 1.f / (1.f + __expf(-__bfloat162float(a.head_gate[row * a.gate_stride + head])));
         }
+        const bool wide = !(((uintptr_t)a.out | (uintptr_t)a.out_stride * 2) & 31);       // rows of the result start on 32 bytes
         const size_t at = (row * a.nqh + head) * a.n_splits + split;
         if (a.n_splits > 1 && valid && half == 0 && !(FA_WIDE && group))
             *reinterpret_cast<float2*>(a.partial + (size_t)a.rows * a.nqh * a.n_splits * BRAID_HD + at * 2) = make_float2(m, l);
@@ -558,18 +565,28 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (ok && valid && a.n_splits > 1) {
                 float* dst = a.partial + at * BRAID_HD + c0;
 #pragma unroll
-                for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(ov[c] * inv, ov[c + 1] * inv, ov[c + 2] * inv, ov[c + 3] * inv);
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(ov[c + i] * inv);
+                    store32(dst + c, w);
+                }
             } else if (ok && valid) {
                 __nv_bfloat16* dst = a.out + row * a.out_stride + (size_t)head * BRAID_HD + c0;
 #pragma unroll
-                for (int c = 0; c < 32; c += 8) {
-                    uint32_t w[4];
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 8; ++i) {
                         __nv_bfloat162 b = __floats2bfloat162_rn(ov[c + 2 * i] * inv, ov[c + 2 * i + 1] * inv);
                         w[i] = *reinterpret_cast<uint32_t*>(&b);
                     }
-                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (wide) {
+                        store32(dst + c, w);
+                    } else {
+                        *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 }
             }
         }
@@ -604,7 +621,7 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     const int g = a.nqh / a.nkh;
     const int hpc = g < FA_BM ? g : FA_BM, tpc = FA_BM / hpc, hchunks = (g + hpc - 1) / hpc;
     if (a.n_splits < 1) a.n_splits = 1;
-    if (a.n_splits > 1 && !a.partial) BRAID_REFUSE("attn_kv4: slices need the partial buffer");
+    if (a.n_splits > 1 && (!a.partial || (uintptr_t)a.partial & 31)) BRAID_REFUSE("attn_kv4: slices need the partial buffer, on 32 bytes");
     // A CTA for every tile that a sequence may have, or, where the rows are too few for that, for every tile that the step may have: those look up
     // whose tile they are.  (A CTA that finds nothing to do still takes an SM for some us.  512 tokens beside 63 single ones, attention as a whole: 387
     // us by sequence, 282 by step; 900 beside 100 sequences of up to 50: 246, 162; 3,000, 100, 200 and 1,500: 118, 114.)

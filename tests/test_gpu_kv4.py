@@ -448,6 +448,10 @@ def test_prompts_keep_the_bits_of_the_codes(K, monkeypatch, hd, slices):
     score = 2 * 2.0 ** -12 * smag[1] + 32 * U * smag[0]
     most = mag * (2 * score[..., None] + 2 * 2.0 ** -12 + 2.0 ** -18) + 2.0 ** -8 * want.abs() + 1e-30
     assert ((out.double().view(want.shape) - want).abs() <= most)[:n].all()
+    # rows of the result that start on 16 bytes, not on 32
+    wide = torch.full((c.rows, c.nqh * hd + 8), 9.0, dtype=BF, device=DEV)
+    again = c.run(K, out=wide[:, 8:])
+    assert torch.equal(again, out) and (wide[:, :8] == 9).all()
 
 
 @pytest.mark.parametrize("seqs", [[(1, 9000), (1, 10), (1, 4000)], [(4, 5000)], [(33, 3000)]])
