@@ -379,14 +379,19 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const bool came = mbar_wait(q_full, 0, abort_flag);
             ok = __all_sync(0xffffffffu, came) && ok;
             uint4 x[CHUNKS];
-            float most = 0.f;
+            uint32_t top2 = 0u;                                // the largest of even and of odd numbers (a NaN is none)
 #pragma unroll
             for (int i = 0; i < CHUNKS; ++i) {
                 x[i] = *reinterpret_cast<const uint4*>(src + (chunk0 + ((i + lane) & (CHUNKS - 1))) * 16);
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t size = w[e] & 0x7fff7fffu;
+                    const __nv_bfloat162 t = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&top2), *reinterpret_cast<const __nv_bfloat162*>(&size));
+                    top2 = *reinterpret_cast<const uint32_t*>(&t);
+                }
             }
+            float most = fmaxf(__uint_as_float(top2 << 16), __uint_as_float(top2 & 0xffff0000u));
             share[group][1][half][r] = most;
             if (FA_WIDE) {                                     // four threads have a row's numbers
                 asm volatile("barrier.cta.sync %0, 128;" ::"r"(9 + quarter) : "memory");

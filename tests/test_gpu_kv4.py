@@ -412,6 +412,20 @@ def test_values_of_all_sizes(K, monkeypatch, name, dt, seqs):
     c.check(K, backend="plain")
 
 
+@pytest.mark.parametrize("hd", [64, 128, 224])
+def test_a_bad_query_spoils_its_row_alone(K, monkeypatch, hd):
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    c = Case(K, [(150, 100), (30, 0)], 4, 2, hd, BF)
+    clean = c.run(K).view(c.rows, 4, hd)
+    c.q = c.q.clone()
+    c.q[5, 3], c.q[140, hd + 1], c.q[160, 2 * hd:3 * hd] = math.nan, math.inf, 0.0
+    out = c.run(K).view(c.rows, 4, hd)
+    assert out[5, 0].isnan().all() and out[140, 1].isnan().all() and out[160, 2].isfinite().all()
+    spoilt = torch.zeros(c.rows, 4, dtype=torch.bool, device=DEV)
+    spoilt[5, 0] = spoilt[140, 1] = spoilt[160, 2] = True
+    assert torch.equal(out[~spoilt], clean[~spoilt])
+
+
 def test_long_float32_sums_have_no_bias(K, monkeypatch):
     """One slice of 40,000 tokens in float32.  Keys' and probabilities' errors are independent, as the values are, so that their share of the
     result is at most a probability's largest error: 16 2^-24 of a score's products and 8 2^-24.  Sums that are cut off at every 16 tokens, 625 times a
