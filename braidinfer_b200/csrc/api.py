@@ -1003,7 +1003,8 @@ class Kernels:
                 args = _KV4_PROMPT_ARGS.pack(
                     q.data_ptr(), pages.data_ptr(), out.data_ptr(), *[t.data_ptr() for t in part], self._error_flag.data_ptr() + 12, sinks,
                     _ptr(gate) or 0, _ptr(bias[0]) or 0, _ptr(bias[1]) or 0, scales.data_ptr(), top + 4 * i * nkh, flags, q.stride(0), out.stride(0),
-                    gate_stride, _ptr(partial) or 0, rows, n, max_q_len, nqh, nkh, cols, window, has_sink, scale, sink, out_scale, options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0, i)
+                    gate_stride, _ptr(partial) or 0, rows, n, max_q_len, nqh, nkh, cols, window, has_sink, scale, sink, out_scale,
+                    options["softcap"] or 0.0, 0.0, 0.0, 0.0, n_splits, q_from, 0, i)
                 self.launches += 1
                 self._check_lib(lib_tc, lib_tc.braid_attn_kv4_prompt(args, stream), "attn_kv4")
             if partial is not None:

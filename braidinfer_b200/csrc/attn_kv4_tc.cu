@@ -1,5 +1,5 @@
 // Attention of prompts over a cache held in 4 bits, on the 5th-generation tensor cores (tcgen05): over the pages that kv4_expand_kernel
-// (kv4.cu) has read back as bfloat16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size:
+// (kv4.cu) has read back as float16 numbers, block c of sequence i as page i * cols + c.  Compiled for one head size:
 // -DBRAID_HD=<32, 64, ... 256>.  The sizes computed with are 64, 128 and 256; a head's further numbers are zero (in the pages, and behind the
 // queries' map).
 //
@@ -21,7 +21,8 @@
 //
 // What bounds it: the exponentials of a tile take the SM 2,048 cycles, and so do its products.  So the two groups have ONE place for their
 // scores: S of one is computed while the other's exponentials run, which keeps the groups half a turn apart without a barrier between them.
-// A tile takes some 3,000 cycles.  Prompts of 1,800, 1,346 and 689 tokens / 700 tokens behind 16,500 (88 of 148 SMs), 32 heads of 128 over 8, us with
+// A tile takes some 3,000 cycles, and a CTA some 14,000 beside its tiles (its start, the queries' way and conversion, the first tile's chain, the
+// result).  Prompts of 1,800, 1,346 and 689 tokens / 700 tokens behind 16,500 (88 of 148 SMs), 32 heads of 128 over 8, us with
 // the reading back, in bfloat16: 83 / 344 by attn_tc.cu (a thread a row, tiles of 64 keys, two CTAs an SM); 89 / 331 the same with two threads a
 // row; 90 / 332 with both groups in a CTA and scores of their own (96 / 376 with barriers that let their exponentials take turns); 104 / 393 with
 // tiles of 128 keys whose probabilities lie over the scores, where all of a group's steps wait for one another; 78 / 237 so, and 78 / 224 with

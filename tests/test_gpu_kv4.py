@@ -282,7 +282,8 @@ def test_prompts(K, route, seqs, nqh, nkh, hd, dt):
 
 
 @pytest.mark.parametrize("slices", [2, 3, 8])
-@pytest.mark.parametrize("name, hd", [("window", 64), ("sink", 128), ("sinks", 64), ("gate", 128), ("bias", 64), ("cap", 128), ("window", 96), ("gate", 32), ("window", 256), ("sinks", 160)])
+@pytest.mark.parametrize("name, hd", [("window", 64), ("sink", 128), ("sinks", 64), ("gate", 128), ("bias", 64), ("cap", 128), ("window", 96), ("gate", 32),
+                                      ("window", 256), ("sinks", 160)])
 def test_prompts_in_slices(K, monkeypatch, name, hd, slices):
     """The context cut into slices, some of them without a key that a row sees, or without any."""
     monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
