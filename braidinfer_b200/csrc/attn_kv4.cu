@@ -224,7 +224,10 @@ attn_kv4_kernel(const Kv4Args a) {
     const int unit = (int)(gridDim.x / heads - part) * (int)gridDim.z - 1 - (int)blockIdx.z;
     const int tile = unit / a.n_splits, split = unit - tile * a.n_splits;
     const int q_len = a.q_len[seq], tok0 = tile * tpc;
-    if (tok0 >= q_len || (a.q_to > 0 && q_len > a.q_to)) return;
+    if (tok0 >= q_len || (a.q_to > 0 && q_len > a.q_to)) {
+        pdl_wait();                                            // all CTAs may leave here, and a grid ends after what is ahead of it (common.cuh)
+        return;
+    }
     const int q_start = a.q_start[seq], kv_before = a.kv_before[seq];
     const int n_tok = min(tpc, q_len - tok0);
     const int head0 = kvh * g + hchunk * hpc, n_heads = min(hpc, g - hchunk * hpc);

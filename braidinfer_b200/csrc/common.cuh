@@ -55,7 +55,9 @@ void braid_set_error(const char* fmt, ...);
 // kernel of a step writes a state, or a key from before the step, that another of its kernels
 // reads.  Anyone else may call the same entry twice on one state with nothing in between.  So a
 // kernel that wants its state early begins with `if (!settled) pdl_wait();` (a second wait returns
-// at once).  BRAIDINFER_PDL=0 in the environment turns the attribute off; the two instructions are
+// at once).  A kernel waits on every way out of it that all of its CTAs may take, also where there is nothing to do:
+// its successor waits for this grid alone, and were that to end before what is ahead of it, nothing would order the successor
+// behind that.  BRAIDINFER_PDL=0 in the environment turns the attribute off; the two instructions are
 // then no-ops.
 int braid_pdl_enabled(void);
 

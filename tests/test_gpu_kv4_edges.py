@@ -1,0 +1,39 @@
+"""The 4-bit cache on the GPU where its kernels meet others: what follows them in the stream, steps that leave them nothing to do."""
+import pytest
+import torch
+
+from braidinfer_b200.csrc.api import Kernels
+from test_gpu_kv4 import BF, DEV, F32, K, Case, dev  # noqa: F401 (K is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def arguments(c, out, max_q=None, window=None):
+    return (c.q, out, c.cache, c.table.to(DEV), c.start.to(DEV), dev(c.q_len), dev(c.before), c.seq.to(DEV), len(c.q_len), max_q or max(c.q_len),
+            max(n + b for n, b in zip(c.q_len, c.before)), c.nqh, c.nkh, c.hd, window, c.hd ** -0.5)
+
+
+@pytest.mark.parametrize("slices", [None, 3])
+@pytest.mark.parametrize("seqs", [[(60, 0), (60, 40)], [(300, 3000), (200, 2500), (9, 4000)]], ids=["short", "long"])
+def test_what_follows_prompts_without_short_sequences(K, monkeypatch, seqs, slices):
+    """A settled step whose bound on the tokens a sequence is its rows: the kernel for sequences of few tokens runs behind the prompts', and
+    finds none.  What comes next in the stream starts as soon as that one has ended, and has to see the prompts' results."""
+    if slices:
+        monkeypatch.setattr(Kernels, "_kv4_prompt_slices", lambda *a: slices)
+    c = Case(K, seqs, 32, 8, 128, BF, pad=8)
+    ran, mma = [], K._attn_kv4_mma
+    monkeypatch.setattr(K, "_attn_kv4_mma", lambda *a: (ran.append(a[-2:]), mma(*a)))
+    out, next_to = torch.empty(c.rows, 32 * 128, dtype=BF, device=DEV), torch.empty(c.rows, 32 * 128, device=DEV)
+    args = arguments(c, out, max_q=c.rows)
+    K.attn_kv4(*args)                                         # (every kernel waits for the one ahead of it from its start)
+    torch.cuda.synchronize()
+    want = out.float()
+    want[sum(c.q_len):] = 9.0
+    ran.clear()
+    for _ in range(30):
+        out.fill_(9.0)
+        K.attn_kv4(*args, settled=True)
+        K.cast(out, next_to)
+        assert torch.equal(next_to, want)
+    K.check_device_errors()
+    assert ran == [(True, 2)] * 30                            # (settled, sequences of up to two tokens)
