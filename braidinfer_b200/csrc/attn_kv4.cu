@@ -359,6 +359,7 @@ attn_kv4_kernel(const Kv4Args a) {
     float o[2 * W][4], zs[2][W], m[2], l[2];
     bool ok = true;
     bool walked = PARTS == 1;
+    uint32_t wrapped = 0;                                      // FAST: its sign says that a scaled step's exponent passed 255
     int st = 0, step_exp[W];                                   // FAST: the steps of a group are scaled by 2^step_exp
     uint32_t phase = 0;
 #pragma unroll
@@ -366,7 +367,8 @@ attn_kv4_kernel(const Kv4Args a) {
     // FAST takes the scaled probabilities as float16 numbers: they are rounded by 2^-11 (a code counts up to 15 steps, which with the 2^-8 of
     // bfloat16 made errors of 0.0046 of the result), and pass the type's range where a group's later steps are much larger than its
     // first ones (2^7 times, at a probability of 1; at the other end, steps of down to 2^-23 of those keep all 11 bits): the results are
-    // then not finite, and the warp walks once more in bfloat16, codes less 8 and nothing scaled.
+    // then not finite, or, where the scaled step has passed float32's range too, its sum of exponents has run into the sign bit, which steps
+    // never have (`wrapped`).  The warp then walks once more in bfloat16, codes less 8 and nothing scaled.
     auto walk = [&](auto FAST) {
     constexpr bool fast = decltype(FAST)::value;
 #pragma unroll
@@ -563,6 +565,10 @@ attn_kv4_kernel(const Kv4Args a) {
                 const uint32_t a0 = codes<fast, 0>(v01[w]), a1 = codes<fast, 1>(v01[w]), a2 = codes<fast, 0>(v89[w]), a3 = codes<fast, 1>(v89[w]);
                 const uint32_t b0 = codes<fast, 2>(v01[w]), b1 = codes<fast, 3>(v01[w]), b2 = codes<fast, 2>(v89[w]), b3 = codes<fast, 3>(v89[w]);
                 float x[4] = {p[0] * sa, p[1] * sa, p[2] * sb, p[3] * sb};
+                if constexpr (fast) {
+                    if (!EDGE.value || s[rec][0] != -INFINITY || s[rec][1] != -INFINITY) wrapped |= __float_as_uint(sa);
+                    if (!EDGE.value || s[rec][2] != -INFINITY || s[rec][3] != -INFINITY) wrapped |= __float_as_uint(sb);
+                }
                 if constexpr (EDGE.value) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -608,7 +614,7 @@ attn_kv4_kernel(const Kv4Args a) {
     };
     if constexpr (PARTS == 1) walk(std::true_type{});
     {
-        float t = walked ? 0.f : INFINITY;
+        float t = walked && (int)wrapped >= 0 ? 0.f : INFINITY;
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) t = fmaf(0.f, o[i][0], fmaf(0.f, o[i][1], fmaf(0.f, o[i][2], fmaf(0.f, o[i][3], t))));
 #pragma unroll

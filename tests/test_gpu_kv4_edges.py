@@ -37,3 +37,35 @@ def test_what_follows_prompts_without_short_sequences(K, monkeypatch, seqs, slic
         assert torch.equal(next_to, want)
     K.check_device_errors()
     assert ran == [(True, 2)] * 30                            # (settled, sequences of up to two tokens)
+
+
+# ------------------------------------------------------------------ warps that walk many units
+HEADS = [64, 128, 160, 256]                                   # units of 64 tokens, and of 32 above 128
+
+
+def one_slice(K, monkeypatch, hd):
+    """A context is not sliced: four warps walk all of it, a unit each in turn."""
+    monkeypatch.setitem(K.kv4_attention_library(hd).plans, 0, (1, [0] * 5))
+    monkeypatch.setitem(K.kv4_attention_library(hd).plans, 1, (1, [0] * 5))
+
+
+def refill(K, c, keys=None, values=None, seed=5):
+    """The sequences' keys and values anew: functions of (numbers [tokens, kv heads, head], positions [tokens, 1, 1], length)."""
+    x = torch.randn(2, c.num * 64, c.nkh, c.hd, generator=torch.Generator().manual_seed(seed))
+    for i, (n, b) in enumerate(zip(c.q_len, c.before)):
+        t = torch.arange(n + b)
+        at = c.table[i].long()[t // 64] * 64 + t % 64
+        for plane, f in enumerate((keys, values)):
+            if f is not None:
+                x[plane, at] = f(x[plane, at], t[:, None, None], n + b)
+    K.kv4_store(x[0].flatten(1).to(DEV), x[1].flatten(1).to(DEV), dev(torch.arange(c.num * 64)), c.cache, c.hd)
+
+
+@pytest.mark.parametrize("hd", HEADS)
+@pytest.mark.parametrize("first, later", [(None, 1e10), (1e-18, 1e21), (1e-24, 1e30)])
+def test_steps_far_above_the_first_units(K, monkeypatch, hd, first, later):
+    """A group's scale comes from the first unit that a warp walks: later steps that pass float32's range times that scale are not lost."""
+    one_slice(K, monkeypatch, hd)
+    c = Case(K, [(1, 700), (3, 600)], 8, 2, hd, BF)
+    refill(K, c, values=lambda x, t, n: torch.where(t < 256, x * first if first else torch.full_like(x, 3.0), x * later))
+    c.check(K)
