@@ -118,6 +118,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // way, a code took 1.75 instructions and the 128 had to be taken off again: 64 requests of 8k 167 us instead of 140.)  Otherwise: the
 // codes less 8, as they are, in bfloat16.
 #define KV4_UNIT 133
+#define KV4_NO_STEP 101                                       // step_exp of a group whose first unit has no range
 template <bool FAST, int N> __device__ __forceinline__ uint32_t codes(uint32_t x) {
     if constexpr (FAST) {
         return (N & 2 ? x >> 8 : x) & (N & 1 ? 0x00f000f0u : 0x000f000fu);
@@ -359,16 +360,18 @@ attn_kv4_kernel(const Kv4Args a) {
     float o[2 * W][4], zs[2][W], m[2], l[2];
     bool ok = true;
     bool walked = PARTS == 1;
-    uint32_t wrapped = 0;                                      // FAST: its sign says that a scaled step's exponent passed 255
+    uint32_t signs = 0;                                        // FAST: of the scaled probabilities; one is negative where its step's exponent passed 255
     int st = 0, step_exp[W];                                   // FAST: the steps of a group are scaled by 2^step_exp
     uint32_t phase = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) step_exp[w] = 0;
     // FAST takes the scaled probabilities as float16 numbers: they are rounded by 2^-11 (a code counts up to 15 steps, which with the 2^-8 of
     // bfloat16 made errors of 0.0046 of the result), and pass the type's range where a group's later steps are much larger than its
-    // first ones (2^7 times, at a probability of 1; at the other end, steps of down to 2^-23 of those keep all 11 bits): the results are
-    // then not finite, or, where the scaled step has passed float32's range too, its sum of exponents has run into the sign bit, which steps
-    // never have (`wrapped`).  The warp then walks once more in bfloat16, codes less 8 and nothing scaled.
+    // first ones (2^7 times, at a probability of 1): the results are then not finite, or, where the scaled step has passed float32's range too, its
+    // sum of exponents has run into the sign bit, which steps and probabilities never have (`signs`).  At the other end, steps of down to 2^-23 of the first
+    // ones keep all 11 bits at a probability of 1, and what lies below is rounded to multiples of 2^-24: where the first unit's
+    // large values have next to no probability, that is all of the result (`low`, below).  Either way the warp walks once more in bfloat16, codes less
+    // 8 and nothing scaled.
     auto walk = [&](auto FAST) {
     constexpr bool fast = decltype(FAST)::value;
 #pragma unroll
@@ -407,8 +410,8 @@ attn_kv4_kernel(const Kv4Args a) {
             for (int i = 0; i < GH; ++i) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], x));
-                const int e = most[i] == 0.f ? 100 : 9 - exponent(most[i]);
-                in &= e >= 0 && e <= 100;
+                const int e = most[i] == 0.f ? KV4_NO_STEP : 9 - exponent(most[i]);
+                in &= e >= 0 && (e <= 100 || most[i] == 0.f);
 #pragma unroll
                 for (int w = 4 * i; w < W && w < 4 * i + 4; ++w) step_exp[w] = __shfl_sync(0xffffffffu, e, w & 3);
             }
@@ -565,10 +568,6 @@ attn_kv4_kernel(const Kv4Args a) {
                 const uint32_t a0 = codes<fast, 0>(v01[w]), a1 = codes<fast, 1>(v01[w]), a2 = codes<fast, 0>(v89[w]), a3 = codes<fast, 1>(v89[w]);
                 const uint32_t b0 = codes<fast, 2>(v01[w]), b1 = codes<fast, 3>(v01[w]), b2 = codes<fast, 2>(v89[w]), b3 = codes<fast, 3>(v89[w]);
                 float x[4] = {p[0] * sa, p[1] * sa, p[2] * sb, p[3] * sb};
-                if constexpr (fast) {
-                    if (!EDGE.value || s[rec][0] != -INFINITY || s[rec][1] != -INFINITY) wrapped |= __float_as_uint(sa);
-                    if (!EDGE.value || s[rec][2] != -INFINITY || s[rec][3] != -INFINITY) wrapped |= __float_as_uint(sb);
-                }
                 if constexpr (EDGE.value) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -581,7 +580,9 @@ attn_kv4_kernel(const Kv4Args a) {
                     for (int e = 0; e < 4; ++e) zs[e & 1][w] = fmaf(p[e], e < 2 ? za : zb, zs[e & 1][w]);
                 }
                 if constexpr (fast) {
-                    const uint32_t p0 = transpose8x8(pack_half(x[0], x[1])), p1 = transpose8x8(pack_half(x[2], x[3]));
+                    const uint32_t x0 = pack_half(x[0], x[1]), x1 = pack_half(x[2], x[3]);
+                    signs |= x0 | x1;
+                    const uint32_t p0 = transpose8x8(x0), p1 = transpose8x8(x1);
                     mma16816_f16(o[2 * w], a0, a1, a2, a3, p0, p1);
                     mma16816_f16(o[2 * w + 1], b0, b1, b2, b3, p0, p1);
                 } else {
@@ -613,8 +614,31 @@ attn_kv4_kernel(const Kv4Args a) {
     }
     };
     if constexpr (PARTS == 1) walk(std::true_type{});
+    bool low = false;
+    if constexpr (PARTS == 1) {
+        // Roundings of small products p step (to half of 2^-24) are at most 15 2^-25 a token of a result's number: less than 2^-11 of the
+        // group's largest number, or that is too small.  (Numbers of odd n count codes 16 times.  A group that had no range in the first unit, and has zeros
+        // for results, had none that counts: p step below 2^-126.)
+        const float least = (float)(n_mine * C::US) * (15.f * 0x1p-38f);
+        auto largest = [&](int w, int c) { return fmaxf(fmaxf(o[2 * w][c], o[2 * w + 1][c]), 0x1p-4f * fmaxf(o[2 * w][2 + c], o[2 * w + 1][2 + c])); };
+        float v = INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v = fminf(v, fminf(largest(w, 0), largest(w, 1)));
+        if (__any_sync(0xffffffffu, v < least)) {              // (of this lane's numbers; of all of a group's?)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t mine = 0x11111111u << j;        // the lanes that have this column
+                const bool sees = __ballot_sync(0xffffffffu, l[c] > 0.f) & mine;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint32_t enough = __ballot_sync(0xffffffffu, largest(w, c) >= least), some = __ballot_sync(0xffffffffu, largest(w, c) != 0.f);
+                    low |= sees && !(enough & mine) && (step_exp[w] != KV4_NO_STEP || (some & mine));
+                }
+            }
+        }
+    }
     {
-        float t = walked && (int)wrapped >= 0 ? 0.f : INFINITY;
+        float t = walked && !(signs & 0x80008000u) && !low ? 0.f : INFINITY;
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) t = fmaf(0.f, o[i][0], fmaf(0.f, o[i][1], fmaf(0.f, o[i][2], fmaf(0.f, o[i][3], t))));
 #pragma unroll

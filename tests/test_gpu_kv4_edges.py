@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from braidinfer_b200.csrc.api import Kernels
-from test_gpu_kv4 import BF, DEV, F32, K, Case, dev  # noqa: F401 (K is a fixture)
+from test_gpu_kv4 import BF, DEV, F32, K, U, Case, dev  # noqa: F401 (K is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,59 @@ def test_steps_far_above_the_first_units(K, monkeypatch, hd, first, later):
     c = Case(K, [(1, 700), (3, 600)], 8, 2, hd, BF)
     refill(K, c, values=lambda x, t, n: torch.where(t < 256, x * first if first else torch.full_like(x, 3.0), x * later))
     c.check(K)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 700), (2, 600)], [(130, 600), (40, 500)]], ids=["few", "prompts"])
+@pytest.mark.parametrize("hd", HEADS)
+@pytest.mark.parametrize("power", [12, 20, 30, 40, 60])
+def test_large_values_without_probability(K, monkeypatch, hd, power, seqs):
+    """The first tokens' values are 2^power times the others', and their scores 50 lower: the result is all the others', whose products with
+    their probabilities must keep their bits."""
+    one_slice(K, monkeypatch, hd)
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    c = Case(K, seqs, 8, 2, hd, BF)
+    c.q = c.q.clone()
+    c.q[:, ::hd] = 8.0
+
+    def keys(x, t, n):
+        x[..., :1] = torch.where(t < 256, -50.0 / 8 * hd ** 0.5, 0.0)
+        return x
+    refill(K, c, keys=keys, values=lambda x, t, n: torch.where(t < 256, x, x * 2.0 ** -power))
+    out = c.check(K)
+    # prompts' float16 operands: half a step of 2^-12 for a key, a query, a value and a probability, and the result's bfloat16
+    want, mag, smag = c.want()
+    most = mag * (2 * (2 * 2.0 ** -12 * smag[1] + 32 * U * smag[0])[..., None] + 2 * 2.0 ** -12 + 2.0 ** -18) + 2.0 ** -8 * want.abs()
+    assert ((out.double().view(want.shape) - want).abs() <= most)[:sum(c.q_len)].all()
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("hd", HEADS)
+@pytest.mark.parametrize("rise", [0.0, 3.0, -3.0])
+def test_many_units_a_warp(K, monkeypatch, hd, rise, dt):
+    """Rings that are filled again and again, and maxima that rise all along the context (or fall: the first keeps to the end)."""
+    one_slice(K, monkeypatch, hd)
+    c = Case(K, [(1, 3000), (4, 2111), (2, 0), (3, 1300)], 8, 2, hd, dt)
+    c.q = c.q.clone()
+    c.q[:, ::hd] = 8.0
+
+    def keys(x, t, n):
+        x[..., :1] = rise * t / n * hd ** 0.5
+        return x
+    refill(K, c, keys=keys)
+    out = c.check(K)
+    assert torch.equal(c.run(K), out)
+    c.check(K, window=1500, head_sinks=torch.linspace(-3, 3, 8, device=DEV))
+    c.check(K, window=700, keep_first=500)
+
+
+@pytest.mark.parametrize("hd", HEADS)
+@pytest.mark.parametrize("at", [0.3, 0.97])
+@pytest.mark.parametrize("factor", [1e6, 1e-12])
+def test_second_walks_after_many_units(K, monkeypatch, hd, at, factor):
+    """The values' sizes change where a warp has walked many units: it begins again, with its ring as it then stands."""
+    one_slice(K, monkeypatch, hd)
+    c = Case(K, [(1, 3000), (4, 2111), (1, 100), (3, 1300)], 8, 2, hd, BF)
+    refill(K, c, values=lambda x, t, n: torch.where(t < at * n, x, x * factor))
+    out = c.check(K)
+    assert torch.equal(c.run(K), out)
+    c.check(K, window=1500)
