@@ -156,7 +156,7 @@ class CacheManager:
     def begin_step(self, slot_ids: Sequence[int], new_tokens: Sequence[int], lists: bool = False) -> List:
         """Reserve pages for the tokens each sequence brings; return, per group, the page
         table [sequences, blocks] (int32, -1 where a block is absent or released), or with `lists` every sequence's
-        list of pages."""
+        list of pages: as many as the step's tokens reach, even where a step that failed has left it more."""
         if len(set(slot_ids)) != len(slot_ids):
             raise CacheError("a slot appears twice in one step")
         for g in self.groups:
@@ -171,7 +171,7 @@ class CacheManager:
             for s, n in zip(slot_ids, new_tokens):
                 g.pages.grow(s, self.lengths[s] + n)
             if lists:
-                tables.append([list(g.pages.blocks[s]) for s in slot_ids])
+                tables.append([g.pages.blocks[s][:-(-(self.lengths[s] + n) // PAGE_SIZE)] for s, n in zip(slot_ids, new_tokens)])
                 continue
             cols = max(1, max(len(g.pages.blocks[s]) for s in slot_ids))
             t = np.full((len(slot_ids), cols), -1, dtype=np.int32)
