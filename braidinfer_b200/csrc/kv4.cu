@@ -75,6 +75,7 @@ step_tables_kernel(TablesArgs a) {
         if (tq > a.rows || tb > a.n_pages_listed) bad = true;
         if (i == a.n - 1) { q0[a.n] = (int)min(tq, (long long)a.rows); b0[a.n] = (int)min(tb, (long long)a.n_pages_listed); }
     }
+    if (a.n == 0 && tid == 0) q0[0] = b0[0] = 0;              // no request: all rows are padding
     if (bad) atomicExch(a.error_flag, 1);
     __syncthreads();
     auto page_of = [&](int i, long long c) {
