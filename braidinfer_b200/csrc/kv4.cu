@@ -125,8 +125,9 @@ extern "C" int braid_step_tables(const TablesArgs* args, void* stream) {
     if (a.n > TABLES_MAX_REQUESTS) BRAID_REFUSE("step_tables: %d requests exceed %d", a.n, TABLES_MAX_REQUESTS);
     if ((long long)a.num_pages * BRAID_PAGE_SIZE > 0x7fffffffLL) BRAID_REFUSE("step_tables: places in %d pages pass 32 bits", a.num_pages);
     const long long items = (long long)a.rows + (long long)a.n * a.cols;
-    if (items == 0) return BRAID_OK;
-    const long long ctas = (items + TABLES_THREADS * TABLES_PER_THREAD - 1) / (TABLES_THREADS * TABLES_PER_THREAD);
+    if (items == 0 && a.n == 0) return BRAID_OK;
+    // (requests without rows and columns still have their first rows written and their lengths looked at)
+    const long long ctas = items == 0 ? 1 : (items + TABLES_THREADS * TABLES_PER_THREAD - 1) / (TABLES_THREADS * TABLES_PER_THREAD);
     if (ctas > 0x7fffffffLL) BRAID_REFUSE("step_tables: the tables exceed the grid limit");
     const size_t smem = 2 * ((size_t)a.n + 1) * sizeof(int);
     cudaError_t e = cudaSuccess;

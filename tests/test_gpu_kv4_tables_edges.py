@@ -17,3 +17,14 @@ def test_no_requests_and_rows_of_padding(K, rows):
     K.check_device_errors()
     assert (place[:rows] == -1).all() and (pos[:rows] == 0).all() and (seq[:rows] == -1).all()
     assert place[rows] == pos[rows] == seq[rows] == 77
+
+
+def test_requests_without_rows_and_blocks(K):
+    start = torch.full((3,), 77, dtype=torch.int32, device=DEV)
+    table = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    K.step_tables(dev([0, 0]), dev([0, 0]), dev([]), table, dev([]), num_pages=3, q_start=start[:2])
+    K.check_device_errors()
+    assert start.tolist() == [0, 0, 77]
+    K.step_tables(dev([0, 0]), dev([0, 9]), dev([]), table, dev([]), num_pages=3)
+    with pytest.raises(KernelError, match="lengths of a step's requests"):
+        K.check_device_errors()
