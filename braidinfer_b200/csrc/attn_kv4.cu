@@ -190,6 +190,9 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     return w;
 }
 
+// The parity of a stage's last use, of `uses` that went through the stages in turn.
+__host__ __device__ constexpr uint32_t kv4_last_parity(int uses, int stage, int stages) { return (uint32_t)((uses - 1 - stage) / stages) & 1u; }
+
 template <int PARTS, int NW, int SR, int ST>
 struct Kv4Cfg {
     static constexpr int HD = BRAID_HD, W = HD / 32;
@@ -256,6 +259,7 @@ attn_kv4_kernel(const Kv4Args a) {
     __syncthreads();
     const int* table = a.page_table + (size_t)seq * a.cols;
     int issued = 0, istage = 0, pages = 0;                     // a lane's page: of this warp's unit (issued & ~31) + lane
+    int earlier = 0;                                           // units that a first walk had asked for
     auto issue = [&]() {
         if ((issued & 31) == 0) {
             pages = 0;
@@ -650,21 +654,22 @@ attn_kv4_kernel(const Kv4Args a) {
         if (__any_sync(0xffffffffu, ok && t != 0.f)) {
             if constexpr (PARTS == 1) for (; st != istage; phase ^= (st == ST - 1), st = st == ST - 1 ? 0 : st + 1)        // (units asked for and not walked)
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], phase, &abort_flag)) && ok;
-            if constexpr (PARTS == 1) {
-                issued = 0;
-                while (issued < min(ST, n_mine)) issue();
+            if (PARTS != 1 || ok) {
+                if constexpr (PARTS == 1) {
+                    earlier = issued;
+                    issued = 0;
+                    while (issued < min(ST, n_mine)) issue();
+                }
+                walk(std::false_type{});
+                walked = false;
             }
-            walk(std::false_type{});
-            walked = false;
         }
     }
     if (!ok) {
         // a copy did not arrive in time: wait for the others (bounded too), so that none lands after the CTA has ended
         if (lane == 0) atomicExch(a.error_flag, 1);
-        for (int s = 0; s < ST; ++s) {
-            const int last = (issued - 1 - s) / ST;            // the last use of stage s
-            if (issued > s) for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&full[warp][s], (uint32_t)(last & 1)); ++i) {}
-        }
+        for (int s = 0; s < ST; ++s)
+            if (earlier + issued > s) for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&full[warp][s], kv4_last_parity(earlier + issued, s, ST)); ++i) {}
     }
 
     // ---- the CTA's warps merge
@@ -904,6 +909,7 @@ static int launch_kv4(const Kv4Args& a, cudaStream_t s) {
 }
 
 extern "C" int braid_attn_kv4_head_dim(void) { return BRAID_HD; }
+extern "C" int braid_attn_kv4_last_parity(int uses, int stage, int stages) { return (int)kv4_last_parity(uses, stage, stages); }
 extern "C" int braid_attn_kv4_args_bytes(void) { return (int)sizeof(Kv4Args); }
 
 // CTAs that the device holds at once.

@@ -1,7 +1,11 @@
 """The 4-bit cache without a GPU: steps that fail or bring nothing, the largest sizes."""
+import ctypes
+
+import pytest
 import torch
 
 from braidinfer_b200.cache import CacheManager
+from braidinfer_b200.csrc import build
 from braidinfer_b200.parts.spec import CacheRequest
 
 
@@ -17,3 +21,24 @@ def test_page_lists_after_a_step_that_failed():
     c.end_step([a, b], [1, 65])
     for full, g in zip(c.begin_step([b, a], [63, 128], lists=True), c.groups):
         assert full == [g.pages.blocks[b][:2], g.pages.blocks[a][:3]]
+
+
+@pytest.mark.parametrize("stages", [2, 3])
+def test_the_last_copies_of_a_ring(stages):
+    """What a warp of attn_kv4_kernel waits for before it gives up: the last use of every stage, over both walks of a context (the second
+    begins where the ring stands, after what the first had asked for and not walked)."""
+    lib = ctypes.CDLL(str(build.kv4_attention_library(64, verbose=False)))
+    for n in range(1, 9):
+        for walked in range(n + 1):                           # units of the first walk
+            phases = [0] * stages                             # copies that each stage has been given
+            uses = 0
+            asked = min(n, walked + stages)
+            for k in range(asked):
+                phases[uses % stages] += 1
+                uses += 1
+            for k in range(min(stages, n) + 1):               # and of the second, before one does not come
+                for s in range(stages):
+                    if phases[s]:                             # a barrier's phase of parity p is over when its copy has come: the last one's
+                        assert lib.braid_attn_kv4_last_parity(uses, s, stages) == (phases[s] - 1) % 2
+                phases[uses % stages] += 1
+                uses += 1
