@@ -952,6 +952,8 @@ class Kernels:
         if max_q_len <= 8 or out.dtype != torch.bfloat16:
             return False
         g = nqh // nkh
+        if not tc and -(-max_q_len // (64 // min(g, 64))) > 65535:
+            return False                                      # the older kernel's tiles of 64 columns pass the depth of a grid
         tiles = -(-g // 16) * -(-max_q_len // (16 // min(g, 16)))
         units = nkh * min(tiles * n_seqs, out.shape[0] * g // 16 + n_seqs)
         least = Kernels.KV4_PAGES_FROM * (max(1, min(3, 128 / hd)) if tc else 1)

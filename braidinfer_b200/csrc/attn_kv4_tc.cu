@@ -176,8 +176,10 @@ attn_kv4_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // CTAs start in the order x, y, z: all kv heads and sequences of the last token tile first, then
     // the tile before, ...: late tokens see the most keys, so the longest CTAs start first and the
     // short ones fill the gaps at the end
-    const int kvh = blockIdx.x / hchunks, hchunk = blockIdx.x - kvh * hchunks;
-    const int unit = gridDim.z - 1 - blockIdx.z, split = unit % a.n_splits;
+    // (more than 65,535 tiles are in parts along x)
+    const int heads = a.nkh * hchunks, part = blockIdx.x / heads, hx = blockIdx.x - part * heads;
+    const int kvh = hx / hchunks, hchunk = hx - kvh * hchunks;
+    const int unit = (int)(gridDim.x / heads - part) * (int)gridDim.z - 1 - (int)blockIdx.z, split = unit % a.n_splits;
     int seq = blockIdx.y, tile = unit / a.n_splits;
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
@@ -634,8 +636,8 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     const long long every = (a.max_q_len + FA_QTILES * tpc - 1) / (FA_QTILES * tpc);
     const long long most = a.rows / (FA_QTILES * tpc) + (a.q_from > 1 ? (a.rows / a.q_from < a.n_seqs ? a.rows / a.q_from : a.n_seqs) : a.n_seqs);
     a.tiles = 2 * most <= every * a.n_seqs ? (int)most : 0;
-    const long long gx = (a.tiles ? most : every) * a.n_splits;
-    if (gx > 65535 || (long long)a.nkh * hchunks > 0x7fffffffLL || a.n_seqs > 65535)
+    const long long gx = (a.tiles ? most : every) * a.n_splits, parts = (gx + 65534) / 65535;
+    if (gx > 0x7fffffffLL - 65535 || (long long)a.nkh * hchunks * parts > 0x7fffffffLL || a.n_seqs > 65535)
         BRAID_REFUSE("attn_kv4: the step exceeds the grid limits (%lld token tiles, %d sequences)", gx, a.n_seqs);
     if ((long long)a.n_seqs * a.cols * 2 * a.nkh * FA_PAGE > 0x7fffffffLL) BRAID_REFUSE("attn_kv4: the pages' rows pass 32 bits");
     CUtensorMap mq, mkv;
@@ -672,6 +674,6 @@ extern "C" int braid_attn_kv4_prompt(const Kv4PromptArgs* args, void* stream) {
     a.sink_log2 = a.sink * log2e;
     a.cap_log2 = a.softcap * log2e;
     braid_launch(a.softcap > 0.f ? attn_kv4_prompt_kernel<FA_CAP> : a.bias_slope ? attn_kv4_prompt_kernel<FA_BIAS> : attn_kv4_prompt_kernel<FA_PLAIN>,
-                 dim3(a.nkh * hchunks, a.tiles ? 1 : a.n_seqs, (unsigned)gx), dim3(FA_THREADS), FA_SMEM, (cudaStream_t)stream, mq, mkv, a);
+                 dim3((unsigned)(a.nkh * hchunks * parts), a.tiles ? 1 : a.n_seqs, (unsigned)((gx + parts - 1) / parts)), dim3(FA_THREADS), FA_SMEM, (cudaStream_t)stream, mq, mkv, a);
     BRAID_LAUNCH_CHECK();
 }

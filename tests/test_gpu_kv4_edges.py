@@ -125,3 +125,33 @@ def test_second_walks_after_many_units(K, monkeypatch, hd, at, factor):
     out = c.check(K)
     assert torch.equal(c.run(K), out)
     c.check(K, window=1500)
+
+
+@pytest.mark.parametrize("hd, tokens", [(32, 131075), (160, 65539)])
+def test_more_tiles_of_prompts_than_a_grid_is_deep(K, hd, tokens):
+    """128 heads a kv head: a CTA takes 2 tokens, one of heads above 128, and the two here are more than 65,535.  Plain attention is within their
+    roundings."""
+    assert -(-tokens // (2 if hd <= 128 else 1)) > 65535
+    g, nqh, window, blocks = torch.Generator(device=DEV).manual_seed(hd), 128, 24, -(-tokens // 64)
+    x = torch.randn(2, 64 * blocks, hd, generator=g, device=DEV).to(BF)
+    cache = torch.zeros(blocks, 1, K.kv4_page_bytes(hd), dtype=torch.uint8, device=DEV)
+    every = torch.arange(64 * blocks, dtype=torch.int32, device=DEV)
+    K.kv4_store(x[0], x[1], every, cache, hd)
+    q = torch.randn(tokens + 3, nqh * hd, generator=g, device=DEV).to(BF)
+    seq = torch.zeros(tokens + 3, dtype=torch.int32, device=DEV)
+    seq[tokens:] = -1
+    assert K._kv4_as_pages(q, q, tokens, tokens, 1, nqh, 1, hd, True)
+    out = []
+    for backend in ("auto", "plain"):
+        out.append(torch.full((tokens + 3, nqh * hd), 9.0, dtype=BF, device=DEV))
+        K.attn_kv4(q, out[-1], cache, every[None, :blocks].contiguous(), dev([0]), dev([tokens]), dev([0]), seq, 1, tokens, tokens, nqh, 1, hd, window, hd ** -0.5,
+                   backend=backend)
+    K.check_device_errors()
+    a, b = out
+    assert (a[tokens:] == 9).all() and (b[tokens:] == 9).all()
+    # a score is off by 2^-12 of its products twice (|q| |k| hd^-1/2 of them: 1.2 hd^1/2), a probability by twice that; these are independent of the values, as
+    # the values are of one another, so that a row of thousands of numbers is off by as much of its length
+    most = 2 * 2 * 2.0 ** -12 * 1.2 * hd ** 0.5 + 2 * 2.0 ** -12 + 2 * 2.0 ** -9
+    for i in range(0, tokens, 8192):
+        x, y = (t[i:min(i + 8192, tokens)].float() for t in out)
+        assert ((x - y).norm(dim=1) <= most * y.norm(dim=1)).all()

@@ -6,6 +6,7 @@ import torch
 
 from braidinfer_b200.cache import CacheManager
 from braidinfer_b200.csrc import build
+from braidinfer_b200.csrc.api import Kernels
 from braidinfer_b200.parts.spec import CacheRequest
 
 
@@ -42,3 +43,12 @@ def test_the_last_copies_of_a_ring(stages):
                         assert lib.braid_attn_kv4_last_parity(uses, s, stages) == (phases[s] - 1) % 2
                 phases[uses % stages] += 1
                 uses += 1
+
+
+def test_prompts_past_a_grids_depth_of_the_older_kernel():
+    """The kernel for ordinary pages refuses more than 65,535 tiles of 64 columns of queries; the others take a grid's tiles in parts."""
+    def over_pages(tokens, heads, tc):
+        x = torch.empty(1, heads * 32, dtype=torch.bfloat16).expand(tokens, heads * 32)
+        return Kernels._kv4_as_pages(x, x, tokens, tokens, 1, heads, 1, 32, tc)
+    for heads, most in ((128, 65535), (64, 65535), (16, 4 * 65535), (1, 64 * 65535)):
+        assert over_pages(most, heads, False) and not over_pages(most + 1, heads, False) and over_pages(2 * most + 1, heads, True)
