@@ -145,6 +145,8 @@ _KV4_PROMPT_ARGS = struct.Struct("<14Q3qQ8i7f4i4x")      # Kv4PromptArgs of csrc
 _TABLES_ARGS, _STORE_ARGS, _EXPAND_ARGS = struct.Struct("<8Q5i4xQ"), struct.Struct("<5Q2q5i4x"), struct.Struct("<10Q11i4x")
 _KV4_SIMPLE_ARGS = struct.Struct("<7Q2q8ifi2f2Qq3Qfi2Q")
 
+_FARTHEST = 0x7fffffff - 64           # a window or kept first tokens, so that the kernels' sums with a tile's length stay within 32 bits
+
 _KV4_PAGE_BYTES = {hd: build.page_size() * (hd + hd // 4) for hd in range(32, 257, 32)}
 
 _NO_SCALE = (None, 0, 0, 0.0, 0.0)
@@ -828,7 +830,10 @@ class Kernels:
             raise KernelError(f"kv4_expand: the cache holds {cache.shape[1]} kv heads, the pages {out.shape[2]}")
         self._i32("kv4_expand", ("page_table", page_table, 0), ("q_len", q_len, n), ("kv_before", kv_before, n))
         self._on_device("kv4_expand", cache, out)
-        self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, int(window or 0), int(keep_first or 0))
+        window, keep_first = min(int(window or 0), _FARTHEST), min(int(keep_first or 0), _FARTHEST)
+        if window < 0 or keep_first < 0:
+            raise KernelError("kv4_expand: window and keep_first must not be negative")
+        self._expand(lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first)
 
     def _expand(self, lib, cache, out, page_table, q_len, kv_before, n, hd, window, keep_first, out_cols=0, out_table=None, repair=None, seq0=0,
                 q_from=0, scales=None, top=0) -> None:
@@ -868,7 +873,8 @@ class Kernels:
             raise KernelError("attn_kv4: a cap on the scores is positive and does not go with a distance bias")
         if page_table.dim() != 2 or page_table.shape[0] < n_seqs:
             raise KernelError(f"attn_kv4: a page table of {n_seqs} sequences is wanted, got {tuple(page_table.shape)}")
-        if int(keep_first or 0) < 0 or int(window or 0) < 0 or max_q_len < 0 or max_kv_len < 0:
+        window, keep_first = min(int(window or 0), _FARTHEST), min(int(keep_first or 0), _FARTHEST)
+        if keep_first < 0 or window < 0 or max_q_len < 0 or max_kv_len < 0:
             raise KernelError("attn_kv4: window, keep_first and lengths must not be negative")
         self._i32(what, ("page_table", page_table, 0), ("q_start", q_start, n_seqs), ("q_len", q_len, n_seqs), ("kv_before", kv_before, n_seqs),
                   ("token_seq", token_seq, rows))
@@ -882,19 +888,19 @@ class Kernels:
         few = max(1, 8 // (nqh // nkh)) if tc and n_seqs > 1 and rows - max_q_len < 8 * (n_seqs - 1) else 0
         if backend == "auto" and self._kv4_as_pages(q, out, max_q_len, max_kv_len, 1 if few else n_seqs, nqh, nkh, hd, tc):
             self._attn_kv4_pages(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
-                                 int(window or 0), scale, int(keep_first or 0), head_scale, dict(
+                                 window, scale, keep_first, head_scale, dict(
                                      sink=sink, out_scale=out_scale, head_sinks=head_sinks, head_gate=head_gate, distance_bias=distance_bias,
                                      softcap=softcap), tc, few + 1 if few else 0)
             if few:
                 self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, few, max_kv_len, nqh, nkh, hd,
-                                   int(window or 0), scale, sink, out_scale, head_sinks, head_gate, 0, None, distance_bias, softcap, settled, few)
+                                   window, scale, sink, out_scale, head_sinks, head_gate, 0, None, distance_bias, softcap, settled, few)
             return
         if backend == "auto":
             self._attn_kv4_mma(q, out, cache, page_table, q_start, q_len, kv_before, token_seq, n_seqs, max_q_len, max_kv_len, nqh, nkh, hd,
-                               int(window or 0), scale, sink, out_scale, head_sinks, head_gate, int(keep_first or 0), head_scale, distance_bias,
+                               window, scale, sink, out_scale, head_sinks, head_gate, keep_first, head_scale, distance_bias,
                                softcap, settled)
             return
-        self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, int(window or 0), scale, int(keep_first or 0),
+        self._attn_kv4_plain(q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first,
                              head_scale, sink, out_scale, head_sinks, head_gate, distance_bias, softcap)
 
     def _attn_kv4_plain(self, q, out, cache, page_table, q_start, kv_before, token_seq, nqh, nkh, hd, window, scale, keep_first, head_scale, sink,

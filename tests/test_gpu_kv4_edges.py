@@ -155,3 +155,21 @@ def test_more_tiles_of_prompts_than_a_grid_is_deep(K, hd, tokens):
     for i in range(0, tokens, 8192):
         x, y = (t[i:min(i + 8192, tokens)].float() for t in out)
         assert ((x - y).norm(dim=1) <= most * y.norm(dim=1)).all()
+
+
+@pytest.mark.parametrize("far", [2 ** 31 - 65, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+def test_windows_and_kept_tokens_of_any_size(K, monkeypatch, dt, new, far):
+    """A window, or kept first tokens, past all there is (and past 32 bits) hide nothing."""
+    monkeypatch.setattr(Kernels, "KV4_PAGES_FROM", 0)
+    c = Case(K, [(new, 500), (new, 0)], 4, 2, 64, dt)
+    for kw in (dict(window=far), dict(window=7, keep_first=far), dict(window=far, keep_first=far)):
+        for backend in ("auto", "plain"):
+            c.check(K, backend=backend, **kw)
+    table = dev(torch.arange(8)[None])
+    pages, want = (torch.zeros(c.num, 2, 2, 64, 64, device=DEV) for _ in range(2))
+    K.kv4_expand(c.cache, pages, table[:, :8].contiguous(), dev([1]), dev([500]), window=3, keep_first=far)
+    K.kv4_expand(c.cache, want, table[:, :8].contiguous(), dev([1]), dev([500]))
+    K.check_device_errors()
+    assert torch.equal(pages, want)
