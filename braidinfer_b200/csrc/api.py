@@ -819,12 +819,15 @@ class Kernels:
         """Read the pages that a step's queries see back into ordinary ones, out [pages, 2, kv_heads, page size, hd] (float32 or
         bfloat16), page for page: with a window, from the first position that a sequence's first new token sees, and its kept first
         ones.  Other places of those pages, behind the sequence's end too, come out zero; other pages stay as they were.  A page belongs
-        to one sequence."""
+        to one sequence.  A visible position whose page is absent, or behind the table's end, raises a device error."""
         lib = self.part_library("kv4")
         if out.dim() != 5 or out.shape[0] != cache.shape[0] or out.shape[1] != 2 or out.shape[3] != build.page_size() or not out.is_contiguous():
             raise KernelError(f"kv4_expand: the pages must be contiguous [{cache.shape[0]}, 2, kv_heads, {build.page_size()}, head_dim], got "
                               f"{tuple(out.shape)}")
+        if page_table.dim() != 2:
+            raise KernelError(f"kv4_expand: the page table must be [sequences, blocks], got {tuple(page_table.shape)}")
         hd, n = out.shape[4], page_table.shape[0]
+        dtype_code(out.dtype)
         self._check_kv4("kv4_expand", cache, hd)
         if out.shape[2] != cache.shape[1]:
             raise KernelError(f"kv4_expand: the cache holds {cache.shape[1]} kv heads, the pages {out.shape[2]}")

@@ -400,6 +400,8 @@ kv4_expand_kernel(const ExpandArgs a) {
         for (int c = blockIdx.x + gridDim.x * threadIdx.x; c < a.out_cols; c += gridDim.x * blockDim.x)
             a.out_table[(size_t)seq * a.out_cols + c] = seq * a.out_cols + c;
     if (end - before < a.q_from) return;
+    // a table that ends before the sequence (whoever reads pages of the other numbering looks after that itself)
+    if (a.out_cols <= 0 && blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0 && end > (long long)a.cols * BRAID_PAGE_SIZE) atomicExch(a.error_flag, 1);
     constexpr bool SCALED = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
     constexpr int OUT = !SCALED ? HD : HD <= 64 ? 64 : HD <= 128 ? 128 : 256;       // numbers of a row that is written, zeros behind the head's
     __shared__ float3 sizes[2][8];

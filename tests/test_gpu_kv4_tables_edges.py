@@ -28,3 +28,23 @@ def test_requests_without_rows_and_blocks(K):
     K.step_tables(dev([0, 0]), dev([0, 9]), dev([]), table, dev([]), num_pages=3)
     with pytest.raises(KernelError, match="lengths of a step's requests"):
         K.check_device_errors()
+
+
+def test_reading_back_past_the_table(K):
+    """A sequence that is longer than its row of the page table is flagged, and what the table holds is read."""
+    cache = torch.zeros(3, 2, K.kv4_page_bytes(64), dtype=torch.uint8, device=DEV)
+    x = torch.randn(64, 128, generator=torch.Generator().manual_seed(1)).to(DEV)
+    K.kv4_store(x, x, dev(torch.arange(64) + 64), cache, 64)
+    out, want = torch.zeros(3, 2, 2, 64, 64, device=DEV), torch.zeros(3, 2, 2, 64, 64, device=DEV)
+    K.kv4_expand(cache, want, dev([[1]]), dev([1]), dev([63]))
+    K.check_device_errors()
+    for before in (64, 5000, 2 ** 31 - 2):
+        K.kv4_expand(cache, out.zero_(), dev([[1]]), dev([1]), dev([before]))
+        with pytest.raises(KernelError, match="visible position"):
+            K.check_device_errors()
+        assert torch.equal(out, want)
+    launched = K.launches
+    for bad in (dict(page_table=dev([1])), dict(out=out.half())):
+        with pytest.raises(KernelError):
+            K.kv4_expand(**{**dict(cache=cache, out=out, page_table=dev([[1]]), q_len=dev([1]), kv_before=dev([5])), **bad})
+    assert K.launches == launched
