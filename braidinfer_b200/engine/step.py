@@ -302,6 +302,8 @@ class StepPacker:
         n = len(slots)
         if token_source_rows is not None and any(len(t) != 1 for t in tokens):
             raise ValueError("tokens can be taken from the device only in steps of one token a sequence")
+        if token_source_rows is not None and len(token_source_rows) != n:
+            raise ValueError(f"{len(token_source_rows)} rows of tokens on the device for {n} sequences")
         q_len = [len(t) for t in tokens]
         n_tokens = sum(q_len)
         rows = -(-max(n_tokens, int(pad_rows_to)) // self.row_multiple) * self.row_multiple

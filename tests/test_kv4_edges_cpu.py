@@ -7,6 +7,7 @@ import torch
 from braidinfer_b200.cache import CacheManager
 from braidinfer_b200.csrc import build
 from braidinfer_b200.csrc.api import Kernels
+from braidinfer_b200.engine.step import StepPacker
 from braidinfer_b200.parts.spec import CacheRequest
 
 
@@ -52,3 +53,10 @@ def test_prompts_past_a_grids_depth_of_the_older_kernel():
         return Kernels._kv4_as_pages(x, x, tokens, tokens, 1, heads, 1, 32, tc)
     for heads, most in ((128, 65535), (64, 65535), (16, 4 * 65535), (1, 64 * 65535)):
         assert over_pages(most, heads, False) and not over_pages(most + 1, heads, False) and over_pages(2 * most + 1, heads, True)
+
+
+@pytest.mark.parametrize("rows", [[], [0], [0, 1, 2]])
+def test_rows_of_device_tokens_are_counted(rows):
+    packer = StepPacker("cpu", 1)
+    with pytest.raises(ValueError, match="rows of tokens"):
+        packer.pack_lengths([0, 1], [[5], [6]], [3, 4], [[0], [0]], [[[0], [1]]], [4], token_source_rows=rows)
