@@ -102,7 +102,8 @@ def load(model: str, dtype: str = "bfloat16", max_seq_len: Optional[int] = None,
     random weights of a named size.  `max_seq_len` caps the context of a sequence
     (default: the config's max_position_embeddings, at most 8192, as in the
     reference); the cache is sized for `max_batch` such sequences.  `cache_format` "int4" holds keys and values in 4 bits a
-    number (see `Engine`): 3.2 times the tokens in the same memory."""
+    number (see `Engine`): 3.2 times the tokens of a bfloat16 cache in the same memory; prompts want up to 1 GiB beside it, or one
+    sequence's context in 16 bits a number if that is more."""
     if model.startswith("random:"):
         cfg_dict = preset(model.split(":", 1)[1])
         source = None

@@ -2,16 +2,19 @@
 //
 // softmax over the visible keys of scale * q . k_j, with k_j = lowest + step * code a group of 32 numbers, so that
 //   q . k_j = sum over groups g of  step_jg (q_g . code_jg) + lowest_jg sum(q_g)
-//   out     = sum over keys of  (p_j step_jg) (code_jg - 8) + sum over keys of p_j (lowest_jg + 8 step_jg)     (for the numbers of group g)
-// (codes less 8: both sums are then about as small as the result.  With the codes as they are, each was some 2 standard deviations of the values
-// and the result what was left of them: errors of 0.0046 of the result in bfloat16 and 7e-6 in float32 behind 128k and 3k tokens.)
+//   out     = sum over keys of  (p_j step_jg) code_jg + sum over keys of p_j lowest_jg                         (for the numbers of group g)
+//           = sum over keys of  (p_j step_jg) (code_jg - 8) + sum over keys of p_j (lowest_jg + 8 step_jg)
+// Each sum of the first form is some 2 standard deviations of the values, and the result what is left of them; those of the second are about as
+// small as the result.  bfloat16 runs take the first, whose codes cost less, with p step in float16 (FAST below; in bfloat16 it made errors
+// of 0.0046 of the result behind 128k tokens).  Float32 runs take the second (the first: 7e-6 behind 3k tokens), and so does a warp of a
+// bfloat16 run whose values float16 does not hold.
 // The codes themselves are the tensor cores' operand (mma.sync m16n8k16, float32 sums): a mask makes two of them a pair of 16-bit
 // numbers, exact, straight from the bytes as they are stored (`codes`).  So neither keys nor values are ever rounded, and what scales
 // them is applied to a group's sums (keys) or to the probabilities (values).  Keys and value columns are the 16 rows of a product and the
 // queries its 8 columns (query heads of one kv head, of up to 8 tokens), so that few queries waste little.
 //
 // What bounds it: reading the cache, 1.25 head-size bytes a token and kv head, at about two instructions a code of which the masks and
-// shifts are half.  Every warp walks units of 32 or 64 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
+// shifts are half (64 requests of 8,000 in bfloat16: 135 us, 3.9 TB/s).  Every warp walks units of 32 or 64 tokens of its own through a ring of its own in shared memory, filled by one bulk copy a unit
 // (the units are contiguous), so that warps never wait for one another before the end, where a CTA's warps merge their maxima, sums
 // and results.  A context is sliced over CTAs where few would work on it: a few slices are a cluster, whose CTAs read one another's
 // results and end together; those of more are merged by a second kernel.
@@ -290,7 +293,7 @@ attn_kv4_kernel(const Kv4Args a) {
     // ---- queries: column r, numbers 32 w + 8 j .. + 7 of the head
     uint32_t q[W][PARTS][4];
     constexpr int GH = W > 4 ? 2 : 1;
-    constexpr int QP = PARTS > 1 ? 3 : 2;                      // 16 bits of it, or all
+    constexpr int QP = PARTS > 1 ? 3 : 2;                      // 16 bits of it (off by 2^-17, below the probabilities' 2^-12), or all
     uint32_t qb[QP][GH];                                       // the sum of group j's (and 4 + j's) numbers beside a zero, in parts
     int q_exp;                                                 // of column r: the queries are scaled by 2^q_exp
     const int col = r, tl = col / hpc, hl = col - tl * hpc;
@@ -864,7 +867,7 @@ attn_kv4_merge_few_kernel(const Kv4Args a) {
 
 // ------------------------------------------------------------------ host side
 // Four warps a CTA.  A unit is SR records of 16 tokens: four of them give a warp enough independent products to work on (one request of
-// 128k, heads of 128: 53 us with two records a unit and 12 warps an SM, 45 with four and 8, which may take 255 registers then; 54 with
+// 128k, heads of 128: 53 us with two records a unit and 12 warps an SM, 45 with four and 8 (42 in all by now), which may take 255 registers then; 54 with
 // 12 warps of four records in parts that come and go by themselves); two where the registers hold no more: float32, heads above 128.
 // More queries than 8 columns hold are more CTAs: 16 columns a CTA, which share the codes' way to the operands but leave room for two records, took
 // longer (us, 16 / 8 columns: 6 sequences of 5 tokens of 4 heads in a window of 4,096, 32 / 27; 64 of 5 behind 4,000, 214 / 179; heads of 64, 141 / 102).

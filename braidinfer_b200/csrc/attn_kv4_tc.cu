@@ -50,7 +50,7 @@ static_assert(FA_PAGE == 64, "a key tile of this kernel is two pages of 64 posit
 #define FA_OD (FA_WIDE ? 128 : FA_HD)            // result columns of a group
 #define FA_QTILES (FA_WIDE ? 1 : 2)              // tiles of 128 rows a CTA
 #define FA_HB (FA_HD / 64)                       // 64-element blocks of it
-#define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] bf16, 128-byte rows
+#define FA_QBLOCK_BYTES (128 * 128)              // [128 rows][64 elements] of 16 bits, 128-byte rows
 #define FA_PBLOCK_BYTES (64 * 128)               // [64 positions][64 elements]: what a copy brings
 #define FA_KBLOCK_BYTES (2 * FA_PBLOCK_BYTES)    // two pages on end
 #define FA_Q_BYTES (FA_HB * FA_QBLOCK_BYTES)
